@@ -104,6 +104,39 @@ class PagedAttn(ctypes.Structure):
                 ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("nsplit", c_int32), ("err", c_void_p)]
 
 
+class PagedCache(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("dtype", c_int32),
+                ("k_page_stride", c_int64), ("k_head_stride", c_int64), ("k_token_stride", c_int64),
+                ("v_page_stride", c_int64), ("v_head_stride", c_int64), ("v_token_stride", c_int64),
+                ("page_size", c_int64), ("num_pages", c_int64),
+                ("page_table", c_void_p), ("page_table_stride", c_int64), ("page_table_cols", c_int64),
+                ("lengths", c_void_p), ("max_length", c_int64),
+                ("requests", c_int64), ("kv_heads", c_int64), ("head_dim", c_int64), ("descales", c_void_p)]
+
+
+class DecodeAttn(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("q_request_stride", c_int64), ("q_head_stride", c_int64), ("heads", c_int64),
+                ("softmax_scale", c_float), ("window", c_int64), ("sinks", c_int64),
+                ("weight_sums", c_void_p), ("sums_request_stride", c_int64), ("sums_head_stride", c_int64),
+                ("out", c_void_p), ("out_request_stride", c_int64), ("out_head_stride", c_int64),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("err", c_void_p)]
+
+
+class WindowAttn(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("q_token_stride", c_int64), ("q_head_stride", c_int64), ("rows", c_int64),
+                ("heads", c_int64), ("cu_seqlens_q", c_void_p), ("max_q", c_int64), ("softmax_scale", c_float),
+                ("window", c_int64), ("sinks", c_int64),
+                ("out", c_void_p), ("out_token_stride", c_int64), ("out_head_stride", c_int64),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("err", c_void_p)]
+
+
+class Evict(ctypes.Structure):
+    _fields_ = [("weight_sums", c_void_p), ("sums_request_stride", c_int64), ("sums_head_stride", c_int64),
+                ("budget", c_int64), ("sinks", c_int64), ("recent", c_int64),
+                ("out_page_table", c_void_p), ("out_page_table_stride", c_int64), ("out_page_table_cols", c_int64),
+                ("kept", c_void_p), ("lengths", c_void_p), ("out_sums", c_void_p), ("err", c_void_p)]
+
+
 _SIGNATURES = {
     "fm_last_error": (ctypes.c_char_p, []),
     "fm_version": (c_int, []),
@@ -137,6 +170,12 @@ _SIGNATURES = {
     "fm_paged_attn_nsplit": (c_int32, [c_int64, c_int64, c_int64, c_int64, c_int32]),
     "fm_paged_attn_workspace_size": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int32]),
     "fm_paged_cross_attn": (c_int, [ctypes.POINTER(PagedAttn), c_void_p]),
+    "fm_paged_decode_attn_workspace_size": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                                       c_int32]),
+    "fm_paged_decode_attn": (c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(DecodeAttn), c_void_p]),
+    "fm_paged_window_attn_workspace_size": (c_size_t, [c_int64] * 9),
+    "fm_paged_window_attn": (c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(WindowAttn), c_void_p]),
+    "fm_paged_evict": (c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(Evict), c_void_p]),
     "fm_tree_build": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
     "fm_tree_commit": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

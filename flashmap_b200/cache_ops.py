@@ -1,0 +1,237 @@
+"""Operators on a paged key/value cache that a target model decodes with:
+
+* ``paged_decode_attention``: attention of one new token per request, split
+  over the cache's length and joined, which can also gather each position's
+  attention weight;
+* ``paged_window_attention``: causal attention of chunks of query rows (a
+  prompt, a drafted block to verify) with a sliding window and first tokens
+  that stay visible;
+* ``evict_paged_context``: cuts contexts to a budget of positions, those that
+  gathered the most attention weight among them.
+
+The cache is given by two views ``k_cache`` and ``v_cache (pages, kv_heads,
+page_size, head_dim)``, bf16 or e4m3, whose rows are contiguous and 16-byte
+aligned; the other strides are free.  For vLLM's joint cache they are
+``kv_cache[..., :head_dim]`` and ``kv_cache[..., head_dim:]``; for a pool of
+rows ``(slots, kv_heads, head_dim)`` they are ``pool.unsqueeze(2)``, a page
+size of 1.  Token i of request r is token ``i % page_size`` of page
+``block_table[r, i // page_size]``.  An e4m3 cache takes ``descales (2,
+requests, kv_heads)``, the factors of keys and values.
+
+Query head h reads kv head ``h // (heads / kv_heads)``.  Scores, softmax sums
+and outputs are held in fp32; the softmax numerators are rounded to bf16 (to
+f16 for an e4m3 cache) for the product with the values, and the output to bf16.
+A row that sees no position is zero.  A position that no row of a request may
+see is never read.  Each call checks its arguments (``OpArgumentError``), runs
+on the current stream without a host synchronisation, and can be captured in a
+CUDA graph.  There is no fallback.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from .serving_ops import OpArgumentError, _err, _need
+
+__all__ = ["OpArgumentError", "paged_decode_attention", "paged_window_attention", "evict_paged_context"]
+
+_FP8 = torch.float8_e4m3fn
+
+
+def _on(t: torch.Tensor, name: str, device) -> None:
+    _need(t.device == device, f"{name} must be on {device}, got {t.device}")
+
+
+def _cache(k_cache, v_cache, lengths, block_table, descales, max_len: int) -> _lib.PagedCache:
+    _need(k_cache.is_cuda, "k_cache must be a CUDA tensor")
+    dev = k_cache.device
+    _need(dev.index == torch.cuda.current_device(), f"the cache is on {dev}, which is not the current device")
+    _on(v_cache, "v_cache", dev)
+    _on(lengths, "the lengths", dev)
+    _on(block_table, "block_table", dev)
+    _need(k_cache.dtype is torch.bfloat16 or k_cache.dtype is _FP8, f"the cache must be bf16 or e4m3, got {k_cache.dtype}")
+    _need(v_cache.dtype is k_cache.dtype, "k_cache and v_cache must share a dtype")
+    _need(k_cache.dim() == 4 and v_cache.shape == k_cache.shape,
+          "k_cache and v_cache must both be (pages, kv_heads, page_size, head_dim)")
+    pages, kv_heads, page, head_dim = k_cache.shape
+    _need(head_dim == 64 or head_dim == 128, f"head_dim must be 64 or 128, got {head_dim}")
+    _need(kv_heads > 0 and page > 0, "the cache needs a kv head and a token to a page")
+    ks, vs = k_cache.stride(), v_cache.stride()
+    _need(ks[3] == 1 and vs[3] == 1, "cache rows must be contiguous")
+    _need(lengths.dtype is torch.int32 and lengths.dim() == 1 and lengths.is_contiguous(),
+          "the lengths must be contiguous int32 (requests,)")
+    requests = lengths.shape[0]
+    _need(block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.shape[0] == requests,
+          "block_table must be int32 (requests, pages)")
+    _need(block_table.shape[1] <= 1 or block_table.stride(1) == 1, "block_table rows must be contiguous")
+    _need(max_len >= 0, "the largest length must not be negative")
+    dp = None
+    if k_cache.dtype is _FP8:
+        if descales is not None:
+            _on(descales, "descales", dev)
+            _need(descales.dtype is torch.float32 and descales.shape == (2, requests, kv_heads)
+                  and descales.is_contiguous(), "descales must be contiguous float32 (2, requests, kv_heads)")
+            dp = descales.data_ptr()
+    else:
+        _need(descales is None, "descales go with an e4m3 cache")
+    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(),
+                           _lib.FM_DT_E4M3 if k_cache.dtype is _FP8 else _lib.FM_DT_BF16,
+                           ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], page, pages, block_table.data_ptr(),
+                           block_table.stride(0), block_table.shape[1], lengths.data_ptr(), max_len, requests,
+                           kv_heads, head_dim, dp)
+
+
+def _query(query, name: str, cache: _lib.PagedCache, device) -> torch.Tensor:
+    _on(query, name, device)
+    _need(query.dtype is torch.bfloat16 and query.dim() == 3, f"{name} must be bf16 (rows, heads, head_dim)")
+    heads, head_dim = query.shape[1], query.shape[2]
+    _need(head_dim == cache.head_dim, f"{name} has rows of {head_dim}, the cache of {cache.head_dim}")
+    _need(heads > 0 and heads % cache.kv_heads == 0, f"{heads} query heads are no multiple of {cache.kv_heads} kv heads")
+    if query.stride(2) != 1 or query.data_ptr() % 16 or query.stride(0) % 8 or query.stride(1) % 8:
+        query = query.contiguous()
+        if query.data_ptr() % 16:  # a contiguous view that starts between two 16-byte lines
+            query = query.clone()
+    return query
+
+
+def _visibility(window: int, sinks: int) -> None:
+    _need(window >= 0 and sinks >= 0, "window and sinks must not be negative")
+
+
+def _sums(weight_sums, cache: _lib.PagedCache, device, least: int) -> None:
+    _on(weight_sums, "weight_sums", device)
+    _need(weight_sums.dtype is torch.float32 and weight_sums.dim() == 3
+          and weight_sums.shape[0] == cache.requests and weight_sums.shape[1] == cache.kv_heads,
+          "weight_sums must be float32 (requests, kv_heads, positions)")
+    _need(weight_sums.shape[2] >= least, f"weight_sums has {weight_sums.shape[2]} positions, {least} are needed")
+    _need(weight_sums.shape[2] <= 1 or weight_sums.stride(2) == 1, "weight_sums rows must be contiguous")
+
+
+def _raw_stream(device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                           seqused_k: torch.Tensor, block_table: torch.Tensor, max_seqlen_k: int,
+                           softmax_scale: float, *, window: int = 0, sinks: int = 0,
+                           descales: Optional[torch.Tensor] = None,
+                           weight_sums: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per request, ``query (requests, heads,
+    head_dim)`` bf16, at position ``seqused_k - 1`` of its context (its own key
+    and value are in the cache already); ``(requests, heads, head_dim)`` bf16.
+
+    It sees every position, or with ``window > 0`` the last ``window`` and the
+    first ``sinks``.  ``weight_sums (requests, kv_heads, >= max_seqlen_k)`` fp32
+    is added to in place: position j of a kv head gathers the attention weights
+    of its query heads, which ``evict_paged_context`` goes by.  A request has at
+    most ``max_seqlen_k`` positions."""
+    cache = _cache(k_cache, v_cache, seqused_k, block_table, descales, int(max_seqlen_k))
+    dev = k_cache.device
+    query = _query(query, "query", cache, dev)
+    _need(query.shape[0] == cache.requests, "one query row per request")
+    _visibility(window, sinks)
+    out = torch.empty(query.shape, dtype=torch.bfloat16, device=dev)
+    if weight_sums is not None:
+        _sums(weight_sums, cache, dev, cache.max_length)
+    if cache.requests == 0:
+        return out
+    lib = _lib.load()
+    heads, qs, os = query.shape[1], query.stride(), out.stride()
+    args = _lib.DecodeAttn(query.data_ptr(), qs[0], qs[1], heads, softmax_scale, window, sinks, None, 0, 0,
+                           out.data_ptr(), os[0], os[1], None, 0, _err(dev).data_ptr())
+    if weight_sums is not None:
+        args.weight_sums = weight_sums.data_ptr()
+        args.sums_request_stride, args.sums_head_stride = weight_sums.stride(0), weight_sums.stride(1)
+    need = lib.fm_paged_decode_attn_workspace_size(cache.requests, heads, cache.kv_heads, cache.head_dim,
+                                                   cache.max_length, window, sinks, weight_sums is not None)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    _lib.call("fm_paged_decode_attn", ctypes.byref(cache), ctypes.byref(args), _raw_stream(dev))
+    return out
+
+
+def paged_window_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                           cu_seqlens_q: torch.Tensor, seqused_k: torch.Tensor, block_table: torch.Tensor,
+                           max_seqlen_q: int, max_seqlen_k: int, softmax_scale: float, *, window: int = 0,
+                           sinks: int = 0, descales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of chunks of query rows: rows ``cu_seqlens_q[r] ..
+    cu_seqlens_q[r + 1]`` of ``query (tokens, heads, head_dim)`` bf16 are the
+    last positions of request r's ``seqused_k[r]`` (their own keys and values
+    are in the cache already); ``(tokens, heads, head_dim)`` bf16.
+
+    The row at position p sees the positions j <= p; with ``window > 0`` of
+    those only p - j < ``window`` or j < ``sinks``.  A request has at most
+    ``max_seqlen_q`` rows and ``max_seqlen_k`` positions.  Values that some rows
+    of a chunk see and others do not must be finite."""
+    cache = _cache(k_cache, v_cache, seqused_k, block_table, descales, int(max_seqlen_k))
+    dev = k_cache.device
+    query = _query(query, "query", cache, dev)
+    _on(cu_seqlens_q, "cu_seqlens_q", dev)
+    _need(cu_seqlens_q.dtype is torch.int32 and cu_seqlens_q.shape == (cache.requests + 1,)
+          and cu_seqlens_q.is_contiguous(), "cu_seqlens_q must be contiguous int32 (requests + 1,)")
+    _need(max_seqlen_q >= 0, "max_seqlen_q must not be negative")
+    _visibility(window, sinks)
+    out = torch.empty(query.shape, dtype=torch.bfloat16, device=dev)
+    tokens, heads = query.shape[0], query.shape[1]
+    if cache.requests == 0 or tokens == 0:
+        return out
+    lib = _lib.load()
+    qs, os = query.stride(), out.stride()
+    args = _lib.WindowAttn(query.data_ptr(), qs[0], qs[1], tokens, heads, cu_seqlens_q.data_ptr(),
+                           int(max_seqlen_q), softmax_scale, window, sinks, out.data_ptr(), os[0], os[1], None, 0,
+                           _err(dev).data_ptr())
+    need = lib.fm_paged_window_attn_workspace_size(cache.requests, tokens, heads, cache.kv_heads, cache.head_dim,
+                                                   int(max_seqlen_q), cache.max_length, window, sinks)
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    _lib.call("fm_paged_window_attn", ctypes.byref(cache), ctypes.byref(args), _raw_stream(dev))
+    return out
+
+
+def evict_paged_context(k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k: torch.Tensor,
+                        block_table: torch.Tensor, weight_sums: torch.Tensor, budget: int, *, sinks: int = 0,
+                        recent: int = 0, out_block_table: Optional[torch.Tensor] = None
+                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Cuts every context to ``budget`` positions, for each kv head its own: the
+    first ``sinks``, the last ``recent`` and, of those between, the ones with
+    the largest ``weight_sums (requests, kv_heads, positions)`` (the lowest
+    position among equal sums; a sum that is no number ranks last).  A context
+    within the budget stays whole.
+
+    The kept rows move, in order of position, to the request's first slots: in
+    place (the pages after them are free then), or with ``out_block_table
+    (requests, pages)`` to its pages of the same pool, which must be none that
+    ``block_table`` names (pages shared between requests keep their rows).
+    Keys move as they are, rotated at their old positions.
+
+    Returns ``kept (requests, kv_heads, budget)`` int32, the kept positions and
+    then -1; the new lengths ``(requests,)`` int32; and the kept positions' sums
+    ``(requests, kv_heads, budget)``, then 0, to go on gathering in."""
+    _need(weight_sums.dim() == 3, "weight_sums must be float32 (requests, kv_heads, positions)")
+    cache = _cache(k_cache, v_cache, seqused_k, block_table, None, weight_sums.shape[2])
+    dev = k_cache.device
+    _sums(weight_sums, cache, dev, 0)
+    _need(budget >= 1, "the budget must be positive")
+    _need(sinks >= 0 and recent >= 0 and sinks + recent <= budget, "sinks + recent must lie within the budget")
+    kept = torch.empty((cache.requests, cache.kv_heads, budget), dtype=torch.int32, device=dev)
+    lengths = torch.empty(cache.requests, dtype=torch.int32, device=dev)
+    sums = torch.empty((cache.requests, cache.kv_heads, budget), dtype=torch.float32, device=dev)
+    args = _lib.Evict(weight_sums.data_ptr(), weight_sums.stride(0), weight_sums.stride(1), budget, sinks, recent,
+                      None, 0, 0, kept.data_ptr(), lengths.data_ptr(), sums.data_ptr(), _err(dev).data_ptr())
+    if out_block_table is not None:
+        _on(out_block_table, "out_block_table", dev)
+        _need(out_block_table.dtype is torch.int32 and out_block_table.dim() == 2
+              and out_block_table.shape[0] == cache.requests, "out_block_table must be int32 (requests, pages)")
+        _need(out_block_table.shape[1] <= 1 or out_block_table.stride(1) == 1, "out_block_table rows must be contiguous")
+        _need(out_block_table.shape[1] * cache.page_size >= budget, "out_block_table does not cover the budget")
+        args.out_page_table = out_block_table.data_ptr()
+        args.out_page_table_stride, args.out_page_table_cols = out_block_table.stride(0), out_block_table.shape[1]
+    if cache.requests:
+        _lib.call("fm_paged_evict", ctypes.byref(cache), ctypes.byref(args), _raw_stream(dev))
+    return kept, lengths, sums

@@ -1,0 +1,562 @@
+// Attention of one new token per request over a paged key/value cache.
+//
+// For request r and query head h of the group that shares kv head c, over the
+// positions j that the token sees:
+//   s_j = scale q_h . k_j,  w_j = exp(s_j - max s) / sum exp(s - max s),
+//   out_h = sum_j w_j v_j,  and, when asked for, sums[r, c, j] += sum over the
+// group's heads of w_j.
+//
+// The keys and values are read once and each takes part in 4 G operations a
+// byte at most (G query heads to a kv head), so the cache's bytes bound it.
+// The visible positions are cut into chunks of equal length, one CTA per
+// (chunk, request, kv head, 8 or 16 query heads): requests of very different
+// lengths then make units of the same size, and one long request fills the
+// GPU.  Each of a CTA's four warps streams its own 16-key tiles through a
+// cp.async pipeline, with its own running maximum and sum, and the warps are
+// merged at the end.  Chunks are joined by a second kernel
+// (decode_join_kernel), which also turns the scores that the first one left
+// into weights, since only then are a row's maximum and sum known.
+#include "paged_cache.cuh"
+
+namespace fm {
+namespace {
+
+constexpr int DA_STAGES = 3;
+constexpr int DA_TILE = 16;  // keys of a warp's tile
+
+struct DecodeArgs {
+  CacheRef c;
+  const uint8_t* q;  // bf16
+  long long q_rs, q_hs;  // elements
+  int H, G, hgroups;     // heads, heads per kv head, CTAs' head groups per kv head
+  float scale;           // softmax_scale * log2(e)
+  int window, sinks;
+  int chunk, chunks;     // keys per chunk, chunks per item
+  __nv_bfloat16* out;
+  long long o_rs, o_hs;
+  float* sums;
+  long long s_rs, s_hs;
+  float* part;    // [R * H][chunks][HD] unnormalised outputs
+  float2* stats;  // [R * H][chunks] (maximum, sum), base-2 scores
+  float* scores;  // [R * H][pitch] base-2 scores, when sums are wanted
+  int pitch;
+  int* err;
+};
+
+template <int HD, bool KV8>
+struct DaLayout {
+  static constexpr int RB = HD * (KV8 ? 1 : 2);       // bytes of a key row
+  static constexpr int PART = DA_TILE * RB;           // K or V of a tile
+  static constexpr int WARP = DA_STAGES * 2 * PART;
+  static constexpr int PIPE = 4 * WARP;
+};
+
+template <int HD, bool KV8, int NG>
+constexpr int da_smem() {
+  constexpr int merge = 4 * 8 * NG * (HD + 4) * 4 + 4 * 8 * NG * 8 + 8 * NG * 8;
+  return (DaLayout<HD, KV8>::PIPE > merge ? DaLayout<HD, KV8>::PIPE : merge) + 4 * DA_STAGES * 4;
+}
+
+// NG: groups of 8 query heads (1 or 2).  Scores: S[heads][keys] = Q K^T with
+// the heads as the 16 rows of the product; then O^T[d][heads] = V^T P^T, whose
+// B operand is the scores' accumulator layout as it stands.
+template <int HD, bool KV8, int NG>
+__global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
+  using Lay = DaLayout<HD, KV8>;
+  constexpr int RB = Lay::RB, MT = HD / 16, KS = HD / 16;
+  extern __shared__ __align__(1024) uint8_t da_smem_buf[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+  pdl_wait();
+  const int items = a.c.R * a.c.KH * a.hgroups;
+  const int chunk = blockIdx.x / items;
+  int rest = blockIdx.x % items;
+  const int hg = rest % a.hgroups;
+  rest /= a.hgroups;
+  const int c = rest % a.c.KH, r = rest / a.c.KH;
+  const int h0 = c * a.G + hg * 8 * NG;                 // first query head
+  const int nh = min(8 * NG, a.G - hg * 8 * NG);        // query heads of this CTA
+  const int len = cache_length(a.c, r, a.err, threadIdx.x == 0 && chunk == 0);
+  const Span sp = visible_span(len, a.window, a.sinks);
+  const int begin = chunk * a.chunk;
+  const int end = min(sp.n, begin + a.chunk);
+  if (begin >= end) {
+    if (chunk == 0)  // nothing to attend to: zero rows
+      for (int i = threadIdx.x; i < nh * HD; i += 128)
+        a.out[(long long)r * a.o_rs + (long long)(h0 + i / HD) * a.o_hs + i % HD] = f2bf(0.0f);
+    return;
+  }
+
+  float kd = 1.0f, vd = 1.0f;
+  if (a.c.descales) {
+    kd = a.c.descales[(long long)r * a.c.KH + c];
+    vd = a.c.descales[(long long)(a.c.R + r) * a.c.KH + c];
+  }
+
+  // Query fragments: head h0 + gid (and + 8).  An 8-bit key row is read four
+  // bytes to a lane, so there a lane holds columns 4 tig .. 4 tig + 3 of each
+  // sixteen, and for 16-bit rows columns 2 tig, 2 tig + 1 and those plus 8.
+  uint32_t qa[NG][KS][2];
+  float sscale[NG];
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    const bool live = gid + 8 * n < nh;
+    const __nv_bfloat16* row =
+        reinterpret_cast<const __nv_bfloat16*>(a.q) + (long long)r * a.q_rs + (long long)(h0 + (live ? gid + 8 * n : 0)) * a.q_hs;
+    float amax = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const int col = ks * 16 + (KV8 ? tig * 4 + f * 2 : tig * 2 + f * 8);
+        qa[n][ks][f] = live ? *reinterpret_cast<const uint32_t*>(row + col) : 0u;
+        if constexpr (KV8) {
+          amax = fmaxf(amax, fabsf(__uint_as_float(qa[n][ks][f] << 16)));
+          amax = fmaxf(amax, fabsf(__uint_as_float(qa[n][ks][f] & 0xffff0000u)));
+        }
+      }
+    sscale[n] = a.scale * kd;
+    if constexpr (KV8) {
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const float f = half_row_scale(amax);
+      sscale[n] = sscale[n] / f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          qa[n][ks][e] = pack16(__uint_as_float(qa[n][ks][e] << 16) * f,
+                                __uint_as_float(qa[n][ks][e] & 0xffff0000u) * f, true);
+    }
+  }
+
+  const uint32_t wbase = smem_u32(da_smem_buf) + warp * Lay::WARP;
+  uint32_t* wok = reinterpret_cast<uint32_t*>(da_smem_buf + da_smem<HD, KV8, NG>() - 4 * DA_STAGES * 4) + warp * DA_STAGES;
+  const int ntiles = (end - begin + 4 * DA_TILE - 1) / (4 * DA_TILE);
+  const long long trow = (long long)r * a.c.tstride;
+  // page of this lane's key of tile t (lanes 0 .. 15), read one tile ahead of its copies
+  auto lookup = [&](int t, int* tok) {
+    const int i = begin + (t * 4 + warp) * DA_TILE + lane;
+    if (lane >= DA_TILE || i >= end) return -1;
+    const int p = sp.pos(i), pg = p / a.c.page;
+    *tok = p - pg * a.c.page;
+    const int page = a.c.table[trow + pg];
+    if (page >= 0 && page < a.c.num_pages) return page;
+    record_error(a.err, DEV_BAD_INDEX);
+    return -1;
+  };
+  int tok_next = 0, page_next = lookup(0, &tok_next);
+  auto issue = [&](int t) {
+    if (t < ntiles) {
+      const int page = page_next, tok = tok_next;
+      page_next = lookup(t + 1, &tok_next);
+      const int st = t % DA_STAGES;
+      const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
+      if (lane == 0) wok[st] = ok;
+      const uint32_t sbase = wbase + st * 2 * Lay::PART;
+      constexpr int CPR = RB / 16, RPI = 32 / CPR;  // copies per row, rows per instruction
+#pragma unroll
+      for (int u = 0; u < DA_TILE / RPI; ++u) {
+        const int row = u * RPI + lane / CPR, ch = lane % CPR;
+        const long long pg = __shfl_sync(0xffffffffu, page, row);
+        const long long tk = __shfl_sync(0xffffffffu, tok, row);
+        const uint32_t dst = sbase + row_sw<RB>(row, ch);
+        const uint8_t* ks = a.c.k;
+        const uint8_t* vs = a.c.v;
+        if (pg >= 0) {
+          ks += pg * a.c.kps + (long long)c * a.c.khs + tk * a.c.kts + ch * 16;
+          vs += pg * a.c.vps + (long long)c * a.c.vhs + tk * a.c.vts + ch * 16;
+        }
+        // rows that no position stands for are zero: what the cache holds there may be no number
+        pc_cp_async16(dst, ks, pg >= 0 ? 16u : 0u);
+        pc_cp_async16(dst + Lay::PART, vs, pg >= 0 ? 16u : 0u);
+      }
+    }
+    pc_cp_commit();
+  };
+#pragma unroll
+  for (int t = 0; t < DA_STAGES - 1; ++t) issue(t);
+
+  float o[NG][MT][4];
+  float m[NG], l[NG];
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+  }
+
+  for (int t = 0; t < ntiles; ++t) {
+    issue(t + DA_STAGES - 1);
+    pc_cp_wait<DA_STAGES - 1>();
+    __syncwarp();
+    const uint32_t kb0 = wbase + (t % DA_STAGES) * 2 * Lay::PART, vb0 = kb0 + Lay::PART;
+    const uint32_t ok = wok[t % DA_STAGES];
+    float sc[2][4];  // keys 8 nt + 2 tig (+ 1) of heads gid, gid + 8
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
+      const int kr = nt * 8 + (lane & 7);
+      if constexpr (KV8) {
+#pragma unroll
+        for (int k4 = 0; k4 < KS; k4 += 4) {
+          uint32_t b[4];
+          ldsm4(kb0 + row_sw<RB>(kr, k4 + (lane >> 3)), b);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            mma16816<true>(sc[nt], qa[0][k4 + e][0], NG == 2 ? qa[NG - 1][k4 + e][0] : 0u, qa[0][k4 + e][1],
+                           NG == 2 ? qa[NG - 1][k4 + e][1] : 0u, e4m3x2_h(b[e] & 0xffffu), e4m3x2_h(b[e] >> 16));
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks += 2) {
+          uint32_t b[4];
+          ldsm4(kb0 + row_sw<RB>(kr, 2 * ks + (lane >> 3)), b);
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            mma16816<false>(sc[nt], qa[0][ks + e][0], NG == 2 ? qa[NG - 1][ks + e][0] : 0u, qa[0][ks + e][1],
+                            NG == 2 ? qa[NG - 1][ks + e][1] : 0u, b[2 * e], b[2 * e + 1]);
+        }
+      }
+    }
+    const int key0 = begin + (t * 4 + warp) * DA_TILE;
+    uint32_t pb[NG][2];
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& s = sc[nt][2 * n + e];
+          s = (ok >> (nt * 8 + tig * 2 + e)) & 1u ? s * sscale[n] : -INFINITY;
+          mx = fmaxf(mx, s);
+        }
+      if (a.scores != nullptr && gid + 8 * n < nh) {
+        float* dst = a.scores + ((long long)r * a.H + h0 + gid + 8 * n) * a.pitch + key0 + tig * 2;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)  // the pitch is even and past every chunk's last whole tile
+          if (key0 + nt * 8 + tig * 2 < end)
+            *reinterpret_cast<float2*>(dst + nt * 8) = make_float2(sc[nt][2 * n], sc[nt][2 * n + 1]);
+      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[n], mx);
+      const float u = mn == -INFINITY ? 0.0f : mn;
+      if (__any_sync(0xffffffffu, mn != m[n])) {
+        const float al = exp2f(m[n] - u);
+        l[n] *= al;
+        // the outputs' columns are heads 2 tig, 2 tig + 1
+        const float a0 = __shfl_sync(0xffffffffu, al, tig * 8), a1 = __shfl_sync(0xffffffffu, al, tig * 8 + 4);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          o[n][i][0] *= a0;
+          o[n][i][1] *= a1;
+          o[n][i][2] *= a0;
+          o[n][i][3] *= a1;
+        }
+        m[n] = mn;
+      }
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const float p0 = exp2f(sc[nt][2 * n] - u), p1 = exp2f(sc[nt][2 * n + 1] - u);
+        l[n] += p0 + p1;
+        pb[n][nt] = pack16(p0, p1, KV8);
+      }
+    }
+    if constexpr (KV8) {
+      // one transposed load of byte pairs holds columns 2 gid and 2 gid + 1 of
+      // two keys: rows gid and gid + 8 of the product stand for those columns
+#pragma unroll
+      for (int i = 0; i < MT; i += 2) {
+        uint32_t b[4];
+        ldsm4_t(vb0 + row_sw<RB>((lane & 7) + ((lane >> 3) & 1) * 8, i + (lane >> 4)), b);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t x = b[2 * e], y = b[2 * e + 1];
+          const uint32_t a0 = e4m3x2_h(__byte_perm(x, 0, 0x4420)), a1 = e4m3x2_h(__byte_perm(x, 0, 0x4431));
+          const uint32_t a2 = e4m3x2_h(__byte_perm(y, 0, 0x4420)), a3 = e4m3x2_h(__byte_perm(y, 0, 0x4431));
+#pragma unroll
+          for (int n = 0; n < NG; ++n) mma16816<true>(o[n][i + e], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        uint32_t b[4];  // (keys 0-7, d 0-7), (keys 0-7, d 8-15), (keys 8-15, d 0-7), (keys 8-15, d 8-15)
+        ldsm4_t(vb0 + row_sw<RB>((lane & 7) + (lane >> 4) * 8, 2 * i + ((lane >> 3) & 1)), b);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) mma16816<false>(o[n][i], b[0], b[1], b[2], b[3], pb[n][0], pb[n][1]);
+      }
+    }
+    __syncwarp();  // the stage may be refilled from here on
+  }
+  pc_cp_wait<0>();
+  __syncthreads();  // every warp's pipeline is drained: its shared memory is free
+
+  // merge the four warps: each head's maximum, sum and output
+  float* mO = reinterpret_cast<float*>(da_smem_buf);  // [4][8 NG][HD + 4]
+  float2* mS = reinterpret_cast<float2*>(mO + 4 * 8 * NG * (HD + 4));
+  float2* mR = mS + 4 * 8 * NG;
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
+    l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
+    if (tig == 0) mS[warp * 8 * NG + n * 8 + gid] = make_float2(m[n], l[n]);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = i * 16 + (KV8 ? 2 * gid + (e >> 1) : gid + (e >> 1) * 8);
+        mO[(warp * 8 * NG + n * 8 + tig * 2 + (e & 1)) * (HD + 4) + d] = o[n][i][e];
+      }
+  }
+  __syncthreads();
+  const bool single = sp.n <= a.chunk;
+  if (threadIdx.x < nh) {
+    float mm = -INFINITY, ll = 0.0f;
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, mS[w * 8 * NG + threadIdx.x].x);
+    const float u = mm == -INFINITY ? 0.0f : mm;
+    for (int w = 0; w < 4; ++w) {
+      float2& s = mS[w * 8 * NG + threadIdx.x];
+      s.x = exp2f(s.x - u);  // from here on the warp's factor
+      ll += s.y * s.x;
+    }
+    mR[threadIdx.x] = make_float2(mm, ll);
+    if (!single || a.scores != nullptr)
+      a.stats[((long long)r * a.H + h0 + threadIdx.x) * a.chunks + chunk] = make_float2(mm, ll);
+  }
+  __syncthreads();
+  for (int v = threadIdx.x; v < nh * (HD / 4); v += 128) {
+    const int h = v / (HD / 4), d = (v % (HD / 4)) * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = mS[w * 8 * NG + h].x;
+      const float4 x = *reinterpret_cast<const float4*>(&mO[(w * 8 * NG + h) * (HD + 4) + d]);
+      acc.x += x.x * f;
+      acc.y += x.y * f;
+      acc.z += x.z * f;
+      acc.w += x.w * f;
+    }
+    acc.x *= vd;
+    acc.y *= vd;
+    acc.z *= vd;
+    acc.w *= vd;
+    if (single) {
+      const float ll = mR[h].y, inv = ll == 0.0f ? 0.0f : 1.0f / ll;  // a row whose scores are all -inf is zero
+      uint2 w2 = make_uint2(pack16(acc.x * inv, acc.y * inv, false), pack16(acc.z * inv, acc.w * inv, false));
+      *reinterpret_cast<uint2*>(a.out + (long long)r * a.o_rs + (long long)(h0 + h) * a.o_hs + d) = w2;
+    } else {
+      *reinterpret_cast<float4*>(a.part + (((long long)r * a.H + h0 + h) * a.chunks + chunk) * HD + d) = acc;
+    }
+  }
+}
+
+// Blocks [0, R H): one (request, head)'s chunks joined to its output row.
+// Blocks from there on: 1024 visible positions of one (request, kv head),
+// whose weights are added to the sums; every sum has one writer, so repeated
+// runs agree bit for bit.
+template <int HD>
+__global__ void __launch_bounds__(128) decode_join_kernel(DecodeArgs a, int key_blocks) {
+  __shared__ float sred[4][HD];
+  __shared__ float2 sst[64];
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto row_stats = [&](long long row, int n) {  // by one warp: (maximum, sum) over the row's chunks
+    float mm = -INFINITY;
+    for (int c = lane; c < n; c += 32) mm = fmaxf(mm, a.stats[row * a.chunks + c].x);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
+    const float u = mm == -INFINITY ? 0.0f : mm;
+    float ll = 0.0f;
+    for (int c = lane; c < n; c += 32) {
+      const float2 s = a.stats[row * a.chunks + c];
+      ll += s.y * exp2f(s.x - u);
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
+    return make_float2(u, ll);
+  };
+  const int rows = a.c.R * a.H;
+  if ((int)blockIdx.x < rows) {
+    const int row = blockIdx.x, r = row / a.H, h = row % a.H;
+    const Span sp = visible_span(cache_length(a.c, r, a.err, false), a.window, a.sinks);
+    const int n = (sp.n + a.chunk - 1) / a.chunk;
+    if (n <= 1) return;  // written by its only chunk
+    const float2 st = row_stats(row, n);
+    constexpr int V = HD / 4, PER = 128 / V;  // threads per chunk's row, chunks at a time
+    const int d = (threadIdx.x % V) * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = threadIdx.x / V; c < n; c += PER) {
+      const float f = exp2f(a.stats[(long long)row * a.chunks + c].x - st.x);
+      const float4 x = *reinterpret_cast<const float4*>(a.part + ((long long)row * a.chunks + c) * HD + d);
+      acc.x += x.x * f;
+      acc.y += x.y * f;
+      acc.z += x.z * f;
+      acc.w += x.w * f;
+    }
+    if constexpr (V == 16) {  // two groups of a warp hold the same columns
+      acc.x += __shfl_xor_sync(0xffffffffu, acc.x, 16);
+      acc.y += __shfl_xor_sync(0xffffffffu, acc.y, 16);
+      acc.z += __shfl_xor_sync(0xffffffffu, acc.z, 16);
+      acc.w += __shfl_xor_sync(0xffffffffu, acc.w, 16);
+    }
+    if (lane < V) *reinterpret_cast<float4*>(&sred[warp][d]) = acc;
+    __syncthreads();
+    const float inv = st.y == 0.0f ? 0.0f : 1.0f / st.y;
+    for (int i = threadIdx.x; i < HD; i += 128)
+      a.out[(long long)r * a.o_rs + (long long)h * a.o_hs + i] =
+          f2bf((sred[0][i] + sred[1][i] + sred[2][i] + sred[3][i]) * inv);
+    return;
+  }
+  const int item = (blockIdx.x - rows) / key_blocks, kb = (blockIdx.x - rows) % key_blocks;
+  const int r = item / a.c.KH, c = item % a.c.KH;
+  const Span sp = visible_span(cache_length(a.c, r, a.err, false), a.window, a.sinks);
+  const int begin = kb * 1024, end = min(sp.n, begin + 1024);
+  if (begin >= end) return;
+  const int n = (sp.n + a.chunk - 1) / a.chunk;
+  const long long row0 = (long long)r * a.H + c * a.G;
+  float* dst = a.sums + (long long)r * a.s_rs + (long long)c * a.s_hs;
+  float add[8] = {};
+  for (int g0 = 0; g0 < a.G; g0 += 64) {
+    for (int g = g0 + warp; g < min(a.G, g0 + 64); g += 4) {
+      const float2 st = row_stats(row0 + g, n);
+      if (lane == 0) sst[g - g0] = make_float2(st.x, st.y == 0.0f ? 0.0f : 1.0f / st.y);
+    }
+    __syncthreads();
+    for (int g = g0; g < min(a.G, g0 + 64); ++g) {
+      const float2 st = sst[g - g0];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = begin + u * 128 + threadIdx.x;
+        if (i < end) add[u] += exp2f(a.scores[(row0 + g) * a.pitch + i] - st.x) * st.y;
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const int i = begin + u * 128 + threadIdx.x;
+    if (i < end) dst[sp.pos(i)] += add[u];
+  }
+}
+
+struct DecodePlan {
+  int ng, hgroups, chunk, chunks, pitch;
+  size_t part, stats, scores, total;
+};
+
+// The visible positions a request can have at most, cut so that the launch has
+// about eight chunks per SM where there are that many positions.
+DecodePlan decode_plan(int64_t R, int64_t H, int64_t KH, int64_t HD, int64_t max_len, int64_t window, bool sums,
+                       int64_t sinks) {
+  DecodePlan p{};
+  const int64_t G = H / KH;
+  p.ng = G > 8 ? 2 : 1;
+  p.hgroups = (int)((G + 8 * p.ng - 1) / (8 * p.ng));
+  const int64_t span = visible_span((int)max_len, (int)window, (int)sinks).n;
+  const int64_t units = R * KH * p.hgroups * span;
+  int64_t chunk = (units / (148 * 8) + 63) / 64 * 64;
+  chunk = chunk < 64 ? 64 : chunk > 512 ? 512 : chunk;
+  p.chunk = (int)chunk;
+  p.chunks = (int)((span + chunk - 1) / chunk);
+  if (p.chunks < 1) p.chunks = 1;
+  p.pitch = (int)((span + 15) / 16 * 16);
+  auto up = [](size_t b) { return (b + 255) / 256 * 256; };
+  const bool join = p.chunks > 1;
+  p.part = join ? up((size_t)(R * H) * p.chunks * HD * 4) : 0;
+  p.stats = join || sums ? up((size_t)(R * H) * p.chunks * 8) : 0;
+  p.scores = sums ? up((size_t)(R * H) * p.pitch * 4) : 0;
+  p.total = p.part + p.stats + p.scores;
+  return p;
+}
+
+template <int HD, bool KV8, int NG>
+fm_status launch_decode(const DecodeArgs& a, unsigned grid, cudaStream_t s) {
+  constexpr int smem = da_smem<HD, KV8, NG>();
+  fm_status st = check_cuda(cudaFuncSetAttribute(decode_attn_kernel<HD, KV8, NG>,
+                                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                            "paged_decode_attn");
+  if (st != FM_OK) return st;
+  return launch_kernel(decode_attn_kernel<HD, KV8, NG>, dim3(grid), dim3(128), smem, s, false, a);
+}
+
+template <int HD>
+fm_status launch_decode_hd(const DecodeArgs& a, bool kv8, int ng, unsigned grid, cudaStream_t s) {
+  if (kv8) return ng == 2 ? launch_decode<HD, true, 2>(a, grid, s) : launch_decode<HD, true, 1>(a, grid, s);
+  return ng == 2 ? launch_decode<HD, false, 2>(a, grid, s) : launch_decode<HD, false, 1>(a, grid, s);
+}
+
+}  // namespace
+}  // namespace fm
+
+using namespace fm;
+
+extern "C" size_t fm_paged_decode_attn_workspace_size(int64_t requests, int64_t heads, int64_t kv_heads,
+                                                      int64_t head_dim, int64_t max_length, int64_t window,
+                                                      int64_t sinks, int32_t with_sums) {
+  if (requests < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || max_length < 0 ||
+      max_length > 0x7ffffff0 || window < 0 || window > 0x7ffffff0 || sinks < 0 || sinks > 0x7ffffff0)
+    return 0;
+  return decode_plan(requests, heads, kv_heads, head_dim, max_length, window, with_sums != 0, sinks).total;
+}
+
+extern "C" fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_decode_attn* p, fm_stream stream) {
+  DecodeArgs a{};
+  fm_status st = cache_ref(cache, "paged_decode_attn", &a.c);
+  if (st != FM_OK) return st;
+  if (!p) return set_error(FM_ERR_INVALID, "paged_decode_attn: null arguments");
+  if (p->heads < 1 || p->heads % cache->kv_heads || p->heads > 65535)
+    return set_error(FM_ERR_SHAPE, "paged_decode_attn: query heads must be a multiple of the kv heads");
+  if (p->window < 0 || p->sinks < 0 || p->window > 0x7ffffff0 || p->sinks > 0x7ffffff0)
+    return set_error(FM_ERR_SHAPE, "paged_decode_attn: window and sinks must not be negative");
+  if (cache->requests == 0) return FM_OK;
+  if (!p->q || !p->out) return set_error(FM_ERR_INVALID, "paged_decode_attn: null pointer");
+  if ((uintptr_t)p->q % 4 || p->q_request_stride % 2 || p->q_head_stride % 2 || (uintptr_t)p->out % 8 ||
+      p->out_request_stride % 4 || p->out_head_stride % 4)
+    return set_error(FM_ERR_ALIGN, "paged_decode_attn: query rows must be 4-byte, output rows 8-byte aligned");
+  const bool sums = p->weight_sums != nullptr;
+  const DecodePlan pl = decode_plan(cache->requests, p->heads, cache->kv_heads, cache->head_dim, a.c.max_len,
+                                    p->window, sums, p->sinks);
+  if (pl.total > p->workspace_bytes || (pl.total && !p->workspace))
+    return set_error(FM_ERR_WORKSPACE, "paged_decode_attn: workspace %zu < %zu", p->workspace_bytes, pl.total);
+  if ((uintptr_t)p->workspace % 16) return set_error(FM_ERR_ALIGN, "paged_decode_attn: workspace not 16-byte aligned");
+  a.q = static_cast<const uint8_t*>(p->q);
+  a.q_rs = p->q_request_stride;
+  a.q_hs = p->q_head_stride;
+  a.H = (int)p->heads;
+  a.G = (int)(p->heads / cache->kv_heads);
+  a.hgroups = pl.hgroups;
+  a.scale = p->softmax_scale * kLog2e;
+  a.window = (int)p->window;
+  a.sinks = (int)p->sinks;
+  a.chunk = pl.chunk;
+  a.chunks = pl.chunks;
+  a.out = static_cast<__nv_bfloat16*>(p->out);
+  a.o_rs = p->out_request_stride;
+  a.o_hs = p->out_head_stride;
+  a.sums = p->weight_sums;
+  a.s_rs = p->sums_request_stride;
+  a.s_hs = p->sums_head_stride;
+  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
+  a.part = reinterpret_cast<float*>(ws);
+  a.stats = reinterpret_cast<float2*>(ws + pl.part);
+  a.scores = sums ? reinterpret_cast<float*>(ws + pl.part + pl.stats) : nullptr;
+  a.pitch = pl.pitch;
+  a.err = p->err;
+  const int64_t items = cache->requests * cache->kv_heads * pl.hgroups;
+  const int64_t key_blocks = sums ? (pl.pitch + 1023) / 1024 : 0;
+  const int64_t join = cache->requests * (p->heads + cache->kv_heads * key_blocks);
+  if (items * pl.chunks > 0x7fffffff || join > 0x7fffffff)
+    return set_error(FM_ERR_SHAPE, "paged_decode_attn: grid too large");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool kv8 = cache->dtype == FM_DT_E4M3;
+  const unsigned grid = (unsigned)(items * pl.chunks);
+  st = cache->head_dim == 128 ? launch_decode_hd<128>(a, kv8, pl.ng, grid, s)
+                              : launch_decode_hd<64>(a, kv8, pl.ng, grid, s);
+  if (st != FM_OK || (pl.chunks == 1 && !sums)) return st;
+  if (cache->head_dim == 128)
+    return launch_kernel(decode_join_kernel<128>, dim3((unsigned)join), dim3(128), 0, s, true, a, (int)key_blocks);
+  return launch_kernel(decode_join_kernel<64>, dim3((unsigned)join), dim3(128), 0, s, true, a, (int)key_blocks);
+}

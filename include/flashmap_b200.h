@@ -400,6 +400,104 @@ FM_API fm_status fm_kv_norm_rope_write_pool(const void* kv, int64_t tokens, int6
                                             float eps, int32_t* err, fm_stream stream);
 
 /* ------------------------------------------------------------------------
+ * Operators on a paged key/value cache that a target model decodes with: one
+ * kv head serves heads / kv_heads query heads.
+ * ------------------------------------------------------------------------ */
+
+/* The cache.  k and v are bf16 or e4m3 rows of head_dim (64 or 128) values,
+ * 16-byte aligned, at page * page_stride + kv_head * head_stride + token *
+ * token_stride elements; token i of request r is token i % page_size of page
+ * page_table[r * page_table_stride + i / page_size].  lengths[r] positions are
+ * held, max_length at most; a length beyond max_length or the table is cut
+ * and DEV_BAD_INDEX recorded, and a position whose page id lies outside
+ * [0, num_pages) is not seen and DEV_BAD_INDEX recorded.  descales: (2,
+ * requests, kv_heads) fp32 factors of keys and values, or NULL (1). */
+typedef struct fm_paged_cache {
+  void* k;
+  void* v;
+  int32_t dtype; /* FM_DT_BF16 or FM_DT_E4M3 */
+  int64_t k_page_stride, k_head_stride, k_token_stride;
+  int64_t v_page_stride, v_head_stride, v_token_stride;
+  int64_t page_size, num_pages;
+  const int32_t* page_table;
+  int64_t page_table_stride, page_table_cols;
+  const int32_t* lengths;
+  int64_t max_length;
+  int64_t requests, kv_heads, head_dim;
+  const float* descales;
+} fm_paged_cache;
+
+/* Attention of one new token per request: q (requests, heads, head_dim) bf16,
+ * the token at position lengths[r] - 1.  It sees every position, or with
+ * window > 0 the last `window` and the first `sinks`.  weight_sums (requests,
+ * kv_heads, >= max_length) fp32 or NULL: position j's sum grows by the
+ * attention weights of the kv head's query heads.  A request without
+ * positions gets zero rows.  The workspace need not be initialised. */
+typedef struct fm_decode_attn {
+  const void* q;
+  int64_t q_request_stride, q_head_stride;
+  int64_t heads;
+  float softmax_scale;
+  int64_t window, sinks;
+  float* weight_sums;
+  int64_t sums_request_stride, sums_head_stride;
+  void* out; /* bf16 */
+  int64_t out_request_stride, out_head_stride;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* err;
+} fm_decode_attn;
+FM_API size_t fm_paged_decode_attn_workspace_size(int64_t requests, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                                  int64_t max_length, int64_t window, int64_t sinks,
+                                                  int32_t with_sums);
+FM_API fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_decode_attn* args, fm_stream stream);
+
+/* Causal attention of query rows cu_seqlens_q[r] .. cu_seqlens_q[r + 1] of q
+ * (rows, heads, head_dim) bf16, which are request r's last positions: row i of
+ * n stands at p = lengths[r] - n + i and sees the positions j <= p with no
+ * window, p - j < window or j < sinks.  A row that sees nothing is zero. */
+typedef struct fm_window_attn {
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  int64_t rows, heads;
+  const int32_t* cu_seqlens_q;
+  int64_t max_q; /* the most query rows of one request */
+  float softmax_scale;
+  int64_t window, sinks;
+  void* out; /* bf16 */
+  int64_t out_token_stride, out_head_stride;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* err;
+} fm_window_attn;
+FM_API size_t fm_paged_window_attn_workspace_size(int64_t requests, int64_t rows, int64_t heads, int64_t kv_heads,
+                                                  int64_t head_dim, int64_t max_q, int64_t max_length, int64_t window,
+                                                  int64_t sinks);
+FM_API fm_status fm_paged_window_attn(const fm_paged_cache* cache, const fm_window_attn* args, fm_stream stream);
+
+/* Eviction by accumulated attention weight, per (request, kv head).  A context
+ * of at most `budget` positions stays whole.  Of a longer one the first
+ * `sinks`, the last `recent`, and of those between the largest weight_sums up
+ * to the budget stay (the lowest position among equal sums; NaN ranks last).
+ * The kept rows move in order of position to slots 0 .. budget - 1: in place,
+ * or with out_page_table (requests, >= ceil(budget / page_size)) to its pages
+ * of the same pool, which must hold no page that page_table uses.
+ * kept (requests, kv_heads, budget) int32: the kept positions, then -1;
+ * out_sums, the same shape, fp32: their sums, then 0; lengths (requests). */
+typedef struct fm_evict {
+  const float* weight_sums;
+  int64_t sums_request_stride, sums_head_stride;
+  int64_t budget, sinks, recent;
+  const int32_t* out_page_table; /* NULL: in place */
+  int64_t out_page_table_stride, out_page_table_cols;
+  int32_t* kept;
+  int32_t* lengths;
+  float* out_sums;
+  int32_t* err;
+} fm_evict;
+FM_API fm_status fm_paged_evict(const fm_paged_cache* cache, const fm_evict* args, fm_stream stream);
+
+/* ------------------------------------------------------------------------
  * Sampling and acceptance (modeling_flashmap.py:553-557, :579-594).
  * Randomness: Philox4x32-10 keyed by seed; counters documented per call.
  * ------------------------------------------------------------------------ */

@@ -1,0 +1,466 @@
+"""The operators on a paged key/value cache against the 64-bit oracle.
+
+Tolerances.  An output is sum_j w_j v_j: the kernels round each softmax
+numerator once, to bf16 (8 significant bits: at most 2^-8 of it) or, for e4m3
+caches, to f16 (11 bits: 2^-11), and the output once to bf16.  Everything else
+is fp32: a score is off by at most 8 partial sums' rounding of 2^-22 of
+sum |q k| scale, under 2^-16 for the unit-variance inputs here, and moves a
+weight by that share.  So outputs are held to u sum_j w_j |v_j| + 2^-8 |out|
+with u = 2^-8 or 2^-11, plus 2^-14 of both, and gathered weights to 2^-16 of the
+weight plus the fp32 rounding of the sum they are added to.
+"""
+
+import math
+
+import pytest
+import torch
+
+from oracle import cache_ops as O
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+FP8 = torch.float8_e4m3fn
+
+
+def ops():
+    from flashmap_b200 import cache_ops
+    return cache_ops
+
+
+def close(got, want, mag, what, fp8=False):
+    err = (got.double().cpu() - want).abs()
+    tol = (2.0 ** (-11 if fp8 else -8) + 2.0 ** -14) * mag + (2.0 ** -8 + 2.0 ** -14) * want.abs() + 1e-30
+    assert torch.isfinite(got.float()).all(), f"{what}: not finite"
+    worst = (err / tol).max().item() if err.numel() else 0.0
+    assert worst <= 1.0, f"{what}: {worst:.3g} times the tolerance"
+
+
+def error_word():
+    from flashmap_b200.serving_ops import _err
+    torch.cuda.synchronize()
+    w = _err(torch.device("cuda", torch.cuda.current_device()))
+    code = int(w)
+    w.zero_()
+    return code
+
+
+def make_cache(g, lengths, KH, D, page, dtype, layout, spare=3):
+    """Pools (CPU), table and descales; unused table entries name page 0, whose values are NaN."""
+    used = [-(-L // page) for L in lengths]
+    cols = max(1, max(used, default=1))
+    total = sum(used) + spare + 1
+    ids = torch.randperm(total - 1, generator=g) + 1
+    table = torch.zeros(len(lengths), cols, dtype=torch.int32)
+    at = 0
+    for r, n in enumerate(used):
+        table[r, :n] = ids[at: at + n].int()
+        at += n
+    width = 2 * D if layout == "joint" else D
+    pools = [torch.randn(total, KH, page, width, generator=g).to(torch.bfloat16) for _ in range(1 if layout == "joint" else 2)]
+    for p in pools:
+        p[0] = math.nan
+    for r, L in enumerate(lengths):  # a page's slots past the length hold anything
+        if L % page:
+            for p in pools:
+                p[table[r, used[r] - 1].item(), :, L % page:] = math.nan
+    descales = None
+    if dtype == FP8:
+        pools = [p.to(FP8) for p in pools]
+        descales = 0.5 + torch.rand(2, len(lengths), KH, generator=g)
+    return pools, table, descales
+
+
+def views(pools, D):
+    dev = [p.to(DEV) for p in pools]
+    return dev, dev[0][..., :D], dev[-1][..., -D:]
+
+
+def cpu_views(pools, D):
+    return pools[0][..., :D], pools[-1][..., -D:]
+
+
+DECODE = [
+    # heads, kv_heads, head_dim, page, dtype, layout, window, sinks, lengths
+    (8, 2, 128, 16, "bf16", "joint", 0, 0, [1, 0, 17, 700, 64, 65, 3]),
+    (8, 8, 128, 16, "bf16", "split", 0, 0, [33, 129, 2]),
+    (10, 2, 64, 24, "bf16", "joint", 0, 0, [257, 1, 600]),
+    (16, 1, 128, 1, "bf16", "split", 0, 0, [300, 77]),
+    (40, 2, 64, 32, "bf16", "joint", 100, 4, [1000, 99, 100, 101, 104, 105, 0]),
+    (8, 2, 128, 16, "bf16", "joint", 1, 0, [1, 2, 500]),
+    (8, 2, 128, 128, "bf16", "joint", 130, 200, [5, 150, 331, 900]),
+    (8, 2, 128, 16, "e4m3", "joint", 0, 0, [1, 0, 17, 700, 64, 65, 3]),
+    (12, 1, 128, 1, "e4m3", "split", 64, 3, [400, 66, 67, 68]),
+    (5, 1, 64, 24, "e4m3", "joint", 0, 0, [333, 16, 15]),
+    (32, 2, 64, 16, "e4m3", "split", 70, 16, [512, 5]),
+]
+
+
+@pytest.mark.parametrize("case", DECODE, ids=lambda c: "-".join(map(str, c[:8])))
+@pytest.mark.parametrize("gather", [False, True])
+def test_decode(case, gather):
+    H, KH, D, page, dt, layout, window, sinks, lengths = case
+    g = torch.Generator().manual_seed(11)
+    dtype = FP8 if dt == "e4m3" else torch.bfloat16
+    pools, table, descales = make_cache(g, lengths, KH, D, page, dtype, layout)
+    q = torch.randn(len(lengths), H, D, generator=g).to(torch.bfloat16)
+    _, k, v = views(pools, D)
+    top = max(lengths)
+    before = torch.rand(len(lengths), KH, top + 5, generator=g)
+    sums = before.to(DEV) if gather else None
+    got = ops().paged_decode_attention(
+        q.to(DEV), k, v, torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV), top, D ** -0.5,
+        window=window, sinks=sinks, descales=None if descales is None else descales.to(DEV), weight_sums=sums)
+    want, mag, w = O.decode_attention(q, *cpu_views(pools, D), lengths, table, D ** -0.5, window, sinks, descales)
+    close(got, want, mag, "decode", dt == "e4m3")
+    assert error_word() == 0
+    if gather:
+        for r, L in enumerate(lengths):
+            s = sums[r].double().cpu()
+            add = torch.zeros_like(s)
+            add[:, :L] = w[r]
+            want_s = before[r].double() + add
+            assert ((s - want_s).abs() <= 2.0 ** -16 * add + 2.0 ** -22 * want_s).all()
+            assert torch.equal(s[:, L:].float(), before[r][:, L:])  # nothing past the length
+
+
+def test_decode_many_chunks_repeats_bit_for_bit():
+    g = torch.Generator().manual_seed(5)
+    lengths, KH, H, D, page = [9001, 40, 5000], 2, 8, 128, 16
+    pools, table, _ = make_cache(g, lengths, KH, D, page, torch.bfloat16, "joint")
+    q = torch.randn(3, H, D, generator=g).to(torch.bfloat16)
+    _, k, v = views(pools, D)
+    L = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    runs = []
+    for _ in range(2):
+        sums = torch.zeros(3, KH, 9001, device=DEV)
+        out = ops().paged_decode_attention(q.to(DEV), k, v, L, table.to(DEV), 9001, D ** -0.5, weight_sums=sums)
+        runs.append((out, sums))
+    assert torch.equal(runs[0][0], runs[1][0]) and torch.equal(runs[0][1], runs[1][1])
+    want, mag, w = O.decode_attention(q, *cpu_views(pools, D), lengths, table, D ** -0.5)
+    close(runs[0][0], want, mag, "decode")
+    total = runs[0][1].double().sum(-1).cpu()  # every head's weights add up to one
+    assert torch.allclose(total, torch.full_like(total, H / KH), atol=1e-4)
+
+
+def test_decode_strided_query_sums_and_other_stream():
+    g = torch.Generator().manual_seed(6)
+    lengths, KH, H, D = [130, 50], 2, 4, 128
+    pools, table, _ = make_cache(g, lengths, KH, D, 16, torch.bfloat16, "joint")
+    _, k, v = views(pools, D)
+    wide = torch.randn(2, H, 3, D, generator=g).to(torch.bfloat16)
+    q = wide.to(DEV)[:, :, 1]
+    big = torch.zeros(4, 3 * KH, 200, device=DEV)
+    sums = big[::2, 1:1 + KH, :130]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = ops().paged_decode_attention(q, k, v, torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV),
+                                           130, D ** -0.5, weight_sums=sums)
+    side.synchronize()
+    want, mag, w = O.decode_attention(wide[:, :, 1], *cpu_views(pools, D), lengths, table, D ** -0.5)
+    close(out, want, mag, "decode")
+    assert torch.allclose(sums[1, :, :50].double().cpu(), w[1], atol=1e-5)
+    assert float(big[1].abs().max()) == 0.0 and float(big[:, 1 + KH:].abs().max()) == 0.0
+
+
+def test_decode_extreme_scores():
+    """Large scores, rows of zeros, infinite keys' scores of -inf and a query with an infinity."""
+    g = torch.Generator().manual_seed(7)
+    lengths, KH, D = [80, 80, 80], 1, 128
+    for dtype in (torch.bfloat16, FP8):
+        pools, table, descales = make_cache(g, lengths, KH, D, 16, dtype, "split")
+        q = torch.randn(3, 2, D, generator=g)
+        q[0] *= 1e4
+        q[1] = 0.0
+        q[2] *= 1e-30
+        q = q.to(torch.bfloat16)
+        _, k, v = views(pools, D)
+        out = ops().paged_decode_attention(q.to(DEV), k, v, torch.tensor(lengths, dtype=torch.int32, device=DEV),
+                                           table.to(DEV), 80, D ** -0.5,
+                                           descales=None if descales is None else descales.to(DEV))
+        want, mag, _ = O.decode_attention(q, *cpu_views(pools, D), lengths, table, D ** -0.5, descales=descales)
+        # scores of 1e4 carry an fp32 error of up to 1e4 2^-20, which moves weights by a percent
+        assert ((out[0].double().cpu() - want[0]).abs() <= 0.03 * mag[0] + 2.0 ** -8 * want[0].abs()).all()
+        close(out[1:], want[1:], mag[1:], "decode", dtype == FP8)
+    k2 = pools[0].float().clone()
+    k2[table[0, :5].long()] = -math.inf  # every score of request 0 is -inf (or the query is zero there)
+    k2 = k2.to(torch.bfloat16).to(DEV)
+    v2 = pools[1].float().to(torch.bfloat16).to(DEV)
+    ones = torch.ones(3, 2, D, dtype=torch.bfloat16, device=DEV)
+    out = ops().paged_decode_attention(ones, k2, v2, torch.tensor(lengths, dtype=torch.int32, device=DEV),
+                                       table.to(DEV), 80, D ** -0.5)
+    assert float(out[0].abs().max()) == 0.0 and torch.isfinite(out.float()).all()
+
+
+WINDOW = [
+    # heads, kv_heads, head_dim, page, dtype, layout, window, sinks, lengths, query rows
+    (8, 2, 128, 16, "bf16", "joint", 0, 0, [1, 0, 17, 200, 64, 65, 300], [1, 0, 17, 5, 64, 3, 150]),
+    (4, 4, 128, 16, "bf16", "split", 0, 0, [70, 129], [70, 129]),
+    (10, 2, 64, 24, "bf16", "joint", 0, 0, [257, 1, 300], [33, 1, 299]),
+    (16, 1, 128, 1, "bf16", "split", 0, 0, [300, 77], [17, 17]),
+    (20, 1, 64, 32, "bf16", "joint", 100, 4, [500, 99, 100, 101, 104, 0], [200, 99, 100, 17, 1, 0]),
+    (8, 2, 128, 16, "bf16", "joint", 1, 0, [1, 2, 200], [1, 2, 100]),
+    (8, 2, 128, 16, "bf16", "joint", 1, 1, [300], [280]),
+    (8, 2, 128, 128, "bf16", "joint", 130, 200, [5, 150, 331, 700], [5, 20, 331, 17]),
+    (2, 1, 128, 16, "bf16", "joint", 37, 70, [900], [500]),
+    (8, 2, 128, 16, "bf16", "joint", 0, 0, [20, 100], [30, 101]),  # more rows than positions: the first see nothing
+    (8, 2, 128, 16, "e4m3", "joint", 0, 0, [1, 0, 17, 200, 64, 65, 300], [1, 0, 17, 5, 64, 3, 150]),
+    (12, 1, 128, 1, "e4m3", "split", 64, 3, [400, 66, 67, 68], [17, 66, 1, 68]),
+    (5, 1, 64, 24, "e4m3", "joint", 0, 0, [333, 16, 15], [300, 16, 2]),
+    (3, 3, 64, 16, "e4m3", "split", 70, 16, [512, 5], [200, 5]),
+]
+
+
+@pytest.mark.parametrize("case", WINDOW, ids=lambda c: "-".join(map(str, c[:8])))
+def test_window(case):
+    H, KH, D, page, dt, layout, window, sinks, lengths, rows = case
+    g = torch.Generator().manual_seed(12)
+    dtype = FP8 if dt == "e4m3" else torch.bfloat16
+    pools, table, descales = make_cache(g, lengths, KH, D, page, dtype, layout)
+    cu = torch.tensor([0] + rows).cumsum(0).int()
+    q = torch.randn(int(cu[-1]), H, D, generator=g).to(torch.bfloat16)
+    _, k, v = views(pools, D)
+    got = ops().paged_window_attention(
+        q.to(DEV), k, v, cu.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV), max(rows),
+        max(lengths), D ** -0.5, window=window, sinks=sinks, descales=None if descales is None else descales.to(DEV))
+    want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu, lengths, table, D ** -0.5, window, sinks, descales)
+    close(got, want, mag, "window", dt == "e4m3")
+    assert error_word() == 0
+
+
+@pytest.mark.parametrize("dt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (700, 5)])
+def test_window_long(dt, window, sinks):
+    """Contexts of thousands: long runs of key tiles, few rows (one verified block) and many."""
+    H, KH, D, page, lengths, rows = 4, 1, 128, 16, [5003, 3100], [17, 600]
+    g = torch.Generator().manual_seed(13)
+    pools, table, descales = make_cache(g, lengths, KH, D, page, FP8 if dt == "e4m3" else torch.bfloat16, "joint")
+    cu = torch.tensor([0] + rows).cumsum(0).int()
+    q = torch.randn(int(cu[-1]), H, D, generator=g).to(torch.bfloat16)
+    _, k, v = views(pools, D)
+    got = ops().paged_window_attention(
+        q.to(DEV), k, v, cu.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV), max(rows),
+        max(lengths), D ** -0.5, window=window, sinks=sinks, descales=None if descales is None else descales.to(DEV))
+    want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu, lengths, table, D ** -0.5, window, sinks, descales)
+    close(got, want, mag, "window", dt == "e4m3")
+
+
+def test_window_of_one_row_is_decode():
+    g = torch.Generator().manual_seed(14)
+    lengths, KH, H, D = [130, 50, 1], 2, 8, 128
+    pools, table, _ = make_cache(g, lengths, KH, D, 16, torch.bfloat16, "joint")
+    _, k, v = views(pools, D)
+    q = torch.randn(3, H, D, generator=g).to(torch.bfloat16).to(DEV)
+    L = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    a = ops().paged_decode_attention(q, k, v, L, table.to(DEV), 130, D ** -0.5, window=40, sinks=3)
+    b = ops().paged_window_attention(q, k, v, torch.arange(4, dtype=torch.int32, device=DEV), L, table.to(DEV), 1, 130,
+                                     D ** -0.5, window=40, sinks=3)
+    assert torch.allclose(a.float(), b.float(), atol=2e-2)
+
+
+def test_rows_past_32_bit_offsets():
+    """A pool whose last pages lie more than 2^32 bytes, and 2^32 elements, from its start."""
+    D, KH, page = 128, 1, 16
+    pages, stride = 3, 2_200_000_000  # elements between pages
+    pool = torch.empty(2 * stride + KH * page * 2 * D, dtype=torch.bfloat16, device=DEV)
+    cache = pool.as_strided((pages, KH, page, 2 * D), (stride, page * 2 * D, 2 * D, 1))
+    g = torch.Generator().manual_seed(15)
+    host = torch.randn(pages, KH, page, 2 * D, generator=g).to(torch.bfloat16)
+    cache.copy_(host.to(DEV))
+    lengths, table = [40], torch.tensor([[2, 0, 1]], dtype=torch.int32)
+    L = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    q = torch.randn(1, 4, D, generator=g).to(torch.bfloat16)
+    k, v = cache[..., :D], cache[..., D:]
+    want, mag, _ = O.decode_attention(q, host[..., :D], host[..., D:], lengths, table, D ** -0.5)
+    close(ops().paged_decode_attention(q.to(DEV), k, v, L, table.to(DEV), 40, D ** -0.5), want, mag, "decode")
+    cu = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    close(ops().paged_window_attention(q.to(DEV), k, v, cu, L, table.to(DEV), 1, 40, D ** -0.5), want, mag, "window")
+    sums = torch.arange(40, dtype=torch.float32, device=DEV).view(1, 1, 40)
+    kept, n, _ = ops().evict_paged_context(k, v, L, table.to(DEV), sums, 20, sinks=2, recent=0)
+    assert kept[0, 0].tolist() == [0, 1] + list(range(22, 40)) and int(n) == 20
+    flat = torch.cat([host[2, 0], host[0, 0], host[1, 0]])[:40]
+    now = torch.cat([cache[2, 0], cache[0, 0]])[:20].cpu()
+    assert torch.equal(now, flat[kept[0, 0].cpu().long()])
+
+
+def test_bad_indices_are_reported_and_not_seen():
+    g = torch.Generator().manual_seed(16)
+    KH, H, D, page = 2, 4, 128, 16
+    pools, table, _ = make_cache(g, [64], KH, D, page, torch.bfloat16, "joint")
+    _, k, v = views(pools, D)
+    q = torch.randn(1, H, D, generator=g).to(torch.bfloat16)
+    bad = table.clone()
+    bad[0, 1] = 10_000
+    L = torch.tensor([64], dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    # the oracle on the 48 positions of the other pages
+    sub = table[:, [0, 2, 3]]
+    want, mag, _ = O.decode_attention(q, *cpu_views(pools, D), [48], sub, D ** -0.5)
+    close(ops().paged_decode_attention(q.to(DEV), k, v, L, bad.to(DEV), 64, D ** -0.5), want, mag, "decode")
+    assert error_word() == 4
+    close(ops().paged_window_attention(q.to(DEV), k, v, cu, L, bad.to(DEV), 1, 64, D ** -0.5), want, mag, "window")
+    assert error_word() == 4
+    # a length past max_seqlen_k is cut, a negative one is none
+    long = torch.tensor([100], dtype=torch.int32, device=DEV)
+    want, mag, _ = O.decode_attention(q, *cpu_views(pools, D), [60], table, D ** -0.5)
+    close(ops().paged_decode_attention(q.to(DEV), k, v, long, table.to(DEV), 60, D ** -0.5), want, mag, "decode")
+    assert error_word() == 4
+    none = torch.tensor([-3], dtype=torch.int32, device=DEV)
+    out = ops().paged_decode_attention(q.to(DEV), k, v, none, table.to(DEV), 60, D ** -0.5)
+    assert float(out.abs().max()) == 0.0 and error_word() == 4
+    sums = torch.rand(1, KH, 64, device=DEV)
+    kept, n, _ = ops().evict_paged_context(k, v, L, bad.to(DEV), sums, 32, recent=4)
+    assert error_word() == 4 and int(n) == 32
+
+
+EVICT = [
+    # kv_heads, head_dim, page, dtype, layout, budget, sinks, recent, lengths
+    (2, 128, 16, "bf16", "joint", 40, 4, 8, [100, 40, 41, 39, 0, 1, 700]),
+    (1, 64, 24, "bf16", "split", 33, 0, 0, [500, 34, 3]),
+    (4, 64, 1, "e4m3", "split", 50, 10, 40, [300, 51, 50]),  # nothing between is kept
+    (2, 128, 32, "e4m3", "joint", 1, 0, 0, [5, 1, 2000]),
+    (2, 128, 16, "bf16", "joint", 600, 1, 100, [1500, 601, 20]),
+]
+
+
+@pytest.mark.parametrize("case", EVICT, ids=lambda c: "-".join(map(str, c[:8])))
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("values", ["ties", "spread", "odd"])
+def test_evict(case, in_place, values):
+    KH, D, page, dt, layout, budget, sinks, recent, lengths = case
+    g = torch.Generator().manual_seed(17)
+    R = len(lengths)
+    out_cols = -(-budget // page)
+    pools, table, _ = make_cache(g, lengths, KH, D, page, FP8 if dt == "e4m3" else torch.bfloat16, layout,
+                                 spare=R * out_cols)
+    free = sorted(set(range(1, pools[0].shape[0])) - set(table.flatten().tolist()))
+    out_table = torch.tensor(free[: R * out_cols], dtype=torch.int32).view(R, out_cols)
+    top = max(lengths)
+    sums = torch.rand(R, KH, top + 3, generator=g)
+    if values == "ties":
+        sums = (sums * 5).floor()
+    if values == "odd":
+        pick = torch.randint(0, 6, sums.shape, generator=g)
+        for i, x in enumerate([math.nan, math.inf, -math.inf, -0.0, 0.0, -1.5]):
+            sums[pick == i] = x
+    dev, k, v = views(pools, D)
+    kept, n, got = ops().evict_paged_context(
+        k, v, torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV), sums.to(DEV), budget, sinks=sinks,
+        recent=recent, out_block_table=None if in_place else out_table.to(DEV))
+    assert error_word() == 0
+    want = O.evict(sums, lengths, budget, sinks, recent)
+    to = table if in_place else out_table
+    untouched = [p.clone().view(torch.uint8) for p in pools]
+    for r, L in enumerate(lengths):
+        m = min(L, budget)
+        assert int(n[r]) == m
+        for h in range(KH):
+            assert kept[r, h].tolist() == want[r][h] + [-1] * (budget - m)
+            assert torch.equal(got[r, h, :m].cpu().nan_to_num(7.0), sums[r, h, want[r][h]].nan_to_num(7.0))
+            assert float(got[r, h, m:].abs().sum()) == 0.0
+            for i, j in enumerate(want[r][h]):
+                a, b = int(table[r, j // page]), int(to[r, i // page])
+                for p, u in zip(pools, untouched):
+                    u[b, h, i % page] = p.view(torch.uint8)[a, h, j % page]
+    for p, u in zip(dev, untouched):  # the moved rows, and no other byte of the pool
+        assert torch.equal(p.view(torch.uint8).cpu(), u)
+
+
+def test_evict_long_rows():
+    """A selection over many positions, where the threshold lies in the last byte of the keys."""
+    g = torch.Generator().manual_seed(18)
+    L, budget, KH = 50_001, 20_000, 2
+    page, D = 16, 64
+    cols = -(-L // page)
+    table = torch.randperm(cols, generator=g).int().view(1, cols)
+    pool = torch.randint(-100, 100, (cols, KH, page, 2 * D), generator=g, dtype=torch.int8).to(torch.bfloat16)
+    sums = 1.0 + torch.randint(0, 4000, (1, KH, L), generator=g).float() * 2.0 ** -23
+    dev = pool.to(DEV)
+    kept, n, _ = ops().evict_paged_context(dev[..., :D], dev[..., D:], torch.tensor([L], dtype=torch.int32, device=DEV),
+                                           table.to(DEV), sums.to(DEV), budget, sinks=4, recent=100)
+    want = O.evict(sums, [L], budget, 4, 100)
+    for h in range(KH):
+        assert kept[0, h].tolist() == want[0][h]
+        src = torch.tensor(want[0][h])
+        i = torch.arange(budget)
+        moved = dev[table[0, i // page].long().to(DEV), h, (i % page).to(DEV)].cpu()
+        assert torch.equal(moved, pool[table[0, src // page].long(), h, src % page])
+
+
+def test_decode_in_a_cuda_graph():
+    g = torch.Generator().manual_seed(19)
+    lengths, KH, H, D = [900, 300], 2, 8, 128
+    pools, table, _ = make_cache(g, lengths, KH, D, 16, torch.bfloat16, "joint")
+    _, k, v = views(pools, D)
+    q = torch.randn(2, H, D, generator=g).to(torch.bfloat16).to(DEV)
+    L = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    t = table.to(DEV)
+    sums = torch.zeros(2, KH, 900, device=DEV)
+    eager = ops().paged_decode_attention(q, k, v, L, t, 900, D ** -0.5, weight_sums=sums)
+    want_sums = sums.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops().paged_decode_attention(q, k, v, L, t, 900, D ** -0.5, weight_sums=sums)
+    sums.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, eager) and torch.equal(sums, want_sums)
+    L.copy_(torch.tensor([450, 0], dtype=torch.int32))  # lengths are read when the graph runs
+    graph.replay()
+    want, mag, _ = O.decode_attention(q.cpu(), *cpu_views(pools, D), [450, 0], table, D ** -0.5)
+    close(out, want, mag, "decode")
+
+
+def test_refusals():
+    c = ops()
+    KH, D, page = 2, 128, 16
+    cache = torch.zeros(4, KH, page, 2 * D, dtype=torch.bfloat16, device=DEV)
+    k, v = cache[..., :D], cache[..., D:]
+    L = torch.tensor([5], dtype=torch.int32, device=DEV)
+    t = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    q = torch.zeros(1, 4, D, dtype=torch.bfloat16, device=DEV)
+    sums = torch.zeros(1, KH, 5, device=DEV)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+
+    def decode(**kw):
+        a = dict(query=q, k_cache=k, v_cache=v, seqused_k=L, block_table=t, max_seqlen_k=5, softmax_scale=1.0)
+        return c.paged_decode_attention(**dict(a, **kw))
+
+    def chunk(**kw):
+        a = dict(query=q, k_cache=k, v_cache=v, cu_seqlens_q=cu, seqused_k=L, block_table=t, max_seqlen_q=1,
+                 max_seqlen_k=5, softmax_scale=1.0)
+        return c.paged_window_attention(**dict(a, **kw))
+
+    def evict(**kw):
+        a = dict(k_cache=k, v_cache=v, seqused_k=L, block_table=t, weight_sums=sums, budget=4)
+        return c.evict_paged_context(**dict(a, **kw))
+
+    decode(), chunk(), evict()
+    bad = [
+        (decode, dict(query=q.float())), (decode, dict(query=q[:, :3])), (decode, dict(query=q[..., :64])),
+        (decode, dict(query=q.expand(2, 4, D))), (decode, dict(query=q.cpu())), (decode, dict(window=-1)),
+        (decode, dict(sinks=-1)), (decode, dict(weight_sums=sums[..., :4])), (decode, dict(weight_sums=sums.double())),
+        (decode, dict(descales=torch.ones(2, 1, KH, device=DEV))), (decode, dict(seqused_k=L.long())),
+        (decode, dict(block_table=t.long())), (decode, dict(block_table=t[:0])), (decode, dict(v_cache=v[:2])),
+        (decode, dict(k_cache=cache[..., :96], v_cache=cache[..., 96:192])), (decode, dict(k_cache=k.float(), v_cache=v.float())),
+        (decode, dict(max_seqlen_k=-1)), (chunk, dict(cu_seqlens_q=cu[:1])), (chunk, dict(cu_seqlens_q=cu.long())),
+        (chunk, dict(max_seqlen_q=-1)), (chunk, dict(sinks=-2)), (evict, dict(budget=0)),
+        (evict, dict(sinks=3, recent=2)), (evict, dict(sinks=-1)), (evict, dict(weight_sums=sums[:, :1])),
+        (evict, dict(out_block_table=t[:, :0])), (evict, dict(out_block_table=t.long())),
+    ]
+    for fn, kw in bad:
+        with pytest.raises(c.OpArgumentError):
+            fn(**kw)
+    from flashmap_b200._lib import FlashMapError
+    odd = torch.zeros(4, KH, page, 2 * D + 4, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(FlashMapError, match="16-byte"):
+        decode(k_cache=odd[..., 4:4 + D], v_cache=odd[..., 4 + D:])
+    with pytest.raises(FlashMapError, match="in place"):
+        evict(out_block_table=t)
+    assert error_word() == 0
+    # nothing to do
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    assert decode(query=q[:0], seqused_k=none, block_table=t[:0]).shape == (0, 4, D)
+    assert chunk(query=q[:0], cu_seqlens_q=torch.zeros(2, dtype=torch.int32, device=DEV)).shape == (0, 4, D)
+    assert evict(seqused_k=none, block_table=t[:0], weight_sums=sums[:0])[0].shape == (0, KH, 4)
