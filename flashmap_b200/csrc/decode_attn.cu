@@ -517,7 +517,7 @@ extern "C" fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_
       p->out_request_stride % 4 || p->out_head_stride % 4)
     return set_error(FM_ERR_ALIGN, "paged_decode_attn: query rows must be 4-byte, output rows 8-byte aligned");
   const bool sums = p->weight_sums != nullptr;
-  const DecodePlan pl = decode_plan(cache->requests, p->heads, cache->kv_heads, cache->head_dim, a.c.max_len,
+  const DecodePlan pl = decode_plan(cache->requests, p->heads, cache->kv_heads, cache->head_dim, cache->max_length,
                                     p->window, sums, p->sinks);
   if (pl.total > p->workspace_bytes || (pl.total && !p->workspace))
     return set_error(FM_ERR_WORKSPACE, "paged_decode_attn: workspace %zu < %zu", p->workspace_bytes, pl.total);
