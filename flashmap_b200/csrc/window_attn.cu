@@ -88,27 +88,45 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const float* v) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// D[tmem] (+)= A[tmem] B[smem], 16-bit operands, fp32 accumulate
-__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+// D[tmem] (+)= A B, 16-bit operands, fp32 accumulate; A from shared memory or
+// from tensor memory.  Descriptors come as their low word (address and leading
+// offset in units of 16 bytes); the high word is the same for every operand
+// here: stride 1024 bytes between 8-row atoms, descriptor version 1, 128-byte
+// swizzling.
+constexpr uint32_t WA_DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
                                         uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(WA_DESC_HI)
       : "memory");
 }
-// Descriptor of a B operand stored row by row of K (a key's values): rows of
-// 128 bytes (64 columns of N) with 128-byte swizzling, 8 keys to a 1024-byte
-// atom; the next 64 columns follow `block` bytes on.
-__device__ __forceinline__ uint64_t sdesc_mn_sw128(uint32_t saddr, uint32_t block) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr & 0x3FFFFu) >> 4);
-  d |= (uint64_t)(block >> 4) << 16;
-  d |= (uint64_t)(1024u >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(WA_DESC_HI)
+      : "memory");
+}
+// Low descriptor words.  K-major (Q, K): the leading offset is unused.  A B
+// operand stored key by key (V, 64 columns of N to a 128-byte row): the next 64
+// columns follow 16384 bytes on.
+__device__ __forceinline__ uint32_t desc_lo_k(uint32_t saddr) { return (saddr >> 4) | 1u << 16; }
+__device__ __forceinline__ uint32_t desc_lo_mn(uint32_t saddr) { return (saddr >> 4) | (16384u >> 4) << 16; }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p)
+      :
+      : "memory");
+  return p != 0;
 }
 // kind::f16 with both operands f16 (half) or both bf16, D fp32
 __host__ __device__ constexpr uint32_t wa_idesc(bool half, int M, int N, bool b_mn) {
@@ -124,6 +142,11 @@ template <int N>
 __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -138,82 +161,63 @@ struct WaLayout {
   static constexpr int SLOTS = HD == 64 ? 8 : KV8 ? 4 : 5;
   static constexpr int RAW = KV8 ? 128 * HD : 0;
   static constexpr int RAWS = KV8 ? 2 : 0;
-  static constexpr int LAG = KV8 ? 0 : 2;  // tiles of copies in flight behind the newest
+  static constexpr int LAG = KV8 ? 1 : 2;  // tiles of copies in flight behind the newest
   static constexpr int CTRL = 2 * TILE + SLOTS * TILE + RAWS * RAW;
-  static constexpr int SMEM = 1024 + CTRL + 2048;
+  static constexpr int SMEM = CTRL + 3072;  // 227 KB at head_dim 128: all that a CTA may have
 };
+
+// One unit of work: 256 rows of a request and kv head, and a range of key tiles.
+struct WaItem {
+  int r, c, split;  // r < 0: no more work
+  int q0;           // the request's first query row
+  int row0, rows;   // rows row0 .. row0 + rows - 1 of its nq G
+  int pos0;         // position of its first query row
+  int p_hi, lo;     // the last row's position; the first key of the first row's window
+  int t_first, t_head, t_lo, n;
+  float scale, vd;
+
+  __device__ __forceinline__ int key0(int j) const {  // first key of tile j
+    const int t = t_first + j;
+    return (t < t_head ? t : t - t_head + t_lo) * WA_KEYS;
+  }
+  __device__ __forceinline__ int mt() const { return rows > 128 ? 2 : 1; }
+};
+
+constexpr int WA_ITEMS = 4;  // ring of work items
 
 struct WaCtrl {
   uint64_t full[8], empty[8];
-  uint64_t s_full[2], p_ready[2], o_done[2], q_full, drain;
+  uint64_t s_full[2], p_ready[2][2], o_done[2], o_empty[2], q_full, q_empty, drain;
+  uint64_t item_full[WA_ITEMS], item_empty[WA_ITEMS];
   int abort;
   uint32_t tmem;
-  uint32_t valid[8][4];  // keys of tile j (mod 8) whose page exists
-  float qinv[256];       // e4m3: what a row's query was multiplied with, inverted
+  alignas(16) uint32_t valid[8][4];  // keys of tile j (mod 8) whose page exists
+  float qinv[2][256];                // e4m3: what a row's query was multiplied with, inverted (items in turn)
+  WaItem item[WA_ITEMS];
 };
 
-// 16 warps: two warpgroups of softmax (one to a row tile of 128), one that
-// loads, and one whose first warp issues the products.  S = Q K^T goes to
-// tensor memory; the softmax threads (one to a row) turn it into P in place,
-// which is the next product's A operand.  While one row tile is in softmax the
-// tensor cores work on the other.
+// 16 warps, persistent over work items, heaviest first: two warpgroups of
+// softmax (one to a row tile of 128), one that loads keys and values, and one
+// whose warps issue the products (12), hand out work items and load queries
+// (13 to 15).  S = Q K^T goes to tensor memory; the softmax threads (one to a
+// row) turn it into P in place, which is the next product's A operand.  While
+// one row tile is in softmax the tensor cores work on the other, and the next
+// item's loads run beside the current one's products.
 template <int HD, bool KV8>
 __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
   using Lay = WaLayout<HD, KV8>;
   constexpr int TILE = Lay::TILE, SLOTS = Lay::SLOTS;
   constexpr int CPR = HD / 8;  // 16-byte chunks of a 16-bit row
   extern __shared__ __align__(1024) uint8_t wa_smem[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-  // the row tile, the latest rows (those with the most keys) first
-  const int bid = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
-  const int c = bid % a.c.KH;
-  const int2 at = find_tile(a.cu, a.c.R, a.G, WA_ROWS, a.tiles - 1 - bid / a.c.KH);
-  if (at.x < 0) return;
-  const int r = at.x, q0 = a.cu[r], nq = a.cu[r + 1] - q0;
-  if (q0 < 0 || nq < 0 || q0 + nq > a.T) {
-    if (tid == 0) record_error(a.err, DEV_BAD_INDEX);
-    return;
-  }
-  const int len = cache_length(a.c, r, a.err, tid == 0);
-  const int row0 = at.y * WA_ROWS, rows = min(WA_ROWS, nq * a.G - row0);
-  const int pos0 = len - nq;  // position of the request's first query row (negative: it sees nothing)
-  const int p_lo = pos0 + row0 / a.G, p_hi = pos0 + (row0 + rows - 1) / a.G;
-  const int mt = rows > 128 ? 2 : 1;
-
-  // key tiles: those of the first tokens, then those from the first row's window on
-  const int lo = a.window > 0 ? max(0, p_lo - a.window + 1) : 0;
-  const int t_end = p_hi < 0 ? 0 : p_hi / WA_KEYS + 1;
-  const int t_lo = lo / WA_KEYS;
-  const int t_head = min((min(a.sinks, lo) + WA_KEYS - 1) / WA_KEYS, t_lo);
-  const int total = max(0, t_head + t_end - t_lo);
-  const int t_first = (int)((long long)total * split / a.splits);
-  const int n = (int)((long long)total * (split + 1) / a.splits) - t_first;
-  auto key0 = [&](int j) {  // first key of this CTA's tile j
-    const int t = t_first + j;
-    return (t < t_head ? t : t - t_head + t_lo) * WA_KEYS;
-  };
-  if (n <= 0) {  // nothing is seen
-    if (a.splits == 1) {
-      for (int i = tid; i < rows * CPR; i += 512) {
-        const int row = row0 + i / CPR;
-        *reinterpret_cast<uint4*>(a.out + (long long)(q0 + row / a.G) * a.o_ts +
-                                  (long long)(c * a.G + row % a.G) * a.o_hs + (i % CPR) * 8) = make_uint4(0, 0, 0, 0);
-      }
-    } else {
-      for (int i = tid; i < rows; i += 512) {
-        const int row = row0 + i;
-        a.stats[((long long)split * a.T + q0 + row / a.G) * a.H + c * a.G + row % a.G] = make_float2(-INFINITY, 0.0f);
-      }
-    }
-    return;
-  }
-
-  uint8_t* base = wa_smem + ((1024 - (smem_u32(wa_smem) & 1023)) & 1023);
-  uint8_t* sQ = base;
-  uint8_t* sKV = base + 2 * TILE;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  uint8_t* sQ = wa_smem;
+  uint8_t* sKV = wa_smem + 2 * TILE;
   uint8_t* sRaw = sKV + SLOTS * TILE;
-  WaCtrl* ctl = reinterpret_cast<WaCtrl*>(base + Lay::CTRL);
+  WaCtrl* ctl = reinterpret_cast<WaCtrl*>(wa_smem + Lay::CTRL);
+  if (smem_u32(wa_smem) & 1023) {  // the swizzled tiles need the alignment that the declaration asks for
+    if (tid == 0) record_error(a.err, DEV_BAD_COPY);
+    return;
+  }
   volatile int* abort = &ctl->abort;
   if (tid == 0) {
     for (int i = 0; i < SLOTS; ++i) {
@@ -222,11 +226,18 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl->s_full[i], 2);
-      mbar_init(&ctl->p_ready[i], 128);
+      mbar_init(&ctl->p_ready[i][0], 128);
+      mbar_init(&ctl->p_ready[i][1], 128);
       mbar_init(&ctl->o_done[i], 1);
+      mbar_init(&ctl->o_empty[i], 128);
     }
-    mbar_init(&ctl->q_full, 256);
+    mbar_init(&ctl->q_full, 96);
+    mbar_init(&ctl->q_empty, 1);
     mbar_init(&ctl->drain, 1);
+    for (int i = 0; i < WA_ITEMS; ++i) {
+      mbar_init(&ctl->item_full[i], 1);
+      mbar_init(&ctl->item_empty[i], 15);  // every warp but the one that hands out
+    }
     ctl->abort = 0;
     fence_mbar_init();
   }
@@ -237,86 +248,70 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
   }
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = ctl->tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem, 0);
 
-  float kd = 1.0f, vd = 1.0f;
-  if (a.c.descales) {
-    kd = a.c.descales[(long long)r * a.c.KH + c];
-    vd = a.c.descales[(long long)(a.c.R + r) * a.c.KH + c];
-  }
-  // |scale| goes with the scores; its sign (or a zero scale) with the queries
-  const float fscale = a.scale * kd;
-  const float sgn = fscale > 0.0f ? 1.0f : fscale < 0.0f ? -1.0f : 0.0f;
+  // item k of this CTA; r < 0 after the last, or when a wait ran out
+  auto take = [&](int k) {
+    WaItem w;
+    if (!mbar_wait(&ctl->item_full[k % WA_ITEMS], (k / WA_ITEMS) & 1, abort)) {
+      *abort = 1;
+      record_error(a.err, DEV_TIMEOUT_OTHER);
+      w.r = -1;
+    } else {
+      w = ctl->item[k % WA_ITEMS];
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctl->item_empty[k % WA_ITEMS]);
+    return w;
+  };
 
   if (warp < 8) {
     regs_inc<192>();
-    // ------------------------------------------------------------- queries
-    {
-      constexpr int RPI = 256 / CPR;  // rows at a time
-      const int ch = tid % CPR;
-#pragma unroll 4
-      for (int i = 0; i < 256; i += RPI) {
-        const int lr = i + tid / CPR;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (lr < rows) {
-          const int row = row0 + lr;
-          v = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.q) +
-                                              (long long)(q0 + row / a.G) * a.q_ts +
-                                              (long long)(c * a.G + row % a.G) * a.q_hs + ch * 8);
-        }
-        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-        if constexpr (KV8) {
-          float amax = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xffff0000u))));
-#pragma unroll
-          for (int off = 1; off < CPR; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-          const float f = half_row_scale(amax);
-          if (ch == 0) ctl->qinv[lr] = 1.0f / f;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = pack16(__uint_as_float(w[e] << 16) * f, __uint_as_float(w[e] & 0xffff0000u) * f, true);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = sgn > 0.0f ? w[e] : sgn < 0.0f ? w[e] ^ 0x80008000u : 0u;
-        const int r128 = lr & 127;
-        *reinterpret_cast<uint4*>(sQ + (lr >> 7) * TILE + (ch >> 3) * 16384 + r128 * 128 +
-                                  (((ch & 7) ^ (r128 & 7)) << 4)) = v;
-      }
-      fence_async_smem();
-      mbar_arrive(&ctl->q_full);
-    }
     // ------------------------------------------------------------- softmax
     const int i = warp >> 2;  // row tile
-    if (i < mt) {
-      const int lr = i * 128 + (tid & 127), row = row0 + lr;
-      const bool live = lr < rows;
-      // sees keys up to p (a row past the end stands where the last one does, and is not written),
-      const int p = pos0 + (live ? row : row0 + rows - 1) / a.G;
-      const int wlo = a.window > 0 ? p - a.window + 1 : 0;  // from wlo on or below sinks
-      float sc = sgn == 0.0f ? 1.0f : fabsf(fscale);
-      if constexpr (KV8) {
-        if (!mbar_wait(&ctl->q_full, 0, abort)) *abort = 1;  // the rows' factors are written
-        sc *= ctl->qinv[lr];
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t tS = tmem + lanes + i * 128, tO = tmem + lanes + 256 + i * 128;
+    uint32_t s_phase = 0, o_phase = 0;
+    int tiles = 0, worked = 0;  // key tiles and items with keys so far
+    for (int k = 0;; ++k) {
+      const WaItem w = take(k);
+      if (w.r < 0) break;
+      const int lr = i * 128 + (tid & 127), row = w.row0 + lr;
+      const bool live = lr < w.rows;
+      const int tok = w.q0 + (live ? row / a.G : 0), h = w.c * a.G + (live ? row % a.G : 0);
+      __nv_bfloat16* out = a.out + (long long)tok * a.o_ts + (long long)h * a.o_hs;
+      const long long prow = ((long long)w.split * a.T + tok) * a.H + h;
+      if (w.n <= 0) {  // nothing is seen
+        if (live && a.splits == 1)
+          for (int e = 0; e < CPR; ++e) reinterpret_cast<uint4*>(out)[e] = make_uint4(0, 0, 0, 0);
+        if (live && a.splits > 1) a.stats[prow] = make_float2(-INFINITY, 0.0f);
+        continue;
       }
-      const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-      const uint32_t tS = tmem + lanes + i * 128, tO = tmem + lanes + 256 + i * 128;
+      const int tile0 = tiles, par = worked & 1;
+      tiles += w.n;
+      ++worked;
+      if (i >= w.mt()) continue;
+      // sees keys up to p (a row past the end stands where the last one does, and is not written),
+      const int p = w.pos0 + (live ? row : w.row0 + w.rows - 1) / a.G;
+      const int wlo = a.window > 0 ? p - a.window + 1 : 0;  // from wlo on or below sinks
+      // |scale| goes with the scores, its sign (or a zero) with the queries
+      float sc = w.scale == 0.0f ? 1.0f : fabsf(w.scale);
       float m = -INFINITY, l = 0.0f;
-      bool ok = true;
-      for (int j = 0; j < n; ++j) {
-        if (!mbar_wait(&ctl->s_full[i], j & 1, abort)) {
+      bool ok = true, nan = false;
+      for (int j = 0; j < w.n; ++j) {
+        if (!mbar_wait(&ctl->s_full[i], s_phase, abort)) {
           ok = false;
           break;
         }
+        s_phase ^= 1;
         tc_fence_after();
         float s[128];
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld_x32(tS + q * 32, s + q * 32);
-        const int j0 = key0(j);
-        uint32_t vm[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) vm[q] = ctl->valid[j & 7][q];
+        if (KV8 && j == 0) sc *= ctl->qinv[par][lr];
+        const int j0 = w.key0(j);
+        const uint4 vm4 = *reinterpret_cast<const uint4*>(ctl->valid[(tile0 + j) & 7]);
+        const uint32_t vm[4] = {vm4.x, vm4.y, vm4.z, vm4.w};
         tmem_wait_ld();
         const bool all = p >= j0 + 127 && (j0 >= wlo || j0 + 127 < a.sinks) && (vm[0] & vm[1] & vm[2] & vm[3]) == ~0u;
         if (!__all_sync(0xffffffffu, all)) {
@@ -331,8 +326,9 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < 128; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+        for (int e = 0; e < 128; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], s[e], s[e + 1]);
+        const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * sc;
+        nan |= top != top;
         // The subtracted maximum may lag behind the true one by a factor 2^8:
         // the numerators stay far inside their type's range, the division by
         // the sum takes the factor out, and O is seldom rescaled.
@@ -354,156 +350,170 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
           m = mn;
         }
         const float neg = m == -INFINITY ? 0.0f : -m;
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float2 sc2 = make_float2(sc, sc), neg2 = make_float2(neg, neg);
+        float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          uint32_t w[32];
+          uint32_t pk[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const float p0 = ex2(fmaf(s[q * 64 + 2 * e], sc, neg)), p1 = ex2(fmaf(s[q * 64 + 2 * e + 1], sc, neg));
-            acc[2 * (e & 1)] += p0;
-            acc[2 * (e & 1) + 1] += p1;
-            w[e] = pack16(p0, p1, KV8);
+            const float2 x = __ffma2_rn(make_float2(s[q * 64 + 2 * e], s[q * 64 + 2 * e + 1]), sc2, neg2);
+            const float2 pr = make_float2(ex2(x.x), ex2(x.y));
+            acc[e & 1] = __fadd2_rn(acc[e & 1], pr);
+            pk[e] = pack16(pr.x, pr.y, KV8);
           }
-          tmem_st_x32(tS + q * 32, w);
+          tmem_st_x32(tS + q * 32, pk);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&ctl->p_ready[i][q]);  // the product may start on these 64 keys
         }
-        l += (acc[0] + acc[1]) + (acc[2] + acc[3]);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&ctl->p_ready[i]);
+        l += (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
       }
-      if (ok && !mbar_wait(&ctl->o_done[i], 0, abort)) ok = false;
-      if (!ok) {
+      if (!ok || !mbar_wait(&ctl->o_done[i], o_phase, abort)) {
         *abort = 1;
         record_error(a.err, DEV_TIMEOUT_ACC);
-      } else {
-        tc_fence_after();
-        const int tok = q0 + (live ? row / a.G : 0), h = c * a.G + (live ? row % a.G : 0);
-        const float inv = l == 0.0f ? 0.0f : vd / l;  // a row that sees nothing is zero
-        const bool whole = a.splits == 1;
-        float* part = whole ? nullptr : a.part + (((long long)split * a.T + tok) * a.H + h) * HD;
-        __nv_bfloat16* out = a.out + (long long)tok * a.o_ts + (long long)h * a.o_hs;
-        if (live && !whole) a.stats[((long long)split * a.T + tok) * a.H + h] = make_float2(m, l);
+        break;
+      }
+      o_phase ^= 1;
+      tc_fence_after();
+      float o[HD];
 #pragma unroll
-        for (int q = 0; q < HD / 32; ++q) {
-          float o[32];
-          tmem_ld_x32(tO + q * 32, o);
-          tmem_wait_ld();
-          if (!live) continue;
-          if (whole) {
+      for (int q = 0; q < HD / 32; ++q) tmem_ld_x32(tO + q * 32, o + q * 32);
+      tmem_wait_ld();
+      tc_fence_before();
+      mbar_arrive(&ctl->o_empty[i]);  // the next item's product may overwrite it
+      if (!live) continue;
+      // no score above -inf: zero; a score that is no number: nor is the row
+      if (m == -INFINITY) l = 0.0f;
+      if (nan) l = NAN;
+      if (a.splits == 1) {
+        const float inv = l == 0.0f ? 0.0f : w.vd / l;
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint4 w;
-              w.x = pack16(o[e] * inv, o[e + 1] * inv, false);
-              w.y = pack16(o[e + 2] * inv, o[e + 3] * inv, false);
-              w.z = pack16(o[e + 4] * inv, o[e + 5] * inv, false);
-              w.w = pack16(o[e + 6] * inv, o[e + 7] * inv, false);
-              *reinterpret_cast<uint4*>(out + q * 32 + e) = w;
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(part + q * 32 + e) =
-                  make_float4(o[e] * vd, o[e + 1] * vd, o[e + 2] * vd, o[e + 3] * vd);
-          }
+        for (int e = 0; e < HD; e += 8) {
+          uint4 x;
+          x.x = pack16(o[e] * inv, o[e + 1] * inv, false);
+          x.y = pack16(o[e + 2] * inv, o[e + 3] * inv, false);
+          x.z = pack16(o[e + 4] * inv, o[e + 5] * inv, false);
+          x.w = pack16(o[e + 6] * inv, o[e + 7] * inv, false);
+          *reinterpret_cast<uint4*>(out + e) = x;
         }
-        tc_fence_before();
+      } else {
+        a.stats[prow] = make_float2(m, l);
+        float* part = a.part + prow * HD;
+#pragma unroll
+        for (int e = 0; e < HD; e += 4)
+          *reinterpret_cast<float4*>(part + e) =
+              make_float4(o[e] * w.vd, o[e + 1] * w.vd, o[e + 2] * w.vd, o[e + 3] * w.vd);
       }
     }
   } else if (warp < 12) {
     regs_dec<64>();
     // ------------------------------------------------------------- keys and values
     const int lw = warp - 8;  // rows 32 lw .. 32 lw + 31 of every tile
-    const long long trow = (long long)r * a.c.tstride;
-    auto lookup = [&](int j, int* tok) {  // page of this lane's key of tile j; -1: none, -2: a bad one
-      if (j >= n) return -1;
-      const int k = key0(j) + lw * 32 + lane;
-      if (k > p_hi || !(k >= lo || k < a.sinks)) return -1;
-      const int pg = k / a.c.page;
-      *tok = k - pg * a.c.page;
-      const int page = a.c.table[trow + pg];
-      if (page >= 0 && page < a.c.num_pages) return page;
-      record_error(a.err, DEV_BAD_INDEX);
-      return -2;
-    };
-    int tok = 0, tok_next = 0, page = -1, page_next = lookup(0, &tok_next);
     bool ok = true;
-    const int items = 2 * n;
-    for (int q = 0; q < items + Lay::LAG + (KV8 ? 1 : 0); ++q) {
-      // ---- issue item q (K and V of a tile in turn)
-      if (q < items) {
-        const int slot = q % SLOTS;
-        if (!KV8 && q >= SLOTS && ok && !mbar_wait(&ctl->empty[slot], (q / SLOTS - 1) & 1, abort)) ok = false;
-        if (!ok) break;
-        const bool is_v = q & 1;
-        if (!is_v) {
-          page = page_next;
-          tok = tok_next;
-          page_next = lookup(q / 2 + 1, &tok_next);
-          const uint32_t good = __ballot_sync(0xffffffffu, page != -2);
-          if (lane == 0) ctl->valid[(q / 2) & 7][lw] = good;
+    int slot = 0, made = 0;  // ring position and entries (K and V of a tile in turn) so far
+    uint32_t phase = 1;      // an empty slot's first wait succeeds at once
+    int done_slot = 0;       // the oldest entry that is not handed over yet
+    uint32_t done_phase = 1;
+    int tiles = 0;
+    // hand the oldest entry to the tensor cores; at most PEND newer ones are in flight
+    auto hand_over = [&]() {
+      if constexpr (KV8) {  // widen it: e4m3 is exact in f16
+        __syncwarp();
+        if (!mbar_wait(&ctl->empty[done_slot], done_phase, abort)) {
+          ok = false;
+          return;
         }
-        const uint8_t* src = is_v ? a.c.v : a.c.k;
-        long long off = -1;
-        if (page >= 0)
-          off = is_v ? page * a.c.vps + (long long)c * a.c.vhs + (long long)tok * a.c.vts
-                     : page * a.c.kps + (long long)c * a.c.khs + (long long)tok * a.c.kts;
-        constexpr int RC = KV8 ? HD / 16 : CPR;  // 16-byte chunks of a cache row
-        constexpr int RPI = 32 / RC;
-        const int ch = lane % RC;
-        const uint32_t dst = KV8 ? smem_u32(sRaw) + (q & 1) * Lay::RAW + lw * 32 * HD
-                                 : smem_u32(sKV) + slot * TILE + (ch >> 3) * 16384 + lw * 32 * 128;
+        constexpr int RC = HD / 16, RPI = 32 / RC;
+        const int ch = lane % RC, odd = (ch >> 2) & 1;  // which half first: no two lanes of a row share a bank
+        const uint8_t* raw = sRaw + ((made - 1) & 1) * Lay::RAW + lw * 32 * HD;
+        uint8_t* dst = sKV + done_slot * TILE + (ch >> 2) * 16384;
 #pragma unroll 4
         for (int u = 0; u < 32 / RPI; ++u) {
-          const int row = u * RPI + lane / RC;
-          const long long o = __shfl_sync(0xffffffffu, off, row);
-          // keys that no row sees are zero: what the cache holds there may be no number
-          pc_cp_async16(KV8 ? dst + row * HD + ch * 16 : dst + row * 128 + (((ch & 7) ^ (row & 7)) << 4),
-                        src + (o < 0 ? 0 : o + ch * 16), o < 0 ? 0u : 16u);
+          const int row = u * RPI + lane / RC, r128 = lw * 32 + row;
+          const uint4 x = *reinterpret_cast<const uint4*>(raw + row * HD + ch * 16);
+          const uint4 h0 = make_uint4(e4m3x2_h(x.x & 0xffffu), e4m3x2_h(x.x >> 16), e4m3x2_h(x.y & 0xffffu),
+                                      e4m3x2_h(x.y >> 16));
+          const uint4 h1 = make_uint4(e4m3x2_h(x.z & 0xffffu), e4m3x2_h(x.z >> 16), e4m3x2_h(x.w & 0xffffu),
+                                      e4m3x2_h(x.w >> 16));
+          uint8_t* drow = dst + r128 * 128;
+          const int c0 = (2 * ch) & 7;
+          *reinterpret_cast<uint4*>(drow + (((c0 + odd) ^ (r128 & 7)) << 4)) = odd ? h1 : h0;
+          *reinterpret_cast<uint4*>(drow + (((c0 + 1 - odd) ^ (r128 & 7)) << 4)) = odd ? h0 : h1;
         }
+        __syncwarp();  // the raw rows may be overwritten from here on
       }
-      pc_cp_commit();
-      if constexpr (KV8) {
-        // ---- widen item q - 1, which this warp copied: e4m3 is exact in f16
-        const int d = q - 1;
-        if (d >= 0) {
-          const int slot = d % SLOTS;
-          pc_cp_wait<1>();
-          __syncwarp();
-          if (d >= SLOTS && !mbar_wait(&ctl->empty[slot], (d / SLOTS - 1) & 1, abort)) {
+      fence_async_smem();
+      mbar_arrive(&ctl->full[done_slot]);
+      if (++done_slot == SLOTS) {
+        done_slot = 0;
+        done_phase ^= 1;
+      }
+    };
+    constexpr int PEND = Lay::LAG;
+    for (int k = 0; ok; ++k) {
+      const WaItem w = take(k);
+      if (w.r < 0) break;
+      const long long trow = (long long)w.r * a.c.tstride;
+      auto lookup = [&](int j, int* tok) {  // page of this lane's key of tile j; -1: none, -2: a bad one
+        if (j >= w.n) return -1;
+        const int key = w.key0(j) + lw * 32 + lane;
+        if (key > w.p_hi || !(key >= w.lo || key < a.sinks)) return -1;
+        const int pg = key / a.c.page;
+        *tok = key - pg * a.c.page;
+        const int page = a.c.table[trow + pg];
+        if (page >= 0 && page < a.c.num_pages) return page;
+        record_error(a.err, DEV_BAD_INDEX);
+        return -2;
+      };
+      int tok_next = 0, page_next = lookup(0, &tok_next);
+      for (int j = 0; j < w.n && ok; ++j, ++tiles) {
+        const int page = page_next, tok = tok_next;
+        page_next = lookup(j + 1, &tok_next);
+        const uint32_t good = __ballot_sync(0xffffffffu, page != -2);
+        if (lane == 0) ctl->valid[tiles & 7][lw] = good;
+#pragma unroll
+        for (int is_v = 0; is_v < 2; ++is_v) {
+          if (!KV8 && !mbar_wait(&ctl->empty[slot], phase, abort)) {
             ok = false;
             break;
           }
-          constexpr int RC = HD / 16, RPI = 32 / RC;
-          const int ch = lane % RC, odd = (ch >> 2) & 1;  // which half first: no two lanes of a row share a bank
-          const uint8_t* raw = sRaw + (d & 1) * Lay::RAW + lw * 32 * HD;
-          uint8_t* dst = sKV + slot * TILE + (ch >> 2) * 16384;
+          const uint8_t* src = is_v ? a.c.v : a.c.k;
+          long long off = -1;
+          if (page >= 0)
+            off = is_v ? page * a.c.vps + (long long)w.c * a.c.vhs + (long long)tok * a.c.vts
+                       : page * a.c.kps + (long long)w.c * a.c.khs + (long long)tok * a.c.kts;
+          constexpr int RC = KV8 ? HD / 16 : CPR;  // 16-byte chunks of a cache row
+          constexpr int RPI = 32 / RC;
+          const int ch = lane % RC;
+          const uint32_t dst = KV8 ? smem_u32(sRaw) + (made & 1) * Lay::RAW + lw * 32 * HD
+                                   : smem_u32(sKV) + slot * TILE + (ch >> 3) * 16384 + lw * 32 * 128;
 #pragma unroll 4
           for (int u = 0; u < 32 / RPI; ++u) {
-            const int row = u * RPI + lane / RC, r128 = lw * 32 + row;
-            const uint4 x = *reinterpret_cast<const uint4*>(raw + row * HD + ch * 16);
-            const uint4 h0 = make_uint4(e4m3x2_h(x.x & 0xffffu), e4m3x2_h(x.x >> 16), e4m3x2_h(x.y & 0xffffu),
-                                        e4m3x2_h(x.y >> 16));
-            const uint4 h1 = make_uint4(e4m3x2_h(x.z & 0xffffu), e4m3x2_h(x.z >> 16), e4m3x2_h(x.w & 0xffffu),
-                                        e4m3x2_h(x.w >> 16));
-            uint8_t* drow = dst + r128 * 128;
-            const int c0 = (2 * ch) & 7;
-            *reinterpret_cast<uint4*>(drow + (((c0 + odd) ^ (r128 & 7)) << 4)) = odd ? h1 : h0;
-            *reinterpret_cast<uint4*>(drow + (((c0 + 1 - odd) ^ (r128 & 7)) << 4)) = odd ? h0 : h1;
+            const int row = u * RPI + lane / RC;
+            const long long o = __shfl_sync(0xffffffffu, off, row);
+            // keys that no row sees are zero: what the cache holds there may be no number
+            pc_cp_async16(KV8 ? dst + row * HD + ch * 16 : dst + row * 128 + (((ch & 7) ^ (row & 7)) << 4),
+                          src + (o < 0 ? 0 : o + ch * 16), o < 0 ? 0u : 16u);
           }
-          __syncwarp();  // the raw rows may be overwritten from here on
-          fence_async_smem();
-          mbar_arrive(&ctl->full[slot]);
-        }
-      } else {
-        // ---- item q - LAG has arrived: hand it to the tensor cores
-        const int d = q - Lay::LAG;
-        if (d >= 0) {
-          pc_cp_wait<Lay::LAG>();
-          fence_async_smem();
-          mbar_arrive(&ctl->full[d % SLOTS]);
+          pc_cp_commit();
+          if (made >= PEND) {
+            pc_cp_wait<PEND>();
+            hand_over();
+            if (!ok) break;
+          }
+          ++made;
+          if (++slot == SLOTS) {
+            slot = 0;
+            phase ^= 1;
+          }
         }
       }
+    }
+    // the last entries
+    if (ok) {
+      pc_cp_wait<0>();
+      for (int e = min(made, PEND); e > 0 && ok; --e) hand_over();
     }
     pc_cp_wait<0>();
     if (!ok) {
@@ -512,63 +522,218 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
     }
   } else {
     regs_dec<64>();
-    if (warp == 12 && lane == 0) {
+    if (warp == 12) {
       // ------------------------------------------------------------- products
+      // The whole warp goes through the loop, so that the operands' addresses
+      // are uniform values; one lane issues.
       constexpr uint32_t ID_S = wa_idesc(KV8, 128, 128, false), ID_O = wa_idesc(KV8, 128, HD, true);
+      const bool leader = elect_one();
+      const uint32_t q_lo = desc_lo_k(smem_u32(sQ)), kv = smem_u32(sKV);
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort)); };
       auto product_s = [&](int i, int slot) {
-        const uint32_t qa = smem_u32(sQ) + i * TILE, kb = smem_u32(sKV) + slot * TILE;
+        const uint32_t qa = q_lo + i * (TILE >> 4), kb = desc_lo_k(kv + slot * TILE), d = tmem + i * 128;
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k) {
-          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-          umma_bf16(tmem + i * 128, sdesc_k_sw128(qa + off), sdesc_k_sw128(kb + off), ID_S, k > 0);
+          for (int k = 0; k < HD / 16; ++k) {
+            const uint32_t off = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
+            umma_ss(d, qa + off, kb + off, ID_S, k > 0);
+          }
+          mbar_arrive(&ctl->s_full[i]);  // the keys' validity words and the rows' factors, too, are there
+          umma_commit(&ctl->s_full[i]);
         }
-        mbar_arrive(&ctl->s_full[i]);  // the keys' validity words, too, are there
-        umma_commit(&ctl->s_full[i]);
       };
-      auto product_o = [&](int i, int slot, bool first) {
-        const uint32_t vb = smem_u32(sKV) + slot * TILE;
+      auto product_o = [&](int i, int slot, int half, uint32_t accumulate) {  // 64 keys
+        const uint32_t vb = desc_lo_mn(kv + slot * TILE) + half * 512, d = tmem + 256 + i * 128;
+        const uint32_t pa = tmem + i * 128 + half * 32;
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < WA_KEYS / 16; ++k)
-          umma_ts(tmem + 256 + i * 128, tmem + i * 128 + k * 8, sdesc_mn_sw128(vb + k * 2048, 16384), ID_O,
-                  !first || k > 0);
+          for (int k = 0; k < 4; ++k) umma_ts(d, pa + k * 8, vb + k * 128, ID_O, k > 0 ? 1u : accumulate);
+        }
       };
-      int code = 0;
-      if (!mbar_wait(&ctl->q_full, 0, abort) || !mbar_wait(&ctl->full[0], 0, abort)) code = DEV_TIMEOUT_FULL;
-      if (!code) {
+      int code = 0, slot = 0;
+      uint32_t phase = 0, q_phase = 0, p_phase[2] = {0, 0}, o_phase[2] = {1, 1};
+      auto next = [&]() {
+        if (++slot == SLOTS) {
+          slot = 0;
+          phase ^= 1;
+        }
+      };
+      for (int k = 0; !code; ++k) {
+        const WaItem w = take(k);
+        const int r = __shfl_sync(0xffffffffu, w.r, 0), n = __shfl_sync(0xffffffffu, w.n, 0);
+        const int mt = __shfl_sync(0xffffffffu, w.mt(), 0);
+        if (r < 0) break;
+        if (n <= 0) continue;
+        if (!wait(&ctl->q_full, q_phase) || !wait(&ctl->full[slot], phase)) {
+          code = DEV_TIMEOUT_FULL;
+          break;
+        }
+        q_phase ^= 1;
         tc_fence_after();
-        for (int i = 0; i < mt; ++i) product_s(i, 0);
-        umma_commit(&ctl->empty[0]);
-      }
-      for (int j = 0; j < n && !code; ++j) {
-        const int qv = 2 * j + 1, qk = 2 * j + 2;
-        const bool more = j + 1 < n;
-        if (!mbar_wait(&ctl->full[qv % SLOTS], (qv / SLOTS) & 1, abort)) code = DEV_TIMEOUT_FULL;
-        for (int i = 0; i < mt && !code; ++i) {
-          if (!mbar_wait(&ctl->p_ready[i], j & 1, abort)) {
-            code = DEV_TIMEOUT_ACC;
-            break;
-          }
-          tc_fence_after();
-          product_o(i, qv % SLOTS, j == 0);
-          if (i == mt - 1) umma_commit(&ctl->empty[qv % SLOTS]);
-          if (!more) {
-            umma_commit(&ctl->o_done[i]);
-            continue;
-          }
-          if (i == 0 && !mbar_wait(&ctl->full[qk % SLOTS], (qk / SLOTS) & 1, abort)) {
+        for (int i = 0; i < mt; ++i) product_s(i, slot);
+        if (leader) {
+          umma_commit(&ctl->empty[slot]);
+          if (n == 1) umma_commit(&ctl->q_empty);
+        }
+        next();
+        for (int j = 0; j < n && !code; ++j) {
+          const bool more = j + 1 < n;
+          const int sv = slot;
+          if (!wait(&ctl->full[sv], phase)) {
             code = DEV_TIMEOUT_FULL;
             break;
           }
-          product_s(i, qk % SLOTS);
-          if (i == mt - 1) umma_commit(&ctl->empty[qk % SLOTS]);
+          next();
+          const int sk = slot;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (i >= mt || code) break;
+            if (j == 0) {  // the item before has read its O
+              if (!wait(&ctl->o_empty[i], o_phase[i])) code = DEV_TIMEOUT_ACC;
+              o_phase[i] ^= 1;
+            }
+            for (int half = 0; half < 2 && !code; ++half) {
+              if (!wait(&ctl->p_ready[i][half], p_phase[i])) {
+                code = DEV_TIMEOUT_ACC;
+                break;
+              }
+              tc_fence_after();
+              product_o(i, sv, half, j > 0 || half > 0);
+            }
+            if (code) break;
+            p_phase[i] ^= 1;
+            if (leader && i == mt - 1) umma_commit(&ctl->empty[sv]);
+            if (!more) {
+              if (leader) umma_commit(&ctl->o_done[i]);
+              continue;
+            }
+            if (i == 0 && !wait(&ctl->full[sk], phase)) {
+              code = DEV_TIMEOUT_FULL;
+              break;
+            }
+            product_s(i, sk);
+            if (leader && i == mt - 1) {
+              umma_commit(&ctl->empty[sk]);
+              if (j + 2 == n) umma_commit(&ctl->q_empty);
+            }
+          }
+          if (more) next();
         }
       }
       if (code) {
-        *abort = 1;
-        record_error(a.err, code);
-        umma_commit(&ctl->drain);  // nothing of this CTA may be in flight when it ends
+        if (leader) {
+          *abort = 1;
+          record_error(a.err, code);
+          umma_commit(&ctl->drain);  // nothing of this CTA may be in flight when it ends
+        }
         mbar_wait(&ctl->drain, 0, nullptr);
       }
+    } else {
+      // ------------------------------------------------------------- work items and queries
+      const int total = a.tiles * a.c.KH * a.splits;
+      int id = blockIdx.x;
+      uint32_t q_phase = 1;
+      int worked = 0;
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        WaItem w;
+        if (warp == 13) {
+          w.r = -1;
+          for (; id < total && w.r < 0; id += gridDim.x) {
+            const int bid = id / a.splits;
+            w.split = id % a.splits;
+            w.c = bid % a.c.KH;
+            // the row tile, the latest rows (those with the most keys) first
+            const int2 at = find_tile(a.cu, a.c.R, a.G, WA_ROWS, a.tiles - 1 - bid / a.c.KH);
+            if (at.x < 0) continue;
+            const int q0 = a.cu[at.x], nq = a.cu[at.x + 1] - q0;
+            const int len = cache_length(a.c, at.x, a.err, lane == 0);
+            if (q0 < 0 || nq < 0 || q0 + nq > a.T) {
+              if (lane == 0) record_error(a.err, DEV_BAD_INDEX);
+              continue;
+            }
+            w.r = at.x;
+            w.q0 = q0;
+            w.row0 = at.y * WA_ROWS;
+            w.rows = min(WA_ROWS, nq * a.G - w.row0);
+            w.pos0 = len - nq;  // negative: the first rows see nothing
+            w.p_hi = w.pos0 + (w.row0 + w.rows - 1) / a.G;
+            // key tiles: those of the first tokens, then those from the first row's window on
+            w.lo = a.window > 0 ? max(0, w.pos0 + w.row0 / a.G - a.window + 1) : 0;
+            const int t_end = w.p_hi < 0 ? 0 : w.p_hi / WA_KEYS + 1;
+            w.t_lo = w.lo / WA_KEYS;
+            w.t_head = min((min(a.sinks, w.lo) + WA_KEYS - 1) / WA_KEYS, w.t_lo);
+            const int tiles = max(0, w.t_head + t_end - w.t_lo);
+            w.t_first = (int)((long long)tiles * w.split / a.splits);
+            w.n = (int)((long long)tiles * (w.split + 1) / a.splits) - w.t_first;
+            w.scale = a.scale;
+            w.vd = 1.0f;
+            if (a.c.descales) {
+              w.scale *= a.c.descales[(long long)w.r * a.c.KH + w.c];
+              w.vd = a.c.descales[(long long)(a.c.R + w.r) * a.c.KH + w.c];
+            }
+          }
+          if (!mbar_wait(&ctl->item_empty[k % WA_ITEMS], ((k / WA_ITEMS) & 1) ^ 1, abort)) {
+            *abort = 1;
+            record_error(a.err, DEV_TIMEOUT_OTHER);
+            break;
+          }
+          if (lane == 0) {
+            ctl->item[k % WA_ITEMS] = w;
+            mbar_arrive(&ctl->item_full[k % WA_ITEMS]);
+          }
+        } else {
+          w = take(k);
+        }
+        if (w.r < 0) break;
+        if (w.n <= 0) continue;
+        // the item's queries, once the one before has no product with its own to come
+        if (!mbar_wait(&ctl->q_empty, q_phase, abort)) {
+          *abort = 1;
+          record_error(a.err, DEV_TIMEOUT_EMPTY);
+          break;
+        }
+        q_phase ^= 1;
+        constexpr int RPI = 32 / CPR;  // rows of a warp at a time
+        const int ch = lane % CPR, rows = w.mt() * 128;
+        auto chunk = [&](int lr) { return sQ + (lr >> 7) * TILE + (ch >> 3) * 16384 + (lr & 127) * 128 + (((ch & 7) ^ (lr & 7)) << 4); };
+        for (int lr = (warp - 13) * RPI + lane / CPR; lr < rows; lr += 3 * RPI) {
+          const bool live = lr < w.rows;
+          const int row = w.row0 + (live ? lr : 0);
+          pc_cp_async16(smem_u32(chunk(lr)),
+                        a.q + 2 * ((long long)(w.q0 + row / a.G) * a.q_ts +
+                                   (long long)(w.c * a.G + row % a.G) * a.q_hs + ch * 8),
+                        live ? 16u : 0u);
+        }
+        pc_cp_commit();
+        pc_cp_wait<0>();
+        if (KV8 || !(w.scale > 0.0f)) {
+          for (int lr = (warp - 13) * RPI + lane / CPR; lr - lane / CPR < rows; lr += 3 * RPI) {
+            uint4 v = lr < rows ? *reinterpret_cast<const uint4*>(chunk(lr)) : make_uint4(0, 0, 0, 0);
+            uint32_t* x = reinterpret_cast<uint32_t*>(&v);
+            if constexpr (KV8) {
+              float amax = 0.0f;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(x[e] << 16)), fabsf(__uint_as_float(x[e] & 0xffff0000u))));
+#pragma unroll
+              for (int off = 1; off < CPR; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+              const float f = half_row_scale(amax);
+              if (ch == 0 && lr < rows) ctl->qinv[worked & 1][lr] = 1.0f / f;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                x[e] = pack16(__uint_as_float(x[e] << 16) * f, __uint_as_float(x[e] & 0xffff0000u) * f, true);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = w.scale > 0.0f ? x[e] : w.scale < 0.0f ? x[e] ^ 0x80008000u : 0u;
+            if (lr < rows) *reinterpret_cast<uint4*>(chunk(lr)) = v;
+          }
+        }
+        ++worked;
+        fence_async_smem();
+        mbar_arrive(&ctl->q_full);
+      }
+      pc_cp_wait<0>();
     }
   }
   __syncthreads();
@@ -631,13 +796,14 @@ WindowPlan window_plan(int64_t R, int64_t T, int64_t H, int64_t KH, int64_t HD, 
 template <int HD, bool KV8>
 fm_status launch_window(const WindowArgs& a, cudaStream_t s) {
   constexpr int smem = WaLayout<HD, KV8>::SMEM;
-  static_assert(sizeof(WaCtrl) <= 2048 && smem <= 232448, "shared memory");
+  static_assert(sizeof(WaCtrl) <= 3072 && smem <= 232448, "shared memory");
   fm_status st = check_cuda(
       cudaFuncSetAttribute(window_attn_kernel<HD, KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
       "paged_window_attn");
   if (st != FM_OK) return st;
-  st = launch_kernel(window_attn_kernel<HD, KV8>, dim3((unsigned)(a.tiles * a.c.KH * a.splits)), dim3(512), smem, s,
-                     false, a);
+  const int items = a.tiles * a.c.KH * a.splits, sms = num_sms();
+  st = launch_kernel(window_attn_kernel<HD, KV8>, dim3((unsigned)(items < sms ? items : sms)), dim3(512), smem, s, false,
+                     a);
   if (st != FM_OK || a.splits == 1) return st;
   return launch_kernel(window_join_kernel<HD>, dim3((unsigned)(((long long)a.T * a.H + 3) / 4)), dim3(128), 0, s, true,
                        a);
