@@ -134,7 +134,8 @@ class Evict(ctypes.Structure):
     _fields_ = [("weight_sums", c_void_p), ("sums_request_stride", c_int64), ("sums_head_stride", c_int64),
                 ("budget", c_int64), ("sinks", c_int64), ("recent", c_int64),
                 ("out_page_table", c_void_p), ("out_page_table_stride", c_int64), ("out_page_table_cols", c_int64),
-                ("kept", c_void_p), ("lengths", c_void_p), ("out_sums", c_void_p), ("err", c_void_p)]
+                ("kept", c_void_p), ("lengths", c_void_p), ("out_sums", c_void_p),
+                ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("err", c_void_p)]
 
 
 _SIGNATURES = {
@@ -175,6 +176,7 @@ _SIGNATURES = {
     "fm_paged_decode_attn": (c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(DecodeAttn), c_void_p]),
     "fm_paged_window_attn_workspace_size": (c_size_t, [c_int64] * 9),
     "fm_paged_window_attn": (c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(WindowAttn), c_void_p]),
+    "fm_paged_evict_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
     "fm_paged_evict": (c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(Evict), c_void_p]),
     "fm_tree_build": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
     "fm_tree_commit": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,

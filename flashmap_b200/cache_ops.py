@@ -223,7 +223,8 @@ def evict_paged_context(k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k:
     lengths = torch.empty(cache.requests, dtype=torch.int32, device=dev)
     sums = torch.empty((cache.requests, cache.kv_heads, budget), dtype=torch.float32, device=dev)
     args = _lib.Evict(weight_sums.data_ptr(), weight_sums.stride(0), weight_sums.stride(1), budget, sinks, recent,
-                      None, 0, 0, kept.data_ptr(), lengths.data_ptr(), sums.data_ptr(), _err(dev).data_ptr())
+                      None, 0, 0, kept.data_ptr(), lengths.data_ptr(), sums.data_ptr(), None, 0,
+                      _err(dev).data_ptr())
     if out_block_table is not None:
         _on(out_block_table, "out_block_table", dev)
         _need(out_block_table.dtype is torch.int32 and out_block_table.dim() == 2
@@ -233,5 +234,8 @@ def evict_paged_context(k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k:
         args.out_page_table = out_block_table.data_ptr()
         args.out_page_table_stride, args.out_page_table_cols = out_block_table.stride(0), out_block_table.shape[1]
     if cache.requests:
+        need = _lib.load().fm_paged_evict_workspace_size(cache.requests, cache.kv_heads, budget)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), need
         _lib.call("fm_paged_evict", ctypes.byref(cache), ctypes.byref(args), _raw_stream(dev))
     return kept, lengths, sums

@@ -7,16 +7,26 @@
 // kept rows move, in order of position, to the first slots of the request: in
 // place, or in the pages of another table.
 //
-// evict_select_kernel finds the kept positions: the threshold is the k-th
-// largest 32-bit key, found eight bits at a time from histograms; then one
-// ordered pass writes the kept positions.  evict_move_kernel moves the rows.
-// Both are bound by memory: the sums are read once from HBM and again from L2.
+// evict_select_kernel finds the kept positions: one cluster of CTAs per
+// (request, kv head), each with a slice of the positions whose keys it holds in
+// shared memory.  The smallest kept key is found 11, 11 and 10 bits at a time
+// from histograms that the cluster adds up; then an ordered count gives every
+// kept position its slot.  evict_move_kernel moves the rows.  Both are bound by
+// memory where there are many rows, by latency where there are few.
+#include <cooperative_groups.h>
+
 #include "paged_cache.cuh"
 
 namespace fm {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int EV_THREADS = 512;
+constexpr int EV_WARPS = EV_THREADS / 32;
+constexpr int EV_BINS = 2048;
+constexpr int EV_KEYS = 24576;  // keys of a slice that shared memory holds; longer slices read theirs from L2 again
+constexpr int EV_UNROLL = 8;    // rows that a thread of the moving kernel has in flight
 
 struct EvictArgs {
   CacheRef c;
@@ -28,8 +38,8 @@ struct EvictArgs {
   float* out_sums;  // [R][KH][budget]
   const int* out_table;
   long long ot_stride;
-  int out_cap;  // slots that a row of out_table covers
-  int row_bytes;
+  int2* from;       // [R][KH][budget] (page, token) of the kept rows
+  int row_bytes, slices, chunk;
   int* err;
 };
 
@@ -41,154 +51,239 @@ __device__ __forceinline__ uint32_t sum_key(float v) {
 }
 
 __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
-  __shared__ int hist[256];
-  __shared__ int wsum[2][EV_THREADS / 32];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
+  extern __shared__ uint32_t ev_keys[];
+  __shared__ int hist[2][EV_BINS];
+  __shared__ int wsum[EV_WARPS], wtie[EV_WARPS];
+  __shared__ int s_total[2];  // this slice's sure positions and ties
+  __shared__ int s_bin, s_left;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r = blockIdx.x / a.c.KH, h = blockIdx.x % a.c.KH;
-  const int len = cache_length(a.c, r, a.err, tid == 0 && h == 0);
+  const int item = blockIdx.x / cs, r = item / a.c.KH, h = item % a.c.KH;
+  const int len = cache_length(a.c, r, a.err, tid == 0 && h == 0 && rank == 0);
   const int n = min(len, a.budget);
-  if (h == 0 && tid == 0) a.lengths[r] = n;
+  if (h == 0 && rank == 0 && tid == 0) a.lengths[r] = n;
   const float* sums = a.sums + (long long)r * a.s_rs + (long long)h * a.s_hs;
-  int* kept = a.kept + (long long)blockIdx.x * a.budget;
-  float* out = a.out_sums + (long long)blockIdx.x * a.budget;
-  for (int i = n + tid; i < a.budget; i += EV_THREADS) {
-    kept[i] = -1;
-    out[i] = 0.0f;
+  const int* table = a.c.table + (long long)r * a.c.tstride;
+  const long long row0 = (long long)item * a.budget;
+  auto keep = [&](int at, int i, float v) {
+    const int pg = i / a.c.page;
+    int page = table[pg];
+    if (page < 0 || page >= a.c.num_pages) {
+      record_error(a.err, DEV_BAD_INDEX);
+      page = -1;
+    }
+    a.kept[row0 + at] = i;
+    a.out_sums[row0 + at] = v;
+    a.from[row0 + at] = make_int2(page, i - pg * a.c.page);
+  };
+  for (int i = n + rank * EV_THREADS + tid; i < a.budget; i += cs * EV_THREADS) {
+    a.kept[row0 + i] = -1;
+    a.out_sums[row0 + i] = 0.0f;
   }
   if (len <= a.budget) {
-    for (int i = tid; i < n; i += EV_THREADS) {
-      kept[i] = i;
-      out[i] = sums[i];
-    }
+    for (int i = rank * EV_THREADS + tid; i < n; i += cs * EV_THREADS) keep(i, i, sums[i]);
     return;
   }
   const int lo = a.sinks, hi = len - a.recent;  // the positions that compete
   int need = a.budget - a.sinks - a.recent;     // and how many of them stay (fewer than there are)
+  const int per = ((len + cs - 1) / cs + 31) & ~31;
+  const int begin = min(len, rank * per), count = min(len, begin + per) - begin;
+  const bool held = count <= EV_KEYS;
+  if (held)
+    for (int i = tid; i < count; i += EV_THREADS) ev_keys[i] = sum_key(sums[begin + i]);
+  auto key = [&](int i) { return held ? ev_keys[i] : sum_key(sums[begin + i]); };
+
   uint32_t prefix = 0, mask = 0;
   if (need > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += EV_THREADS) hist[i] = 0;
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const uint32_t digit = pass == 2 ? 1023u : 2047u;
+      int* hp = hist[pass & 1];
+      for (int i = tid; i < EV_BINS; i += EV_THREADS) hp[i] = 0;
       __syncthreads();
-      for (int i = lo + tid; i < hi; i += EV_THREADS) {
-        const uint32_t k = sum_key(sums[i]);
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1);
+      for (int i0 = warp * 32; i0 < count; i0 += EV_THREADS) {
+        const int i = i0 + lane, p = begin + i;
+        int bin = -1;
+        if (i < count && p >= lo && p < hi) {
+          const uint32_t k = key(i);
+          if ((k & mask) == prefix) bin = (int)((k >> shift) & digit);
+        }
+        // equal sums are common (positions that were never looked at): one addition for all of a warp's
+        const unsigned peers = __match_any_sync(0xffffffffu, bin);
+        if (bin >= 0 && lane == __ffs(peers) - 1) atomicAdd(&hp[bin], __popc(peers));
+      }
+      cluster.sync();
+      // thread t: bins 4 t .. 4 t + 3 over the cluster, and the count in all higher bins
+      int4 mine = make_int4(0, 0, 0, 0);
+      for (int q = 0; q < cs; ++q) {
+        const int4 x = reinterpret_cast<const int4*>(cluster.map_shared_rank(hp, q))[tid];
+        mine.x += x.x;
+        mine.y += x.y;
+        mine.z += x.z;
+        mine.w += x.w;
+      }
+      const int all = mine.x + mine.y + mine.z + mine.w;
+      int above = all;  // inclusive suffix sum over lanes
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int v = __shfl_down_sync(0xffffffffu, above, off);
+        if (lane + off < 32) above += v;
+      }
+      if (lane == 0) wsum[warp] = above;
+      __syncthreads();
+      for (int w = warp + 1; w < EV_WARPS; ++w) above += wsum[w];
+      above -= all;
+      // the bin in which the need-th largest lies belongs to exactly one thread
+      const int c4[4] = {mine.w, mine.z, mine.y, mine.x};
+      int before = above;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (before < need && need <= before + c4[e]) {
+          s_bin = 4 * tid + 3 - e;
+          s_left = need - before;
+        }
+        before += c4[e];
       }
       __syncthreads();
-      if (tid == 0) {
-        int left = need, b = 255;
-        while (b > 0 && hist[b] < left) left -= hist[b--];
-        s_need = left;
-        s_prefix = prefix | ((uint32_t)b << shift);
-      }
-      __syncthreads();
-      need = s_need;
-      prefix = s_prefix;
-      mask |= 255u << shift;
+      need = s_left;
+      prefix |= (uint32_t)s_bin << shift;
+      mask |= digit << shift;
     }
   }
-  // prefix is the smallest kept key, and `need` of the positions that hold it stay
-  int base_keep = 0, base_tie = 0;
-  for (int i0 = 0; i0 < len; i0 += EV_THREADS) {
-    const int i = i0 + tid;
-    bool sure = false, tie = false;
-    float v = 0.0f;
-    if (i < len) {
-      v = sums[i];
-      sure = i < lo || i >= hi;
-      if (!sure && need > 0) {
-        const uint32_t k = sum_key(v);
-        sure = k > prefix;
-        tie = k == prefix;
-      }
+  // prefix is the smallest kept key, and the first `need` positions that hold it stay
+  auto kind = [&](int i, bool* tie) {  // whether position begin + i stays for sure, or shares the smallest key
+    const int p = begin + i;
+    *tie = false;
+    if (i >= count) return false;
+    if (p < lo || p >= hi) return true;
+    if (a.budget == a.sinks + a.recent) return false;
+    const uint32_t k = key(i);
+    *tie = k == prefix;
+    return k > prefix;
+  };
+  const int seg = ((count + EV_WARPS - 1) / EV_WARPS + 31) & ~31;  // a warp's run of positions
+  const int s0 = warp * seg, s1 = min(count, s0 + seg);
+  __syncthreads();  // the keys are there where there was no pass
+  int sure = 0, ties = 0;
+  for (int i0 = s0; i0 < s1; i0 += 32) {
+    bool tie;
+    const bool yes = kind(i0 + lane, &tie);
+    sure += __popc(__ballot_sync(0xffffffffu, yes));
+    ties += __popc(__ballot_sync(0xffffffffu, tie));
+  }
+  if (lane == 0) {
+    wsum[warp] = sure;
+    wtie[warp] = ties;
+  }
+  __syncthreads();
+  int sb = 0, tb = 0, st = 0, tt = 0;  // before this warp, and of the slice
+  for (int w = 0; w < EV_WARPS; ++w) {
+    if (w < warp) {
+      sb += wsum[w];
+      tb += wtie[w];
     }
-    // ties before this position decide whether it stays, kept positions before it where it goes
-    const unsigned below = (1u << lane) - 1u;
-    const unsigned tb = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) wsum[0][warp] = __popc(tb);
-    __syncthreads();
-    int tbefore = base_tie, ttotal = 0;
-    for (int w = 0; w < EV_THREADS / 32; ++w) {
-      if (w < warp) tbefore += wsum[0][w];
-      ttotal += wsum[0][w];
+    st += wsum[w];
+    tt += wtie[w];
+  }
+  if (tid == 0) {
+    s_total[0] = st;
+    s_total[1] = tt;
+  }
+  cluster.sync();
+  for (int q = 0; q < rank; ++q) {
+    const int* other = cluster.map_shared_rank(s_total, q);
+    sb += other[0];
+    tb += other[1];
+  }
+  cluster.sync();  // no CTA ends, or counts anew, while another reads its totals
+  const unsigned below = (1u << lane) - 1u;
+  for (int i0 = s0; i0 < s1; i0 += 32) {
+    bool tie;
+    const bool yes = kind(i0 + lane, &tie);
+    const unsigned yb = __ballot_sync(0xffffffffu, yes), eb = __ballot_sync(0xffffffffu, tie);
+    const int t = tb + __popc(eb & below);  // ties before this position
+    if (yes || (tie && t < need)) {
+      const int at = sb + __popc(yb & below) + min(t, need);
+      if (at < a.budget) keep(at, begin + i0 + lane, sums[begin + i0 + lane]);
     }
-    const bool stay = sure || (tie && tbefore + __popc(tb & below) < need);
-    const unsigned kb = __ballot_sync(0xffffffffu, stay);
-    if (lane == 0) wsum[1][warp] = __popc(kb);
-    __syncthreads();
-    int kbefore = base_keep, ktotal = 0;
-    for (int w = 0; w < EV_THREADS / 32; ++w) {
-      if (w < warp) kbefore += wsum[1][w];
-      ktotal += wsum[1][w];
-    }
-    if (stay) {
-      const int at = kbefore + __popc(kb & below);
-      if (at < a.budget) {
-        kept[at] = i;
-        out[at] = v;
-      }
-    }
-    base_tie += ttotal;
-    base_keep += ktotal;
-    __syncthreads();
+    sb += __popc(yb);
+    tb += __popc(eb);
   }
 }
 
-// One CTA per (request, kv head, keys or values).  A row only moves down
-// (kept[i] >= i), so in place the CTA reads a block of rows before it writes
-// the slots of that block: no later block reads a slot below its own first.
+// One CTA per (request, kv head, keys or values, slice of the row's bytes), and
+// for a copy to other pages per `chunk` rows.  In place a row only moves down
+// (kept[i] >= i): the CTA reads a block of rows, all its threads meet, and it
+// writes them.  No later block reads a slot below its own first one, so that
+// one meeting a block is all that is needed.
+template <bool IN_PLACE>
 __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
-  const int part = blockIdx.x & 1, item = blockIdx.x >> 1;
+  pdl_wait();
+  int b = blockIdx.x;
+  const int slice = b % a.slices;
+  b /= a.slices;
+  const int part = b & 1, item = b >> 1;
   const int r = item / a.c.KH, h = item % a.c.KH;
   const int len = cache_length(a.c, r, a.err, false);
-  const int n = min(len, a.budget);
-  const bool in_place = a.out_table == nullptr;
-  if (in_place && len <= a.budget) return;
-  const int* kept = a.kept + (long long)item * a.budget;
-  uint8_t* base = (part ? a.c.v + (long long)h * a.c.vhs : a.c.k + (long long)h * a.c.khs);
+  if (IN_PLACE && len <= a.budget) return;
+  const int begin = blockIdx.y * a.chunk, end = min(min(len, a.budget), begin + a.chunk);
+  const int bytes = a.row_bytes / a.slices, per_row = bytes / 16;
+  const int rows = 256 / per_row, mine = threadIdx.x / per_row;
+  uint8_t* base = (part ? a.c.v + (long long)h * a.c.vhs : a.c.k + (long long)h * a.c.khs) + slice * bytes +
+                  (threadIdx.x % per_row) * 16;
   const long long ps = part ? a.c.vps : a.c.kps, ts = part ? a.c.vts : a.c.kts;
-  const int* src_table = a.c.table + (long long)r * a.c.tstride;
-  const int* dst_table = in_place ? src_table : a.out_table + (long long)r * a.ot_stride;
-  auto row_at = [&](const int* table, int i) -> uint8_t* {
-    const int page = table[i / a.c.page];
-    if (page < 0 || page >= a.c.num_pages) {
-      record_error(a.err, DEV_BAD_INDEX);
-      return nullptr;
+  const int2* from = a.from + (long long)item * a.budget;
+  const int* to = IN_PLACE ? a.c.table + (long long)r * a.c.tstride : a.out_table + (long long)r * a.ot_stride;
+  int2 src[EV_UNROLL];
+  int dst[EV_UNROLL];
+  auto look = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < EV_UNROLL; ++u) {
+      const int i = i0 + u * rows + mine;
+      src[u] = i < end ? from[i] : make_int2(-1, 0);
+      dst[u] = i < end ? to[i / a.c.page] : 0;
     }
-    return base + page * ps + (i % a.c.page) * ts;
   };
-  const int per_row = a.row_bytes / 16, rows = 256 / per_row;
-  const int slot = threadIdx.x / per_row, off = (threadIdx.x % per_row) * 16;
-  constexpr int U = 4;
-  for (int i0 = 0; i0 < n; i0 += rows * U) {
-    uint4 v[U];
-    uint8_t* to[U];
+  look(begin);
+  for (int i0 = begin; i0 < end; i0 += rows * EV_UNROLL) {
+    uint4 v[EV_UNROLL];
+    uint8_t* at[EV_UNROLL];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * rows + slot;
-      to[u] = nullptr;
-      if (i >= n) continue;
-      const int from = kept[i];
-      if (from < 0 || from >= len || (in_place && from == i)) continue;
-      const uint8_t* src = row_at(src_table, from);
-      uint8_t* dst = i < a.out_cap || in_place ? row_at(dst_table, i) : nullptr;
-      if (src == nullptr || dst == nullptr) continue;
-      v[u] = *reinterpret_cast<const uint4*>(src + off);
-      to[u] = dst + off;
+    for (int u = 0; u < EV_UNROLL; ++u) {
+      const int i = i0 + u * rows + mine, tok = i % a.c.page;
+      at[u] = nullptr;
+      if (src[u].x < 0 || (IN_PLACE && src[u].x == dst[u] && src[u].y == tok)) continue;
+      if (dst[u] < 0 || dst[u] >= a.c.num_pages) {
+        record_error(a.err, DEV_BAD_INDEX);
+        continue;
+      }
+      at[u] = base + dst[u] * ps + tok * ts;
+      v[u] = *reinterpret_cast<const uint4*>(base + src[u].x * ps + src[u].y * ts);
     }
-    __syncthreads();
+    look(i0 + rows * EV_UNROLL);
+    if (IN_PLACE) __syncthreads();
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (to[u] != nullptr) *reinterpret_cast<uint4*>(to[u]) = v[u];
-    __syncthreads();
+    for (int u = 0; u < EV_UNROLL; ++u)
+      if (at[u] != nullptr) *reinterpret_cast<uint4*>(at[u]) = v[u];
   }
+}
+
+// CTAs of a cluster: as many as leave one to an SM, with 2048 positions each at least.
+int evict_cluster(int64_t items, int64_t positions) {
+  int cs = 1;
+  while (cs < 8 && items * cs * 2 <= 148 && positions >= 2048 * 2 * cs) cs *= 2;
+  return cs;
 }
 
 }  // namespace
 }  // namespace fm
 
 using namespace fm;
+
+extern "C" size_t fm_paged_evict_workspace_size(int64_t requests, int64_t kv_heads, int64_t budget) {
+  return requests < 1 || kv_heads < 1 || budget < 1 ? 0 : (size_t)requests * kv_heads * budget * sizeof(int2);
+}
 
 extern "C" fm_status fm_paged_evict(const fm_paged_cache* cache, const fm_evict* p, fm_stream stream) {
   EvictArgs a{};
@@ -207,6 +302,10 @@ extern "C" fm_status fm_paged_evict(const fm_paged_cache* cache, const fm_evict*
     return set_error(FM_ERR_INVALID, "paged_evict: the new lengths must not overwrite the old");
   if (p->out_page_table == cache->page_table)
     return set_error(FM_ERR_INVALID, "paged_evict: pass no new page table to evict in place");
+  const size_t need = fm_paged_evict_workspace_size(cache->requests, cache->kv_heads, p->budget);
+  if (!p->workspace || p->workspace_bytes < need)
+    return set_error(FM_ERR_WORKSPACE, "paged_evict: workspace %zu < %zu", p->workspace_bytes, need);
+  if ((uintptr_t)p->workspace % 8) return set_error(FM_ERR_ALIGN, "paged_evict: workspace not 8-byte aligned");
   a.sums = p->weight_sums;
   a.s_rs = p->sums_request_stride;
   a.s_hs = p->sums_head_stride;
@@ -218,13 +317,49 @@ extern "C" fm_status fm_paged_evict(const fm_paged_cache* cache, const fm_evict*
   a.out_sums = p->out_sums;
   a.out_table = p->out_page_table;
   a.ot_stride = p->out_page_table_stride;
-  a.out_cap = a.budget;
+  a.from = static_cast<int2*>(p->workspace);
   a.row_bytes = (int)cache->head_dim * (cache->dtype == FM_DT_E4M3 ? 1 : 2);
   a.err = p->err;
   const int64_t items = cache->requests * cache->kv_heads;
-  if (items > 0x3fffffff) return set_error(FM_ERR_SHAPE, "paged_evict: grid too large");
+  if (items > 0x3ffffff) return set_error(FM_ERR_SHAPE, "paged_evict: grid too large");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  st = launch_kernel(evict_select_kernel, dim3((unsigned)items), dim3(EV_THREADS), 0, s, false, a);
+
+  const int cs = evict_cluster(items, cache->max_length);
+  int64_t keys = (cache->max_length + cs - 1) / cs + 32;
+  if (keys > EV_KEYS) keys = EV_KEYS;
+  st = check_cuda(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_KEYS * 4),
+                  "paged_evict");
   if (st != FM_OK) return st;
-  return launch_kernel(evict_move_kernel, dim3((unsigned)items * 2), dim3(256), 0, s, false, a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(items * cs));
+  cfg.blockDim = dim3(EV_THREADS);
+  cfg.dynamicSmemBytes = (size_t)keys * 4;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)cs, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, evict_select_kernel, a);
+  if (e != cudaSuccess) return set_error(FM_ERR_LAUNCH, "paged_evict: %s", cudaGetErrorString(e));
+  ++launch_counter();
+
+  // Rows are cut into slices of 32 bytes at least while there are fewer than
+  // two CTAs to an SM; a copy is cut along the rows instead.
+  a.slices = 1;
+  a.chunk = a.budget;
+  unsigned chunks = 1;
+  if (a.out_table) {
+    a.chunk = 512;
+    chunks = (unsigned)((a.budget + a.chunk - 1) / a.chunk);
+    if (chunks > 65535) {
+      a.chunk = (a.budget + 65534) / 65535;
+      chunks = (unsigned)((a.budget + a.chunk - 1) / a.chunk);
+    }
+  } else {
+    while (items * 2 * a.slices < 2 * 148 && a.row_bytes / a.slices > 32) a.slices *= 2;
+  }
+  const dim3 grid((unsigned)(items * 2 * a.slices), chunks);
+  if (a.out_table) return launch_kernel(evict_move_kernel<false>, grid, dim3(256), 0, s, true, a);
+  return launch_kernel(evict_move_kernel<true>, grid, dim3(256), 0, s, true, a);
 }

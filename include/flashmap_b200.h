@@ -493,8 +493,11 @@ typedef struct fm_evict {
   int32_t* kept;
   int32_t* lengths;
   float* out_sums;
+  void* workspace; /* need not be initialised */
+  size_t workspace_bytes;
   int32_t* err;
 } fm_evict;
+FM_API size_t fm_paged_evict_workspace_size(int64_t requests, int64_t kv_heads, int64_t budget);
 FM_API fm_status fm_paged_evict(const fm_paged_cache* cache, const fm_evict* args, fm_stream stream);
 
 /* ------------------------------------------------------------------------
