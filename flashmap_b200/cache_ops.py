@@ -43,22 +43,26 @@ _FP8 = torch.float8_e4m3fn
 
 
 def _on(t: torch.Tensor, name: str, device) -> None:
-    _need(t.device == device, f"{name} must be on {device}, got {t.device}")
+    if t.device != device:
+        raise OpArgumentError(f"{name} must be on {device}, got {t.device}")
 
 
 def _cache(k_cache, v_cache, lengths, block_table, descales, max_len: int) -> _lib.PagedCache:
     _need(k_cache.is_cuda, "k_cache must be a CUDA tensor")
     dev = k_cache.device
-    _need(dev.index == torch.cuda.current_device(), f"the cache is on {dev}, which is not the current device")
+    if not (dev.index == torch.cuda.current_device()):
+        raise OpArgumentError(f"the cache is on {dev}, which is not the current device")
     _on(v_cache, "v_cache", dev)
     _on(lengths, "the lengths", dev)
     _on(block_table, "block_table", dev)
-    _need(k_cache.dtype is torch.bfloat16 or k_cache.dtype is _FP8, f"the cache must be bf16 or e4m3, got {k_cache.dtype}")
+    if not (k_cache.dtype is torch.bfloat16 or k_cache.dtype is _FP8):
+        raise OpArgumentError(f"the cache must be bf16 or e4m3, got {k_cache.dtype}")
     _need(v_cache.dtype is k_cache.dtype, "k_cache and v_cache must share a dtype")
     _need(k_cache.dim() == 4 and v_cache.shape == k_cache.shape,
           "k_cache and v_cache must both be (pages, kv_heads, page_size, head_dim)")
     pages, kv_heads, page, head_dim = k_cache.shape
-    _need(head_dim == 64 or head_dim == 128, f"head_dim must be 64 or 128, got {head_dim}")
+    if not (head_dim == 64 or head_dim == 128):
+        raise OpArgumentError(f"head_dim must be 64 or 128, got {head_dim}")
     _need(kv_heads > 0 and page > 0, "the cache needs a kv head and a token to a page")
     ks, vs = k_cache.stride(), v_cache.stride()
     _need(ks[3] == 1 and vs[3] == 1, "cache rows must be contiguous")
@@ -87,10 +91,13 @@ def _cache(k_cache, v_cache, lengths, block_table, descales, max_len: int) -> _l
 
 def _query(query, name: str, cache: _lib.PagedCache, device) -> torch.Tensor:
     _on(query, name, device)
-    _need(query.dtype is torch.bfloat16 and query.dim() == 3, f"{name} must be bf16 (rows, heads, head_dim)")
+    if not (query.dtype is torch.bfloat16 and query.dim() == 3):
+        raise OpArgumentError(f"{name} must be bf16 (rows, heads, head_dim)")
     heads, head_dim = query.shape[1], query.shape[2]
-    _need(head_dim == cache.head_dim, f"{name} has rows of {head_dim}, the cache of {cache.head_dim}")
-    _need(heads > 0 and heads % cache.kv_heads == 0, f"{heads} query heads are no multiple of {cache.kv_heads} kv heads")
+    if not (head_dim == cache.head_dim):
+        raise OpArgumentError(f"{name} has rows of {head_dim}, the cache of {cache.head_dim}")
+    if not (heads > 0 and heads % cache.kv_heads == 0):
+        raise OpArgumentError(f"{heads} query heads are no multiple of {cache.kv_heads} kv heads")
     if query.stride(2) != 1 or query.data_ptr() % 16 or query.stride(0) % 8 or query.stride(1) % 8:
         query = query.contiguous()
         if query.data_ptr() % 16:  # a contiguous view that starts between two 16-byte lines
@@ -107,7 +114,8 @@ def _sums(weight_sums, cache: _lib.PagedCache, device, least: int) -> None:
     _need(weight_sums.dtype is torch.float32 and weight_sums.dim() == 3
           and weight_sums.shape[0] == cache.requests and weight_sums.shape[1] == cache.kv_heads,
           "weight_sums must be float32 (requests, kv_heads, positions)")
-    _need(weight_sums.shape[2] >= least, f"weight_sums has {weight_sums.shape[2]} positions, {least} are needed")
+    if not (weight_sums.shape[2] >= least):
+        raise OpArgumentError(f"weight_sums has {weight_sums.shape[2]} positions, {least} are needed")
     _need(weight_sums.shape[2] <= 1 or weight_sums.stride(2) == 1, "weight_sums rows must be contiguous")
 
 

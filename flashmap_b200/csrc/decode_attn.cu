@@ -21,7 +21,7 @@
 namespace fm {
 namespace {
 
-constexpr int DA_STAGES = 3;
+constexpr int DA_STAGES = 2;
 constexpr int DA_TILE = 16;  // keys of a warp's tile
 
 struct DecodeArgs {
@@ -133,11 +133,11 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
   uint32_t* wok = reinterpret_cast<uint32_t*>(da_smem_buf + da_smem<HD, KV8, NG>() - 4 * DA_STAGES * 4) + warp * DA_STAGES;
   const int ntiles = (end - begin + 4 * DA_TILE - 1) / (4 * DA_TILE);
   const long long trow = (long long)r * a.c.tstride;
-  // page of this lane's key of tile t (lanes 0 .. 15), read one tile ahead of its copies
+  // page and token of this lane's key of tile t (lanes 0 .. 15), read one tile ahead of its copies
   auto lookup = [&](int t, int* tok) {
     const int i = begin + (t * 4 + warp) * DA_TILE + lane;
     if (lane >= DA_TILE || i >= end) return -1;
-    const int p = sp.pos(i), pg = p / a.c.page;
+    const int p = sp.pos(i), pg = a.c.by_page.div(p);
     *tok = p - pg * a.c.page;
     const int page = a.c.table[trow + pg];
     if (page >= 0 && page < a.c.num_pages) return page;
@@ -145,6 +145,10 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
     return -1;
   };
   int tok_next = 0, page_next = lookup(0, &tok_next);
+  constexpr int CPR = RB / 16, RPI = 32 / CPR;  // copies per row, rows per instruction
+  const int ch = lane % CPR, sub = lane / CPR;
+  const uint8_t* kbase = a.c.k + (long long)c * a.c.khs + ch * 16;
+  const uint8_t* vbase = a.c.v + (long long)c * a.c.vhs + ch * 16;
   auto issue = [&](int t) {
     if (t < ntiles) {
       const int page = page_next, tok = tok_next;
@@ -153,22 +157,27 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
       const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
       if (lane == 0) wok[st] = ok;
       const uint32_t sbase = wbase + st * 2 * Lay::PART;
-      constexpr int CPR = RB / 16, RPI = 32 / CPR;  // copies per row, rows per instruction
+      const long long koff = page >= 0 ? page * a.c.kps + tok * a.c.kts : 0;
+      const uint32_t mine = ok >> sub;
+      // rows that no position stands for are zero: what the cache holds there may be no number
+      if (a.c.same) {
 #pragma unroll
-      for (int u = 0; u < DA_TILE / RPI; ++u) {
-        const int row = u * RPI + lane / CPR, ch = lane % CPR;
-        const long long pg = __shfl_sync(0xffffffffu, page, row);
-        const long long tk = __shfl_sync(0xffffffffu, tok, row);
-        const uint32_t dst = sbase + row_sw<RB>(row, ch);
-        const uint8_t* ks = a.c.k;
-        const uint8_t* vs = a.c.v;
-        if (pg >= 0) {
-          ks += pg * a.c.kps + (long long)c * a.c.khs + tk * a.c.kts + ch * 16;
-          vs += pg * a.c.vps + (long long)c * a.c.vhs + tk * a.c.vts + ch * 16;
+        for (int u = 0; u < DA_TILE / RPI; ++u) {
+          const long long o = __shfl_sync(0xffffffffu, koff, u * RPI + sub);
+          const uint32_t dst = sbase + row_sw<RB>(u * RPI + sub, ch), n = (mine >> (u * RPI)) & 1u ? 16u : 0u;
+          pc_cp_async16(dst, kbase + o, n);
+          pc_cp_async16(dst + Lay::PART, vbase + o, n);
         }
-        // rows that no position stands for are zero: what the cache holds there may be no number
-        pc_cp_async16(dst, ks, pg >= 0 ? 16u : 0u);
-        pc_cp_async16(dst + Lay::PART, vs, pg >= 0 ? 16u : 0u);
+      } else {
+        const long long voff = page >= 0 ? page * a.c.vps + tok * a.c.vts : 0;
+#pragma unroll
+        for (int u = 0; u < DA_TILE / RPI; ++u) {
+          const long long o = __shfl_sync(0xffffffffu, koff, u * RPI + sub);
+          const long long w = __shfl_sync(0xffffffffu, voff, u * RPI + sub);
+          const uint32_t dst = sbase + row_sw<RB>(u * RPI + sub, ch), n = (mine >> (u * RPI)) & 1u ? 16u : 0u;
+          pc_cp_async16(dst, kbase + o, n);
+          pc_cp_async16(dst + Lay::PART, vbase + w, n);
+        }
       }
     }
     pc_cp_commit();
@@ -203,9 +212,12 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
           uint32_t b[4];
           ldsm4(kb0 + row_sw<RB>(kr, k4 + (lane >> 3)), b);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < 4; ++e) {
+            uint32_t b0, b1;
+            e4m3x4_h(b[e], b0, b1);
             mma16816<true>(sc[nt], qa[0][k4 + e][0], NG == 2 ? qa[NG - 1][k4 + e][0] : 0u, qa[0][k4 + e][1],
-                           NG == 2 ? qa[NG - 1][k4 + e][1] : 0u, e4m3x2_h(b[e] & 0xffffu), e4m3x2_h(b[e] >> 16));
+                           NG == 2 ? qa[NG - 1][k4 + e][1] : 0u, b0, b1);
+          }
         }
       } else {
 #pragma unroll
@@ -244,7 +256,7 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
       const float mn = fmaxf(m[n], mx);
       const float u = mn == -INFINITY ? 0.0f : mn;
       if (__any_sync(0xffffffffu, mn != m[n])) {
-        const float al = exp2f(m[n] - u);
+        const float al = ex2(m[n] - u);
         l[n] *= al;
         // the outputs' columns are heads 2 tig, 2 tig + 1
         const float a0 = __shfl_sync(0xffffffffu, al, tig * 8), a1 = __shfl_sync(0xffffffffu, al, tig * 8 + 4);
@@ -259,7 +271,7 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
       }
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
-        const float p0 = exp2f(sc[nt][2 * n] - u), p1 = exp2f(sc[nt][2 * n + 1] - u);
+        const float p0 = ex2(sc[nt][2 * n] - u), p1 = ex2(sc[nt][2 * n + 1] - u);
         l[n] += p0 + p1;
         pb[n][nt] = pack16(p0, p1, KV8);
       }
@@ -273,9 +285,9 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
         ldsm4_t(vb0 + row_sw<RB>((lane & 7) + ((lane >> 3) & 1) * 8, i + (lane >> 4)), b);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t x = b[2 * e], y = b[2 * e + 1];
-          const uint32_t a0 = e4m3x2_h(__byte_perm(x, 0, 0x4420)), a1 = e4m3x2_h(__byte_perm(x, 0, 0x4431));
-          const uint32_t a2 = e4m3x2_h(__byte_perm(y, 0, 0x4420)), a3 = e4m3x2_h(__byte_perm(y, 0, 0x4431));
+          uint32_t a0, a1, a2, a3;
+          e4m3x4_h(__byte_perm(b[2 * e], 0, 0x3120), a0, a1);
+          e4m3x4_h(__byte_perm(b[2 * e + 1], 0, 0x3120), a2, a3);
 #pragma unroll
           for (int n = 0; n < NG; ++n) mma16816<true>(o[n][i + e], a0, a1, a2, a3, pb[n][0], pb[n][1]);
         }
@@ -353,44 +365,55 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
   }
 }
 
+// (maximum, sum) of a row over its n chunks, by one warp; the maximum of a row
+// whose scores are all -inf comes back as 0.
+__device__ __forceinline__ float2 row_stats(const float2* stats, int n) {
+  const int lane = threadIdx.x & 31;
+  float2 first = lane < n ? stats[lane] : make_float2(-INFINITY, 0.0f);
+  float mm = first.x;
+  for (int c = lane + 32; c < n; c += 32) mm = fmaxf(mm, stats[c].x);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
+  const float u = mm == -INFINITY ? 0.0f : mm;
+  float ll = first.y * exp2f(first.x - u);
+  for (int c = lane + 32; c < n; c += 32) {
+    const float2 s = stats[c];
+    ll += s.y * exp2f(s.x - u);
+  }
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
+  return make_float2(u, ll);
+}
+
+constexpr int DJ_THREADS = 256;
+constexpr int DJ_KEYS = 4 * DJ_THREADS;  // positions of a block that adds weights to the sums
+constexpr int DJ_HEADS = 8;              // heads whose scores a thread has in flight
+
 // Blocks [0, R H): one (request, head)'s chunks joined to its output row.
-// Blocks from there on: 1024 visible positions of one (request, kv head),
+// Blocks from there on: DJ_KEYS visible positions of one (request, kv head),
 // whose weights are added to the sums; every sum has one writer, so repeated
 // runs agree bit for bit.
 template <int HD>
-__global__ void __launch_bounds__(128) decode_join_kernel(DecodeArgs a, int key_blocks) {
-  __shared__ float sred[4][HD];
-  __shared__ float2 sst[64];
-  pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto row_stats = [&](long long row, int n) {  // by one warp: (maximum, sum) over the row's chunks
-    float mm = -INFINITY;
-    for (int c = lane; c < n; c += 32) mm = fmaxf(mm, a.stats[row * a.chunks + c].x);
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
-    const float u = mm == -INFINITY ? 0.0f : mm;
-    float ll = 0.0f;
-    for (int c = lane; c < n; c += 32) {
-      const float2 s = a.stats[row * a.chunks + c];
-      ll += s.y * exp2f(s.x - u);
-    }
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
-    return make_float2(u, ll);
-  };
+__global__ void __launch_bounds__(DJ_THREADS) decode_join_kernel(DecodeArgs a, int key_blocks) {
+  __shared__ float4 sred[DJ_THREADS / 32][HD / 4];
+  __shared__ float2 sst[DJ_HEADS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = a.c.R * a.H;
+  pdl_wait();
   if ((int)blockIdx.x < rows) {
     const int row = blockIdx.x, r = row / a.H, h = row % a.H;
     const Span sp = visible_span(cache_length(a.c, r, a.err, false), a.window, a.sinks);
     const int n = (sp.n + a.chunk - 1) / a.chunk;
     if (n <= 1) return;  // written by its only chunk
-    const float2 st = row_stats(row, n);
-    constexpr int V = HD / 4, PER = 128 / V;  // threads per chunk's row, chunks at a time
-    const int d = (threadIdx.x % V) * 4;
+    const float2* stats = a.stats + (long long)row * a.chunks;
+    const float2 st = row_stats(stats, n);
+    constexpr int V = HD / 4, PER = DJ_THREADS / V;  // threads per chunk's row, chunks at a time
+    const float4* part = reinterpret_cast<const float4*>(a.part + (long long)row * a.chunks * HD) + tid % V;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = threadIdx.x / V; c < n; c += PER) {
-      const float f = exp2f(a.stats[(long long)row * a.chunks + c].x - st.x);
-      const float4 x = *reinterpret_cast<const float4*>(a.part + ((long long)row * a.chunks + c) * HD + d);
+#pragma unroll 4
+    for (int c = tid / V; c < n; c += PER) {
+      const float4 x = part[(long long)c * V];
+      const float f = exp2f(stats[c].x - st.x);
       acc.x += x.x * f;
       acc.y += x.y * f;
       acc.z += x.z * f;
@@ -402,45 +425,64 @@ __global__ void __launch_bounds__(128) decode_join_kernel(DecodeArgs a, int key_
       acc.z += __shfl_xor_sync(0xffffffffu, acc.z, 16);
       acc.w += __shfl_xor_sync(0xffffffffu, acc.w, 16);
     }
-    if (lane < V) *reinterpret_cast<float4*>(&sred[warp][d]) = acc;
+    if (lane < V) sred[warp][lane] = acc;
     __syncthreads();
-    const float inv = st.y == 0.0f ? 0.0f : 1.0f / st.y;
-    for (int i = threadIdx.x; i < HD; i += 128)
-      a.out[(long long)r * a.o_rs + (long long)h * a.o_hs + i] =
-          f2bf((sred[0][i] + sred[1][i] + sred[2][i] + sred[3][i]) * inv);
+    if (tid < V) {
+      const float inv = st.y == 0.0f ? 0.0f : 1.0f / st.y;
+      float4 o = sred[0][tid];
+#pragma unroll
+      for (int w = 1; w < DJ_THREADS / 32; ++w) {
+        const float4 x = sred[w][tid];
+        o.x += x.x;
+        o.y += x.y;
+        o.z += x.z;
+        o.w += x.w;
+      }
+      *reinterpret_cast<uint2*>(a.out + (long long)r * a.o_rs + (long long)h * a.o_hs + tid * 4) =
+          make_uint2(pack16(o.x * inv, o.y * inv, false), pack16(o.z * inv, o.w * inv, false));
+    }
     return;
   }
   const int item = (blockIdx.x - rows) / key_blocks, kb = (blockIdx.x - rows) % key_blocks;
   const int r = item / a.c.KH, c = item % a.c.KH;
   const Span sp = visible_span(cache_length(a.c, r, a.err, false), a.window, a.sinks);
-  const int begin = kb * 1024, end = min(sp.n, begin + 1024);
-  if (begin >= end) return;
+  const int begin = kb * DJ_KEYS;
+  if (begin >= sp.n) return;
   const int n = (sp.n + a.chunk - 1) / a.chunk;
   const long long row0 = (long long)r * a.H + c * a.G;
   float* dst = a.sums + (long long)r * a.s_rs + (long long)c * a.s_hs;
-  float add[8] = {};
-  for (int g0 = 0; g0 < a.G; g0 += 64) {
-    for (int g = g0 + warp; g < min(a.G, g0 + 64); g += 4) {
-      const float2 st = row_stats(row0 + g, n);
-      if (lane == 0) sst[g - g0] = make_float2(st.x, st.y == 0.0f ? 0.0f : 1.0f / st.y);
+  const int i = begin + tid * 4;  // this thread's four positions (the pitch is a multiple of 16)
+  float old[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) old[e] = i + e < sp.n ? dst[sp.pos(i + e)] : 0.0f;
+  float4 add = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int g0 = 0; g0 < a.G; g0 += DJ_HEADS) {
+    float4 s[DJ_HEADS];
+#pragma unroll
+    for (int g = 0; g < DJ_HEADS; ++g)
+      if (g0 + g < a.G && i < sp.n) s[g] = *reinterpret_cast<const float4*>(a.scores + (row0 + g0 + g) * a.pitch + i);
+    if (g0 + warp < a.G) {
+      const float2 st = row_stats(a.stats + (row0 + g0 + warp) * a.chunks, n);
+      if (lane == 0) sst[warp] = make_float2(st.x, st.y == 0.0f ? 0.0f : 1.0f / st.y);
     }
     __syncthreads();
-    for (int g = g0; g < min(a.G, g0 + 64); ++g) {
-      const float2 st = sst[g - g0];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int i = begin + u * 128 + threadIdx.x;
-        if (i < end) add[u] += exp2f(a.scores[(row0 + g) * a.pitch + i] - st.x) * st.y;
+    for (int g = 0; g < DJ_HEADS; ++g)
+      if (g0 + g < a.G && i < sp.n) {
+        const float2 st = sst[g];
+        add.x += exp2f(s[g].x - st.x) * st.y;
+        add.y += exp2f(s[g].y - st.x) * st.y;
+        add.z += exp2f(s[g].z - st.x) * st.y;
+        add.w += exp2f(s[g].w - st.x) * st.y;
       }
-    }
     __syncthreads();
   }
+  const float w[4] = {add.x, add.y, add.z, add.w};
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const int i = begin + u * 128 + threadIdx.x;
-    if (i < end) dst[sp.pos(i)] += add[u];
-  }
+  for (int e = 0; e < 4; ++e)
+    if (i + e < sp.n) dst[sp.pos(i + e)] = old[e] + w[e];
 }
+static_assert(DJ_THREADS / 32 == DJ_HEADS, "a warp to a head's statistics");
 
 struct DecodePlan {
   int ng, hgroups, chunk, chunks, pitch;
@@ -458,7 +500,7 @@ DecodePlan decode_plan(int64_t R, int64_t H, int64_t KH, int64_t HD, int64_t max
   const int64_t span = visible_span((int)max_len, (int)window, (int)sinks).n;
   const int64_t units = R * KH * p.hgroups * span;
   int64_t chunk = (units / (148 * 8) + 63) / 64 * 64;
-  chunk = chunk < 64 ? 64 : chunk > 512 ? 512 : chunk;
+  chunk = chunk < 64 ? 64 : chunk > 1024 ? 1024 : chunk;
   p.chunk = (int)chunk;
   p.chunks = (int)((span + chunk - 1) / chunk);
   if (p.chunks < 1) p.chunks = 1;
@@ -546,7 +588,7 @@ extern "C" fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_
   a.pitch = pl.pitch;
   a.err = p->err;
   const int64_t items = cache->requests * cache->kv_heads * pl.hgroups;
-  const int64_t key_blocks = sums ? (pl.pitch + 1023) / 1024 : 0;
+  const int64_t key_blocks = sums ? (pl.pitch + DJ_KEYS - 1) / DJ_KEYS : 0;
   const int64_t join = cache->requests * (p->heads + cache->kv_heads * key_blocks);
   if (items * pl.chunks > 0x7fffffff || join > 0x7fffffff)
     return set_error(FM_ERR_SHAPE, "paged_decode_attn: grid too large");
@@ -557,6 +599,6 @@ extern "C" fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_
                               : launch_decode_hd<64>(a, kv8, pl.ng, grid, s);
   if (st != FM_OK || (pl.chunks == 1 && !sums)) return st;
   if (cache->head_dim == 128)
-    return launch_kernel(decode_join_kernel<128>, dim3((unsigned)join), dim3(128), 0, s, true, a, (int)key_blocks);
-  return launch_kernel(decode_join_kernel<64>, dim3((unsigned)join), dim3(128), 0, s, true, a, (int)key_blocks);
+    return launch_kernel(decode_join_kernel<128>, dim3((unsigned)join), dim3(DJ_THREADS), 0, s, true, a, (int)key_blocks);
+  return launch_kernel(decode_join_kernel<64>, dim3((unsigned)join), dim3(DJ_THREADS), 0, s, true, a, (int)key_blocks);
 }

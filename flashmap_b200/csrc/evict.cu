@@ -22,11 +22,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int EV_THREADS = 512;
+constexpr int EV_THREADS = 1024;
 constexpr int EV_WARPS = EV_THREADS / 32;
+static_assert(EV_WARPS == 32, "a warp adds up the warps' counts");
 constexpr int EV_BINS = 2048;
-constexpr int EV_KEYS = 24576;  // keys of a slice that shared memory holds; longer slices read theirs from L2 again
-constexpr int EV_UNROLL = 8;    // rows that a thread of the moving kernel has in flight
+constexpr int EV_KEYS = 49152;  // keys of a slice that shared memory holds; longer slices read theirs from L2 again
+constexpr int EV_UNROLL = 4;    // rows that a thread of the moving kernel has in flight
 
 struct EvictArgs {
   CacheRef c;
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
   const int* table = a.c.table + (long long)r * a.c.tstride;
   const long long row0 = (long long)item * a.budget;
   auto keep = [&](int at, int i, float v) {
-    const int pg = i / a.c.page;
+    const int pg = a.c.by_page.div(i);
     int page = table[pg];
     if (page < 0 || page >= a.c.num_pages) {
       record_error(a.err, DEV_BAD_INDEX);
@@ -91,6 +92,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
   const int begin = min(len, rank * per), count = min(len, begin + per) - begin;
   const bool held = count <= EV_KEYS;
   if (held)
+#pragma unroll 8
     for (int i = tid; i < count; i += EV_THREADS) ev_keys[i] = sum_key(sums[begin + i]);
   auto key = [&](int i) { return held ? ev_keys[i] : sum_key(sums[begin + i]); };
 
@@ -114,16 +116,14 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
         if (bin >= 0 && lane == __ffs(peers) - 1) atomicAdd(&hp[bin], __popc(peers));
       }
       cluster.sync();
-      // thread t: bins 4 t .. 4 t + 3 over the cluster, and the count in all higher bins
-      int4 mine = make_int4(0, 0, 0, 0);
+      // thread t: bins 2 t and 2 t + 1 over the cluster, and the count in all higher bins
+      int2 mine = make_int2(0, 0);
       for (int q = 0; q < cs; ++q) {
-        const int4 x = reinterpret_cast<const int4*>(cluster.map_shared_rank(hp, q))[tid];
+        const int2 x = reinterpret_cast<const int2*>(cluster.map_shared_rank(hp, q))[tid];
         mine.x += x.x;
         mine.y += x.y;
-        mine.z += x.z;
-        mine.w += x.w;
       }
-      const int all = mine.x + mine.y + mine.z + mine.w;
+      const int all = mine.x + mine.y;
       int above = all;  // inclusive suffix sum over lanes
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -132,18 +132,15 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
       }
       if (lane == 0) wsum[warp] = above;
       __syncthreads();
-      for (int w = warp + 1; w < EV_WARPS; ++w) above += wsum[w];
-      above -= all;
+      const int later = __reduce_add_sync(0xffffffffu, lane > warp ? wsum[lane] : 0);
+      above += later - all;
       // the bin in which the need-th largest lies belongs to exactly one thread
-      const int c4[4] = {mine.w, mine.z, mine.y, mine.x};
-      int before = above;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (before < need && need <= before + c4[e]) {
-          s_bin = 4 * tid + 3 - e;
-          s_left = need - before;
-        }
-        before += c4[e];
+      if (above < need && need <= above + mine.y) {
+        s_bin = 2 * tid + 1;
+        s_left = need - above;
+      } else if (above + mine.y < need && need <= above + all) {
+        s_bin = 2 * tid;
+        s_left = need - above - mine.y;
       }
       __syncthreads();
       need = s_left;
@@ -177,15 +174,10 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
     wtie[warp] = ties;
   }
   __syncthreads();
-  int sb = 0, tb = 0, st = 0, tt = 0;  // before this warp, and of the slice
-  for (int w = 0; w < EV_WARPS; ++w) {
-    if (w < warp) {
-      sb += wsum[w];
-      tb += wtie[w];
-    }
-    st += wsum[w];
-    tt += wtie[w];
-  }
+  // before this warp, and of the slice
+  const int ws = wsum[lane], wt = wtie[lane];
+  int sb = __reduce_add_sync(0xffffffffu, lane < warp ? ws : 0), tb = __reduce_add_sync(0xffffffffu, lane < warp ? wt : 0);
+  const int st = __reduce_add_sync(0xffffffffu, ws), tt = __reduce_add_sync(0xffffffffu, wt);
   if (tid == 0) {
     s_total[0] = st;
     s_total[1] = tt;
@@ -218,7 +210,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
 // writes them.  No later block reads a slot below its own first one, so that
 // one meeting a block is all that is needed.
 template <bool IN_PLACE>
-__global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
+__global__ void __launch_bounds__(256, 4) evict_move_kernel(EvictArgs a) {
   pdl_wait();
   int b = blockIdx.x;
   const int slice = b % a.slices;
@@ -242,7 +234,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
     for (int u = 0; u < EV_UNROLL; ++u) {
       const int i = i0 + u * rows + mine;
       src[u] = i < end ? from[i] : make_int2(-1, 0);
-      dst[u] = i < end ? to[i / a.c.page] : 0;
+      dst[u] = i < end ? to[a.c.by_page.div(i)] : 0;
     }
   };
   look(begin);
@@ -251,7 +243,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
     uint8_t* at[EV_UNROLL];
 #pragma unroll
     for (int u = 0; u < EV_UNROLL; ++u) {
-      const int i = i0 + u * rows + mine, tok = i % a.c.page;
+      const int i = i0 + u * rows + mine, tok = i - a.c.by_page.div(i) * a.c.page;
       at[u] = nullptr;
       if (src[u].x < 0 || (IN_PLACE && src[u].x == dst[u] && src[u].y == tok)) continue;
       if (dst[u] < 0 || dst[u] >= a.c.num_pages) {
@@ -269,10 +261,10 @@ __global__ void __launch_bounds__(256) evict_move_kernel(EvictArgs a) {
   }
 }
 
-// CTAs of a cluster: as many as leave one to an SM, with 2048 positions each at least.
+// CTAs of a cluster: as many as leave one to an SM, with 8192 positions each at least.
 int evict_cluster(int64_t items, int64_t positions) {
   int cs = 1;
-  while (cs < 8 && items * cs * 2 <= 148 && positions >= 2048 * 2 * cs) cs *= 2;
+  while (cs < 8 && items * cs * 2 <= 148 && positions >= 8192 * 2 * cs) cs *= 2;
   return cs;
 }
 
@@ -350,7 +342,7 @@ extern "C" fm_status fm_paged_evict(const fm_paged_cache* cache, const fm_evict*
   a.chunk = a.budget;
   unsigned chunks = 1;
   if (a.out_table) {
-    a.chunk = 512;
+    a.chunk = 256;
     chunks = (unsigned)((a.budget + a.chunk - 1) / a.chunk);
     if (chunks > 65535) {
       a.chunk = (a.budget + 65534) / 65535;

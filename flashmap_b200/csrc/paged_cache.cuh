@@ -11,6 +11,20 @@
 
 namespace fm {
 
+// n / d for 0 <= n < 2^31 by a multiplication: with s = ceil(log2 d) and
+// m = ceil(2^(31 + s) / d), n m / 2^(31 + s) exceeds n / d by n (m d - 2^(31 + s)) /
+// (d 2^(31 + s)) < 1 / d, too little to reach the next whole number.
+struct Divider {
+  uint32_t d, m, s;
+  __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> (s - 1)); }
+};
+inline Divider make_divider(uint32_t d) {
+  Divider v{d, 0, 0};
+  while ((1ull << v.s) < d) ++v.s;
+  v.m = (uint32_t)(((1ull << (31 + v.s)) + d - 1) / d);
+  return v;
+}
+
 // Strides in bytes: a pool's offsets pass 32 bits, so every one is 64-bit.
 struct CacheRef {
   uint8_t* k;
@@ -22,6 +36,8 @@ struct CacheRef {
   const float* descales;  // (2, R, KH) or null
   int page, num_pages, max_len;
   int R, KH;
+  Divider by_page;
+  bool same;  // keys and values have the same strides: one offset serves both
 };
 
 // The length of request r, cut to what the call was sized for.
@@ -51,7 +67,9 @@ inline fm_status cache_ref(const fm_paged_cache* p, const char* who, CacheRef* c
                 p->k_page_stride * esz, p->k_head_stride * esz, p->k_token_stride * esz,
                 p->v_page_stride * esz, p->v_head_stride * esz, p->v_token_stride * esz,
                 p->page_table, p->page_table_stride, p->lengths, p->descales,
-                (int)p->page_size, (int)p->num_pages, 0, (int)p->requests, (int)p->kv_heads};
+                (int)p->page_size, (int)p->num_pages, 0, (int)p->requests, (int)p->kv_heads,
+                make_divider((uint32_t)p->page_size), false};
+  c->same = c->kps == c->vps && c->khs == c->vhs && c->kts == c->vts;
   const long long cap = p->page_table_cols > p->max_length / p->page_size ? p->max_length
                                                                            : p->page_table_cols * p->page_size;
   c->max_len = (int)(p->max_length < cap ? p->max_length : cap);
@@ -123,11 +141,17 @@ __device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uin
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// two e4m3 values (low byte first) as f16x2
-__device__ __forceinline__ uint32_t e4m3x2_h(uint32_t two) {
-  uint32_t r;
-  asm("{.reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t;}" : "=r"(r) : "r"(two));
-  return r;
+// four e4m3 values (low byte first) as two f16x2
+__device__ __forceinline__ void e4m3x4_h(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{.reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b;}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four));
+}
+// 2^x; results under 2^-126 are zero
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, bool half) {
   if (half) {

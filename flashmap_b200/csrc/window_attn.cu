@@ -147,11 +147,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // Shared memory: two row tiles of Q, a ring of K and V tiles (16-bit, 128-byte
 // swizzled in blocks of 64 columns), for e4m3 caches two tiles of raw bytes.
@@ -432,10 +427,11 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
         for (int u = 0; u < 32 / RPI; ++u) {
           const int row = u * RPI + lane / RC, r128 = lw * 32 + row;
           const uint4 x = *reinterpret_cast<const uint4*>(raw + row * HD + ch * 16);
-          const uint4 h0 = make_uint4(e4m3x2_h(x.x & 0xffffu), e4m3x2_h(x.x >> 16), e4m3x2_h(x.y & 0xffffu),
-                                      e4m3x2_h(x.y >> 16));
-          const uint4 h1 = make_uint4(e4m3x2_h(x.z & 0xffffu), e4m3x2_h(x.z >> 16), e4m3x2_h(x.w & 0xffffu),
-                                      e4m3x2_h(x.w >> 16));
+          uint4 h0, h1;
+          e4m3x4_h(x.x, h0.x, h0.y);
+          e4m3x4_h(x.y, h0.z, h0.w);
+          e4m3x4_h(x.z, h1.x, h1.y);
+          e4m3x4_h(x.w, h1.z, h1.w);
           uint8_t* drow = dst + r128 * 128;
           const int c0 = (2 * ch) & 7;
           *reinterpret_cast<uint4*>(drow + (((c0 + odd) ^ (r128 & 7)) << 4)) = odd ? h1 : h0;
@@ -459,7 +455,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
         if (j >= w.n) return -1;
         const int key = w.key0(j) + lw * 32 + lane;
         if (key > w.p_hi || !(key >= w.lo || key < a.sinks)) return -1;
-        const int pg = key / a.c.page;
+        const int pg = a.c.by_page.div(key);
         *tok = key - pg * a.c.page;
         const int page = a.c.table[trow + pg];
         if (page >= 0 && page < a.c.num_pages) return page;
