@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
     const float u = mm == -INFINITY ? 0.0f : mm;
     for (int w = 0; w < 4; ++w) {
       float2& s = mS[w * 8 * NG + threadIdx.x];
-      s.x = exp2f(s.x - u);  // from here on the warp's factor
+      s.x = ex2(s.x - u);  // from here on the warp's factor
       ll += s.y * s.x;
     }
     mR[threadIdx.x] = make_float2(mm, ll);
@@ -375,10 +375,10 @@ __device__ __forceinline__ float2 row_stats(const float2* stats, int n) {
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, off));
   const float u = mm == -INFINITY ? 0.0f : mm;
-  float ll = first.y * exp2f(first.x - u);
+  float ll = first.y * ex2(first.x - u);
   for (int c = lane + 32; c < n; c += 32) {
     const float2 s = stats[c];
-    ll += s.y * exp2f(s.x - u);
+    ll += s.y * ex2(s.x - u);
   }
 #pragma unroll
   for (int off = 16; off >= 1; off >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, off);
@@ -389,18 +389,47 @@ constexpr int DJ_THREADS = 256;
 constexpr int DJ_KEYS = 4 * DJ_THREADS;  // positions of a block that adds weights to the sums
 constexpr int DJ_HEADS = 8;              // heads whose scores a thread has in flight
 
-// Blocks [0, R H): one (request, head)'s chunks joined to its output row.
+// Blocks [0, row_blocks): (request, head) rows whose chunks are joined, one row
+// to a block, or to a warp where a row has few chunks (WARP_ROWS).
 // Blocks from there on: DJ_KEYS visible positions of one (request, kv head),
 // whose weights are added to the sums; every sum has one writer, so repeated
 // runs agree bit for bit.
-template <int HD>
-__global__ void __launch_bounds__(DJ_THREADS) decode_join_kernel(DecodeArgs a, int key_blocks) {
+template <int HD, bool WARP_ROWS>
+__global__ void __launch_bounds__(DJ_THREADS) decode_join_kernel(DecodeArgs a, int row_blocks, int key_blocks) {
   __shared__ float4 sred[DJ_THREADS / 32][HD / 4];
   __shared__ float2 sst[DJ_HEADS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = a.c.R * a.H;
   pdl_wait();
-  if ((int)blockIdx.x < rows) {
+  if (WARP_ROWS && (int)blockIdx.x < row_blocks) {
+    const int row = blockIdx.x * (DJ_THREADS / 32) + warp, r = row / a.H, h = row % a.H;
+    if (row >= rows) return;
+    const Span sp = visible_span(cache_length(a.c, r, a.err, false), a.window, a.sinks);
+    const int n = (sp.n + a.chunk - 1) / a.chunk;
+    if (n <= 1) return;  // written by its only chunk
+    const float2* stats = a.stats + (long long)row * a.chunks;
+    const float* part = a.part + (long long)row * a.chunks * HD + lane * (HD / 32);
+    float o[HD / 32] = {};
+    const float2 st = row_stats(stats, n);
+#pragma unroll 4
+    for (int c = 0; c < n; ++c) {
+      float x[HD / 32];
+      if constexpr (HD == 128)
+        *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(part + (long long)c * HD);
+      else
+        *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(part + (long long)c * HD);
+      const float f = ex2(stats[c].x - st.x);
+#pragma unroll
+      for (int e = 0; e < HD / 32; ++e) o[e] += x[e] * f;
+    }
+    const float inv = st.y == 0.0f ? 0.0f : 1.0f / st.y;
+    __nv_bfloat16* out = a.out + (long long)r * a.o_rs + (long long)h * a.o_hs + lane * (HD / 32);
+#pragma unroll
+    for (int e = 0; e < HD / 32; e += 2)
+      *reinterpret_cast<uint32_t*>(out + e) = pack16(o[e] * inv, o[e + 1] * inv, false);
+    return;
+  }
+  if (!WARP_ROWS && (int)blockIdx.x < row_blocks) {
     const int row = blockIdx.x, r = row / a.H, h = row % a.H;
     const Span sp = visible_span(cache_length(a.c, r, a.err, false), a.window, a.sinks);
     const int n = (sp.n + a.chunk - 1) / a.chunk;
@@ -413,7 +442,7 @@ __global__ void __launch_bounds__(DJ_THREADS) decode_join_kernel(DecodeArgs a, i
 #pragma unroll 4
     for (int c = tid / V; c < n; c += PER) {
       const float4 x = part[(long long)c * V];
-      const float f = exp2f(stats[c].x - st.x);
+      const float f = ex2(stats[c].x - st.x);
       acc.x += x.x * f;
       acc.y += x.y * f;
       acc.z += x.z * f;
@@ -443,7 +472,7 @@ __global__ void __launch_bounds__(DJ_THREADS) decode_join_kernel(DecodeArgs a, i
     }
     return;
   }
-  const int item = (blockIdx.x - rows) / key_blocks, kb = (blockIdx.x - rows) % key_blocks;
+  const int item = (blockIdx.x - row_blocks) / key_blocks, kb = (blockIdx.x - row_blocks) % key_blocks;
   const int r = item / a.c.KH, c = item % a.c.KH;
   const Span sp = visible_span(cache_length(a.c, r, a.err, false), a.window, a.sinks);
   const int begin = kb * DJ_KEYS;
@@ -470,10 +499,10 @@ __global__ void __launch_bounds__(DJ_THREADS) decode_join_kernel(DecodeArgs a, i
     for (int g = 0; g < DJ_HEADS; ++g)
       if (g0 + g < a.G && i < sp.n) {
         const float2 st = sst[g];
-        add.x += exp2f(s[g].x - st.x) * st.y;
-        add.y += exp2f(s[g].y - st.x) * st.y;
-        add.z += exp2f(s[g].z - st.x) * st.y;
-        add.w += exp2f(s[g].w - st.x) * st.y;
+        add.x += ex2(s[g].x - st.x) * st.y;
+        add.y += ex2(s[g].y - st.x) * st.y;
+        add.z += ex2(s[g].z - st.x) * st.y;
+        add.w += ex2(s[g].w - st.x) * st.y;
       }
     __syncthreads();
   }
@@ -489,8 +518,10 @@ struct DecodePlan {
   size_t part, stats, scores, total;
 };
 
-// The visible positions a request can have at most, cut so that the launch has
-// about eight chunks per SM where there are that many positions.
+// Chunks of equal length, so many that the launch has DA_CTAS CTAs when every
+// request is as long as the longest may be, of DA_TILE keys to a warp at least.
+constexpr int DA_CTAS = 148 * 12;
+
 DecodePlan decode_plan(int64_t R, int64_t H, int64_t KH, int64_t HD, int64_t max_len, int64_t window, bool sums,
                        int64_t sinks) {
   DecodePlan p{};
@@ -498,9 +529,9 @@ DecodePlan decode_plan(int64_t R, int64_t H, int64_t KH, int64_t HD, int64_t max
   p.ng = G > 8 ? 2 : 1;
   p.hgroups = (int)((G + 8 * p.ng - 1) / (8 * p.ng));
   const int64_t span = visible_span((int)max_len, (int)window, (int)sinks).n;
-  const int64_t units = R * KH * p.hgroups * span;
-  int64_t chunk = (units / (148 * 8) + 63) / 64 * 64;
-  chunk = chunk < 64 ? 64 : chunk > 1024 ? 1024 : chunk;
+  const int64_t items = R * KH * p.hgroups, cut = (DA_CTAS + items - 1) / items;
+  int64_t chunk = ((span + cut - 1) / cut + 63) / 64 * 64;
+  if (chunk < 64) chunk = 64;
   p.chunk = (int)chunk;
   p.chunks = (int)((span + chunk - 1) / chunk);
   if (p.chunks < 1) p.chunks = 1;
@@ -589,7 +620,11 @@ extern "C" fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_
   a.err = p->err;
   const int64_t items = cache->requests * cache->kv_heads * pl.hgroups;
   const int64_t key_blocks = sums ? (pl.pitch + DJ_KEYS - 1) / DJ_KEYS : 0;
-  const int64_t join = cache->requests * (p->heads + cache->kv_heads * key_blocks);
+  // a warp to a row where that leaves no warp more than 16 chunks
+  const bool warp_rows = pl.chunks <= 16;
+  const int64_t per = warp_rows ? DJ_THREADS / 32 : 1;
+  const int64_t row_blocks = pl.chunks > 1 ? (cache->requests * p->heads + per - 1) / per : 0;
+  const int64_t join = row_blocks + cache->requests * cache->kv_heads * key_blocks;
   if (items * pl.chunks > 0x7fffffff || join > 0x7fffffff)
     return set_error(FM_ERR_SHAPE, "paged_decode_attn: grid too large");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -598,7 +633,11 @@ extern "C" fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_
   st = cache->head_dim == 128 ? launch_decode_hd<128>(a, kv8, pl.ng, grid, s)
                               : launch_decode_hd<64>(a, kv8, pl.ng, grid, s);
   if (st != FM_OK || (pl.chunks == 1 && !sums)) return st;
+  const dim3 grid2((unsigned)join), block(DJ_THREADS);
+  auto join_launch = [&](auto kernel) {
+    return launch_kernel(kernel, grid2, block, 0, s, true, a, (int)row_blocks, (int)key_blocks);
+  };
   if (cache->head_dim == 128)
-    return launch_kernel(decode_join_kernel<128>, dim3((unsigned)join), dim3(DJ_THREADS), 0, s, true, a, (int)key_blocks);
-  return launch_kernel(decode_join_kernel<64>, dim3((unsigned)join), dim3(DJ_THREADS), 0, s, true, a, (int)key_blocks);
+    return warp_rows ? join_launch(decode_join_kernel<128, true>) : join_launch(decode_join_kernel<128, false>);
+  return warp_rows ? join_launch(decode_join_kernel<64, true>) : join_launch(decode_join_kernel<64, false>);
 }
