@@ -14,45 +14,77 @@ namespace {
 constexpr int WA_ROWS = 256;  // (token, head of the group) rows of a CTA, in two tiles
 constexpr int WA_KEYS = 128;  // keys of a tile
 
+// What a CTA says of the items that are cut at the ends of its share.
+enum { WA_NONE = 0, WA_MORE = 1, WA_LAST = 2, WA_EMPTY = 3 };
+struct WaCutItem {
+  int starts;              // its last item goes on in the next CTA: slot 2 b + 1
+  int q0, row0, rows, c;   // which item that is
+  int goes_on;             // its first item began before (slot 2 b): WA_MORE also goes on after, WA_LAST ends here
+};
+
 struct WindowArgs {
   CacheRef c;
   const uint8_t* q;  // bf16
   long long q_ts, q_hs;
   const int* cu;
   int T, H, G;
+  Divider by_g;
   float scale;  // softmax_scale * log2(e)
   int window, sinks;
   __nv_bfloat16* out;
   long long o_ts, o_hs;
-  int tiles, splits;
-  float* part;    // [splits][T][H][HD] unnormalised outputs, when splits > 1
-  float2* stats;  // [splits][T][H] (maximum, sum), base-2 scores
+  float* part;    // [2 CTAs][256][HD] outputs of items that are cut, not yet divided by their sums
+  float2* stats;  // [2 CTAs][256] (maximum, sum), base-2 scores
+  WaCutItem* cuts;  // [CTAs]
   int* err;
 };
 
-// Row tile `tile` of the flattened batch: request and its tile, or request -1.
-// Request r has ceil(n_r G / ROWS) tiles; the search runs by one warp.
-__device__ __forceinline__ int2 find_tile(const int* cu, int R, int G, int rows, int tile) {
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int r0 = 0; r0 < R; r0 += 32) {
-    const int r = r0 + lane;
-    int n = r < R ? (int)(((long long)max(0, cu[r + 1] - cu[r]) * G + rows - 1) / rows) : 0;
-    int scan = n;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, scan, off);
-      if (lane >= off) scan += v;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + scan > tile);
-    if (hit) {
-      const int w = __ffs(hit) - 1;
-      const int first = __shfl_sync(0xffffffffu, before + scan - n, w);
-      return make_int2(r0 + w, tile - first);
-    }
-    before += __shfl_sync(0xffffffffu, scan, 31);
-  }
-  return make_int2(-1, 0);
+// The key tiles that rows row0 .. of request r see: those of the first tokens,
+// then those from the first row's window on.
+struct WaKeys {
+  int pos0, p_hi, lo;       // position of the request's first row, of the last row here; first key of the window
+  int t_head, t_lo, tiles;  // tiles 0 .. t_head - 1, then t_lo on
+};
+__device__ __forceinline__ WaKeys wa_keys(const WindowArgs& a, int len, int nq, int row0) {
+  WaKeys k;
+  const int rows = min(WA_ROWS, nq * a.G - row0);
+  k.pos0 = len - nq;  // negative: the first rows see nothing
+  k.p_hi = k.pos0 + a.by_g.div(row0 + rows - 1);
+  k.lo = a.window > 0 ? max(0, k.pos0 + a.by_g.div(row0) - a.window + 1) : 0;
+  const int t_end = k.p_hi < 0 ? 0 : k.p_hi / WA_KEYS + 1;
+  k.t_lo = k.lo / WA_KEYS;
+  k.t_head = min((min(a.sinks, k.lo) + WA_KEYS - 1) / WA_KEYS, k.t_lo);
+  k.tiles = max(0, k.t_head + t_end - k.t_lo);
+  return k;
+}
+// Query rows of request r; 0 where its bounds make no sense.
+__device__ __forceinline__ int wa_queries(const WindowArgs& a, int r, bool report) {
+  const int q0 = a.cu[r], nq = a.cu[r + 1] - q0;
+  if (q0 >= 0 && nq >= 0 && nq <= a.T - q0) return nq;
+  if (report) record_error(a.err, DEV_BAD_INDEX);
+  return 0;
+}
+__device__ __forceinline__ int wa_row_tiles(const WindowArgs& a, int nq) {
+  return (int)(((long long)nq * a.G + WA_ROWS - 1) / WA_ROWS);
+}
+
+// Work is dealt out by key tiles: the items (row tile by row tile, kv head by
+// kv head) lie end to end, each as long as its key tiles plus WA_ITEM for what
+// an item costs besides, and every CTA takes an equal length.  An item that
+// lies across a border is cut there and joined by window_join_kernel, unless
+// less than WA_CUT tiles would be cut off.
+constexpr int WA_ITEM = 5;
+constexpr int WA_CUT = 3;
+constexpr int WA_SHARE = WA_ITEM + 4;  // the least length of a CTA's share
+struct WaBorder {
+  int r, y, c, t;  // request, row tile, kv head, and the first tile after the border
+};
+// Where a border `o` into an item of n tiles (one, if it has none) cuts it.
+__device__ __forceinline__ int wa_cut(int o, int n) {
+  if (o <= 0) return 0;
+  const int t = o - WA_ITEM;
+  if (n < 2 * WA_CUT) return o < (n + WA_ITEM + 1) / 2 ? 0 : n;
+  return t < WA_CUT ? 0 : t > n - WA_CUT ? n : t;
 }
 
 // ----------------------------------------------------------------- tensor memory
@@ -163,7 +195,8 @@ struct WaLayout {
 
 // One unit of work: 256 rows of a request and kv head, and a range of key tiles.
 struct WaItem {
-  int r, c, split;  // r < 0: no more work
+  int r, c;         // r < 0: no more work
+  int slot;         // where its output goes if it is cut, or -1
   int q0;           // the request's first query row
   int row0, rows;   // rows row0 .. row0 + rows - 1 of its nq G
   int pos0;         // position of its first query row
@@ -178,7 +211,9 @@ struct WaItem {
   __device__ __forceinline__ int mt() const { return rows > 128 ? 2 : 1; }
 };
 
-constexpr int WA_ITEMS = 4;  // ring of work items
+constexpr int WA_ITEMS = 4;              // ring of work items
+constexpr int WA_REQUESTS = 16384;       // requests of a call
+constexpr int WA_ROW_TILES = 4096 * 512;  // row tiles of a call
 
 struct WaCtrl {
   uint64_t full[8], empty[8];
@@ -189,9 +224,11 @@ struct WaCtrl {
   alignas(16) uint32_t valid[8][4];  // keys of tile j (mod 8) whose page exists
   float qinv[2][256];                // e4m3: what a row's query was multiplied with, inverted (items in turn)
   WaItem item[WA_ITEMS];
+  WaBorder border[2];
+  long long scan[17];
 };
 
-// 16 warps, persistent over work items, heaviest first: two warpgroups of
+// 16 warps, persistent over work items: two warpgroups of
 // softmax (one to a row tile of 128), one that loads keys and values, and one
 // whose warps issue the products (12), hand out work items and load queries
 // (13 to 15).  S = Q K^T goes to tensor memory; the softmax threads (one to a
@@ -245,6 +282,90 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem, 0);
 
+  // ------------------------------------------------------------- this CTA's share
+  // sum over the CTA of the values before this thread's, and of all
+  auto scan = [&](long long v, long long* all) {
+    long long x = v;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, off);
+      if (lane >= off) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) ctl->scan[warp] = x;
+    __syncthreads();
+    long long before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+      const long long y = ctl->scan[w];
+      before += w < warp ? y : 0;
+      sum += y;
+    }
+    *all = sum;
+    return before + x - v;
+  };
+  {
+    int* pre = reinterpret_cast<int*>(sKV);                                // row tiles before request r
+    long long* chunk = reinterpret_cast<long long*>(sKV + WA_REQUESTS * 4);  // length of 512 row tiles
+    long long row_tiles = 0;
+    for (int r0 = 0; r0 < a.c.R; r0 += 512) {
+      const int r = r0 + tid;
+      const int m = r < a.c.R ? wa_row_tiles(a, wa_queries(a, r, blockIdx.x == 0)) : 0;
+      long long all;
+      const long long before = scan(m, &all);
+      if (r < a.c.R) pre[r] = (int)(row_tiles + before);
+      row_tiles += all;
+    }
+    __syncthreads();
+    auto tiles_of = [&](int idx, int* req, int* y) {  // key tiles of row tile idx (one, if it has none)
+      int lo = 0, hi = a.c.R - 1;                     // the last request with pre[r] <= idx has it
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (pre[mid] <= idx)
+          lo = mid;
+        else
+          hi = mid - 1;
+      }
+      *req = lo;
+      *y = idx - pre[lo];
+      return max(1, wa_keys(a, cache_length(a.c, lo, a.err, false), a.cu[lo + 1] - a.cu[lo], *y * WA_ROWS).tiles);
+    };
+    long long total = 0, before = 0;
+    int r = 0, y = 0, n = 0;  // this thread's row tile of the newest 512
+    for (int i0 = 0; i0 < row_tiles; i0 += 512) {
+      n = i0 + tid < row_tiles ? tiles_of(i0 + tid, &r, &y) : 0;
+      long long all;
+      before = scan(n ? n + WA_ITEM : 0, &all);
+      if (tid == 0) chunk[i0 >> 9] = all;
+      total += all;
+    }
+    total *= a.c.KH;
+    const int shares = (int)min((long long)gridDim.x, (total + WA_SHARE - 1) / WA_SHARE);
+    if (tid < 2) ctl->border[tid] = WaBorder{a.c.R, 0, 0, 0};
+    __syncthreads();
+    for (int e = 0; e < 2; ++e) {
+      const int b = blockIdx.x + e;
+      const long long x = b >= shares ? total : total * b / shares;
+      if (x >= total) continue;
+      int i0 = 0;
+      long long at = 0;
+      if (row_tiles > 512) {
+        while (at + chunk[i0] * a.c.KH <= x) at += chunk[i0++] * a.c.KH;
+        i0 <<= 9;
+        n = i0 + tid < row_tiles ? tiles_of(i0 + tid, &r, &y) : 0;
+        long long all;
+        before = scan(n ? n + WA_ITEM : 0, &all);
+      }
+      const long long into = x - at - before * a.c.KH;
+      const int w = n + WA_ITEM;
+      if (n && into >= 0 && into < (long long)w * a.c.KH) {
+        const int c = (int)(into / w);
+        ctl->border[e] = WaBorder{r, y, c, wa_cut((int)(into - (long long)c * w), n)};
+      }
+    }
+    __syncthreads();
+  }
+
   // item k of this CTA; r < 0 after the last, or when a wait ran out
   auto take = [&](int k) {
     WaItem w;
@@ -273,13 +394,13 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       if (w.r < 0) break;
       const int lr = i * 128 + (tid & 127), row = w.row0 + lr;
       const bool live = lr < w.rows;
-      const int tok = w.q0 + (live ? row / a.G : 0), h = w.c * a.G + (live ? row % a.G : 0);
-      __nv_bfloat16* out = a.out + (long long)tok * a.o_ts + (long long)h * a.o_hs;
-      const long long prow = ((long long)w.split * a.T + tok) * a.H + h;
+      auto out_row = [&](int at) {
+        const int tok = a.by_g.div(at);
+        return a.out + (long long)(w.q0 + tok) * a.o_ts + (long long)(w.c * a.G + at - tok * a.G) * a.o_hs;
+      };
       if (w.n <= 0) {  // nothing is seen
-        if (live && a.splits == 1)
-          for (int e = 0; e < CPR; ++e) reinterpret_cast<uint4*>(out)[e] = make_uint4(0, 0, 0, 0);
-        if (live && a.splits > 1) a.stats[prow] = make_float2(-INFINITY, 0.0f);
+        if (live)
+          for (int e = 0; e < CPR; ++e) reinterpret_cast<uint4*>(out_row(row))[e] = make_uint4(0, 0, 0, 0);
         continue;
       }
       const int tile0 = tiles, par = worked & 1;
@@ -287,7 +408,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       ++worked;
       if (i >= w.mt()) continue;
       // sees keys up to p (a row past the end stands where the last one does, and is not written),
-      const int p = w.pos0 + (live ? row : w.row0 + w.rows - 1) / a.G;
+      const int p = w.pos0 + a.by_g.div(live ? row : w.row0 + w.rows - 1);
       const int wlo = a.window > 0 ? p - a.window + 1 : 0;  // from wlo on or below sinks
       // |scale| goes with the scores, its sign (or a zero) with the queries
       float sc = w.scale == 0.0f ? 1.0f : fabsf(w.scale);
@@ -377,28 +498,57 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       tmem_wait_ld();
       tc_fence_before();
       mbar_arrive(&ctl->o_empty[i]);  // the next item's product may overwrite it
-      if (!live) continue;
       // no score above -inf: zero; a score that is no number: nor is the row
-      if (m == -INFINITY) l = 0.0f;
+      if (m == -INFINITY) {
+        l = 0.0f;
+#pragma unroll
+        for (int e = 0; e < HD; ++e) o[e] = 0.0f;
+      }
       if (nan) l = NAN;
-      if (a.splits == 1) {
+      if (w.slot < 0) {
         const float inv = l == 0.0f ? 0.0f : w.vd / l;
+        // Four lanes hand one another 16-byte pieces, so that they write 64
+        // consecutive bytes of one row at a time instead of 16 of four rows.
+        uint4 x[CPR];
 #pragma unroll
-        for (int e = 0; e < HD; e += 8) {
-          uint4 x;
-          x.x = pack16(o[e] * inv, o[e + 1] * inv, false);
-          x.y = pack16(o[e + 2] * inv, o[e + 3] * inv, false);
-          x.z = pack16(o[e + 4] * inv, o[e + 5] * inv, false);
-          x.w = pack16(o[e + 6] * inv, o[e + 7] * inv, false);
-          *reinterpret_cast<uint4*>(out + e) = x;
+        for (int e = 0; e < CPR; ++e) {
+          x[e].x = pack16(o[8 * e] * inv, o[8 * e + 1] * inv, false);
+          x[e].y = pack16(o[8 * e + 2] * inv, o[8 * e + 3] * inv, false);
+          x[e].z = pack16(o[8 * e + 4] * inv, o[8 * e + 5] * inv, false);
+          x[e].w = pack16(o[8 * e + 6] * inv, o[8 * e + 7] * inv, false);
         }
-      } else {
-        a.stats[prow] = make_float2(m, l);
-        float* part = a.part + prow * HD;
+        auto trade = [&](uint4& lo, uint4& hi, int bit) {  // the lane with the bit gives lo, the one without hi
+          const bool up = lane & bit;
+          const uint4 give = up ? lo : hi;
+          uint4 got;
+          got.x = __shfl_xor_sync(0xffffffffu, give.x, bit);
+          got.y = __shfl_xor_sync(0xffffffffu, give.y, bit);
+          got.z = __shfl_xor_sync(0xffffffffu, give.z, bit);
+          got.w = __shfl_xor_sync(0xffffffffu, give.w, bit);
+          (up ? lo : hi) = got;
+        };
 #pragma unroll
-        for (int e = 0; e < HD; e += 4)
-          *reinterpret_cast<float4*>(part + e) =
-              make_float4(o[e] * w.vd, o[e + 1] * w.vd, o[e + 2] * w.vd, o[e + 3] * w.vd);
+        for (int e = 0; e < CPR; e += 4) {
+          trade(x[e], x[e + 1], 1);
+          trade(x[e + 2], x[e + 3], 1);
+          trade(x[e], x[e + 2], 2);
+          trade(x[e + 1], x[e + 3], 2);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {  // x[e + u] is piece e + lane % 4 of row u of the four
+          const int at = (lr & ~3) + u;
+          if (at >= w.rows) continue;
+          uint4* dst = reinterpret_cast<uint4*>(out_row(w.row0 + at)) + (lane & 3);
+#pragma unroll
+          for (int e = 0; e < CPR; e += 4) dst[e] = x[e + u];
+        }
+      } else {  // piece by piece of four columns, rows side by side
+        a.stats[w.slot * WA_ROWS + lr] = make_float2(m, l);
+        float4* part = reinterpret_cast<float4*>(a.part) + (long long)w.slot * WA_ROWS * (HD / 4) + lr;
+#pragma unroll
+        for (int e = 0; e < HD / 4; ++e)
+          part[e * WA_ROWS] =
+              make_float4(o[4 * e] * w.vd, o[4 * e + 1] * w.vd, o[4 * e + 2] * w.vd, o[4 * e + 3] * w.vd);
       }
     }
   } else if (warp < 12) {
@@ -626,8 +776,9 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       }
     } else {
       // ------------------------------------------------------------- work items and queries
-      const int total = a.tiles * a.c.KH * a.splits;
-      int id = blockIdx.x;
+      WaBorder cur = ctl->border[0];
+      const WaBorder end = ctl->border[1];
+      WaCutItem cut{0, 0, 0, 0, 0, WA_NONE};
       uint32_t q_phase = 1;
       int worked = 0;
       bool ok = true;
@@ -635,40 +786,51 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
         WaItem w;
         if (warp == 13) {
           w.r = -1;
-          for (; id < total && w.r < 0; id += gridDim.x) {
-            const int bid = id / a.splits;
-            w.split = id % a.splits;
-            w.c = bid % a.c.KH;
-            // the row tile, the latest rows (those with the most keys) first
-            const int2 at = find_tile(a.cu, a.c.R, a.G, WA_ROWS, a.tiles - 1 - bid / a.c.KH);
-            if (at.x < 0) continue;
-            const int q0 = a.cu[at.x], nq = a.cu[at.x + 1] - q0;
-            const int len = cache_length(a.c, at.x, a.err, lane == 0);
-            if (q0 < 0 || nq < 0 || q0 + nq > a.T) {
-              if (lane == 0) record_error(a.err, DEV_BAD_INDEX);
+          while (w.r < 0 && cur.r < a.c.R) {
+            const int nq = wa_queries(a, cur.r, false), row0 = cur.y * WA_ROWS;
+            if (cur.y >= wa_row_tiles(a, nq)) {
+              cur = WaBorder{cur.r + 1, 0, 0, 0};
               continue;
             }
-            w.r = at.x;
-            w.q0 = q0;
-            w.row0 = at.y * WA_ROWS;
-            w.rows = min(WA_ROWS, nq * a.G - w.row0);
-            w.pos0 = len - nq;  // negative: the first rows see nothing
-            w.p_hi = w.pos0 + (w.row0 + w.rows - 1) / a.G;
-            // key tiles: those of the first tokens, then those from the first row's window on
-            w.lo = a.window > 0 ? max(0, w.pos0 + w.row0 / a.G - a.window + 1) : 0;
-            const int t_end = w.p_hi < 0 ? 0 : w.p_hi / WA_KEYS + 1;
-            w.t_lo = w.lo / WA_KEYS;
-            w.t_head = min((min(a.sinks, w.lo) + WA_KEYS - 1) / WA_KEYS, w.t_lo);
-            const int tiles = max(0, w.t_head + t_end - w.t_lo);
-            w.t_first = (int)((long long)tiles * w.split / a.splits);
-            w.n = (int)((long long)tiles * (w.split + 1) / a.splits) - w.t_first;
-            w.scale = a.scale;
-            w.vd = 1.0f;
-            if (a.c.descales) {
-              w.scale *= a.c.descales[(long long)w.r * a.c.KH + w.c];
-              w.vd = a.c.descales[(long long)(a.c.R + w.r) * a.c.KH + w.c];
+            const int len = cache_length(a.c, cur.r, a.err, lane == 0);
+            const WaKeys keys = wa_keys(a, len, nq, row0);
+            const int tiles = max(1, keys.tiles);
+            const bool last = cur.r == end.r && cur.y == end.y && cur.c == end.c;
+            const int t1 = last ? end.t : tiles;
+            if (cur.t < t1) {
+              w.r = cur.r;
+              w.c = cur.c;
+              w.q0 = a.cu[cur.r];
+              w.row0 = row0;
+              w.rows = min(WA_ROWS, nq * a.G - row0);
+              w.pos0 = keys.pos0;
+              w.p_hi = keys.p_hi;
+              w.lo = keys.lo;
+              w.t_first = cur.t;
+              w.t_head = keys.t_head;
+              w.t_lo = keys.t_lo;
+              w.n = keys.tiles ? t1 - cur.t : 0;
+              w.slot = cur.t > 0 ? 2 * (int)blockIdx.x : t1 < tiles ? 2 * (int)blockIdx.x + 1 : -1;
+              w.scale = a.scale;
+              w.vd = 1.0f;
+              if (a.c.descales) {
+                w.scale *= a.c.descales[(long long)w.r * a.c.KH + w.c];
+                w.vd = a.c.descales[(long long)(a.c.R + w.r) * a.c.KH + w.c];
+              }
+              if (cur.t > 0) cut.goes_on = t1 < tiles ? WA_MORE : WA_LAST;
+              if (cur.t == 0 && t1 < tiles) cut = WaCutItem{1, w.q0, w.row0, w.rows, w.c, cut.goes_on};
+            } else if (cur.t > 0 && cur.t < tiles) {
+              cut.goes_on = WA_EMPTY;
+            }
+            cur.t = 0;
+            if (last) {
+              cur.r = a.c.R;
+            } else if (++cur.c == a.c.KH) {
+              cur.c = 0;
+              ++cur.y;
             }
           }
+          if (w.r < 0 && lane == 0) a.cuts[blockIdx.x] = cut;
           if (!mbar_wait(&ctl->item_empty[k % WA_ITEMS], ((k / WA_ITEMS) & 1) ^ 1, abort)) {
             *abort = 1;
             record_error(a.err, DEV_TIMEOUT_OTHER);
@@ -693,13 +855,12 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
         constexpr int RPI = 32 / CPR;  // rows of a warp at a time
         const int ch = lane % CPR, rows = w.mt() * 128;
         auto chunk = [&](int lr) { return sQ + (lr >> 7) * TILE + (ch >> 3) * 16384 + (lr & 127) * 128 + (((ch & 7) ^ (lr & 7)) << 4); };
+        const uint8_t* qbase = a.q + 2 * ((long long)w.q0 * a.q_ts + (long long)w.c * a.G * a.q_hs + ch * 8);
+#pragma unroll 4
         for (int lr = (warp - 13) * RPI + lane / CPR; lr < rows; lr += 3 * RPI) {
           const bool live = lr < w.rows;
-          const int row = w.row0 + (live ? lr : 0);
-          pc_cp_async16(smem_u32(chunk(lr)),
-                        a.q + 2 * ((long long)(w.q0 + row / a.G) * a.q_ts +
-                                   (long long)(w.c * a.G + row % a.G) * a.q_hs + ch * 8),
-                        live ? 16u : 0u);
+          const int row = w.row0 + (live ? lr : 0), tok = a.by_g.div(row);
+          pc_cp_async16(smem_u32(chunk(lr)), qbase + 2 * (tok * a.q_ts + (row - tok * a.G) * a.q_hs), live ? 16u : 0u);
         }
         pc_cp_commit();
         pc_cp_wait<0>();
@@ -739,70 +900,79 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
   }
 }
 
-// A row's splits joined, one warp to a row (token, head).
+// Rows of items that were cut: block (b, y) joins columns 16 y .. 16 y + 15 of
+// the item that CTA b began and left to the next ones, one thread to a row.
 template <int HD>
-__global__ void __launch_bounds__(128) window_join_kernel(WindowArgs a) {
+__global__ void __launch_bounds__(WA_ROWS) window_join_kernel(WindowArgs a, int ctas) {
   pdl_wait();
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5), rows = (long long)a.T * a.H;
-  const int lane = threadIdx.x & 31;
-  if (row >= rows) return;
-  float top = -INFINITY;
-  for (int z = 0; z < a.splits; ++z) top = fmaxf(top, a.stats[z * rows + row].x);
-  const float u = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f, o[HD / 32];
+  const int b = blockIdx.x, lr = threadIdx.x;
+  const WaCutItem cut = a.cuts[b];
+  if (!cut.starts || lr >= cut.rows) return;
+  float top = -INFINITY, sum = 0.0f;
+  float4 o[4] = {};
+  auto add = [&](int slot) {
+    const float2 st = a.stats[slot * WA_ROWS + lr];
+    const float4* part = reinterpret_cast<const float4*>(a.part) + (long long)slot * WA_ROWS * (HD / 4) + lr;
+    const float m = fmaxf(top, st.x), u = m == -INFINITY ? 0.0f : m, f = ex2(top - u), g = ex2(st.x - u);
+    sum = sum * f + st.y * g;
 #pragma unroll
-  for (int e = 0; e < HD / 32; ++e) o[e] = 0.0f;
-  for (int z = 0; z < a.splits; ++z) {
-    const float2 st = a.stats[z * rows + row];
-    if (st.x == -INFINITY && st.y == 0.0f) continue;  // saw nothing: its output was not written
-    const float f = ex2(st.x - u);
-    sum += st.y * f;
-#pragma unroll
-    for (int e = 0; e < HD / 32; ++e) o[e] += a.part[(z * rows + row) * HD + lane * (HD / 32) + e] * f;
+    for (int e = 0; e < 4; ++e) {
+      const float4 x = part[(blockIdx.y * 4 + e) * WA_ROWS];
+      o[e] = make_float4(o[e].x * f + x.x * g, o[e].y * f + x.y * g, o[e].z * f + x.z * g, o[e].w * f + x.w * g);
+    }
+    top = m;
+  };
+  add(2 * b + 1);
+  for (int q = b + 1; q < ctas; ++q) {
+    const int goes_on = a.cuts[q].goes_on;
+    if (goes_on != WA_EMPTY) add(2 * q);
+    if (goes_on == WA_LAST) break;
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  __nv_bfloat16* out = a.out + (row / a.H) * a.o_ts + (row % a.H) * a.o_hs + lane * (HD / 32);
+  const int row = cut.row0 + lr, tok = a.by_g.div(row);
+  uint4* out = reinterpret_cast<uint4*>(a.out + (long long)(cut.q0 + tok) * a.o_ts +
+                                        (long long)(cut.c * a.G + row - tok * a.G) * a.o_hs + blockIdx.y * 16);
 #pragma unroll
-  for (int e = 0; e < HD / 32; e += 2) *reinterpret_cast<uint32_t*>(out + e) = pack16(o[e] * inv, o[e + 1] * inv, false);
+  for (int e = 0; e < 2; ++e)
+    out[e] = make_uint4(pack16(o[2 * e].x * inv, o[2 * e].y * inv, false), pack16(o[2 * e].z * inv, o[2 * e].w * inv, false),
+                        pack16(o[2 * e + 1].x * inv, o[2 * e + 1].y * inv, false),
+                        pack16(o[2 * e + 1].z * inv, o[2 * e + 1].w * inv, false));
 }
 
 struct WindowPlan {
-  int64_t tiles;
-  int splits;
-  size_t part, total;
+  int ctas;
+  bool cuts;  // whether an item can be long enough to be cut
+  size_t part, stats, total;
 };
-// Row tiles (every request ends in one of its own at most), and the splits of
-// their keys: as many as give two CTAs to an SM, of 512 keys at least.
 WindowPlan window_plan(int64_t R, int64_t T, int64_t H, int64_t KH, int64_t HD, int64_t max_q, int64_t max_len,
                        int64_t window, int64_t sinks) {
   WindowPlan p{};
-  p.tiles = (T * (H / KH) + WA_ROWS - 1) / WA_ROWS + R;
+  const int64_t items = (T * (H / KH) / WA_ROWS + R) * KH, sms = num_sms();
   int64_t span = max_len;
-  if (window > 0 && window + max_q + sinks < span) span = window + max_q + sinks;
-  const int64_t want = (2 * 148 + p.tiles * KH - 1) / (p.tiles * KH), most = span / 512;
-  p.splits = (int)(want < most ? want : most);
-  if (p.splits < 1) p.splits = 1;
-  if (p.splits > 1) {
-    p.part = (size_t)p.splits * T * H * HD * 4;
-    p.total = p.part + (size_t)p.splits * T * H * 8;
-  }
+  const int64_t tokens = max_q < WA_ROWS ? max_q : WA_ROWS;
+  if (window > 0 && window + tokens + sinks < span) span = window + tokens + sinks;
+  const int64_t tiles = span / WA_KEYS + 3;
+  p.cuts = tiles >= 2 * WA_CUT;
+  // an item that can be cut gives work to as many CTAs as it has tiles at most
+  const int64_t most = p.cuts ? items * tiles : items;
+  p.ctas = (int)(most < sms ? most : sms);
+  p.part = p.cuts ? (size_t)p.ctas * 2 * WA_ROWS * HD * 4 : 0;
+  p.stats = p.cuts ? (size_t)p.ctas * 2 * WA_ROWS * 8 : 0;
+  p.total = p.part + p.stats + (size_t)p.ctas * sizeof(WaCutItem);
   return p;
 }
 
 template <int HD, bool KV8>
-fm_status launch_window(const WindowArgs& a, cudaStream_t s) {
+fm_status launch_window(const WindowArgs& a, const WindowPlan& pl, cudaStream_t s) {
   constexpr int smem = WaLayout<HD, KV8>::SMEM;
   static_assert(sizeof(WaCtrl) <= 3072 && smem <= 232448, "shared memory");
   fm_status st = check_cuda(
       cudaFuncSetAttribute(window_attn_kernel<HD, KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
       "paged_window_attn");
   if (st != FM_OK) return st;
-  const int items = a.tiles * a.c.KH * a.splits, sms = num_sms();
-  st = launch_kernel(window_attn_kernel<HD, KV8>, dim3((unsigned)(items < sms ? items : sms)), dim3(512), smem, s, false,
-                     a);
-  if (st != FM_OK || a.splits == 1) return st;
-  return launch_kernel(window_join_kernel<HD>, dim3((unsigned)(((long long)a.T * a.H + 3) / 4)), dim3(128), 0, s, true,
-                       a);
+  st = launch_kernel(window_attn_kernel<HD, KV8>, dim3((unsigned)pl.ctas), dim3(512), smem, s, false, a);
+  if (st != FM_OK || !pl.cuts) return st;
+  return launch_kernel(window_join_kernel<HD>, dim3((unsigned)pl.ctas, HD / 16), dim3(WA_ROWS), 0, s, true, a, pl.ctas);
 }
 
 }  // namespace
@@ -842,6 +1012,7 @@ extern "C" fm_status fm_paged_window_attn(const fm_paged_cache* cache, const fm_
   a.T = (int)p->rows;
   a.H = (int)p->heads;
   a.G = (int)(p->heads / cache->kv_heads);
+  a.by_g = make_divider((uint32_t)a.G);
   a.scale = p->softmax_scale * kLog2e;
   a.window = (int)p->window;
   a.sinks = (int)p->sinks;
@@ -854,14 +1025,14 @@ extern "C" fm_status fm_paged_window_attn(const fm_paged_cache* cache, const fm_
   if (pl.total > p->workspace_bytes || (pl.total && !p->workspace))
     return set_error(FM_ERR_WORKSPACE, "paged_window_attn: workspace %zu < %zu", p->workspace_bytes, pl.total);
   if ((uintptr_t)p->workspace % 16) return set_error(FM_ERR_ALIGN, "paged_window_attn: workspace not 16-byte aligned");
-  if (pl.tiles * cache->kv_heads * pl.splits > 0x7fffffff)
-    return set_error(FM_ERR_SHAPE, "paged_window_attn: grid too large");
-  a.tiles = (int)pl.tiles;
-  a.splits = pl.splits;
-  a.part = static_cast<float*>(p->workspace);
-  a.stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(p->workspace) + pl.part);
+  if (cache->requests > WA_REQUESTS || p->rows * a.G / WA_ROWS + cache->requests > WA_ROW_TILES)
+    return set_error(FM_ERR_SHAPE, "paged_window_attn: more than %d requests or %d row tiles", WA_REQUESTS, WA_ROW_TILES);
+  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
+  a.part = reinterpret_cast<float*>(ws);
+  a.stats = reinterpret_cast<float2*>(ws + pl.part);
+  a.cuts = reinterpret_cast<WaCutItem*>(ws + pl.part + pl.stats);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool kv8 = cache->dtype == FM_DT_E4M3;
-  if (cache->head_dim == 128) return kv8 ? launch_window<128, true>(a, s) : launch_window<128, false>(a, s);
-  return kv8 ? launch_window<64, true>(a, s) : launch_window<64, false>(a, s);
+  if (cache->head_dim == 128) return kv8 ? launch_window<128, true>(a, pl, s) : launch_window<128, false>(a, pl, s);
+  return kv8 ? launch_window<64, true>(a, pl, s) : launch_window<64, false>(a, pl, s);
 }
