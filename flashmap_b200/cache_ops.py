@@ -47,58 +47,67 @@ def _on(t: torch.Tensor, name: str, device) -> None:
         raise OpArgumentError(f"{name} must be on {device}, got {t.device}")
 
 
-def _cache(k_cache, v_cache, lengths, block_table, descales, max_len: int) -> _lib.PagedCache:
+def _refuse_cache(k_cache, v_cache, lengths, block_table, descales, max_len: int) -> None:
+    """Raises for the argument that ``_cache`` could not take."""
     _need(k_cache.is_cuda, "k_cache must be a CUDA tensor")
     dev = k_cache.device
-    if not (dev.index == torch.cuda.current_device()):
-        raise OpArgumentError(f"the cache is on {dev}, which is not the current device")
+    _need(dev.index == torch.cuda.current_device(), f"the cache is on {dev}, which is not the current device")
     _on(v_cache, "v_cache", dev)
     _on(lengths, "the lengths", dev)
     _on(block_table, "block_table", dev)
-    if not (k_cache.dtype is torch.bfloat16 or k_cache.dtype is _FP8):
-        raise OpArgumentError(f"the cache must be bf16 or e4m3, got {k_cache.dtype}")
-    _need(v_cache.dtype is k_cache.dtype, "k_cache and v_cache must share a dtype")
+    _need(k_cache.dtype in (torch.bfloat16, _FP8), f"the cache must be bf16 or e4m3, got {k_cache.dtype}")
+    _need(v_cache.dtype == k_cache.dtype, "k_cache and v_cache must share a dtype")
     _need(k_cache.dim() == 4 and v_cache.shape == k_cache.shape,
           "k_cache and v_cache must both be (pages, kv_heads, page_size, head_dim)")
-    pages, kv_heads, page, head_dim = k_cache.shape
-    if not (head_dim == 64 or head_dim == 128):
-        raise OpArgumentError(f"head_dim must be 64 or 128, got {head_dim}")
-    _need(kv_heads > 0 and page > 0, "the cache needs a kv head and a token to a page")
-    ks, vs = k_cache.stride(), v_cache.stride()
-    _need(ks[3] == 1 and vs[3] == 1, "cache rows must be contiguous")
-    _need(lengths.dtype is torch.int32 and lengths.dim() == 1 and lengths.is_contiguous(),
+    _need(k_cache.shape[3] in (64, 128), f"head_dim must be 64 or 128, got {k_cache.shape[3]}")
+    _need(k_cache.shape[1] > 0 and k_cache.shape[2] > 0, "the cache needs a kv head and a token to a page")
+    _need(k_cache.stride(3) == 1 and v_cache.stride(3) == 1, "cache rows must be contiguous")
+    _need(lengths.dtype == torch.int32 and lengths.dim() == 1 and lengths.is_contiguous(),
           "the lengths must be contiguous int32 (requests,)")
-    requests = lengths.shape[0]
-    _need(block_table.dtype is torch.int32 and block_table.dim() == 2 and block_table.shape[0] == requests,
+    _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == lengths.shape[0],
           "block_table must be int32 (requests, pages)")
     _need(block_table.shape[1] <= 1 or block_table.stride(1) == 1, "block_table rows must be contiguous")
     _need(max_len >= 0, "the largest length must not be negative")
-    dp = None
-    if k_cache.dtype is _FP8:
-        if descales is not None:
-            _on(descales, "descales", dev)
-            _need(descales.dtype is torch.float32 and descales.shape == (2, requests, kv_heads)
-                  and descales.is_contiguous(), "descales must be contiguous float32 (2, requests, kv_heads)")
-            dp = descales.data_ptr()
-    else:
+    if k_cache.dtype == torch.bfloat16:
         _need(descales is None, "descales go with an e4m3 cache")
+    elif descales is not None:
+        _on(descales, "descales", dev)
+        _need(descales.dtype == torch.float32 and descales.is_contiguous()
+              and descales.shape == (2, lengths.shape[0], k_cache.shape[1]),
+              "descales must be contiguous float32 (2, requests, kv_heads)")
+
+
+def _cache(k_cache, v_cache, lengths, block_table, descales, max_len: int) -> _lib.PagedCache:
+    # one condition on the way through; which part of it failed is found out only then
+    dev, dtype = k_cache.device, k_cache.dtype
+    shape, ks, vs, ts, table = k_cache.shape, k_cache.stride(), v_cache.stride(), block_table.stride(), block_table.shape
+    if not (dev.type == "cuda" and dev.index == torch._C._cuda_getDevice() and v_cache.device == dev
+            and lengths.device == dev and block_table.device == dev and v_cache.dtype == dtype
+            and (dtype == torch.bfloat16 and descales is None or dtype == _FP8)
+            and len(shape) == 4 and v_cache.shape == shape and shape[3] in (64, 128) and shape[1] > 0 and shape[2] > 0
+            and ks[3] == 1 and vs[3] == 1 and lengths.dtype == torch.int32 and block_table.dtype == torch.int32
+            and lengths.dim() == 1 and lengths.is_contiguous() and len(table) == 2 and table[0] == lengths.shape[0]
+            and (table[1] <= 1 or ts[1] == 1) and max_len >= 0
+            and (descales is None or descales.device == dev and descales.dtype == torch.float32
+                 and descales.is_contiguous() and descales.shape == (2, table[0], shape[1]))):
+        _refuse_cache(k_cache, v_cache, lengths, block_table, descales, max_len)
+        raise OpArgumentError("the cache's tensors do not go together")
     return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(),
-                           _lib.FM_DT_E4M3 if k_cache.dtype is _FP8 else _lib.FM_DT_BF16,
-                           ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], page, pages, block_table.data_ptr(),
-                           block_table.stride(0), block_table.shape[1], lengths.data_ptr(), max_len, requests,
-                           kv_heads, head_dim, dp)
+                           _lib.FM_DT_BF16 if descales is None and dtype == torch.bfloat16 else _lib.FM_DT_E4M3,
+                           ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], shape[2], shape[0], block_table.data_ptr(),
+                           ts[0], table[1], lengths.data_ptr(), max_len, table[0], shape[1], shape[3],
+                           None if descales is None else descales.data_ptr())
 
 
-def _query(query, name: str, cache: _lib.PagedCache, device) -> torch.Tensor:
-    _on(query, name, device)
-    if not (query.dtype is torch.bfloat16 and query.dim() == 3):
-        raise OpArgumentError(f"{name} must be bf16 (rows, heads, head_dim)")
-    heads, head_dim = query.shape[1], query.shape[2]
-    if not (head_dim == cache.head_dim):
-        raise OpArgumentError(f"{name} has rows of {head_dim}, the cache of {cache.head_dim}")
-    if not (heads > 0 and heads % cache.kv_heads == 0):
-        raise OpArgumentError(f"{heads} query heads are no multiple of {cache.kv_heads} kv heads")
-    if query.stride(2) != 1 or query.data_ptr() % 16 or query.stride(0) % 8 or query.stride(1) % 8:
+def _query(query, cache: _lib.PagedCache, device) -> torch.Tensor:
+    shape, stride = query.shape, query.stride()
+    if not (query.device == device and query.dtype == torch.bfloat16 and len(shape) == 3
+            and shape[2] == cache.head_dim and shape[1] > 0 and shape[1] % cache.kv_heads == 0):
+        _on(query, "query", device)
+        _need(query.dtype == torch.bfloat16 and query.dim() == 3, "query must be bf16 (rows, heads, head_dim)")
+        _need(shape[2] == cache.head_dim, f"query has rows of {shape[2]}, the cache of {cache.head_dim}")
+        raise OpArgumentError(f"{shape[1]} query heads are no multiple of {cache.kv_heads} kv heads")
+    if stride[2] != 1 or stride[0] % 8 or stride[1] % 8 or query.data_ptr() % 16:
         query = query.contiguous()
         if query.data_ptr() % 16:  # a contiguous view that starts between two 16-byte lines
             query = query.clone()
@@ -119,8 +128,19 @@ def _sums(weight_sums, cache: _lib.PagedCache, device, least: int) -> None:
     _need(weight_sums.shape[2] <= 1 or weight_sums.stride(2) == 1, "weight_sums rows must be contiguous")
 
 
-def _raw_stream(device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
+_ERR_WORDS: dict = {}  # device index -> address of its error word, which lives as long as the process
+
+
+def _launch(name: str, cache: _lib.PagedCache, args, device) -> None:
+    index = device.index
+    err = _ERR_WORDS.get(index)
+    if err is None:
+        err = _ERR_WORDS[index] = _err(device).data_ptr()
+    args.err = err
+    lib = _lib.load()
+    status = getattr(lib, name)(ctypes.byref(cache), ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, name)
 
 
 def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -139,7 +159,7 @@ def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     most ``max_seqlen_k`` positions."""
     cache = _cache(k_cache, v_cache, seqused_k, block_table, descales, int(max_seqlen_k))
     dev = k_cache.device
-    query = _query(query, "query", cache, dev)
+    query = _query(query, cache, dev)
     _need(query.shape[0] == cache.requests, "one query row per request")
     _visibility(window, sinks)
     out = torch.empty(query.shape, dtype=torch.bfloat16, device=dev)
@@ -150,7 +170,7 @@ def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     lib = _lib.load()
     heads, qs, os = query.shape[1], query.stride(), out.stride()
     args = _lib.DecodeAttn(query.data_ptr(), qs[0], qs[1], heads, softmax_scale, window, sinks, None, 0, 0,
-                           out.data_ptr(), os[0], os[1], None, 0, _err(dev).data_ptr())
+                           out.data_ptr(), os[0], os[1], None, 0, None)
     if weight_sums is not None:
         args.weight_sums = weight_sums.data_ptr()
         args.sums_request_stride, args.sums_head_stride = weight_sums.stride(0), weight_sums.stride(1)
@@ -159,7 +179,7 @@ def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     if need:
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         args.workspace, args.workspace_bytes = ws.data_ptr(), need
-    _lib.call("fm_paged_decode_attn", ctypes.byref(cache), ctypes.byref(args), _raw_stream(dev))
+    _launch("fm_paged_decode_attn", cache, args, dev)
     return out
 
 
@@ -178,7 +198,7 @@ def paged_window_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     of a chunk see and others do not must be finite."""
     cache = _cache(k_cache, v_cache, seqused_k, block_table, descales, int(max_seqlen_k))
     dev = k_cache.device
-    query = _query(query, "query", cache, dev)
+    query = _query(query, cache, dev)
     _on(cu_seqlens_q, "cu_seqlens_q", dev)
     _need(cu_seqlens_q.dtype is torch.int32 and cu_seqlens_q.shape == (cache.requests + 1,)
           and cu_seqlens_q.is_contiguous(), "cu_seqlens_q must be contiguous int32 (requests + 1,)")
@@ -192,13 +212,13 @@ def paged_window_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     qs, os = query.stride(), out.stride()
     args = _lib.WindowAttn(query.data_ptr(), qs[0], qs[1], tokens, heads, cu_seqlens_q.data_ptr(),
                            int(max_seqlen_q), softmax_scale, window, sinks, out.data_ptr(), os[0], os[1], None, 0,
-                           _err(dev).data_ptr())
+                           None)
     need = lib.fm_paged_window_attn_workspace_size(cache.requests, tokens, heads, cache.kv_heads, cache.head_dim,
                                                    int(max_seqlen_q), cache.max_length, window, sinks)
     if need:
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         args.workspace, args.workspace_bytes = ws.data_ptr(), need
-    _lib.call("fm_paged_window_attn", ctypes.byref(cache), ctypes.byref(args), _raw_stream(dev))
+    _launch("fm_paged_window_attn", cache, args, dev)
     return out
 
 
@@ -231,8 +251,7 @@ def evict_paged_context(k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k:
     lengths = torch.empty(cache.requests, dtype=torch.int32, device=dev)
     sums = torch.empty((cache.requests, cache.kv_heads, budget), dtype=torch.float32, device=dev)
     args = _lib.Evict(weight_sums.data_ptr(), weight_sums.stride(0), weight_sums.stride(1), budget, sinks, recent,
-                      None, 0, 0, kept.data_ptr(), lengths.data_ptr(), sums.data_ptr(), None, 0,
-                      _err(dev).data_ptr())
+                      None, 0, 0, kept.data_ptr(), lengths.data_ptr(), sums.data_ptr(), None, 0, None)
     if out_block_table is not None:
         _on(out_block_table, "out_block_table", dev)
         _need(out_block_table.dtype is torch.int32 and out_block_table.dim() == 2
@@ -245,5 +264,5 @@ def evict_paged_context(k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k:
         need = _lib.load().fm_paged_evict_workspace_size(cache.requests, cache.kv_heads, budget)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         args.workspace, args.workspace_bytes = ws.data_ptr(), need
-        _lib.call("fm_paged_evict", ctypes.byref(cache), ctypes.byref(args), _raw_stream(dev))
+        _launch("fm_paged_evict", cache, args, dev)
     return kept, lengths, sums

@@ -319,8 +319,7 @@ extern "C" fm_status fm_paged_evict(const fm_paged_cache* cache, const fm_evict*
   const int cs = evict_cluster(items, cache->max_length);
   int64_t keys = (cache->max_length + cs - 1) / cs + 32;
   if (keys > EV_KEYS) keys = EV_KEYS;
-  st = check_cuda(cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_KEYS * 4),
-                  "paged_evict");
+  st = allow_smem<evict_select_kernel>(EV_KEYS * 4, "paged_evict");
   if (st != FM_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(items * cs));

@@ -6,6 +6,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "launch.cuh"
 
@@ -77,6 +79,19 @@ inline fm_status cache_ref(const fm_paged_cache* p, const char* who, CacheRef* c
       c->vhs % 16 || c->vts % 16)
     return set_error(FM_ERR_ALIGN, "%s: cache rows must be 16-byte aligned", who);
   return FM_OK;
+}
+
+// Lets kernel K have `bytes` of dynamic shared memory, once per device.
+template <auto K>
+inline fm_status allow_smem(int bytes, const char* who) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return FM_OK;
+  const fm_status st = check_cuda(cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), who);
+  if (st == FM_OK) done.fetch_or(bit, std::memory_order_release);
+  return st;
 }
 
 // The positions of a context of `len` that its last token sees, numbered

@@ -966,9 +966,7 @@ template <int HD, bool KV8>
 fm_status launch_window(const WindowArgs& a, const WindowPlan& pl, cudaStream_t s) {
   constexpr int smem = WaLayout<HD, KV8>::SMEM;
   static_assert(sizeof(WaCtrl) <= 3072 && smem <= 232448, "shared memory");
-  fm_status st = check_cuda(
-      cudaFuncSetAttribute(window_attn_kernel<HD, KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-      "paged_window_attn");
+  fm_status st = allow_smem<window_attn_kernel<HD, KV8>>(smem, "paged_window_attn");
   if (st != FM_OK) return st;
   st = launch_kernel(window_attn_kernel<HD, KV8>, dim3((unsigned)pl.ctas), dim3(512), smem, s, false, a);
   if (st != FM_OK || !pl.cuts) return st;
