@@ -385,24 +385,24 @@ __device__ __forceinline__ float2 row_stats(const float2* stats, int n) {
   return make_float2(u, ll);
 }
 
-constexpr int DJ_THREADS = 256;
-constexpr int DJ_KEYS = 4 * DJ_THREADS;  // positions of a block that adds weights to the sums
-constexpr int DJ_HEADS = 8;              // heads whose scores a thread has in flight
+constexpr int DJ_HEADS = 8;  // heads whose scores a thread has in flight
 
 // Blocks [0, row_blocks): (request, head) rows whose chunks are joined, one row
 // to a block, or to a warp where a row has few chunks (WARP_ROWS).
-// Blocks from there on: DJ_KEYS visible positions of one (request, kv head),
+// Blocks from there on: 4 NT visible positions of one (request, kv head),
 // whose weights are added to the sums; every sum has one writer, so repeated
 // runs agree bit for bit.
-template <int HD, bool WARP_ROWS>
-__global__ void __launch_bounds__(DJ_THREADS) decode_join_kernel(DecodeArgs a, int row_blocks, int key_blocks) {
-  __shared__ float4 sred[DJ_THREADS / 32][HD / 4];
+template <int HD, bool WARP_ROWS, int NT>
+__global__ void __launch_bounds__(NT) decode_join_kernel(DecodeArgs a, int row_blocks, int key_blocks) {
+  constexpr int DJ_KEYS = 4 * NT;
+  static_assert(NT / 32 >= DJ_HEADS, "a warp to a head's statistics");
+  __shared__ float4 sred[NT / 32][HD / 4];
   __shared__ float2 sst[DJ_HEADS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = a.c.R * a.H;
   pdl_wait();
   if (WARP_ROWS && (int)blockIdx.x < row_blocks) {
-    const int row = blockIdx.x * (DJ_THREADS / 32) + warp, r = row / a.H, h = row % a.H;
+    const int row = blockIdx.x * (NT / 32) + warp, r = row / a.H, h = row % a.H;
     if (row >= rows) return;
     const Span sp = visible_span(cache_length(a.c, r, a.err, false), a.window, a.sinks);
     const int n = (sp.n + a.chunk - 1) / a.chunk;
@@ -436,7 +436,7 @@ __global__ void __launch_bounds__(DJ_THREADS) decode_join_kernel(DecodeArgs a, i
     if (n <= 1) return;  // written by its only chunk
     const float2* stats = a.stats + (long long)row * a.chunks;
     const float2 st = row_stats(stats, n);
-    constexpr int V = HD / 4, PER = DJ_THREADS / V;  // threads per chunk's row, chunks at a time
+    constexpr int V = HD / 4, PER = NT / V;  // threads per chunk's row, chunks at a time
     const float4* part = reinterpret_cast<const float4*>(a.part + (long long)row * a.chunks * HD) + tid % V;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -459,8 +459,8 @@ __global__ void __launch_bounds__(DJ_THREADS) decode_join_kernel(DecodeArgs a, i
     if (tid < V) {
       const float inv = st.y == 0.0f ? 0.0f : 1.0f / st.y;
       float4 o = sred[0][tid];
-#pragma unroll
-      for (int w = 1; w < DJ_THREADS / 32; ++w) {
+#pragma unroll 8
+      for (int w = 1; w < NT / 32; ++w) {
         const float4 x = sred[w][tid];
         o.x += x.x;
         o.y += x.y;
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(DJ_THREADS) decode_join_kernel(DecodeArgs a, i
 #pragma unroll
     for (int g = 0; g < DJ_HEADS; ++g)
       if (g0 + g < a.G && i < sp.n) s[g] = *reinterpret_cast<const float4*>(a.scores + (row0 + g0 + g) * a.pitch + i);
-    if (g0 + warp < a.G) {
+    if (warp < DJ_HEADS && g0 + warp < a.G) {
       const float2 st = row_stats(a.stats + (row0 + g0 + warp) * a.chunks, n);
       if (lane == 0) sst[warp] = make_float2(st.x, st.y == 0.0f ? 0.0f : 1.0f / st.y);
     }
@@ -511,8 +511,6 @@ __global__ void __launch_bounds__(DJ_THREADS) decode_join_kernel(DecodeArgs a, i
   for (int e = 0; e < 4; ++e)
     if (i + e < sp.n) dst[sp.pos(i + e)] = old[e] + w[e];
 }
-static_assert(DJ_THREADS / 32 == DJ_HEADS, "a warp to a head's statistics");
-
 struct DecodePlan {
   int ng, hgroups, chunk, chunks, pitch;
   size_t part, stats, scores, total;
@@ -624,10 +622,10 @@ extern "C" fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_
   a.pitch = pl.pitch;
   a.err = p->err;
   const int64_t items = cache->requests * cache->kv_heads * pl.hgroups;
-  const int64_t key_blocks = sums ? (pl.pitch + DJ_KEYS - 1) / DJ_KEYS : 0;
   // a warp to a row where that leaves no warp more than 16 chunks
   const bool warp_rows = pl.chunks <= 16;
-  const int64_t per = warp_rows ? DJ_THREADS / 32 : 1;
+  const int nt = warp_rows ? 256 : 1024;
+  const int64_t per = warp_rows ? nt / 32 : 1, key_blocks = sums ? (pl.pitch + 4 * nt - 1) / (4 * nt) : 0;
   const int64_t row_blocks = pl.chunks > 1 ? (cache->requests * p->heads + per - 1) / per : 0;
   const int64_t join = row_blocks + cache->requests * cache->kv_heads * key_blocks;
   if (items * pl.chunks > 0x7fffffff || join > 0x7fffffff)
@@ -638,11 +636,11 @@ extern "C" fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_
   st = cache->head_dim == 128 ? launch_decode_hd<128>(a, kv8, pl.ng, grid, s)
                               : launch_decode_hd<64>(a, kv8, pl.ng, grid, s);
   if (st != FM_OK || (pl.chunks == 1 && !sums)) return st;
-  const dim3 grid2((unsigned)join), block(DJ_THREADS);
+  const dim3 grid2((unsigned)join), block(nt);
   auto join_launch = [&](auto kernel) {
     return launch_kernel(kernel, grid2, block, 0, s, true, a, (int)row_blocks, (int)key_blocks);
   };
   if (cache->head_dim == 128)
-    return warp_rows ? join_launch(decode_join_kernel<128, true>) : join_launch(decode_join_kernel<128, false>);
-  return warp_rows ? join_launch(decode_join_kernel<64, true>) : join_launch(decode_join_kernel<64, false>);
+    return warp_rows ? join_launch(decode_join_kernel<128, true, 256>) : join_launch(decode_join_kernel<128, false, 1024>);
+  return warp_rows ? join_launch(decode_join_kernel<64, true, 256>) : join_launch(decode_join_kernel<64, false, 1024>);
 }

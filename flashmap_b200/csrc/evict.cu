@@ -22,9 +22,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int EV_THREADS = 1024;
+constexpr int EV_THREADS = 512;
 constexpr int EV_WARPS = EV_THREADS / 32;
-static_assert(EV_WARPS == 32, "a warp adds up the warps' counts");
 constexpr int EV_BINS = 2048;
 constexpr int EV_KEYS = 49152;  // keys of a slice that shared memory holds; longer slices read theirs from L2 again
 constexpr int EV_UNROLL = 4;    // rows that a thread of the moving kernel has in flight
@@ -51,7 +50,7 @@ __device__ __forceinline__ uint32_t sum_key(float v) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-__global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
+__global__ void __launch_bounds__(EV_THREADS, 3) evict_select_kernel(EvictArgs a) {
   extern __shared__ uint32_t ev_keys[];
   __shared__ int hist[2][EV_BINS];
   __shared__ int wsum[EV_WARPS], wtie[EV_WARPS];
@@ -67,23 +66,27 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
   const float* sums = a.sums + (long long)r * a.s_rs + (long long)h * a.s_hs;
   const int* table = a.c.table + (long long)r * a.c.tstride;
   const long long row0 = (long long)item * a.budget;
-  auto keep = [&](int at, int i, float v) {
-    const int pg = a.c.by_page.div(i);
-    int page = table[pg];
-    if (page < 0 || page >= a.c.num_pages) {
-      record_error(a.err, DEV_BAD_INDEX);
-      page = -1;
-    }
-    a.kept[row0 + at] = i;
-    a.out_sums[row0 + at] = v;
-    a.from[row0 + at] = make_int2(page, i - pg * a.c.page);
-  };
   for (int i = n + rank * EV_THREADS + tid; i < a.budget; i += cs * EV_THREADS) {
     a.kept[row0 + i] = -1;
     a.out_sums[row0 + i] = 0.0f;
   }
+  // what goes with the kept positions of slots b .. e - 1, once their numbers are written
+  auto fill = [&](int b, int e) {
+#pragma unroll 4
+    for (int at = b + tid; at < e; at += EV_THREADS) {
+      const int i = a.kept[row0 + at], pg = a.c.by_page.div(i);
+      const int page = table[pg];
+      const bool ok = page >= 0 && page < a.c.num_pages;
+      if (!ok) record_error(a.err, DEV_BAD_INDEX);
+      a.out_sums[row0 + at] = sums[i];
+      a.from[row0 + at] = make_int2(ok ? page : -1, i - pg * a.c.page);
+    }
+  };
   if (len <= a.budget) {
-    for (int i = rank * EV_THREADS + tid; i < n; i += cs * EV_THREADS) keep(i, i, sums[i]);
+    const int part = (n + cs - 1) / cs, b = min(n, rank * part), e = min(n, b + part);
+    for (int i = b + tid; i < e; i += EV_THREADS) a.kept[row0 + i] = i;
+    __syncthreads();
+    fill(b, e);
     return;
   }
   const int lo = a.sinks, hi = len - a.recent;  // the positions that compete
@@ -116,14 +119,16 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
         if (bin >= 0 && lane == __ffs(peers) - 1) atomicAdd(&hp[bin], __popc(peers));
       }
       cluster.sync();
-      // thread t: bins 2 t and 2 t + 1 over the cluster, and the count in all higher bins
-      int2 mine = make_int2(0, 0);
+      // thread t: bins 4 t .. 4 t + 3 over the cluster, and the count in all higher bins
+      int4 mine = make_int4(0, 0, 0, 0);
       for (int q = 0; q < cs; ++q) {
-        const int2 x = reinterpret_cast<const int2*>(cluster.map_shared_rank(hp, q))[tid];
+        const int4 x = reinterpret_cast<const int4*>(cluster.map_shared_rank(hp, q))[tid];
         mine.x += x.x;
         mine.y += x.y;
+        mine.z += x.z;
+        mine.w += x.w;
       }
-      const int all = mine.x + mine.y;
+      const int all = mine.x + mine.y + mine.z + mine.w;
       int above = all;  // inclusive suffix sum over lanes
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -132,15 +137,16 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
       }
       if (lane == 0) wsum[warp] = above;
       __syncthreads();
-      const int later = __reduce_add_sync(0xffffffffu, lane > warp ? wsum[lane] : 0);
-      above += later - all;
+      above += __reduce_add_sync(0xffffffffu, lane > warp && lane < EV_WARPS ? wsum[lane] : 0) - all;
       // the bin in which the need-th largest lies belongs to exactly one thread
-      if (above < need && need <= above + mine.y) {
-        s_bin = 2 * tid + 1;
-        s_left = need - above;
-      } else if (above + mine.y < need && need <= above + all) {
-        s_bin = 2 * tid;
-        s_left = need - above - mine.y;
+      const int c4[4] = {mine.w, mine.z, mine.y, mine.x};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (above < need && need <= above + c4[e]) {
+          s_bin = 4 * tid + 3 - e;
+          s_left = need - above;
+        }
+        above += c4[e];
       }
       __syncthreads();
       need = s_left;
@@ -175,7 +181,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
   }
   __syncthreads();
   // before this warp, and of the slice
-  const int ws = wsum[lane], wt = wtie[lane];
+  const int ws = lane < EV_WARPS ? wsum[lane] : 0, wt = lane < EV_WARPS ? wtie[lane] : 0;
   int sb = __reduce_add_sync(0xffffffffu, lane < warp ? ws : 0), tb = __reduce_add_sync(0xffffffffu, lane < warp ? wt : 0);
   const int st = __reduce_add_sync(0xffffffffu, ws), tt = __reduce_add_sync(0xffffffffu, wt);
   if (tid == 0) {
@@ -183,11 +189,14 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
     s_total[1] = tt;
   }
   cluster.sync();
+  int slice_sure = 0, slice_ties = 0;  // before this slice
   for (int q = 0; q < rank; ++q) {
     const int* other = cluster.map_shared_rank(s_total, q);
-    sb += other[0];
-    tb += other[1];
+    slice_sure += other[0];
+    slice_ties += other[1];
   }
+  sb += slice_sure;
+  tb += slice_ties;
   cluster.sync();  // no CTA ends, or counts anew, while another reads its totals
   const unsigned below = (1u << lane) - 1u;
   for (int i0 = s0; i0 < s1; i0 += 32) {
@@ -197,11 +206,14 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(EvictArgs a) {
     const int t = tb + __popc(eb & below);  // ties before this position
     if (yes || (tie && t < need)) {
       const int at = sb + __popc(yb & below) + min(t, need);
-      if (at < a.budget) keep(at, begin + i0 + lane, sums[begin + i0 + lane]);
+      if (at < a.budget) a.kept[row0 + at] = begin + i0 + lane;
     }
     sb += __popc(yb);
     tb += __popc(eb);
   }
+  __syncthreads();
+  fill(min(a.budget, slice_sure + min(slice_ties, need)),
+       min(a.budget, slice_sure + st + min(slice_ties + tt, need)));
 }
 
 // One CTA per (request, kv head, keys or values, slice of the row's bytes), and
@@ -261,10 +273,10 @@ __global__ void __launch_bounds__(256, 4) evict_move_kernel(EvictArgs a) {
   }
 }
 
-// CTAs of a cluster: as many as leave one to an SM, with 8192 positions each at least.
+// CTAs of a cluster: as many as leave three to an SM, with 4096 positions each at least.
 int evict_cluster(int64_t items, int64_t positions) {
   int cs = 1;
-  while (cs < 8 && items * cs * 2 <= 148 && positions >= 8192 * 2 * cs) cs *= 2;
+  while (cs < 8 && items * cs * 2 <= 3 * 148 && positions >= 4096 * 2 * cs) cs *= 2;
   return cs;
 }
 
