@@ -99,6 +99,13 @@ __global__ void __launch_bounds__(EV_THREADS, 3) evict_select_kernel(EvictArgs a
     for (int i = tid; i < count; i += EV_THREADS) ev_keys[i] = sum_key(sums[begin + i]);
   auto key = [&](int i) { return held ? ev_keys[i] : sum_key(sums[begin + i]); };
 
+  auto meet = [&]() {
+    if (cs > 1)
+      cluster.sync();
+    else
+      __syncthreads();
+  };
+
   uint32_t prefix = 0, mask = 0;
   if (need > 0) {
     for (int pass = 0; pass < 3; ++pass) {
@@ -114,11 +121,15 @@ __global__ void __launch_bounds__(EV_THREADS, 3) evict_select_kernel(EvictArgs a
           const uint32_t k = key(i);
           if ((k & mask) == prefix) bin = (int)((k >> shift) & digit);
         }
-        // equal sums are common (positions that were never looked at): one addition for all of a warp's
-        const unsigned peers = __match_any_sync(0xffffffffu, bin);
-        if (bin >= 0 && lane == __ffs(peers) - 1) atomicAdd(&hp[bin], __popc(peers));
+        // equal sums are common (positions that were never looked at): one addition for a whole warp's
+        const int lead = __shfl_sync(0xffffffffu, bin, 0);
+        if (__all_sync(0xffffffffu, bin == lead)) {
+          if (lane == 0 && bin >= 0) atomicAdd(&hp[bin], 32);
+        } else if (bin >= 0) {
+          atomicAdd(&hp[bin], 1);
+        }
       }
-      cluster.sync();
+      meet();
       // thread t: bins 4 t .. 4 t + 3 over the cluster, and the count in all higher bins
       int4 mine = make_int4(0, 0, 0, 0);
       for (int q = 0; q < cs; ++q) {
@@ -167,13 +178,21 @@ __global__ void __launch_bounds__(EV_THREADS, 3) evict_select_kernel(EvictArgs a
   };
   const int seg = ((count + EV_WARPS - 1) / EV_WARPS + 31) & ~31;  // a warp's run of positions
   const int s0 = warp * seg, s1 = min(count, s0 + seg);
-  __syncthreads();  // the keys are there where there was no pass
-  int sure = 0, ties = 0;
-  for (int i0 = s0; i0 < s1; i0 += 32) {
+  // what the count finds out about 32 positions is kept for when their slots are known
+  uint2* found = reinterpret_cast<uint2*>(&hist[0][0]);
+  const bool noted = count <= 32 * EV_BINS;
+  meet();  // the keys are there where there was no pass, and no CTA reads these bins any more
+  auto look = [&](int i0) {
     bool tie;
     const bool yes = kind(i0 + lane, &tie);
-    sure += __popc(__ballot_sync(0xffffffffu, yes));
-    ties += __popc(__ballot_sync(0xffffffffu, tie));
+    return make_uint2(__ballot_sync(0xffffffffu, yes), __ballot_sync(0xffffffffu, tie));
+  };
+  int sure = 0, ties = 0;
+  for (int i0 = s0; i0 < s1; i0 += 32) {
+    const uint2 f = look(i0);
+    if (noted && lane == 0) found[i0 >> 5] = f;
+    sure += __popc(f.x);
+    ties += __popc(f.y);
   }
   if (lane == 0) {
     wsum[warp] = sure;
@@ -188,7 +207,7 @@ __global__ void __launch_bounds__(EV_THREADS, 3) evict_select_kernel(EvictArgs a
     s_total[0] = st;
     s_total[1] = tt;
   }
-  cluster.sync();
+  meet();
   int slice_sure = 0, slice_ties = 0;  // before this slice
   for (int q = 0; q < rank; ++q) {
     const int* other = cluster.map_shared_rank(s_total, q);
@@ -197,19 +216,40 @@ __global__ void __launch_bounds__(EV_THREADS, 3) evict_select_kernel(EvictArgs a
   }
   sb += slice_sure;
   tb += slice_ties;
-  cluster.sync();  // no CTA ends, or counts anew, while another reads its totals
+  if (cs > 1) cluster.sync();  // no CTA ends while another reads its totals
   const unsigned below = (1u << lane) - 1u;
-  for (int i0 = s0; i0 < s1; i0 += 32) {
-    bool tie;
-    const bool yes = kind(i0 + lane, &tie);
-    const unsigned yb = __ballot_sync(0xffffffffu, yes), eb = __ballot_sync(0xffffffffu, tie);
-    const int t = tb + __popc(eb & below);  // ties before this position
-    if (yes || (tie && t < need)) {
-      const int at = sb + __popc(yb & below) + min(t, need);
-      if (at < a.budget) a.kept[row0 + at] = begin + i0 + lane;
+  for (int i0 = s0; i0 < s1; i0 += 1024) {  // lane l: positions i0 + 32 l .. i0 + 32 l + 31
+    uint2 mine = make_uint2(0, 0);
+    if (noted) {
+      if (i0 + 32 * lane < s1) mine = found[(i0 >> 5) + lane];
+    } else {
+      for (int l = 0; l < 32; ++l) {
+        const uint2 f = look(i0 + 32 * l < s1 ? i0 + 32 * l : count);
+        if (lane == l) mine = f;
+      }
     }
-    sb += __popc(yb);
-    tb += __popc(eb);
+    int ys = __popc(mine.x), es = __popc(mine.y);
+    const int y1 = ys, e1 = es;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, ys, off), e = __shfl_up_sync(0xffffffffu, es, off);
+      if (lane >= off) {
+        ys += y;
+        es += e;
+      }
+    }
+    const int steps = min(32, (s1 - i0 + 31) / 32);
+#pragma unroll 4
+    for (int l = 0; l < steps; ++l) {
+      const unsigned yb = __shfl_sync(0xffffffffu, mine.x, l), eb = __shfl_sync(0xffffffffu, mine.y, l);
+      const int sy = sb + __shfl_sync(0xffffffffu, ys - y1, l), se = tb + __shfl_sync(0xffffffffu, es - e1, l);
+      const int t = se + __popc(eb & below);  // ties before this position
+      const int at = sy + __popc(yb & below) + min(t, need);
+      const bool stay = (yb >> lane & 1u) || ((eb >> lane & 1u) && t < need);
+      if (stay && at < a.budget) a.kept[row0 + at] = begin + i0 + 32 * l + lane;
+    }
+    sb += __shfl_sync(0xffffffffu, ys, 31);
+    tb += __shfl_sync(0xffffffffu, es, 31);
   }
   __syncthreads();
   fill(min(a.budget, slice_sure + min(slice_ties, need)),

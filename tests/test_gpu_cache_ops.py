@@ -464,3 +464,23 @@ def test_refusals():
     assert decode(query=q[:0], seqused_k=none, block_table=t[:0]).shape == (0, 4, D)
     assert chunk(query=q[:0], cu_seqlens_q=torch.zeros(2, dtype=torch.int32, device=DEV)).shape == (0, 4, D)
     assert evict(seqused_k=none, block_table=t[:0], weight_sums=sums[:0])[0].shape == (0, KH, 4)
+
+
+def test_evict_slices_past_shared_memory():
+    """So many positions of one kv head that a CTA's slice of them does not fit its shared memory."""
+    g = torch.Generator().manual_seed(20)
+    L, budget, page, D = 600_000, 100_000, 128, 64
+    cols = -(-L // page)
+    table = torch.randperm(cols, generator=g).int().view(1, cols)
+    pool = torch.randint(-100, 100, (cols, 1, page, 2 * D), generator=g, dtype=torch.int8).to(torch.bfloat16)
+    sums = torch.randint(0, 50, (1, 1, L), generator=g).float()
+    dev = pool.to(DEV)
+    kept, n, got = ops().evict_paged_context(dev[..., :D], dev[..., D:], torch.tensor([L], dtype=torch.int32, device=DEV),
+                                             table.to(DEV), sums.to(DEV), budget, sinks=4, recent=1000)
+    want = O.evict(sums, [L], budget, 4, 1000)
+    assert int(n) == budget and kept[0, 0].tolist() == want[0][0]
+    src = torch.tensor(want[0][0])
+    assert torch.equal(got[0, 0].cpu(), sums[0, 0, src])
+    i = torch.arange(budget)
+    moved = dev[table[0, i // page].long().to(DEV), 0, (i % page).to(DEV)].cpu()
+    assert torch.equal(moved, pool[table[0, src // page].long(), 0, src % page])
