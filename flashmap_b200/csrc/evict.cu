@@ -50,7 +50,7 @@ __device__ __forceinline__ uint32_t sum_key(float v) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-__global__ void __launch_bounds__(EV_THREADS, 3) evict_select_kernel(EvictArgs a) {
+__global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(EvictArgs a) {
   extern __shared__ uint32_t ev_keys[];
   __shared__ int hist[2][EV_BINS];
   __shared__ int wsum[EV_WARPS], wtie[EV_WARPS];
