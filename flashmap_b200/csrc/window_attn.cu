@@ -13,6 +13,7 @@ namespace {
 
 constexpr int WA_ROWS = 256;  // (token, head of the group) rows of a CTA, in two tiles
 constexpr int WA_KEYS = 128;  // keys of a tile
+constexpr int WA_LAG = 1;     // 16-bit tiles whose copies are in flight behind the newest
 
 // What a CTA says of the items that are cut at the ends of its share.
 enum { WA_NONE = 0, WA_MORE = 1, WA_LAST = 2, WA_EMPTY = 3 };
@@ -73,8 +74,8 @@ __device__ __forceinline__ int wa_row_tiles(const WindowArgs& a, int nq) {
 // an item costs besides, and every CTA takes an equal length.  An item that
 // lies across a border is cut there and joined by window_join_kernel, unless
 // less than WA_CUT tiles would be cut off.
-constexpr int WA_ITEM = 5;
-constexpr int WA_CUT = 3;
+constexpr int WA_ITEM = 2;
+constexpr int WA_CUT = 2;
 constexpr int WA_SHARE = WA_ITEM + 4;  // the least length of a CTA's share
 struct WaBorder {
   int r, y, c, t;  // request, row tile, kv head, and the first tile after the border
@@ -118,6 +119,12 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const float* v) {
       "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
       "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
       : "memory");
+}
+__device__ __forceinline__ void tmem_st_x2(uint32_t taddr, float x, float y) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1,%2};" ::"r"(taddr), "f"(x), "f"(y) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x2(uint32_t taddr, float& x, float& y) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];" : "=f"(x), "=f"(y) : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // D[tmem] (+)= A B, 16-bit operands, fp32 accumulate; A from shared memory or
@@ -180,16 +187,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return y;
 }
 
-// Shared memory: two row tiles of Q, a ring of K and V tiles (16-bit, 128-byte
-// swizzled in blocks of 64 columns), for e4m3 caches two tiles of raw bytes.
-template <int HD, bool KV8>
+// Shared memory: two row tiles of Q and a ring of K and V tiles (16-bit,
+// 128-byte swizzled in blocks of 64 columns).
+template <int HD>
 struct WaLayout {
   static constexpr int TILE = 128 * HD * 2;  // Q, K or V tile
-  static constexpr int SLOTS = HD == 64 ? 8 : KV8 ? 4 : 5;
-  static constexpr int RAW = KV8 ? 128 * HD : 0;
-  static constexpr int RAWS = KV8 ? 2 : 0;
-  static constexpr int LAG = KV8 ? 1 : 2;  // tiles of copies in flight behind the newest
-  static constexpr int CTRL = 2 * TILE + SLOTS * TILE + RAWS * RAW;
+  static constexpr int SLOTS = HD == 64 ? 8 : 5;
+  static constexpr int CTRL = 2 * TILE + SLOTS * TILE;
   static constexpr int SMEM = CTRL + 3072;  // 227 KB at head_dim 128: all that a CTA may have
 };
 
@@ -209,6 +213,7 @@ struct WaItem {
     return (t < t_head ? t : t - t_head + t_lo) * WA_KEYS;
   }
   __device__ __forceinline__ int mt() const { return rows > 128 ? 2 : 1; }
+  __device__ __forceinline__ bool duo() const { return rows <= 128 && n >= 2; }
 };
 
 constexpr int WA_ITEMS = 4;              // ring of work items
@@ -217,7 +222,7 @@ constexpr int WA_ROW_TILES = 4096 * 512;  // row tiles of a call
 
 struct WaCtrl {
   uint64_t full[8], empty[8];
-  uint64_t s_full[2], p_ready[2][2], o_done[2], o_empty[2], q_full, q_empty, drain;
+  uint64_t s_full[2], p_ready[2][2], o_done[2], o_empty[2], other, q_raw, q_full, q_empty, drain;
   uint64_t item_full[WA_ITEMS], item_empty[WA_ITEMS];
   int abort;
   uint32_t tmem;
@@ -235,16 +240,24 @@ struct WaCtrl {
 // row) turn it into P in place, which is the next product's A operand.  While
 // one row tile is in softmax the tensor cores work on the other, and the next
 // item's loads run beside the current one's products.
-template <int HD, bool KV8>
+//
+// DUO is the kernel for calls whose requests have 128 rows at most, so that an
+// item has one row tile: both softmax warpgroups take its rows, each every
+// other key tile, so that here, too, one is in softmax while the other's
+// products run, and join their halves at the end (24 x 17 rows on 512 .. 4096
+// positions: 70 us with one warpgroup, 64 us with both; in the same kernel as
+// the rest it costs that 4 percent).
+template <int HD, bool KV8, bool DUO>
 __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
-  using Lay = WaLayout<HD, KV8>;
+  using Lay = WaLayout<HD>;
   constexpr int TILE = Lay::TILE, SLOTS = Lay::SLOTS;
   constexpr int CPR = HD / 8;  // 16-byte chunks of a 16-bit row
+  // registers: 2 x 184 + 64 + 80, or 2 x 176 + 96 + 64 where e4m3 rows pass
+  // through the loading warps, is what 4 x 128 threads are launched with
   extern __shared__ __align__(1024) uint8_t wa_smem[];
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   uint8_t* sQ = wa_smem;
   uint8_t* sKV = wa_smem + 2 * TILE;
-  uint8_t* sRaw = sKV + SLOTS * TILE;
   WaCtrl* ctl = reinterpret_cast<WaCtrl*>(wa_smem + Lay::CTRL);
   if (smem_u32(wa_smem) & 1023) {  // the swizzled tiles need the alignment that the declaration asks for
     if (tid == 0) record_error(a.err, DEV_BAD_COPY);
@@ -263,7 +276,9 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       mbar_init(&ctl->o_done[i], 1);
       mbar_init(&ctl->o_empty[i], 128);
     }
-    mbar_init(&ctl->q_full, 96);
+    mbar_init(&ctl->other, 128);
+    mbar_init(&ctl->q_raw, 96);
+    mbar_init(&ctl->q_full, KV8 ? 256 : 96);
     mbar_init(&ctl->q_empty, 1);
     mbar_init(&ctl->drain, 1);
     for (int i = 0; i < WA_ITEMS; ++i) {
@@ -382,17 +397,18 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
   };
 
   if (warp < 8) {
-    regs_inc<192>();
+    regs_inc<KV8 ? 176 : 184>();
     // ------------------------------------------------------------- softmax
     const int i = warp >> 2;  // row tile
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t tS = tmem + lanes + i * 128, tO = tmem + lanes + 256 + i * 128;
-    uint32_t s_phase = 0, o_phase = 0;
+    uint32_t s_phase = 0, o_phase = 0, other_phase = 0;
     int tiles = 0, worked = 0;  // key tiles and items with keys so far
     for (int k = 0;; ++k) {
       const WaItem w = take(k);
       if (w.r < 0) break;
-      const int lr = i * 128 + (tid & 127), row = w.row0 + lr;
+      const bool duo = DUO && w.duo();
+      const int lr = (duo ? 0 : i * 128) + (tid & 127), row = w.row0 + lr;
       const bool live = lr < w.rows;
       auto out_row = [&](int at) {
         const int tok = a.by_g.div(at);
@@ -406,7 +422,42 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       const int tile0 = tiles, par = worked & 1;
       tiles += w.n;
       ++worked;
-      if (i >= w.mt()) continue;
+      if constexpr (KV8) {  // this row tile's queries to f16, each row with a power of two of its own
+        if (!mbar_wait(&ctl->q_raw, par, abort)) {
+          *abort = 1;
+          record_error(a.err, DEV_TIMEOUT_FULL);
+          break;
+        }
+        if (i < w.mt()) {
+          const int r128 = tid & 127;
+          uint8_t* qrow = sQ + i * TILE + r128 * 128;
+          auto piece = [&](int e) { return reinterpret_cast<uint4*>(qrow + (e >> 3) * 16384 + (((e & 7) ^ (r128 & 7)) << 4)); };
+          float amax = 0.0f;
+#pragma unroll 4
+          for (int e = 0; e < CPR; ++e) {
+            const uint4 v = *piece(e);
+            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(x[q] << 16)), fabsf(__uint_as_float(x[q] & 0xffff0000u))));
+          }
+          const float up = half_row_scale(amax), f = w.scale > 0.0f ? up : w.scale < 0.0f ? -up : 0.0f;
+#pragma unroll 4
+          for (int e = 0; e < CPR; ++e) {
+            const uint4 v = *piece(e);
+            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+            uint32_t y[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              y[q] = pack16(__uint_as_float(x[q] << 16) * f, __uint_as_float(x[q] & 0xffff0000u) * f, true);
+            *piece(e) = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+          ctl->qinv[par][i * 128 + r128] = 1.0f / up;
+        }
+        fence_async_smem();
+        mbar_arrive(&ctl->q_full);
+      }
+      if (!duo && i >= w.mt()) continue;
       // sees keys up to p (a row past the end stands where the last one does, and is not written),
       const int p = w.pos0 + a.by_g.div(live ? row : w.row0 + w.rows - 1);
       const int wlo = a.window > 0 ? p - a.window + 1 : 0;  // from wlo on or below sinks
@@ -414,7 +465,8 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       float sc = w.scale == 0.0f ? 1.0f : fabsf(w.scale);
       float m = -INFINITY, l = 0.0f;
       bool ok = true, nan = false;
-      for (int j = 0; j < w.n; ++j) {
+      const int first = duo ? i : 0, step = duo ? 2 : 1;
+      for (int j = first; j < w.n; j += step) {
         if (!mbar_wait(&ctl->s_full[i], s_phase, abort)) {
           ok = false;
           break;
@@ -424,7 +476,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
         float s[128];
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld_x32(tS + q * 32, s + q * 32);
-        if (KV8 && j == 0) sc *= ctl->qinv[par][lr];
+        if (KV8 && j == first) sc *= ctl->qinv[par][lr];
         const int j0 = w.key0(j);
         const uint4 vm4 = *reinterpret_cast<const uint4*>(ctl->valid[(tile0 + j) & 7]);
         const uint32_t vm[4] = {vm4.x, vm4.y, vm4.z, vm4.w};
@@ -451,7 +503,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
         const float mn = top > m + 8.0f || m == -INFINITY ? fmaxf(m, top) : m;
         if (__any_sync(0xffffffffu, mn != m)) {
           const float f = m == mn ? 1.0f : ex2(m - mn);
-          if (j > 0) {  // S is complete, so the product before it, P V of tile j - 1, is too
+          if (j > first) {  // S is complete, so the product with the V before it is too
 #pragma unroll
             for (int q = 0; q < HD / 16; ++q) {
               float o[16];
@@ -492,19 +544,50 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       }
       o_phase ^= 1;
       tc_fence_after();
+      if (m == -INFINITY) l = 0.0f;  // no score above -inf: zero
+      if (nan) l = NAN;              // a score that is no number: nor is the row
+      if (duo && i == 1) {  // the other warpgroup joins the two halves; S is free by now
+        tmem_st_x2(tS, m, l);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&ctl->other);
+        continue;
+      }
       float o[HD];
 #pragma unroll
       for (int q = 0; q < HD / 32; ++q) tmem_ld_x32(tO + q * 32, o + q * 32);
-      tmem_wait_ld();
+      if (duo) {
+        if (!mbar_wait(&ctl->other, other_phase, abort)) {
+          *abort = 1;
+          record_error(a.err, DEV_TIMEOUT_ACC);
+          break;
+        }
+        other_phase ^= 1;
+        tc_fence_after();
+        float m1, l1;
+        tmem_ld_x2(tS + 128, m1, l1);
+        tmem_wait_ld();
+        const float mm = fmaxf(m, m1), u = mm == -INFINITY ? 0.0f : mm, f = ex2(m - u), g = ex2(m1 - u);
+        l = l * f + l1 * g;
+        m = mm;
+#pragma unroll
+        for (int q = 0; q < HD / 16; ++q) {
+          float x[16];
+          tmem_ld_x16(tO + 128 + q * 16, x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[q * 16 + e] = o[q * 16 + e] * f + x[e] * g;
+        }
+      } else {
+        tmem_wait_ld();
+      }
       tc_fence_before();
       mbar_arrive(&ctl->o_empty[i]);  // the next item's product may overwrite it
-      // no score above -inf: zero; a score that is no number: nor is the row
-      if (m == -INFINITY) {
-        l = 0.0f;
+      if (duo) mbar_arrive(&ctl->o_empty[1]);
+      if (m == -INFINITY) {  // whatever 0 times the values was
 #pragma unroll
         for (int e = 0; e < HD; ++e) o[e] = 0.0f;
       }
-      if (nan) l = NAN;
       if (w.slot < 0) {
         const float inv = l == 0.0f ? 0.0f : w.vd / l;
         // Four lanes hand one another 16-byte pieces, so that they write 64
@@ -552,51 +635,27 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       }
     }
   } else if (warp < 12) {
-    regs_dec<64>();
+    regs_dec<KV8 ? 96 : 64>();
     // ------------------------------------------------------------- keys and values
     const int lw = warp - 8;  // rows 32 lw .. 32 lw + 31 of every tile
     bool ok = true;
-    int slot = 0, made = 0;  // ring position and entries (K and V of a tile in turn) so far
-    uint32_t phase = 1;      // an empty slot's first wait succeeds at once
-    int done_slot = 0;       // the oldest entry that is not handed over yet
-    uint32_t done_phase = 1;
-    int tiles = 0;
-    // hand the oldest entry to the tensor cores; at most PEND newer ones are in flight
-    auto hand_over = [&]() {
-      if constexpr (KV8) {  // widen it: e4m3 is exact in f16
-        __syncwarp();
-        if (!mbar_wait(&ctl->empty[done_slot], done_phase, abort)) {
-          ok = false;
-          return;
-        }
-        constexpr int RC = HD / 16, RPI = 32 / RC;
-        const int ch = lane % RC, odd = (ch >> 2) & 1;  // which half first: no two lanes of a row share a bank
-        const uint8_t* raw = sRaw + ((made - 1) & 1) * Lay::RAW + lw * 32 * HD;
-        uint8_t* dst = sKV + done_slot * TILE + (ch >> 2) * 16384;
-#pragma unroll 4
-        for (int u = 0; u < 32 / RPI; ++u) {
-          const int row = u * RPI + lane / RC, r128 = lw * 32 + row;
-          const uint4 x = *reinterpret_cast<const uint4*>(raw + row * HD + ch * 16);
-          uint4 h0, h1;
-          e4m3x4_h(x.x, h0.x, h0.y);
-          e4m3x4_h(x.y, h0.z, h0.w);
-          e4m3x4_h(x.z, h1.x, h1.y);
-          e4m3x4_h(x.w, h1.z, h1.w);
-          uint8_t* drow = dst + r128 * 128;
-          const int c0 = (2 * ch) & 7;
-          *reinterpret_cast<uint4*>(drow + (((c0 + odd) ^ (r128 & 7)) << 4)) = odd ? h1 : h0;
-          *reinterpret_cast<uint4*>(drow + (((c0 + 1 - odd) ^ (r128 & 7)) << 4)) = odd ? h0 : h1;
-        }
-        __syncwarp();  // the raw rows may be overwritten from here on
-      }
-      fence_async_smem();
-      mbar_arrive(&ctl->full[done_slot]);
-      if (++done_slot == SLOTS) {
-        done_slot = 0;
-        done_phase ^= 1;
+    int slot = 0, tiles = 0;
+    uint32_t phase = 1;  // an empty slot's first wait succeeds at once
+    constexpr int RC = HD * (KV8 ? 1 : 2) / 16, RPI = 32 / RC, U = 32 / RPI;  // 16-byte chunks of a cache row, rows at a time
+    const int ch = lane % RC, sub = lane / RC;
+    auto advance = [&]() {
+      if (++slot == SLOTS) {
+        slot = 0;
+        phase ^= 1;
       }
     };
-    constexpr int PEND = Lay::LAG;
+    int behind = 0, oldest = 0;  // entries whose copies are not handed over, and the first of them
+    auto hand_over = [&]() {
+      fence_async_smem();
+      mbar_arrive(&ctl->full[oldest]);
+      oldest = oldest + 1 == SLOTS ? 0 : oldest + 1;
+      --behind;
+    };
     for (int k = 0; ok; ++k) {
       const WaItem w = take(k);
       if (w.r < 0) break;
@@ -612,62 +671,100 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
         record_error(a.err, DEV_BAD_INDEX);
         return -2;
       };
+      // byte offsets of this lane's key and value, -1 where there is none:
+      // rows that are not seen are zero, what the cache holds there may be no number
+      auto k_off = [&](int page, int tok) {
+        return page < 0 ? -1ll : page * a.c.kps + (long long)w.c * a.c.khs + tok * a.c.kts;
+      };
+      auto v_off = [&](int page, int tok) {
+        return page < 0 ? -1ll : page * a.c.vps + (long long)w.c * a.c.vhs + tok * a.c.vts;
+      };
       int tok_next = 0, page_next = lookup(0, &tok_next);
-      for (int j = 0; j < w.n && ok; ++j, ++tiles) {
-        const int page = page_next, tok = tok_next;
-        page_next = lookup(j + 1, &tok_next);
-        const uint32_t good = __ballot_sync(0xffffffffu, page != -2);
-        if (lane == 0) ctl->valid[tiles & 7][lw] = good;
+      if constexpr (KV8) {
+        // e4m3 rows come into registers, one tile ahead, and go on as f16, which holds them exactly
+        uint4 xk[U], xv[U];
+        auto fetch = [&](uint4* x, const uint8_t* from, long long off) {
 #pragma unroll
-        for (int is_v = 0; is_v < 2; ++is_v) {
-          if (!KV8 && !mbar_wait(&ctl->empty[slot], phase, abort)) {
+          for (int u = 0; u < U; ++u) {
+            const long long o = __shfl_sync(0xffffffffu, off, u * RPI + sub);
+            x[u] = o < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(from + o + ch * 16);
+          }
+        };
+        auto widen = [&](const uint4* x) {
+          if (!mbar_wait(&ctl->empty[slot], phase, abort)) {
             ok = false;
-            break;
+            return;
           }
-          const uint8_t* src = is_v ? a.c.v : a.c.k;
-          long long off = -1;
-          if (page >= 0)
-            off = is_v ? page * a.c.vps + (long long)w.c * a.c.vhs + (long long)tok * a.c.vts
-                       : page * a.c.kps + (long long)w.c * a.c.khs + (long long)tok * a.c.kts;
-          constexpr int RC = KV8 ? HD / 16 : CPR;  // 16-byte chunks of a cache row
-          constexpr int RPI = 32 / RC;
-          const int ch = lane % RC;
-          const uint32_t dst = KV8 ? smem_u32(sRaw) + (made & 1) * Lay::RAW + lw * 32 * HD
-                                   : smem_u32(sKV) + slot * TILE + (ch >> 3) * 16384 + lw * 32 * 128;
-#pragma unroll 4
-          for (int u = 0; u < 32 / RPI; ++u) {
-            const int row = u * RPI + lane / RC;
-            const long long o = __shfl_sync(0xffffffffu, off, row);
-            // keys that no row sees are zero: what the cache holds there may be no number
-            pc_cp_async16(KV8 ? dst + row * HD + ch * 16 : dst + row * 128 + (((ch & 7) ^ (row & 7)) << 4),
-                          src + (o < 0 ? 0 : o + ch * 16), o < 0 ? 0u : 16u);
+          uint8_t* dst = sKV + slot * TILE + (ch >> 2) * 16384 + (lw * 32 + sub) * 128;
+          const int c0 = (2 * ch) & 7, odd = (ch >> 2) & 1;  // which half first: no two lanes of a row share a bank
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            uint4 h0, h1;
+            e4m3x4_h(x[u].x, h0.x, h0.y);
+            e4m3x4_h(x[u].y, h0.z, h0.w);
+            e4m3x4_h(x[u].z, h1.x, h1.y);
+            e4m3x4_h(x[u].w, h1.z, h1.w);
+            const int sw = (u * RPI + sub) & 7;
+            *reinterpret_cast<uint4*>(dst + u * RPI * 128 + (((c0 + odd) ^ sw) << 4)) = odd ? h1 : h0;
+            *reinterpret_cast<uint4*>(dst + u * RPI * 128 + (((c0 + 1 - odd) ^ sw) << 4)) = odd ? h0 : h1;
           }
-          pc_cp_commit();
-          if (made >= PEND) {
-            pc_cp_wait<PEND>();
-            hand_over();
-            if (!ok) break;
-          }
-          ++made;
-          if (++slot == SLOTS) {
-            slot = 0;
-            phase ^= 1;
+          fence_async_smem();
+          mbar_arrive(&ctl->full[slot]);
+          advance();
+        };
+        int page = page_next, tok = tok_next;
+        if (w.n > 0) fetch(xk, a.c.k, k_off(page, tok));
+        for (int j = 0; j < w.n && ok; ++j, ++tiles) {
+          page_next = lookup(j + 1, &tok_next);
+          const uint32_t good = __ballot_sync(0xffffffffu, page != -2);
+          if (lane == 0) ctl->valid[tiles & 7][lw] = good;
+          fetch(xv, a.c.v, v_off(page, tok));
+          widen(xk);
+          page = page_next;
+          tok = tok_next;
+          if (j + 1 < w.n) fetch(xk, a.c.k, k_off(page, tok));
+          if (ok) widen(xv);
+        }
+      } else {
+        for (int j = 0; j < w.n && ok; ++j, ++tiles) {
+          const int page = page_next, tok = tok_next;
+          page_next = lookup(j + 1, &tok_next);
+          const uint32_t good = __ballot_sync(0xffffffffu, page != -2);
+          if (lane == 0) ctl->valid[tiles & 7][lw] = good;
+#pragma unroll
+          for (int is_v = 0; is_v < 2; ++is_v) {
+            const long long off = is_v ? v_off(page, tok) : k_off(page, tok);
+            const uint8_t* from = (is_v ? a.c.v : a.c.k) + ch * 16;
+            if (!mbar_wait(&ctl->empty[slot], phase, abort)) {
+              ok = false;
+              break;
+            }
+            const uint32_t dst = smem_u32(sKV) + slot * TILE + (ch >> 3) * 16384 + (lw * 32 + sub) * 128;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const long long o = __shfl_sync(0xffffffffu, off, u * RPI + sub);
+              pc_cp_async16(dst + u * RPI * 128 + (((ch & 7) ^ ((u * RPI + sub) & 7)) << 4), from + (o < 0 ? 0 : o),
+                            o < 0 ? 0u : 16u);
+            }
+            pc_cp_commit();
+            advance();
+            // the entry WA_LAG before this one has arrived: hand it to the tensor cores
+            if (++behind > WA_LAG) {
+              pc_cp_wait<WA_LAG>();
+              hand_over();
+            }
           }
         }
       }
     }
-    // the last entries
-    if (ok) {
-      pc_cp_wait<0>();
-      for (int e = min(made, PEND); e > 0 && ok; --e) hand_over();
-    }
-    pc_cp_wait<0>();
+    pc_cp_wait<0>();  // nothing of this CTA may be in flight when it ends
+    while (!KV8 && ok && behind > 0) hand_over();
     if (!ok) {
       *abort = 1;
       record_error(a.err, DEV_TIMEOUT_EMPTY);
     }
   } else {
-    regs_dec<64>();
+    regs_dec<KV8 ? 64 : 80>();
     if (warp == 12) {
       // ------------------------------------------------------------- products
       // The whole warp goes through the loop, so that the operands' addresses
@@ -676,8 +773,8 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       const bool leader = elect_one();
       const uint32_t q_lo = desc_lo_k(smem_u32(sQ)), kv = smem_u32(sKV);
       auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort)); };
-      auto product_s = [&](int i, int slot) {
-        const uint32_t qa = q_lo + i * (TILE >> 4), kb = desc_lo_k(kv + slot * TILE), d = tmem + i * 128;
+      auto product_s = [&](int i, int rows_of, int slot) {
+        const uint32_t qa = q_lo + rows_of * (TILE >> 4), kb = desc_lo_k(kv + slot * TILE), d = tmem + i * 128;
         if (leader) {
 #pragma unroll
           for (int k = 0; k < HD / 16; ++k) {
@@ -696,74 +793,117 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
           for (int k = 0; k < 4; ++k) umma_ts(d, pa + k * 8, vb + k * 128, ID_O, k > 0 ? 1u : accumulate);
         }
       };
-      int code = 0, slot = 0;
+      auto release = [&](uint64_t* bar) {
+        if (leader) umma_commit(bar);
+      };
+      int code = 0, slot = 0;  // slot and phase: the ring's entry that comes next in this item
       uint32_t phase = 0, q_phase = 0, p_phase[2] = {0, 0}, o_phase[2] = {1, 1};
-      auto next = [&]() {
-        if (++slot == SLOTS) {
-          slot = 0;
+      bool s1_read = false;  // the second S holds what the last item's epilogue still reads
+      auto slot_of = [&](int e) { return slot + e >= SLOTS ? slot + e - SLOTS : slot + e; };  // e < SLOTS
+      // entry e from the next one on is in shared memory
+      auto filled = [&](int e) {
+        if (!wait(&ctl->full[slot_of(e)], slot + e >= SLOTS ? phase ^ 1 : phase)) code = DEV_TIMEOUT_FULL;
+        return !code;
+      };
+      auto skip = [&](int e) {
+        slot += e;
+        if (slot >= SLOTS) {
+          slot -= SLOTS;
           phase ^= 1;
         }
+      };
+      auto emptied = [&](int i) {  // what row tile i of the item before left in tensor memory is read
+        if (!wait(&ctl->o_empty[i], o_phase[i])) code = DEV_TIMEOUT_ACC;
+        o_phase[i] ^= 1;
+        return !code;
+      };
+      // O_i += P_i V, as P's halves arrive
+      auto add_pv = [&](int i, int sv, bool fresh) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (!wait(&ctl->p_ready[i][half], p_phase[i])) {
+            code = DEV_TIMEOUT_ACC;
+            return false;
+          }
+          tc_fence_after();
+          product_o(i, sv, half, !fresh || half > 0);
+        }
+        p_phase[i] ^= 1;
+        return true;
       };
       for (int k = 0; !code; ++k) {
         const WaItem w = take(k);
         const int r = __shfl_sync(0xffffffffu, w.r, 0), n = __shfl_sync(0xffffffffu, w.n, 0);
         const int mt = __shfl_sync(0xffffffffu, w.mt(), 0);
+        const bool duo = DUO && __shfl_sync(0xffffffffu, (int)w.duo(), 0);
         if (r < 0) break;
         if (n <= 0) continue;
-        if (!wait(&ctl->q_full, q_phase) || !wait(&ctl->full[slot], phase)) {
-          code = DEV_TIMEOUT_FULL;
-          break;
-        }
+        if (!wait(&ctl->q_full, q_phase)) code = DEV_TIMEOUT_FULL;
         q_phase ^= 1;
+        if (code || !filled(0)) break;
         tc_fence_after();
-        for (int i = 0; i < mt; ++i) product_s(i, slot);
-        if (leader) {
-          umma_commit(&ctl->empty[slot]);
-          if (n == 1) umma_commit(&ctl->q_empty);
+        bool early = false;  // emptied(1) is done
+        if ((duo || mt == 2) && s1_read) {
+          if (!emptied(1)) break;
+          early = true;
+          s1_read = false;
         }
-        next();
-        for (int j = 0; j < n && !code; ++j) {
-          const bool more = j + 1 < n;
-          const int sv = slot;
-          if (!wait(&ctl->full[sv], phase)) {
-            code = DEV_TIMEOUT_FULL;
-            break;
-          }
-          next();
-          const int sk = slot;
+        if (duo) {
+          // ring entries from here: K0 V0 K1 V1 ...; warpgroup i has the key tiles j with j % 2 == i
+          product_s(0, 0, slot);
+          release(&ctl->empty[slot]);
+          if (!filled(2)) break;
+          product_s(1, 0, slot_of(2));
+          release(&ctl->empty[slot_of(2)]);
+          if (n == 2) release(&ctl->q_empty);
+          skip(1);
+          for (int j = 0; j < n; j += 2) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (i >= mt || code) break;
-            if (j == 0) {  // the item before has read its O
-              if (!wait(&ctl->o_empty[i], o_phase[i])) code = DEV_TIMEOUT_ACC;
-              o_phase[i] ^= 1;
-            }
-            for (int half = 0; half < 2 && !code; ++half) {
-              if (!wait(&ctl->p_ready[i][half], p_phase[i])) {
-                code = DEV_TIMEOUT_ACC;
-                break;
+            for (int i = 0; i < 2; ++i) {  // the next entry is the V of tile j + i
+              if (j + i >= n || code) break;
+              if (j == 0 && !(i == 1 && early) && !emptied(i)) break;
+              if (!filled(0) || !add_pv(i, slot, j == 0)) break;
+              release(&ctl->empty[slot]);
+              if (j + i + 2 < n) {
+                if (!filled(3)) break;
+                product_s(i, 0, slot_of(3));
+                release(&ctl->empty[slot_of(3)]);
+                if (j + i + 3 == n) release(&ctl->q_empty);
+              } else {
+                release(&ctl->o_done[i]);
               }
-              tc_fence_after();
-              product_o(i, sv, half, j > 0 || half > 0);
+              skip(j + i + 1 < n ? 2 : 1);
             }
             if (code) break;
-            p_phase[i] ^= 1;
-            if (leader && i == mt - 1) umma_commit(&ctl->empty[sv]);
-            if (!more) {
-              if (leader) umma_commit(&ctl->o_done[i]);
-              continue;
-            }
-            if (i == 0 && !wait(&ctl->full[sk], phase)) {
-              code = DEV_TIMEOUT_FULL;
-              break;
-            }
-            product_s(i, sk);
-            if (leader && i == mt - 1) {
-              umma_commit(&ctl->empty[sk]);
-              if (j + 2 == n) umma_commit(&ctl->q_empty);
-            }
           }
-          if (more) next();
+          s1_read = true;
+        } else {
+          for (int i = 0; i < mt; ++i) product_s(i, i, slot);
+          release(&ctl->empty[slot]);
+          if (n == 1) release(&ctl->q_empty);
+          skip(1);
+          for (int j = 0; j < n && !code; ++j) {
+            const bool more = j + 1 < n;
+            if (!filled(0)) break;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (i >= mt || code) break;
+              if (j == 0 && !(i == 1 && early) && !emptied(i)) break;
+              if (!add_pv(i, slot, j == 0)) break;
+              if (i == mt - 1) release(&ctl->empty[slot]);
+              if (!more) {
+                release(&ctl->o_done[i]);
+                continue;
+              }
+              if (i == 0 && !filled(1)) break;
+              product_s(i, i, slot_of(1));
+              if (i == mt - 1) {
+                release(&ctl->empty[slot_of(1)]);
+                if (j + 2 == n) release(&ctl->q_empty);
+              }
+            }
+            skip(more ? 2 : 1);
+          }
         }
       }
       if (code) {
@@ -780,7 +920,6 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       const WaBorder end = ctl->border[1];
       WaCutItem cut{0, 0, 0, 0, 0, WA_NONE};
       uint32_t q_phase = 1;
-      int worked = 0;
       bool ok = true;
       for (int k = 0; ok; ++k) {
         WaItem w;
@@ -864,31 +1003,18 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
         }
         pc_cp_commit();
         pc_cp_wait<0>();
-        if (KV8 || !(w.scale > 0.0f)) {
-          for (int lr = (warp - 13) * RPI + lane / CPR; lr - lane / CPR < rows; lr += 3 * RPI) {
-            uint4 v = lr < rows ? *reinterpret_cast<const uint4*>(chunk(lr)) : make_uint4(0, 0, 0, 0);
-            uint32_t* x = reinterpret_cast<uint32_t*>(&v);
-            if constexpr (KV8) {
-              float amax = 0.0f;
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(x[e] << 16)), fabsf(__uint_as_float(x[e] & 0xffff0000u))));
-#pragma unroll
-              for (int off = 1; off < CPR; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-              const float f = half_row_scale(amax);
-              if (ch == 0 && lr < rows) ctl->qinv[worked & 1][lr] = 1.0f / f;
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                x[e] = pack16(__uint_as_float(x[e] << 16) * f, __uint_as_float(x[e] & 0xffff0000u) * f, true);
+        if constexpr (KV8) {  // the softmax threads turn them into f16
+          mbar_arrive(&ctl->q_raw);
+        } else {
+          if (!(w.scale > 0.0f))
+            for (int lr = (warp - 13) * RPI + lane / CPR; lr < rows; lr += 3 * RPI) {
+              uint4* at = reinterpret_cast<uint4*>(chunk(lr));
+              const uint32_t keep = w.scale < 0.0f ? ~0u : 0u, flip = w.scale < 0.0f ? 0x80008000u : 0u;
+              *at = make_uint4((at->x & keep) ^ flip, (at->y & keep) ^ flip, (at->z & keep) ^ flip, (at->w & keep) ^ flip);
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = w.scale > 0.0f ? x[e] : w.scale < 0.0f ? x[e] ^ 0x80008000u : 0u;
-            if (lr < rows) *reinterpret_cast<uint4*>(chunk(lr)) = v;
-          }
+          fence_async_smem();
+          mbar_arrive(&ctl->q_full);
         }
-        ++worked;
-        fence_async_smem();
-        mbar_arrive(&ctl->q_full);
       }
       pc_cp_wait<0>();
     }
@@ -962,15 +1088,20 @@ WindowPlan window_plan(int64_t R, int64_t T, int64_t H, int64_t KH, int64_t HD, 
   return p;
 }
 
-template <int HD, bool KV8>
+template <int HD, bool KV8, bool DUO>
 fm_status launch_window(const WindowArgs& a, const WindowPlan& pl, cudaStream_t s) {
-  constexpr int smem = WaLayout<HD, KV8>::SMEM;
+  constexpr int smem = WaLayout<HD>::SMEM;
   static_assert(sizeof(WaCtrl) <= 3072 && smem <= 232448, "shared memory");
-  fm_status st = allow_smem<window_attn_kernel<HD, KV8>>(smem, "paged_window_attn");
+  fm_status st = allow_smem<window_attn_kernel<HD, KV8, DUO>>(smem, "paged_window_attn");
   if (st != FM_OK) return st;
-  st = launch_kernel(window_attn_kernel<HD, KV8>, dim3((unsigned)pl.ctas), dim3(512), smem, s, false, a);
+  st = launch_kernel(window_attn_kernel<HD, KV8, DUO>, dim3((unsigned)pl.ctas), dim3(512), smem, s, false, a);
   if (st != FM_OK || !pl.cuts) return st;
   return launch_kernel(window_join_kernel<HD>, dim3((unsigned)pl.ctas, HD / 16), dim3(WA_ROWS), 0, s, true, a, pl.ctas);
+}
+
+template <int HD, bool KV8>
+fm_status launch_window(const WindowArgs& a, const WindowPlan& pl, bool duo, cudaStream_t s) {
+  return duo ? launch_window<HD, KV8, true>(a, pl, s) : launch_window<HD, KV8, false>(a, pl, s);
 }
 
 }  // namespace
@@ -1030,7 +1161,7 @@ extern "C" fm_status fm_paged_window_attn(const fm_paged_cache* cache, const fm_
   a.stats = reinterpret_cast<float2*>(ws + pl.part);
   a.cuts = reinterpret_cast<WaCutItem*>(ws + pl.part + pl.stats);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool kv8 = cache->dtype == FM_DT_E4M3;
-  if (cache->head_dim == 128) return kv8 ? launch_window<128, true>(a, pl, s) : launch_window<128, false>(a, pl, s);
-  return kv8 ? launch_window<64, true>(a, pl, s) : launch_window<64, false>(a, pl, s);
+  const bool kv8 = cache->dtype == FM_DT_E4M3, duo = p->max_q * a.G <= 128;
+  if (cache->head_dim == 128) return kv8 ? launch_window<128, true>(a, pl, duo, s) : launch_window<128, false>(a, pl, duo, s);
+  return kv8 ? launch_window<64, true>(a, pl, duo, s) : launch_window<64, false>(a, pl, duo, s);
 }
