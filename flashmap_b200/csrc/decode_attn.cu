@@ -31,7 +31,7 @@ struct DecodeArgs {
   int H, G, hgroups;     // heads, heads per kv head, CTAs' head groups per kv head
   float scale;           // softmax_scale * log2(e)
   int window, sinks;
-  int chunk, chunks;     // keys per chunk, chunks per item
+  int least, chunks;     // keys of a chunk at least, chunks of an item at most
   __nv_bfloat16* out;
   long long o_rs, o_hs;
   float* sums;
@@ -42,6 +42,15 @@ struct DecodeArgs {
   int pitch;
   int* err;
 };
+
+// Keys of a chunk of n visible positions.  Up to DA_WHOLE stay one chunk, which
+// needs no join (201 positions, 1 request: 5.2 us against 6.3 us in chunks of 128).
+constexpr int DA_WHOLE = 256;
+__device__ __forceinline__ int chunk_of(const DecodeArgs& a, int n) {
+  if (n <= DA_WHOLE) return DA_WHOLE;
+  const int even = (((n + a.chunks - 1) / a.chunks) + 63) & ~63;
+  return even > a.least ? even : a.least;
+}
 
 template <int HD, bool KV8>
 struct DaLayout {
@@ -65,7 +74,8 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
   using Lay = DaLayout<HD, KV8>;
   constexpr int RB = Lay::RB, MT = HD / 16, KS = HD / 16;
   extern __shared__ __align__(1024) uint8_t da_smem_buf[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+  // a uniform warp number spares the e4m3 kernel the registers that keep a fourth CTA off the SM
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   pdl_wait();
   const int items = a.c.R * a.c.KH * a.hgroups;
   const int chunk = blockIdx.x / items;
@@ -77,14 +87,14 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
   const int nh = min(8 * NG, a.G - hg * 8 * NG);        // query heads of this CTA
   const int len = cache_length(a.c, r, a.err, threadIdx.x == 0 && chunk == 0);
   const Span sp = visible_span(len, a.window, a.sinks);
-  const int begin = chunk * a.chunk;
-  const int end = min(sp.n, begin + a.chunk);
-  if (begin >= end) {
+  const int size = chunk_of(a, sp.n);
+  if ((long long)chunk * size >= sp.n) {
     if (chunk == 0)  // nothing to attend to: zero rows
       for (int i = threadIdx.x; i < nh * HD; i += 128)
         a.out[(long long)r * a.o_rs + (long long)(h0 + i / HD) * a.o_hs + i % HD] = f2bf(0.0f);
     return;
   }
+  const int begin = chunk * size, end = min(sp.n, begin + size);
 
   float kd = 1.0f, vd = 1.0f;
   if (a.c.descales) {
@@ -324,7 +334,7 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
       }
   }
   __syncthreads();
-  const bool single = sp.n <= a.chunk;
+  const bool single = sp.n <= chunk_of(a, sp.n);
   if (threadIdx.x < nh) {
     float mm = -INFINITY, ll = 0.0f;
     for (int w = 0; w < 4; ++w) mm = fmaxf(mm, mS[w * 8 * NG + threadIdx.x].x);
@@ -405,7 +415,7 @@ __global__ void __launch_bounds__(NT) decode_join_kernel(DecodeArgs a, int row_b
     const int row = blockIdx.x * (NT / 32) + warp, r = row / a.H, h = row % a.H;
     if (row >= rows) return;
     const Span sp = visible_span(cache_length(a.c, r, a.err, false), a.window, a.sinks);
-    const int n = (sp.n + a.chunk - 1) / a.chunk;
+    const int size = chunk_of(a, sp.n), n = (sp.n + size - 1) / size;
     if (n <= 1) return;  // written by its only chunk
     const float2* stats = a.stats + (long long)row * a.chunks;
     const float* part = a.part + (long long)row * a.chunks * HD + lane * (HD / 32);
@@ -432,7 +442,7 @@ __global__ void __launch_bounds__(NT) decode_join_kernel(DecodeArgs a, int row_b
   if (!WARP_ROWS && (int)blockIdx.x < row_blocks) {
     const int row = blockIdx.x, r = row / a.H, h = row % a.H;
     const Span sp = visible_span(cache_length(a.c, r, a.err, false), a.window, a.sinks);
-    const int n = (sp.n + a.chunk - 1) / a.chunk;
+    const int size = chunk_of(a, sp.n), n = (sp.n + size - 1) / size;
     if (n <= 1) return;  // written by its only chunk
     const float2* stats = a.stats + (long long)row * a.chunks;
     const float2 st = row_stats(stats, n);
@@ -477,7 +487,7 @@ __global__ void __launch_bounds__(NT) decode_join_kernel(DecodeArgs a, int row_b
   const Span sp = visible_span(cache_length(a.c, r, a.err, false), a.window, a.sinks);
   const int begin = kb * DJ_KEYS;
   if (begin >= sp.n) return;
-  const int n = (sp.n + a.chunk - 1) / a.chunk;
+  const int size = chunk_of(a, sp.n), n = (sp.n + size - 1) / size;
   const long long row0 = (long long)r * a.H + c * a.G;
   float* dst = a.sums + (long long)r * a.s_rs + (long long)c * a.s_hs;
   const int i = begin + tid * 4;  // this thread's four positions (the pitch is a multiple of 16)
@@ -512,19 +522,20 @@ __global__ void __launch_bounds__(NT) decode_join_kernel(DecodeArgs a, int row_b
     if (i + e < sp.n) dst[sp.pos(i + e)] = old[e] + w[e];
 }
 struct DecodePlan {
-  int ng, hgroups, chunk, chunks, pitch;
+  int ng, hgroups, least, chunks, pitch;
   size_t part, stats, scores, total;
 };
 
-// Chunks of equal length, so many that the launch has DA_CTAS CTAs when every
-// request is as long as the longest may be.  Up to DA_WHOLE positions stay one
-// chunk, which needs no join (201 positions, 1 request: 5.2 us against 6.3 us in
-// chunks of 128); longer spans are cut into 128 at least (500 positions: 6.0 us
-// against 7.8 us in chunks of 256 and 6.0 us in chunks of 64, 8 requests of 1000:
-// 10.9, 8.9 and 12.3 us).
-constexpr int DA_WHOLE = 256;
-constexpr int DA_CHUNK = 128;
+// Every request is cut into equal chunks, so many that the launch has DA_CTAS
+// CTAs; the kernel finds their size from the request's own length, so that a
+// call sized for far longer contexts than it meets still uses the whole GPU.
+// Chunks have DA_CHUNK keys at least (500 positions, 1 request: 6.0 us against
+// 7.8 us in chunks of 256 and 6.0 us in chunks of 64), and more where there are
+// enough (request, kv head) pairs to fill the GPU without cutting, three CTAs
+// to an SM: then a cut only makes a join.
 constexpr int DA_CTAS = 148 * 12;
+constexpr int DA_CHUNK = 128;
+constexpr int DA_ENOUGH = 1024;
 
 DecodePlan decode_plan(int64_t R, int64_t H, int64_t KH, int64_t HD, int64_t max_len, int64_t window, bool sums,
                        int64_t sinks) {
@@ -534,11 +545,11 @@ DecodePlan decode_plan(int64_t R, int64_t H, int64_t KH, int64_t HD, int64_t max
   p.hgroups = (int)((G + 8 * p.ng - 1) / (8 * p.ng));
   const int64_t span = visible_span((int)max_len, (int)window, (int)sinks).n;
   const int64_t items = R * KH * p.hgroups, cut = (DA_CTAS + items - 1) / items;
-  int64_t chunk = ((span + cut - 1) / cut + 63) / 64 * 64;
-  if (span <= DA_WHOLE) chunk = DA_WHOLE;
-  if (chunk < DA_CHUNK) chunk = DA_CHUNK;
-  p.chunk = (int)chunk;
-  p.chunks = (int)((span + chunk - 1) / chunk);
+  int64_t least = DA_ENOUGH * items / (3 * 148) / 64 * 64;
+  least = least < DA_CHUNK ? DA_CHUNK : least > DA_ENOUGH ? DA_ENOUGH : least;
+  p.least = (int)least;
+  const int64_t most = span <= DA_WHOLE ? 1 : (span + least - 1) / least;
+  p.chunks = (int)(cut < most ? cut : most);
   if (p.chunks < 1) p.chunks = 1;
   p.pitch = (int)((span + 15) / 16 * 16);
   auto up = [](size_t b) { return (b + 255) / 256 * 256; };
@@ -607,7 +618,7 @@ extern "C" fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_
   a.scale = p->softmax_scale * kLog2e;
   a.window = (int)p->window;
   a.sinks = (int)p->sinks;
-  a.chunk = pl.chunk;
+  a.least = pl.least;
   a.chunks = pl.chunks;
   a.out = static_cast<__nv_bfloat16*>(p->out);
   a.o_rs = p->out_request_stride;
