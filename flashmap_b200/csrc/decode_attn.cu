@@ -535,7 +535,7 @@ struct DecodePlan {
 // to an SM: then a cut only makes a join.
 constexpr int DA_CTAS = 148 * 12;
 constexpr int DA_CHUNK = 128;
-constexpr int DA_ENOUGH = 1024;
+constexpr int DA_ENOUGH = 1536;
 
 DecodePlan decode_plan(int64_t R, int64_t H, int64_t KH, int64_t HD, int64_t max_len, int64_t window, bool sums,
                        int64_t sinks) {
