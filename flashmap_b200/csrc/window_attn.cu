@@ -36,7 +36,8 @@ struct WindowArgs {
   long long o_ts, o_hs;
   float* part;    // [2 CTAs][256][HD] outputs of items that are cut, not yet divided by their sums
   float2* stats;  // [2 CTAs][256] (maximum, sum), base-2 scores
-  WaCutItem* cuts;  // [CTAs]
+  WaCutItem* cuts;  // [CTAs], or null: items are not cut
+  int row_tiles;    // no fewer than there are
   int* err;
 };
 
@@ -69,6 +70,28 @@ __device__ __forceinline__ int wa_row_tiles(const WindowArgs& a, int nq) {
   return (int)(((long long)nq * a.G + WA_ROWS - 1) / WA_ROWS);
 }
 
+// Request and row tile that come at `tile` in the batch, or request -1; by one warp.
+__device__ __forceinline__ int2 wa_find(const WindowArgs& a, int tile) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int r0 = 0; r0 < a.c.R; r0 += 32) {
+    const int r = r0 + lane, n = r < a.c.R ? wa_row_tiles(a, wa_queries(a, r, true)) : 0;
+    int scan = n;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, scan, off);
+      if (lane >= off) scan += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + scan > tile);
+    if (hit) {
+      const int w = __ffs(hit) - 1;
+      return make_int2(r0 + w, tile - __shfl_sync(0xffffffffu, before + scan - n, w));
+    }
+    before += __shfl_sync(0xffffffffu, scan, 31);
+  }
+  return make_int2(-1, 0);
+}
+
 // Work is dealt out by key tiles: the items (row tile by row tile, kv head by
 // kv head) lie end to end, each as long as its key tiles plus WA_ITEM for what
 // an item costs besides, and every CTA takes an equal length.  An item that
@@ -77,6 +100,10 @@ __device__ __forceinline__ int wa_row_tiles(const WindowArgs& a, int nq) {
 constexpr int WA_ITEM = 2;
 constexpr int WA_CUT = 2;
 constexpr int WA_SHARE = WA_ITEM + 4;  // the least length of a CTA's share
+//
+// Where items are too short to cut and there are enough of them, CTA b simply
+// takes items b, b + CTAs, .. from the last row tile on (the longest of a
+// prompt): no shares, no join (12 windowed prompts: 65 us, with shares 68 us).
 struct WaBorder {
   int r, y, c, t;  // request, row tile, kv head, and the first tile after the border
 };
@@ -319,7 +346,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
     *all = sum;
     return before + x - v;
   };
-  {
+  if (a.cuts != nullptr) {
     int* pre = reinterpret_cast<int*>(sKV);                                // row tiles before request r
     long long* chunk = reinterpret_cast<long long*>(sKV + WA_REQUESTS * 4);  // length of 512 row tiles
     long long row_tiles = 0;
@@ -916,8 +943,14 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       }
     } else {
       // ------------------------------------------------------------- work items and queries
-      WaBorder cur = ctl->border[0];
-      const WaBorder end = ctl->border[1];
+      const bool shares = a.cuts != nullptr;
+      const long long items = (long long)a.row_tiles * a.c.KH;
+      long long id = blockIdx.x;  // the next item, where there are no shares
+      WaBorder cur{0, 0, 0, 0}, end{a.c.R, 0, 0, 0};
+      if (shares) {
+        cur = ctl->border[0];
+        end = ctl->border[1];
+      }
       WaCutItem cut{0, 0, 0, 0, 0, WA_NONE};
       uint32_t q_phase = 1;
       bool ok = true;
@@ -926,6 +959,17 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
         if (warp == 13) {
           w.r = -1;
           while (w.r < 0 && cur.r < a.c.R) {
+            if (!shares) {
+              if (id >= items) break;
+              const int back = (int)(id / a.c.KH);
+              const int2 at = wa_find(a, a.row_tiles - 1 - back);
+              cur = WaBorder{at.x, at.y, (int)(id - (long long)back * a.c.KH), 0};
+              id += gridDim.x;
+              if (at.x < 0) {  // the bound on the row tiles was above their number
+                cur.r = 0;
+                continue;
+              }
+            }
             const int nq = wa_queries(a, cur.r, false), row0 = cur.y * WA_ROWS;
             if (cur.y >= wa_row_tiles(a, nq)) {
               cur = WaBorder{cur.r + 1, 0, 0, 0};
@@ -962,6 +1006,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
               cut.goes_on = WA_EMPTY;
             }
             cur.t = 0;
+            if (!shares) continue;
             if (last) {
               cur.r = a.c.R;
             } else if (++cur.c == a.c.KH) {
@@ -969,7 +1014,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
               ++cur.y;
             }
           }
-          if (w.r < 0 && lane == 0) a.cuts[blockIdx.x] = cut;
+          if (w.r < 0 && shares && lane == 0) a.cuts[blockIdx.x] = cut;
           if (!mbar_wait(&ctl->item_empty[k % WA_ITEMS], ((k / WA_ITEMS) & 1) ^ 1, abort)) {
             *abort = 1;
             record_error(a.err, DEV_TIMEOUT_OTHER);
@@ -1078,13 +1123,13 @@ WindowPlan window_plan(int64_t R, int64_t T, int64_t H, int64_t KH, int64_t HD, 
   const int64_t tokens = max_q < WA_ROWS ? max_q : WA_ROWS;
   if (window > 0 && window + tokens + sinks < span) span = window + tokens + sinks;
   const int64_t tiles = span / WA_KEYS + 3;
-  p.cuts = tiles >= 2 * WA_CUT;
+  p.cuts = tiles >= (items >= sms ? 8 : 2 * WA_CUT);
   // an item that can be cut gives work to as many CTAs as it has tiles at most
   const int64_t most = p.cuts ? items * tiles : items;
   p.ctas = (int)(most < sms ? most : sms);
   p.part = p.cuts ? (size_t)p.ctas * 2 * WA_ROWS * HD * 4 : 0;
   p.stats = p.cuts ? (size_t)p.ctas * 2 * WA_ROWS * 8 : 0;
-  p.total = p.part + p.stats + (size_t)p.ctas * sizeof(WaCutItem);
+  p.total = p.part + p.stats + (p.cuts ? (size_t)p.ctas * sizeof(WaCutItem) : 0);
   return p;
 }
 
@@ -1159,7 +1204,8 @@ extern "C" fm_status fm_paged_window_attn(const fm_paged_cache* cache, const fm_
   uint8_t* ws = static_cast<uint8_t*>(p->workspace);
   a.part = reinterpret_cast<float*>(ws);
   a.stats = reinterpret_cast<float2*>(ws + pl.part);
-  a.cuts = reinterpret_cast<WaCutItem*>(ws + pl.part + pl.stats);
+  a.cuts = pl.cuts ? reinterpret_cast<WaCutItem*>(ws + pl.part + pl.stats) : nullptr;
+  a.row_tiles = (int)(p->rows * a.G / WA_ROWS + cache->requests);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool kv8 = cache->dtype == FM_DT_E4M3, duo = p->max_q * a.G <= 128;
   if (cache->head_dim == 128) return kv8 ? launch_window<128, true>(a, pl, duo, s) : launch_window<128, false>(a, pl, duo, s);

@@ -246,6 +246,26 @@ def test_window_long(dt, window, sinks):
     close(got, want, mag, "window", dt == "e4m3")
 
 
+@pytest.mark.parametrize("dt", ["bf16", "e4m3"])
+def test_window_many_short_items(dt):
+    """More (row tile, kv head) items than SMs, each too short to be cut; some requests without rows."""
+    H, KH, D, page = 16, 8, 64, 16
+    lengths = [37 * (i % 13) + (i % 3) for i in range(40)]
+    rows = [min(L, 5 * i % 211) for i, L in enumerate(lengths)]
+    g = torch.Generator().manual_seed(21)
+    pools, table, descales = make_cache(g, lengths, KH, D, page, FP8 if dt == "e4m3" else torch.bfloat16, "joint")
+    cu = torch.tensor([0] + rows).cumsum(0).int()
+    q = torch.randn(int(cu[-1]), H, D, generator=g).to(torch.bfloat16)
+    _, k, v = views(pools, D)
+    for window, sinks in ((0, 0), (100, 3)):
+        got = ops().paged_window_attention(
+            q.to(DEV), k, v, cu.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV), max(rows),
+            max(lengths), D ** -0.5, window=window, sinks=sinks, descales=None if descales is None else descales.to(DEV))
+        want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu, lengths, table, D ** -0.5, window, sinks, descales)
+        close(got, want, mag, "window", dt == "e4m3")
+    assert error_word() == 0
+
+
 def test_window_of_one_row_is_decode():
     g = torch.Generator().manual_seed(14)
     lengths, KH, H, D = [130, 50, 1], 2, 8, 128
