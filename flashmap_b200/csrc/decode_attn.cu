@@ -8,14 +8,19 @@
 //
 // The keys and values are read once and each takes part in 4 G operations a
 // byte at most (G query heads to a kv head), so the cache's bytes bound it.
-// The visible positions are cut into chunks of equal length, one CTA per
-// (chunk, request, kv head, 8 or 16 query heads): requests of very different
-// lengths then make units of the same size, and one long request fills the
+// A request's visible positions are cut into equal chunks, one CTA per (chunk,
+// request, kv head, 8 or 16 query heads), so that one long request fills the
 // GPU.  Each of a CTA's four warps streams its own 16-key tiles through a
 // cp.async pipeline, with its own running maximum and sum, and the warps are
 // merged at the end.  Chunks are joined by a second kernel
 // (decode_join_kernel), which also turns the scores that the first one left
 // into weights, since only then are a row's maximum and sum known.
+//
+// Measured, 32 heads on 8 of 128: 1 request of 49157, 46 us (4.4 TB/s, of which
+// 7 us are the join); 64 requests of 1024 .. 8192 with sums, 222 us (5.5 TB/s,
+// the scores and the join included); 40 heads on 8, e4m3, 192 requests of
+// 512 .. 4096, 186 us (4.9 TB/s: the widening to f16 takes the issue slots);
+// 64 heads on 8 of 64, a window of 2048, 94 us (5.5 TB/s).
 #include "paged_cache.cuh"
 
 namespace fm {

@@ -11,8 +11,12 @@
 // (request, kv head), each with a slice of the positions whose keys it holds in
 // shared memory.  The smallest kept key is found 11, 11 and 10 bits at a time
 // from histograms that the cluster adds up; then an ordered count gives every
-// kept position its slot.  evict_move_kernel moves the rows.  Both are bound by
-// memory where there are many rows, by latency where there are few.
+// kept position its slot.  The rows are moved by evict_move_kernel, or, where
+// there are CTAs enough, by the CTA that chose them (64 requests, 8 kv heads,
+// 2000 .. 8192 to 2048 positions: 214 us in two launches, 210 us in one, of
+// which 166 us are the rows' bytes; 8 e4m3 contexts of 20000 .. 65000 copied
+// to 8192: 94 and 91 us).  A few rows are bound by latency: one request of 4096
+// to 2048, 25 us, half of it choosing, in three rounds of counting and meeting.
 #include <cooperative_groups.h>
 
 #include "paged_cache.cuh"
@@ -26,6 +30,7 @@ constexpr int EV_THREADS = 512;
 constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_BINS = 2048;
 constexpr int EV_KEYS = 49152;  // keys of a slice that shared memory holds; longer slices read theirs from L2 again
+constexpr int EV_FUSE = 148;    // CTAs that choose from which on they move the rows, too
 constexpr int EV_UNROLL = 4;    // rows that a thread of the moving kernel has in flight
 
 struct EvictArgs {
@@ -50,6 +55,58 @@ __device__ __forceinline__ uint32_t sum_key(float v) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
+// Moves rows begin .. end - 1 of (r, h)'s keys or values, `slice` of their
+// bytes, by 256 threads.  In place a row only moves down (kept[i] >= i): the
+// CTA reads a block of rows, all its threads meet, and it writes them.  No later
+// block reads a slot below its own first one, so one meeting a block is all
+// that is needed.
+template <bool IN_PLACE>
+__device__ __forceinline__ void move_rows(const EvictArgs& a, int r, int h, int part, int slice, int begin, int end,
+                                          int tid) {
+  const int bytes = a.row_bytes / a.slices, per_row = bytes / 16;
+  const int rows = 256 / per_row, mine = tid / per_row;
+  uint8_t* base = (part ? a.c.v + (long long)h * a.c.vhs : a.c.k + (long long)h * a.c.khs) + slice * bytes +
+                  (tid % per_row) * 16;
+  const long long ps = part ? a.c.vps : a.c.kps, ts = part ? a.c.vts : a.c.kts;
+  const int2* from = a.from + ((long long)r * a.c.KH + h) * a.budget;
+  const int* to = IN_PLACE ? a.c.table + (long long)r * a.c.tstride : a.out_table + (long long)r * a.ot_stride;
+  int2 src[EV_UNROLL];
+  int dst[EV_UNROLL];
+  auto look = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < EV_UNROLL; ++u) {
+      const int i = i0 + u * rows + mine;
+      src[u] = i < end ? from[i] : make_int2(-1, 0);
+      dst[u] = i < end ? to[a.c.by_page.div(i)] : 0;
+    }
+  };
+  look(begin);
+  for (int i0 = begin; i0 < end; i0 += rows * EV_UNROLL) {
+    uint4 v[EV_UNROLL];
+    uint8_t* at[EV_UNROLL];
+#pragma unroll
+    for (int u = 0; u < EV_UNROLL; ++u) {
+      const int i = i0 + u * rows + mine, tok = i - a.c.by_page.div(i) * a.c.page;
+      at[u] = nullptr;
+      if (src[u].x < 0 || (IN_PLACE && src[u].x == dst[u] && src[u].y == tok)) continue;
+      if (dst[u] < 0 || dst[u] >= a.c.num_pages) {
+        record_error(a.err, DEV_BAD_INDEX);
+        continue;
+      }
+      at[u] = base + dst[u] * ps + tok * ts;
+      v[u] = *reinterpret_cast<const uint4*>(base + src[u].x * ps + src[u].y * ts);
+    }
+    look(i0 + rows * EV_UNROLL);
+    if (IN_PLACE) __syncthreads();
+#pragma unroll
+    for (int u = 0; u < EV_UNROLL; ++u)
+      if (at[u] != nullptr) *reinterpret_cast<uint4*>(at[u]) = v[u];
+  }
+}
+
+// MOVE: what the CTA does with the rows that it has chosen.
+enum { EV_LEAVE, EV_IN_PLACE, EV_COPY };
+template <int MOVE>
 __global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(EvictArgs a) {
   extern __shared__ uint32_t ev_keys[];
   __shared__ int hist[2][EV_BINS];
@@ -87,6 +144,10 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(EvictArgs a
     for (int i = b + tid; i < e; i += EV_THREADS) a.kept[row0 + i] = i;
     __syncthreads();
     fill(b, e);
+    if constexpr (MOVE == EV_COPY) {
+      __syncthreads();
+      move_rows<false>(a, r, h, tid >> 8, 0, b, e, tid & 255);
+    }
     return;
   }
   const int lo = a.sinks, hi = len - a.recent;  // the positions that compete
@@ -252,15 +313,17 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(EvictArgs a
     tb += __shfl_sync(0xffffffffu, es, 31);
   }
   __syncthreads();
-  fill(min(a.budget, slice_sure + min(slice_ties, need)),
-       min(a.budget, slice_sure + st + min(slice_ties + tt, need)));
+  const int slot0 = min(a.budget, slice_sure + min(slice_ties, need));
+  const int slot1 = min(a.budget, slice_sure + st + min(slice_ties + tt, need));
+  fill(slot0, slot1);
+  if constexpr (MOVE != EV_LEAVE) {
+    __syncthreads();
+    move_rows<MOVE == EV_IN_PLACE>(a, r, h, tid >> 8, 0, slot0, slot1, tid & 255);
+  }
 }
 
 // One CTA per (request, kv head, keys or values, slice of the row's bytes), and
-// for a copy to other pages per `chunk` rows.  In place a row only moves down
-// (kept[i] >= i): the CTA reads a block of rows, all its threads meet, and it
-// writes them.  No later block reads a slot below its own first one, so that
-// one meeting a block is all that is needed.
+// for a copy to other pages per `chunk` rows.
 template <bool IN_PLACE>
 __global__ void __launch_bounds__(256, 4) evict_move_kernel(EvictArgs a) {
   pdl_wait();
@@ -272,45 +335,7 @@ __global__ void __launch_bounds__(256, 4) evict_move_kernel(EvictArgs a) {
   const int len = cache_length(a.c, r, a.err, false);
   if (IN_PLACE && len <= a.budget) return;
   const int begin = blockIdx.y * a.chunk, end = min(min(len, a.budget), begin + a.chunk);
-  const int bytes = a.row_bytes / a.slices, per_row = bytes / 16;
-  const int rows = 256 / per_row, mine = threadIdx.x / per_row;
-  uint8_t* base = (part ? a.c.v + (long long)h * a.c.vhs : a.c.k + (long long)h * a.c.khs) + slice * bytes +
-                  (threadIdx.x % per_row) * 16;
-  const long long ps = part ? a.c.vps : a.c.kps, ts = part ? a.c.vts : a.c.kts;
-  const int2* from = a.from + (long long)item * a.budget;
-  const int* to = IN_PLACE ? a.c.table + (long long)r * a.c.tstride : a.out_table + (long long)r * a.ot_stride;
-  int2 src[EV_UNROLL];
-  int dst[EV_UNROLL];
-  auto look = [&](int i0) {
-#pragma unroll
-    for (int u = 0; u < EV_UNROLL; ++u) {
-      const int i = i0 + u * rows + mine;
-      src[u] = i < end ? from[i] : make_int2(-1, 0);
-      dst[u] = i < end ? to[a.c.by_page.div(i)] : 0;
-    }
-  };
-  look(begin);
-  for (int i0 = begin; i0 < end; i0 += rows * EV_UNROLL) {
-    uint4 v[EV_UNROLL];
-    uint8_t* at[EV_UNROLL];
-#pragma unroll
-    for (int u = 0; u < EV_UNROLL; ++u) {
-      const int i = i0 + u * rows + mine, tok = i - a.c.by_page.div(i) * a.c.page;
-      at[u] = nullptr;
-      if (src[u].x < 0 || (IN_PLACE && src[u].x == dst[u] && src[u].y == tok)) continue;
-      if (dst[u] < 0 || dst[u] >= a.c.num_pages) {
-        record_error(a.err, DEV_BAD_INDEX);
-        continue;
-      }
-      at[u] = base + dst[u] * ps + tok * ts;
-      v[u] = *reinterpret_cast<const uint4*>(base + src[u].x * ps + src[u].y * ts);
-    }
-    look(i0 + rows * EV_UNROLL);
-    if (IN_PLACE) __syncthreads();
-#pragma unroll
-    for (int u = 0; u < EV_UNROLL; ++u)
-      if (at[u] != nullptr) *reinterpret_cast<uint4*>(at[u]) = v[u];
-  }
+  move_rows<IN_PLACE>(a, r, h, part, slice, begin, end, threadIdx.x);
 }
 
 // CTAs of a cluster: as many as leave three to an SM, with 4096 positions each at least.
@@ -371,25 +396,38 @@ extern "C" fm_status fm_paged_evict(const fm_paged_cache* cache, const fm_evict*
   const int cs = evict_cluster(items, cache->max_length);
   int64_t keys = (cache->max_length + cs - 1) / cs + 32;
   if (keys > EV_KEYS) keys = EV_KEYS;
-  st = allow_smem<evict_select_kernel>(EV_KEYS * 4, "paged_evict");
+  const size_t smem = (size_t)keys * 4;
+  auto select = [&](auto kernel, fm_status allowed) {
+    if (allowed != FM_OK) return allowed;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(items * cs));
+    cfg.blockDim = dim3(EV_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)cs, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    if (e != cudaSuccess) return set_error(FM_ERR_LAUNCH, "paged_evict: %s", cudaGetErrorString(e));
+    ++launch_counter();
+    return (fm_status)FM_OK;
+  };
+  constexpr int most = EV_KEYS * 4;
+  // Where there is a CTA to every SM that can move what it has chosen, it does
+  // so at once: the moving of some runs beside the choosing of others.  In
+  // place only one CTA may move a (request, kv head)'s rows.
+  a.slices = 1;
+  if (a.out_table && items * cs >= EV_FUSE)
+    return select(evict_select_kernel<EV_COPY>, allow_smem<evict_select_kernel<EV_COPY>>(most, "paged_evict"));
+  if (!a.out_table && cs == 1 && items >= EV_FUSE)
+    return select(evict_select_kernel<EV_IN_PLACE>, allow_smem<evict_select_kernel<EV_IN_PLACE>>(most, "paged_evict"));
+  st = select(evict_select_kernel<EV_LEAVE>, allow_smem<evict_select_kernel<EV_LEAVE>>(most, "paged_evict"));
   if (st != FM_OK) return st;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(items * cs));
-  cfg.blockDim = dim3(EV_THREADS);
-  cfg.dynamicSmemBytes = (size_t)keys * 4;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {(unsigned)cs, 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, evict_select_kernel, a);
-  if (e != cudaSuccess) return set_error(FM_ERR_LAUNCH, "paged_evict: %s", cudaGetErrorString(e));
-  ++launch_counter();
 
   // Rows are cut into slices of 32 bytes at least while there are fewer than
   // two CTAs to an SM; a copy is cut along the rows instead.
-  a.slices = 1;
   a.chunk = a.budget;
   unsigned chunks = 1;
   if (a.out_table) {
