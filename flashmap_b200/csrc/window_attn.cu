@@ -268,7 +268,7 @@ struct WaCtrl {
   float qinv[2][256];                // e4m3: what a row's query was multiplied with, inverted (items in turn)
   WaItem item[WA_ITEMS];
   WaBorder border[2];
-  long long scan[17];
+  int scan[16];
 };
 
 // 16 warps, persistent over work items: two warpgroups of
@@ -337,11 +337,12 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
 
   // ------------------------------------------------------------- this CTA's share
   // sum over the CTA of the values before this thread's, and of all
-  auto scan = [&](long long v, long long* all) {
-    long long x = v;
+  // (a key tile count is under 2^24, so a warp's sum fits 32 bits)
+  auto scan = [&](int v, long long* all) {
+    int x = v;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x, off);
+      const int y = __shfl_up_sync(0xffffffffu, x, off);
       if (lane >= off) x += y;
     }
     __syncthreads();
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
     long long before = 0, sum = 0;
 #pragma unroll
     for (int w = 0; w < 16; ++w) {
-      const long long y = ctl->scan[w];
+      const int y = ctl->scan[w];
       before += w < warp ? y : 0;
       sum += y;
     }
@@ -398,7 +399,9 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
     __syncthreads();
     for (int e = 0; e < 2; ++e) {
       const int b = blockIdx.x + e;
-      const long long x = b >= shares ? total : total * b / shares;
+      const long long x = b >= shares ? total
+                          : total < (1 << 20) ? (long long)((unsigned)total * (unsigned)b / (unsigned)shares)
+                                              : total * b / shares;
       if (x >= total) continue;
       int i0 = 0;
       long long at = 0;
@@ -412,7 +415,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       const long long into = x - at - before * a.c.KH;
       const int w = n + WA_ITEM;
       if (n && into >= 0 && into < (long long)w * a.c.KH) {
-        const int c = (int)(into / w);
+        const int c = into < 0x7fffffff ? (int)into / w : (int)(into / w);
         ctl->border[e] = WaBorder{r, y, c, wa_cut((int)(into - (long long)c * w), n)};
       }
     }
@@ -1047,15 +1050,19 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
           break;
         }
         q_phase ^= 1;
-        constexpr int RPI = 32 / CPR;  // rows of a warp at a time
-        const int ch = lane % CPR, rows = w.mt() * 128;
-        auto chunk = [&](int lr) { return sQ + (lr >> 7) * TILE + (ch >> 3) * 16384 + (lr & 127) * 128 + (((ch & 7) ^ (lr & 7)) << 4); };
+        constexpr int RPI = 4;  // rows of a warp at a time: eight lanes to a row, CPR / 8 pieces to a lane
+        const int ch = lane & 7, rows = w.mt() * 128;
+        auto chunk = [&](int lr, int blk) {
+          return sQ + (lr >> 7) * TILE + blk * 16384 + (lr & 127) * 128 + ((ch ^ (lr & 7)) << 4);
+        };
         const uint8_t* qbase = a.q + 2 * ((long long)w.q0 * a.q_ts + (long long)w.c * a.G * a.q_hs + ch * 8);
 #pragma unroll 4
-        for (int lr = (warp - 13) * RPI + lane / CPR; lr < rows; lr += 3 * RPI) {
+        for (int lr = (warp - 13) * RPI + (lane >> 3); lr < rows; lr += 3 * RPI) {
           const bool live = lr < w.rows;
           const int row = w.row0 + (live ? lr : 0), tok = a.by_g.div(row);
-          pc_cp_async16(smem_u32(chunk(lr)), qbase + 2 * (tok * a.q_ts + (row - tok * a.G) * a.q_hs), live ? 16u : 0u);
+          const uint8_t* src = qbase + 2 * (tok * a.q_ts + (row - tok * a.G) * a.q_hs);
+#pragma unroll
+          for (int blk = 0; blk < CPR / 8; ++blk) pc_cp_async16(smem_u32(chunk(lr, blk)), src + blk * 128, live ? 16u : 0u);
         }
         pc_cp_commit();
         pc_cp_wait<0>();
@@ -1063,11 +1070,12 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
           mbar_arrive(&ctl->q_raw);
         } else {
           if (!(w.scale > 0.0f))
-            for (int lr = (warp - 13) * RPI + lane / CPR; lr < rows; lr += 3 * RPI) {
-              uint4* at = reinterpret_cast<uint4*>(chunk(lr));
-              const uint32_t keep = w.scale < 0.0f ? ~0u : 0u, flip = w.scale < 0.0f ? 0x80008000u : 0u;
-              *at = make_uint4((at->x & keep) ^ flip, (at->y & keep) ^ flip, (at->z & keep) ^ flip, (at->w & keep) ^ flip);
-            }
+            for (int lr = (warp - 13) * RPI + (lane >> 3); lr < rows; lr += 3 * RPI)
+              for (int blk = 0; blk < CPR / 8; ++blk) {
+                uint4* at = reinterpret_cast<uint4*>(chunk(lr, blk));
+                const uint32_t keep = w.scale < 0.0f ? ~0u : 0u, flip = w.scale < 0.0f ? 0x80008000u : 0u;
+                *at = make_uint4((at->x & keep) ^ flip, (at->y & keep) ^ flip, (at->z & keep) ^ flip, (at->w & keep) ^ flip);
+              }
           fence_async_smem();
           mbar_arrive(&ctl->q_full);
         }
@@ -1131,7 +1139,7 @@ WindowPlan window_plan(int64_t R, int64_t T, int64_t H, int64_t KH, int64_t HD, 
   WindowPlan p{};
   const int64_t items = (T * (H / KH) / WA_ROWS + R) * KH, sms = num_sms();
   int64_t span = max_len;
-  const int64_t tokens = max_q < WA_ROWS ? max_q : WA_ROWS;
+  const int64_t per = WA_ROWS / (H / KH) + 2, tokens = max_q < per ? max_q : per;  // that a row tile touches
   if (window > 0 && window + tokens + sinks < span) span = window + tokens + sinks;
   const int64_t tiles = span / WA_KEYS + 3;
   p.cuts = tiles >= (items >= sms ? 8 : 2 * WA_CUT);
