@@ -173,11 +173,11 @@ _SIGNATURES = {
     "fm_paged_cross_attn": (c_int, [ctypes.POINTER(PagedAttn), c_void_p]),
     "fm_paged_decode_attn_workspace_size": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
                                                        c_int32]),
-    "fm_paged_decode_attn": (c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(DecodeAttn), c_void_p]),
+    "fm_paged_decode_attn": (c_int, [c_void_p, c_void_p, c_void_p]),  # PagedCache, DecodeAttn
     "fm_paged_window_attn_workspace_size": (c_size_t, [c_int64] * 9),
-    "fm_paged_window_attn": (c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(WindowAttn), c_void_p]),
+    "fm_paged_window_attn": (c_int, [c_void_p, c_void_p, c_void_p]),  # PagedCache, WindowAttn
     "fm_paged_evict_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
-    "fm_paged_evict": (c_int, [ctypes.POINTER(PagedCache), ctypes.POINTER(Evict), c_void_p]),
+    "fm_paged_evict": (c_int, [c_void_p, c_void_p, c_void_p]),  # PagedCache, Evict
     "fm_tree_build": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
     "fm_tree_commit": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

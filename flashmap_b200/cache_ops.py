@@ -29,8 +29,9 @@ CUDA graph.  There is no fallback.
 
 from __future__ import annotations
 
-import ctypes
-from typing import Optional, Tuple
+import functools
+import struct
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -40,6 +41,25 @@ from .serving_ops import OpArgumentError, _err, _need
 __all__ = ["OpArgumentError", "paged_decode_attention", "paged_window_attention", "evict_paged_context"]
 
 _FP8 = torch.float8_e4m3fn
+
+# fm_paged_cache, fm_decode_attn, fm_window_attn and fm_evict as the C entries
+# read them (native sizes and alignment): packing one takes a fifth of the time
+# that filling a ctypes.Structure of these fields does.
+_CACHE = struct.Struct("@PPiqqqqqqqqPqqPqqqqP")
+_DECODE = struct.Struct("@PqqqfqqPqqPqqPNP")
+_WINDOW = struct.Struct("@PqqqqPqfqqPqqPNP")
+_EVICT = struct.Struct("@PqqqqqPqqPPPPNP")
+
+
+class _Cache(NamedTuple):
+    """A checked cache: its packed fm_paged_cache and the sizes that calls go by."""
+    packed: bytes
+    device: torch.device
+    requests: int
+    kv_heads: int
+    page_size: int
+    head_dim: int
+    max_length: int
 
 
 def _on(t: torch.Tensor, name: str, device) -> None:
@@ -77,7 +97,7 @@ def _refuse_cache(k_cache, v_cache, lengths, block_table, descales, max_len: int
               "descales must be contiguous float32 (2, requests, kv_heads)")
 
 
-def _cache(k_cache, v_cache, lengths, block_table, descales, max_len: int) -> _lib.PagedCache:
+def _cache(k_cache, v_cache, lengths, block_table, descales, max_len: int) -> _Cache:
     # one condition on the way through; which part of it failed is found out only then
     dev, dtype = k_cache.device, k_cache.dtype
     shape, ks, vs, ts, table = k_cache.shape, k_cache.stride(), v_cache.stride(), block_table.stride(), block_table.shape
@@ -92,14 +112,15 @@ def _cache(k_cache, v_cache, lengths, block_table, descales, max_len: int) -> _l
                  and descales.is_contiguous() and descales.shape == (2, table[0], shape[1]))):
         _refuse_cache(k_cache, v_cache, lengths, block_table, descales, max_len)
         raise OpArgumentError("the cache's tensors do not go together")
-    return _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(),
-                           _lib.FM_DT_BF16 if descales is None and dtype == torch.bfloat16 else _lib.FM_DT_E4M3,
-                           ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], shape[2], shape[0], block_table.data_ptr(),
-                           ts[0], table[1], lengths.data_ptr(), max_len, table[0], shape[1], shape[3],
-                           None if descales is None else descales.data_ptr())
+    return _Cache(_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(),
+                              _lib.FM_DT_BF16 if dtype == torch.bfloat16 else _lib.FM_DT_E4M3,
+                              ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], shape[2], shape[0], block_table.data_ptr(),
+                              ts[0], table[1], lengths.data_ptr(), max_len, table[0], shape[1], shape[3],
+                              0 if descales is None else descales.data_ptr()),
+                  dev, table[0], shape[1], shape[2], shape[3], max_len)
 
 
-def _query(query, cache: _lib.PagedCache, device) -> torch.Tensor:
+def _query(query, cache: _Cache, device) -> torch.Tensor:
     shape, stride = query.shape, query.stride()
     if not (query.device == device and query.dtype == torch.bfloat16 and len(shape) == 3
             and shape[2] == cache.head_dim and shape[1] > 0 and shape[1] % cache.kv_heads == 0):
@@ -118,7 +139,7 @@ def _visibility(window: int, sinks: int) -> None:
     _need(window >= 0 and sinks >= 0, "window and sinks must not be negative")
 
 
-def _sums(weight_sums, cache: _lib.PagedCache, device, least: int) -> None:
+def _sums(weight_sums, cache: _Cache, device, least: int) -> None:
     _on(weight_sums, "weight_sums", device)
     _need(weight_sums.dtype is torch.float32 and weight_sums.dim() == 3
           and weight_sums.shape[0] == cache.requests and weight_sums.shape[1] == cache.kv_heads,
@@ -131,14 +152,20 @@ def _sums(weight_sums, cache: _lib.PagedCache, device, least: int) -> None:
 _ERR_WORDS: dict = {}  # device index -> address of its error word, which lives as long as the process
 
 
-def _launch(name: str, cache: _lib.PagedCache, args, device) -> None:
-    index = device.index
-    err = _ERR_WORDS.get(index)
+def _err_word(device) -> int:
+    err = _ERR_WORDS.get(device.index)
     if err is None:
-        err = _ERR_WORDS[index] = _err(device).data_ptr()
-    args.err = err
-    lib = _lib.load()
-    status = getattr(lib, name)(ctypes.byref(cache), ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+        err = _ERR_WORDS[device.index] = _err(device).data_ptr()
+    return err
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_size(name: str, *sizes: int) -> int:
+    return getattr(_lib.load(), name)(*sizes)
+
+
+def _launch(name: str, cache: _Cache, args: bytes) -> None:
+    status = getattr(_lib.load(), name)(cache.packed, args, torch._C._cuda_getCurrentRawStream(cache.device.index))
     if status:
         _lib.check(status, name)
 
@@ -162,24 +189,20 @@ def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     query = _query(query, cache, dev)
     _need(query.shape[0] == cache.requests, "one query row per request")
     _visibility(window, sinks)
-    out = torch.empty(query.shape, dtype=torch.bfloat16, device=dev)
+    out = query.new_empty(query.shape)
+    sums, s0, s1 = 0, 0, 0
     if weight_sums is not None:
         _sums(weight_sums, cache, dev, cache.max_length)
+        sums, s0, s1 = weight_sums.data_ptr(), weight_sums.stride(0), weight_sums.stride(1)
     if cache.requests == 0:
         return out
-    lib = _lib.load()
     heads, qs, os = query.shape[1], query.stride(), out.stride()
-    args = _lib.DecodeAttn(query.data_ptr(), qs[0], qs[1], heads, softmax_scale, window, sinks, None, 0, 0,
-                           out.data_ptr(), os[0], os[1], None, 0, None)
-    if weight_sums is not None:
-        args.weight_sums = weight_sums.data_ptr()
-        args.sums_request_stride, args.sums_head_stride = weight_sums.stride(0), weight_sums.stride(1)
-    need = lib.fm_paged_decode_attn_workspace_size(cache.requests, heads, cache.kv_heads, cache.head_dim,
-                                                   cache.max_length, window, sinks, weight_sums is not None)
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), need
-    _launch("fm_paged_decode_attn", cache, args, dev)
+    need = _workspace_size("fm_paged_decode_attn_workspace_size", cache.requests, heads, cache.kv_heads, cache.head_dim,
+                           cache.max_length, window, sinks, int(weight_sums is not None))
+    ws = seqused_k.new_empty(need // 4) if need else None  # sizes are multiples of 8
+    _launch("fm_paged_decode_attn", cache,
+            _DECODE.pack(query.data_ptr(), qs[0], qs[1], heads, softmax_scale, window, sinks, sums, s0, s1,
+                         out.data_ptr(), os[0], os[1], ws.data_ptr() if need else 0, need, _err_word(dev)))
     return out
 
 
@@ -204,21 +227,18 @@ def paged_window_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
           and cu_seqlens_q.is_contiguous(), "cu_seqlens_q must be contiguous int32 (requests + 1,)")
     _need(max_seqlen_q >= 0, "max_seqlen_q must not be negative")
     _visibility(window, sinks)
-    out = torch.empty(query.shape, dtype=torch.bfloat16, device=dev)
+    out = query.new_empty(query.shape)
     tokens, heads = query.shape[0], query.shape[1]
     if cache.requests == 0 or tokens == 0:
         return out
-    lib = _lib.load()
     qs, os = query.stride(), out.stride()
-    args = _lib.WindowAttn(query.data_ptr(), qs[0], qs[1], tokens, heads, cu_seqlens_q.data_ptr(),
-                           int(max_seqlen_q), softmax_scale, window, sinks, out.data_ptr(), os[0], os[1], None, 0,
-                           None)
-    need = lib.fm_paged_window_attn_workspace_size(cache.requests, tokens, heads, cache.kv_heads, cache.head_dim,
-                                                   int(max_seqlen_q), cache.max_length, window, sinks)
-    if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), need
-    _launch("fm_paged_window_attn", cache, args, dev)
+    need = _workspace_size("fm_paged_window_attn_workspace_size", cache.requests, tokens, heads, cache.kv_heads,
+                           cache.head_dim, int(max_seqlen_q), cache.max_length, window, sinks)
+    ws = seqused_k.new_empty(need // 4) if need else None  # sizes are multiples of 8
+    _launch("fm_paged_window_attn", cache,
+            _WINDOW.pack(query.data_ptr(), qs[0], qs[1], tokens, heads, cu_seqlens_q.data_ptr(), int(max_seqlen_q),
+                         softmax_scale, window, sinks, out.data_ptr(), os[0], os[1], ws.data_ptr() if need else 0, need,
+                         _err_word(dev)))
     return out
 
 
@@ -247,22 +267,22 @@ def evict_paged_context(k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k:
     _sums(weight_sums, cache, dev, 0)
     _need(budget >= 1, "the budget must be positive")
     _need(sinks >= 0 and recent >= 0 and sinks + recent <= budget, "sinks + recent must lie within the budget")
-    kept = torch.empty((cache.requests, cache.kv_heads, budget), dtype=torch.int32, device=dev)
-    lengths = torch.empty(cache.requests, dtype=torch.int32, device=dev)
-    sums = torch.empty((cache.requests, cache.kv_heads, budget), dtype=torch.float32, device=dev)
-    args = _lib.Evict(weight_sums.data_ptr(), weight_sums.stride(0), weight_sums.stride(1), budget, sinks, recent,
-                      None, 0, 0, kept.data_ptr(), lengths.data_ptr(), sums.data_ptr(), None, 0, None)
+    kept = seqused_k.new_empty((cache.requests, cache.kv_heads, budget))
+    lengths = seqused_k.new_empty(cache.requests)
+    sums = weight_sums.new_empty((cache.requests, cache.kv_heads, budget))
+    to, to_stride, to_cols = 0, 0, 0
     if out_block_table is not None:
         _on(out_block_table, "out_block_table", dev)
         _need(out_block_table.dtype is torch.int32 and out_block_table.dim() == 2
               and out_block_table.shape[0] == cache.requests, "out_block_table must be int32 (requests, pages)")
         _need(out_block_table.shape[1] <= 1 or out_block_table.stride(1) == 1, "out_block_table rows must be contiguous")
         _need(out_block_table.shape[1] * cache.page_size >= budget, "out_block_table does not cover the budget")
-        args.out_page_table = out_block_table.data_ptr()
-        args.out_page_table_stride, args.out_page_table_cols = out_block_table.stride(0), out_block_table.shape[1]
+        to, to_stride, to_cols = out_block_table.data_ptr(), out_block_table.stride(0), out_block_table.shape[1]
     if cache.requests:
-        need = _lib.load().fm_paged_evict_workspace_size(cache.requests, cache.kv_heads, budget)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        args.workspace, args.workspace_bytes = ws.data_ptr(), need
-        _launch("fm_paged_evict", cache, args, dev)
+        need = _workspace_size("fm_paged_evict_workspace_size", cache.requests, cache.kv_heads, budget)
+        ws = seqused_k.new_empty(need // 4)
+        _launch("fm_paged_evict", cache,
+                _EVICT.pack(weight_sums.data_ptr(), weight_sums.stride(0), weight_sums.stride(1), budget, sinks, recent,
+                            to, to_stride, to_cols, kept.data_ptr(), lengths.data_ptr(), sums.data_ptr(), ws.data_ptr(),
+                            need, _err_word(dev)))
     return kept, lengths, sums

@@ -75,16 +75,27 @@ def test_argument_refusals():
         st, msg = _status("fm_paged_decode_attn", _cache(), _decode(**kw))
         assert st == want, (kw, st, msg)
     for kw, want in ((dict(heads=3), SHAPE), (dict(rows=-1), SHAPE), (dict(rows=1 << 40), SHAPE), (dict(window=-1), SHAPE),
-                     (dict(cu_seqlens_q=None), INVALID), (dict(q=(1 << 24) + 8), ALIGN), (dict(out_head_stride=132), ALIGN),
-                     ({}, WORKSPACE)):
+                     (dict(cu_seqlens_q=None), INVALID), (dict(q=(1 << 24) + 8), ALIGN), (dict(out_head_stride=132), ALIGN)):
         st, msg = _status("fm_paged_window_attn", _cache(), _window(**kw))
         assert st == want, (kw, st, msg)
+    # contexts long enough to be cut need room for the parts
+    st, msg = _status("fm_paged_window_attn", _cache(max_length=4096, page_table_cols=256), _window())
+    assert st == WORKSPACE, (st, msg)
     for kw, want in ((dict(budget=0), SHAPE), (dict(sinks=30, recent=3), SHAPE), (dict(recent=-1), SHAPE),
                      (dict(weight_sums=None), INVALID), (dict(kept=None), INVALID), (dict(lengths=1 << 23), INVALID),
                      (dict(out_page_table=1 << 22, out_page_table_cols=4), INVALID),
                      (dict(out_page_table=1 << 28, out_page_table_cols=1), SHAPE), ({}, WORKSPACE)):
         st, msg = _status("fm_paged_evict", _cache(), _evict(**kw))
         assert st == want, (kw, st, msg)
+
+
+def test_packed_arguments_have_the_structures_layout():
+    from flashmap_b200 import cache_ops as C
+    for packed, fields in ((C._CACHE, _lib.PagedCache), (C._DECODE, _lib.DecodeAttn), (C._WINDOW, _lib.WindowAttn),
+                           (C._EVICT, _lib.Evict)):
+        assert packed.size == ctypes.sizeof(fields)
+        values = [0.5 if t is ctypes.c_float else 3 + i for i, (_, t) in enumerate(fields._fields_)]
+        assert packed.pack(*values) == bytes(fields(*values))
 
 
 def test_workspace_sizes():
