@@ -571,7 +571,7 @@ fm_status launch_decode(const DecodeArgs& a, unsigned grid, cudaStream_t s) {
   constexpr int smem = da_smem<HD, KV8, NG>();
   const fm_status st = allow_smem<decode_attn_kernel<HD, KV8, NG>>(smem, "paged_decode_attn");
   if (st != FM_OK) return st;
-  return launch_kernel(decode_attn_kernel<HD, KV8, NG>, dim3(grid), dim3(128), smem, s, false, a);
+  return launch_kernel(decode_attn_kernel<HD, KV8, NG>, dim3(grid), dim3(128), smem, s, true, a);
 }
 
 template <int HD>

@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(EvictArgs a
   const int cs = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int item = blockIdx.x / cs, r = item / a.c.KH, h = item % a.c.KH;
+  pdl_wait();
   const int len = cache_length(a.c, r, a.err, tid == 0 && h == 0 && rank == 0);
   const int n = min(len, a.budget);
   if (h == 0 && rank == 0 && tid == 0) a.lengths[r] = n;
@@ -405,11 +406,13 @@ extern "C" fm_status fm_paged_evict(const fm_paged_cache* cache, const fm_evict*
     cfg.blockDim = dim3(EV_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim = {(unsigned)cs, 1, 1};
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
     if (e != cudaSuccess) return set_error(FM_ERR_LAUNCH, "paged_evict: %s", cudaGetErrorString(e));
     ++launch_counter();

@@ -334,6 +334,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, ctl->tmem, 0);
+  pdl_wait();
 
   // ------------------------------------------------------------- this CTA's share
   // sum over the CTA of the values before this thread's, and of all
@@ -1158,7 +1159,7 @@ fm_status launch_window(const WindowArgs& a, const WindowPlan& pl, cudaStream_t 
   static_assert(sizeof(WaCtrl) <= 3072 && smem <= 232448, "shared memory");
   fm_status st = allow_smem<window_attn_kernel<HD, KV8, DUO>>(smem, "paged_window_attn");
   if (st != FM_OK) return st;
-  st = launch_kernel(window_attn_kernel<HD, KV8, DUO>, dim3((unsigned)pl.ctas), dim3(512), smem, s, false, a);
+  st = launch_kernel(window_attn_kernel<HD, KV8, DUO>, dim3((unsigned)pl.ctas), dim3(512), smem, s, true, a);
   if (st != FM_OK || !pl.cuts) return st;
   return launch_kernel(window_join_kernel<HD>, dim3((unsigned)pl.ctas, HD / 16), dim3(WA_ROWS), 0, s, true, a, pl.ctas);
 }
