@@ -16,7 +16,7 @@
 // 2000 .. 8192 to 2048 positions: 214 us in two launches, 210 us in one, of
 // which 166 us are the rows' bytes; 8 e4m3 contexts of 20000 .. 65000 copied
 // to 8192: 94 and 91 us).  A few rows are bound by latency: one request of 4096
-// to 2048, 25 us, half of it choosing, in three rounds of counting and meeting.
+// to 2048, 18 us, half of it choosing, in three rounds of counting and meeting.
 #include <cooperative_groups.h>
 
 #include "paged_cache.cuh"

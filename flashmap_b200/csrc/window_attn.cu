@@ -12,7 +12,7 @@
 // keys and values of their kv head, so a cache row is read once for the whole
 // group.  Chunks of prompts are bound by the chain S -> softmax -> P -> P V of
 // the two row tiles in flight and by the exponentials (4096 rows of 32 heads on
-// 12300 positions with a window of 4000: 309 us, 873 TFLOP/s of the visible
+// 12300 positions with a window of 4000: 308 us, 874 TFLOP/s of the visible
 // pairs, 52 percent of a large matrix product's rate; 32768 positions without a
 // window: 1040 at clocks that the power limit sets).  Calls with few rows are
 // bound by the cache's bytes and the latency of a CTA's first tiles (24 x 17 rows
@@ -114,7 +114,7 @@ constexpr int WA_SHARE = WA_ITEM + 4;  // the least length of a CTA's share
 //
 // Where items are too short to cut and there are enough of them, CTA b simply
 // takes items b, b + CTAs, .. from the last row tile on (the longest of a
-// prompt): no shares, no join (12 windowed prompts: 65 us, with shares 68 us).
+// prompt): no shares, no join (12 windowed prompts: 60 us, with shares 65 us).
 struct WaBorder {
   int r, y, c, t;  // request, row tile, kv head, and the first tile after the border
 };
