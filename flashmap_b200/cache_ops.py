@@ -218,7 +218,8 @@ def paged_window_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     The row at position p sees the positions j <= p; with ``window > 0`` of
     those only p - j < ``window`` or j < ``sinks``.  A request has at most
     ``max_seqlen_q`` rows and ``max_seqlen_k`` positions.  Values that some rows
-    of a chunk see and others do not must be finite."""
+    of a chunk see and others do not must be finite.  Rows that ``cu_seqlens_q``
+    gives to no request are not written."""
     cache = _cache(k_cache, v_cache, seqused_k, block_table, descales, int(max_seqlen_k))
     dev = k_cache.device
     query = _query(query, cache, dev)

@@ -371,6 +371,10 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       if (r < a.c.R) pre[r] = (int)(row_tiles + before);
       row_tiles += all;
     }
+    if (row_tiles > a.row_tiles) {  // bounds that run back, so that requests share rows: nothing is done
+      if (blockIdx.x == 0 && tid == 0) record_error(a.err, DEV_BAD_INDEX);
+      row_tiles = 0;
+    }
     __syncthreads();
     auto tiles_of = [&](int idx, int* req, int* y) {  // key tiles of row tile idx (one, if it has none)
       int lo = 0, hi = a.c.R - 1;                     // the last request with pre[r] <= idx has it
@@ -1178,7 +1182,7 @@ extern "C" size_t fm_paged_window_attn_workspace_size(int64_t requests, int64_t 
                                                       int64_t head_dim, int64_t max_q, int64_t max_length,
                                                       int64_t window, int64_t sinks) {
   if (requests < 1 || rows < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || max_q < 0 || max_length < 0 ||
-      window < 0 || sinks < 0)
+      window < 0 || window > 0x7ffffff0 || sinks < 0 || sinks > 0x7ffffff0)
     return 0;
   return window_plan(requests, rows, heads, kv_heads, head_dim, max_q, max_length, window, sinks).total;
 }
@@ -1192,7 +1196,7 @@ extern "C" fm_status fm_paged_window_attn(const fm_paged_cache* cache, const fm_
     return set_error(FM_ERR_SHAPE, "paged_window_attn: query heads must be a multiple of the kv heads");
   if (p->window < 0 || p->sinks < 0 || p->window > 0x7ffffff0 || p->sinks > 0x7ffffff0)
     return set_error(FM_ERR_SHAPE, "paged_window_attn: window and sinks must not be negative");
-  if (p->rows < 0 || p->rows * p->heads > 0x7ffffff0)
+  if (p->rows < 0 || p->rows > 0x7ffffff0 || p->rows * p->heads > 0x7ffffff0)
     return set_error(FM_ERR_SHAPE, "paged_window_attn: too many query rows");
   if (cache->requests == 0 || p->rows == 0) return FM_OK;
   if (!p->q || !p->out || !p->cu_seqlens_q) return set_error(FM_ERR_INVALID, "paged_window_attn: null pointer");

@@ -504,3 +504,24 @@ def test_evict_slices_past_shared_memory():
     i = torch.arange(budget)
     moved = dev[table[0, i // page].long().to(DEV), 0, (i % page).to(DEV)].cpu()
     assert torch.equal(moved, pool[table[0, src // page].long(), 0, src % page])
+
+
+@pytest.mark.parametrize("max_len", [64, 4096])
+def test_window_bounds_that_run_back_are_reported(max_len):
+    """Bounds 0, T, 0, T, .. give the same rows to several requests, more row
+    tiles than T rows can have: with shares nothing is done, without them no
+    more than fit; the next call is as ever."""
+    g = torch.Generator().manual_seed(23)
+    KH, H, D, page, T, R = 1, 16, 128, 16, 64, 9
+    pools, table, _ = make_cache(g, [max_len], KH, D, page, torch.bfloat16, "joint")
+    _, k, v = views(pools, D)
+    q = torch.randn(T, H, D, generator=g).to(torch.bfloat16)
+    L = torch.tensor([max_len] * R, dtype=torch.int32, device=DEV)
+    many = table.expand(R, -1).contiguous().to(DEV)
+    back = torch.tensor([0, T] * (R // 2) + [0, T], dtype=torch.int32, device=DEV)
+    ops().paged_window_attention(q.to(DEV), k, v, back, L, many, T, max_len, D ** -0.5)
+    assert error_word() == 4
+    cu = torch.tensor([0] + [T] * R, dtype=torch.int32, device=DEV)
+    want, mag, _ = O.window_attention(q, *cpu_views(pools, D), [0, T], [max_len], table, D ** -0.5)
+    close(ops().paged_window_attention(q.to(DEV), k, v, cu, L, many, T, max_len, D ** -0.5), want, mag, "window")
+    assert error_word() == 0
