@@ -298,7 +298,11 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
   uint8_t* sKV = wa_smem + 2 * TILE;
   WaCtrl* ctl = reinterpret_cast<WaCtrl*>(wa_smem + Lay::CTRL);
   if (smem_u32(wa_smem) & 1023) {  // the swizzled tiles need the alignment that the declaration asks for
-    if (tid == 0) record_error(a.err, DEV_BAD_COPY);
+    pdl_wait();
+    if (tid == 0) {
+      record_error(a.err, DEV_BAD_COPY);
+      if (a.cuts != nullptr) a.cuts[blockIdx.x] = WaCutItem{0, 0, 0, 0, 0, WA_NONE};
+    }
     return;
   }
   volatile int* abort = &ctl->abort;
@@ -952,14 +956,14 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
           }
         }
       }
-      if (code) {
-        if (leader) {
+      if (leader) {
+        if (code) {
           *abort = 1;
           record_error(a.err, code);
-          umma_commit(&ctl->drain);  // nothing of this CTA may be in flight when it ends
         }
-        mbar_wait(&ctl->drain, 0, nullptr);
+        umma_commit(&ctl->drain);  // nothing of this CTA may be in flight when it ends, whichever wait ran out
       }
+      mbar_wait(&ctl->drain, 0, nullptr);
     } else {
       // ------------------------------------------------------------- work items and queries
       const bool shares = a.cuts != nullptr;
@@ -971,6 +975,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
         end = ctl->border[1];
       }
       WaCutItem cut{0, 0, 0, 0, 0, WA_NONE};
+      if (shares && warp == 13 && lane == 0) a.cuts[blockIdx.x] = cut;  // what the join reads where a wait runs out
       uint32_t q_phase = 1;
       bool ok = true;
       for (int k = 0; ok; ++k) {
