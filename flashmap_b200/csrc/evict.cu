@@ -109,7 +109,7 @@ enum { EV_LEAVE, EV_IN_PLACE, EV_COPY };
 template <int MOVE>
 __global__ void __launch_bounds__(EV_THREADS, 2) evict_select_kernel(EvictArgs a) {
   extern __shared__ uint32_t ev_keys[];
-  __shared__ int hist[2][EV_BINS];
+  __shared__ alignas(16) int hist[2][EV_BINS];  // read four bins at a time
   __shared__ int wsum[EV_WARPS], wtie[EV_WARPS];
   __shared__ int s_total[2];  // this slice's sure positions and ties
   __shared__ int s_bin, s_left;
