@@ -149,6 +149,16 @@ def _sums(weight_sums, cache: _Cache, device, least: int) -> None:
     _need(weight_sums.shape[2] <= 1 or weight_sums.stride(2) == 1, "weight_sums rows must be contiguous")
 
 
+def _apart(sums) -> bool:
+    """Whether no two of the rows share memory, for strides that do not show it at a glance."""
+    reach = sums.shape[2]
+    for stride, size in sorted((sums.stride(d), sums.shape[d]) for d in (0, 1) if sums.shape[d] > 1):
+        if stride < reach:
+            return False
+        reach += stride * (size - 1)
+    return True
+
+
 _ERR_WORDS: dict = {}  # device index -> address of its error word, which lives as long as the process
 
 
@@ -182,8 +192,8 @@ def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     It sees every position, or with ``window > 0`` the last ``window`` and the
     first ``sinks``.  ``weight_sums (requests, kv_heads, >= max_seqlen_k)`` fp32
     is added to in place: position j of a kv head gathers the attention weights
-    of its query heads, which ``evict_paged_context`` goes by.  A request has at
-    most ``max_seqlen_k`` positions."""
+    of its query heads, which ``evict_paged_context`` goes by; no two of its rows
+    may share memory.  A request has at most ``max_seqlen_k`` positions."""
     cache = _cache(k_cache, v_cache, seqused_k, block_table, descales, int(max_seqlen_k))
     dev = k_cache.device
     query = _query(query, cache, dev)
@@ -194,6 +204,9 @@ def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     if weight_sums is not None:
         _sums(weight_sums, cache, dev, cache.max_length)
         sums, s0, s1 = weight_sums.data_ptr(), weight_sums.stride(0), weight_sums.stride(1)
+        inner, outer, n = (s1, s0, cache.kv_heads) if s1 <= s0 else (s0, s1, cache.requests)
+        if inner < weight_sums.shape[2] or outer < inner * (n - 1) + weight_sums.shape[2]:  # a dimension of size 1 may have any stride
+            _need(_apart(weight_sums), "rows of weight_sums must not share memory")
     if cache.requests == 0:
         return out
     heads, qs, os = query.shape[1], query.stride(), out.stride()
@@ -254,9 +267,10 @@ def evict_paged_context(k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k:
     within the budget stays whole.
 
     The kept rows move, in order of position, to the request's first slots: in
-    place (the pages after them are free then), or with ``out_block_table
-    (requests, pages)`` to its pages of the same pool, which must be none that
-    ``block_table`` names (pages shared between requests keep their rows).
+    place (the pages after them are free then; no other request may share the
+    pages), or with ``out_block_table (requests, pages)`` to its pages of the
+    same pool, which must be none that ``block_table`` names (pages shared
+    between requests keep their rows).
     Keys move as they are, rotated at their old positions.
 
     Returns ``kept (requests, kv_heads, budget)`` int32, the kept positions and

@@ -525,3 +525,29 @@ def test_window_bounds_that_run_back_are_reported(max_len):
     want, mag, _ = O.window_attention(q, *cpu_views(pools, D), [0, T], [max_len], table, D ** -0.5)
     close(ops().paged_window_attention(q.to(DEV), k, v, cu, L, many, T, max_len, D ** -0.5), want, mag, "window")
     assert error_word() == 0
+
+
+def test_sums_that_share_memory_are_refused():
+    """Sums are added to in place: two rows of them in the same memory would lose additions."""
+    c = ops()
+    KH, D, page, R = 2, 128, 16, 3
+    cache = torch.zeros(4, KH, page, 2 * D, dtype=torch.bfloat16, device=DEV)
+    L = torch.full((R,), 5, dtype=torch.int32, device=DEV)
+    t = torch.zeros(R, 1, dtype=torch.int32, device=DEV)
+    q = torch.zeros(R, 4, D, dtype=torch.bfloat16, device=DEV)
+
+    def decode(sums):
+        return c.paged_decode_attention(q, cache[..., :D], cache[..., D:], L, t, 5, 1.0, weight_sums=sums)
+
+    base = torch.zeros(64, device=DEV)
+    for strides in ((0, 5, 1), (10, 0, 1), (10, 4, 1), (5, 5, 1), (9, 5, 1)):
+        with pytest.raises(c.OpArgumentError, match="share memory"):
+            decode(base.as_strided((R, KH, 5), strides))
+    assert float(base.abs().max()) == 0.0 and error_word() == 0
+    for strides in ((10, 5, 1), (5, 15, 1), (12, 6, 1), (15, 10, 1)):
+        base.zero_()
+        decode(base.as_strided((R, KH, 5), strides))
+        assert torch.allclose(base.as_strided((R, KH, 5), strides), torch.full((R, KH, 5), 0.4, device=DEV))  # 2 heads / 5
+    # rows that are only read may share memory
+    kept, _, sums = c.evict_paged_context(cache[..., :D], cache[..., D:], L[:1], t[:1], base[:5].expand(1, KH, 5), 4)
+    assert kept.shape == (1, KH, 4) and error_word() == 0
