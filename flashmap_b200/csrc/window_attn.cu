@@ -776,6 +776,12 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
           if (ok) widen(xv);
         }
       } else {
+        if (w.n <= 0) {
+          // No copy of this item hands over what is behind, and the warps that wait for that take no further
+          // items: without this, a run of items that see no key would fill the ring of items and stop here.
+          pc_cp_wait<0>();
+          while (behind > 0) hand_over();
+        }
         for (int j = 0; j < w.n && ok; ++j, ++tiles) {
           const int page = page_next, tok = tok_next;
           page_next = lookup(j + 1, &tok_next);

@@ -551,3 +551,34 @@ def test_sums_that_share_memory_are_refused():
     # rows that are only read may share memory
     kept, _, sums = c.evict_paged_context(cache[..., :D], cache[..., D:], L[:1], t[:1], base[:5].expand(1, KH, 5), 4)
     assert kept.shape == (1, KH, 4) and error_word() == 0
+
+
+RUNS_OF_NOTHING = [
+    # heads, kv_heads, lengths, query rows
+    # a verify batch padded with requests that hold nothing: items one by one, then in shares
+    (8, 8, [37 * i % 290 + 1 if i % 8 == 3 else 0 for i in range(150)], [17] * 150),
+    (8, 8, [171 * i % 890 + 11 if i % 8 == 3 else 0 for i in range(200)], [17] * 200),
+    # requests that hold nothing, or less than their rows, between chunks
+    (16, 8, [2304, 0, 2304, 0, 2304], [800, 1, 900, 1, 1000]),
+    (32, 8, [900, 30, 900, 25, 700], [700, 3000, 800, 4000, 600]),
+]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("case", RUNS_OF_NOTHING, ids=["padded", "padded_shares", "between", "rows_before"])
+def test_window_runs_of_items_that_see_nothing(case, dt):
+    """Several items of a CTA in a row whose rows see no key, after one that has keys: what it still waits for
+    must not be held back by them."""
+    H, KH, lengths, rows = case
+    D, page = 64, 16
+    g = torch.Generator().manual_seed(24)
+    pools, table, descales = make_cache(g, lengths, KH, D, page, FP8 if dt == "e4m3" else torch.bfloat16, "joint")
+    cu = torch.tensor([0] + rows).cumsum(0).int()
+    q = torch.randn(int(cu[-1]), H, D, generator=g).to(torch.bfloat16)
+    _, k, v = views(pools, D)
+    got = ops().paged_window_attention(
+        q.to(DEV), k, v, cu.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV), max(rows),
+        max(lengths), D ** -0.5, descales=None if descales is None else descales.to(DEV))
+    assert error_word() == 0
+    want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu, lengths, table, D ** -0.5, descales=descales)
+    close(got, want, mag, "window", dt == "e4m3")
