@@ -582,3 +582,74 @@ def test_window_runs_of_items_that_see_nothing(case, dt):
     assert error_word() == 0
     want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu, lengths, table, D ** -0.5, descales=descales)
     close(got, want, mag, "window", dt == "e4m3")
+
+
+def evicted(pools, table, to, want, lengths, budget, page):
+    """The pools' bytes with each (request, kv head)'s kept rows moved to the first slots of `to`."""
+    now = [p.view(torch.uint8).clone() for p in pools]
+    for r, L in enumerate(lengths):
+        i = torch.arange(min(L, budget))
+        dst = to[r, i // page].long()
+        for h, rows in enumerate(want[r]):
+            src = torch.tensor(rows, dtype=torch.long)
+            for p, u in zip(pools, now):
+                u[dst, h, i % page] = p.view(torch.uint8)[table[r, src // page].long(), h, src % page]
+    return now
+
+
+def spread(n, top, odd=37):
+    return [odd * i * i % top for i in range(n)]
+
+
+EVICT_MANY = [
+    # kv_heads, head_dim, page, dtype, layout, budget, sinks, recent, in place, lengths
+    # 148 (request, kv head) pairs or more, moved by the CTA that chose them
+    (4, 128, 16, "bf16", "joint", 50, 4, 8, True, [0, 1, 49, 50, 51, 52, 900] + spread(33, 400)),
+    (8, 64, 24, "e4m3", "split", 33, 0, 0, True, [0, 1, 33, 34] + spread(16, 300)),
+    (4, 128, 1, "e4m3", "joint", 300, 16, 100, True, [299, 300, 301, 1800] + spread(33, 900)),
+    (4, 64, 16, "bf16", "split", 700, 0, 64, True, [700, 701, 2500, 2040] + spread(33, 1100)),
+    # one CTA to a pair however long the context, and more slots than its shared memory stages
+    (4, 64, 32, "e4m3", "split", 5000, 4, 4900, True, [6000, 5001, 5000, 4999] + spread(52, 100)),
+    # copies to other pages: one, two and four CTAs to a pair
+    (4, 128, 16, "bf16", "joint", 50, 4, 8, False, [0, 1, 49, 50, 51, 52, 900] + spread(33, 400)),
+    (4, 128, 32, "bf16", "split", 600, 4, 100, False, [5000, 4097, 601, 600, 599, 1] + spread(14, 3000)),
+    (4, 64, 24, "e4m3", "joint", 1100, 1, 0, False, [9000, 8191, 1101, 1100] + spread(6, 6000)),
+    # too few pairs for that: two launches, four CTAs choosing for a pair
+    (4, 128, 16, "bf16", "joint", 1100, 4, 300, True, [9000, 1101, 8200, 40, 3000]),
+]
+
+
+@pytest.mark.parametrize("case", EVICT_MANY, ids=lambda c: "-".join(map(str, c[:9])))
+@pytest.mark.parametrize("values", ["ties", "spread", "odd"])
+def test_evict_many(case, values):
+    KH, D, page, dt, layout, budget, sinks, recent, in_place, lengths = case
+    g = torch.Generator().manual_seed(25)
+    R, out_cols = len(lengths), -(-budget // page)
+    pools, table, _ = make_cache(g, lengths, KH, D, page, FP8 if dt == "e4m3" else torch.bfloat16, layout,
+                                 spare=0 if in_place else R * out_cols)
+    to = table
+    if not in_place:
+        free = sorted(set(range(1, pools[0].shape[0])) - set(table.flatten().tolist()))
+        to = torch.tensor(free, dtype=torch.int32)[torch.randperm(len(free), generator=g)][: R * out_cols].view(R, out_cols)
+    sums = torch.rand(R, KH, max(lengths) + 3, generator=g)
+    if values == "ties":
+        sums = (sums * 5).floor()
+    if values == "odd":
+        pick = torch.randint(0, 6, sums.shape, generator=g)
+        for i, x in enumerate([math.nan, math.inf, -math.inf, -0.0, 0.0, -1.5]):
+            sums[pick == i] = x
+    dev, k, v = views(pools, D)
+    kept, n, got = ops().evict_paged_context(
+        k, v, torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV), sums.to(DEV), budget, sinks=sinks,
+        recent=recent, out_block_table=None if in_place else to.to(DEV))
+    assert error_word() == 0
+    want = O.evict(sums, lengths, budget, sinks, recent)
+    assert n.tolist() == [min(L, budget) for L in lengths]
+    for r, L in enumerate(lengths):
+        m = min(L, budget)
+        for h in range(KH):
+            assert kept[r, h].tolist() == want[r][h] + [-1] * (budget - m)
+            assert torch.equal(got[r, h, :m].cpu().nan_to_num(7.0), sums[r, h, want[r][h]].nan_to_num(7.0))
+            assert float(got[r, h, m:].abs().sum()) == 0.0
+    for p, u in zip(dev, evicted(pools, table, to, want, lengths, budget, page)):
+        assert torch.equal(p.view(torch.uint8).cpu(), u)
