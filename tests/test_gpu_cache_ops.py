@@ -653,3 +653,34 @@ def test_evict_many(case, values):
             assert float(got[r, h, m:].abs().sum()) == 0.0
     for p, u in zip(dev, evicted(pools, table, to, want, lengths, budget, page)):
         assert torch.equal(p.view(torch.uint8).cpu(), u)
+
+
+VERIFY = [
+    # heads, kv_heads, most rows, page, layout, lengths: at most 128 (row, head of the group) rows to a request
+    (8, 2, 17, 16, "joint", [1, 2, 17, 100, 128, 129, 200, 256, 257, 300, 384, 385, 500, 513, 640, 800, 1000, 1500, 2049,
+                             3000, 4096, 5, 64, 700]),  # one key tile to many, shares and cut items
+    (32, 8, 17, 64, "split", [4096, 1, 129, 2500, 257, 60, 900, 385, 3333, 128, 1700, 30, 513, 641, 2048, 1, 200, 300, 256, 4000]),
+    (16, 8, 5, 24, "joint", [(97 * i) % 520 + 1 for i in range(60)]),  # many short items, one by one
+    (8, 1, 16, 1, "split", [1000, 127, 300, 16]),  # all 128 rows
+    (3, 1, 1, 16, "joint", [700, 1, 129, 0, 5000]),  # a new token each
+]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 5)])
+@pytest.mark.parametrize("case", VERIFY, ids=["shares", "groups", "short", "full", "one"])
+def test_window_verify(case, window, sinks, D, dt):
+    H, KH, most, page, layout, lengths = case
+    g = torch.Generator().manual_seed(26)
+    rows = [min(L, most - i % 3 if most > 3 else most) for i, L in enumerate(lengths)]
+    pools, table, descales = make_cache(g, lengths, KH, D, page, FP8 if dt == "e4m3" else torch.bfloat16, layout)
+    cu = torch.tensor([0] + rows).cumsum(0).int()
+    q = torch.randn(int(cu[-1]), H, D, generator=g).to(torch.bfloat16)
+    _, k, v = views(pools, D)
+    got = ops().paged_window_attention(
+        q.to(DEV), k, v, cu.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV), most,
+        max(lengths), D ** -0.5, window=window, sinks=sinks, descales=None if descales is None else descales.to(DEV))
+    assert error_word() == 0
+    want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu, lengths, table, D ** -0.5, window, sinks, descales)
+    close(got, want, mag, "window", dt == "e4m3")
