@@ -684,3 +684,151 @@ def test_window_verify(case, window, sinks, D, dt):
     assert error_word() == 0
     want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu, lengths, table, D ** -0.5, window, sinks, descales)
     close(got, want, mag, "window", dt == "e4m3")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (3500, 20)])
+def test_decode_joins_many_chunks_at_head_dim_64(dt, window, sinks):
+    """Few requests with long contexts: more than 16 chunks to a row."""
+    H, KH, D, page, lengths = 12, 1, 64, 16, [5003, 300, 0, 4000]
+    g = torch.Generator().manual_seed(27)
+    pools, table, descales = make_cache(g, lengths, KH, D, page, FP8 if dt == "e4m3" else torch.bfloat16, "joint")
+    q = torch.randn(len(lengths), H, D, generator=g).to(torch.bfloat16)
+    _, k, v = views(pools, D)
+    want, mag, w = O.decode_attention(q, *cpu_views(pools, D), lengths, table, D ** -0.5, window, sinks, descales)
+    for gather in (False, True):
+        sums = torch.zeros(len(lengths), KH, 5003, device=DEV) if gather else None
+        got = ops().paged_decode_attention(
+            q.to(DEV), k, v, torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV), 5003, D ** -0.5,
+            window=window, sinks=sinks, descales=None if descales is None else descales.to(DEV), weight_sums=sums)
+        assert error_word() == 0
+        close(got, want, mag, "decode", dt == "e4m3")
+    for r, L in enumerate(lengths):
+        s = sums[r].double().cpu()
+        assert ((s[:, :L] - w[r]).abs() <= (2.0 ** -16 + 2.0 ** -22) * w[r]).all() and float(s[:, L:].abs().sum()) == 0.0
+
+
+@pytest.mark.parametrize("dt", ["bf16", "e4m3"])
+def test_window_of_many_row_tiles(dt):
+    """More than 512 row tiles and requests, dealt out in shares."""
+    H, KH, D, page = 16, 1, 64, 16
+    lengths = [(53 * i) % 90 + 1 + (800 if i % 61 == 7 else 0) for i in range(530)]
+    rows = [min(L, 1 + (7 * i) % 40) for i, L in enumerate(lengths)]
+    g = torch.Generator().manual_seed(28)
+    pools, table, descales = make_cache(g, lengths, KH, D, page, FP8 if dt == "e4m3" else torch.bfloat16, "split")
+    cu = torch.tensor([0] + rows).cumsum(0).int()
+    q = torch.randn(int(cu[-1]), H, D, generator=g).to(torch.bfloat16)
+    _, k, v = views(pools, D)
+    for window, sinks in ((0, 0), (600, 3)):
+        got = ops().paged_window_attention(
+            q.to(DEV), k, v, cu.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV), max(rows),
+            max(lengths), D ** -0.5, window=window, sinks=sinks, descales=None if descales is None else descales.to(DEV))
+        assert error_word() == 0
+        want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu, lengths, table, D ** -0.5, window, sinks, descales)
+        close(got, want, mag, "window", dt == "e4m3")
+
+
+@pytest.mark.parametrize("rows", [[17, 9], [300, 40]], ids=["verify", "chunk"])
+def test_window_in_a_cuda_graph(rows):
+    g = torch.Generator().manual_seed(29)
+    lengths, KH, H, D = [900, 300], 2, 8, 128
+    pools, table, _ = make_cache(g, lengths, KH, D, 16, torch.bfloat16, "joint")
+    _, k, v = views(pools, D)
+    q = torch.randn(sum(rows), H, D, generator=g).to(torch.bfloat16)
+    dq, t = q.to(DEV), table.to(DEV)
+    L = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, rows[0], sum(rows)], dtype=torch.int32, device=DEV)
+
+    def call():
+        return ops().paged_window_attention(dq, k, v, cu, L, t, max(rows), 900, D ** -0.5, window=500, sinks=4)
+
+    eager = call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    out.fill_(math.nan)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, eager)
+    L.copy_(torch.tensor([450, 0], dtype=torch.int32))  # lengths and bounds are read when the graph runs
+    cu.copy_(torch.tensor([0, rows[0] - 3, sum(rows)], dtype=torch.int32))
+    graph.replay()
+    assert error_word() == 0
+    want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu.tolist(), [450, 0], table, D ** -0.5, 500, 4)
+    close(out, want, mag, "window")
+
+
+@pytest.mark.parametrize("case", [(2, [900, 300, 200], True), (50, [900, 300, 200], True), (50, [900, 300, 200], False),
+                                  (5, [9000, 300, 200], True)], ids=["few", "many", "copied", "clusters"])
+def test_evict_in_a_cuda_graph(case):
+    times, some, in_place = case
+    lengths, KH, D, page, budget = some * times, 2, 64, 16, 250
+    g = torch.Generator().manual_seed(30)
+    R, out_cols = len(lengths), -(-budget // page)
+    pools, table, _ = make_cache(g, lengths, KH, D, page, torch.bfloat16, "joint", spare=0 if in_place else R * out_cols)
+    to = table
+    if not in_place:
+        free = sorted(set(range(1, pools[0].shape[0])) - set(table.flatten().tolist()))
+        to = torch.tensor(free, dtype=torch.int32)[: R * out_cols].view(R, out_cols)
+    dev, k, v = views(pools, D)
+    first = dev[0].clone()
+    L, t, dto = torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV), to.to(DEV)
+    values = torch.rand(R, KH, max(lengths), generator=g)
+    sums = values.to(DEV)
+
+    def call():
+        return ops().evict_paged_context(k, v, L, t, sums, budget, sinks=4, recent=30,
+                                         out_block_table=None if in_place else dto)
+
+    call()
+    dev[0].copy_(first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept, n, got = call()
+    for now in (lengths, [max(0, x - 270) for x in lengths]):  # lengths and sums are read when the graph runs
+        dev[0].copy_(first)
+        values = torch.rand(R, KH, max(lengths), generator=g)
+        sums.copy_(values.to(DEV))
+        L.copy_(torch.tensor(now, dtype=torch.int32))
+        graph.replay()
+        assert error_word() == 0
+        want = O.evict(values, now, budget, 4, 30)
+        assert n.tolist() == [min(x, budget) for x in now]
+        assert kept.tolist() == [[w + [-1] * (budget - len(w)) for w in per] for per in want]
+        assert torch.equal(dev[0].view(torch.uint8).cpu(), evicted(pools, table, to, want, now, budget, page)[0])
+
+
+def test_window_and_eviction_of_strided_tensors_on_another_stream():
+    g = torch.Generator().manual_seed(31)
+    lengths, rows, KH, H, D, page, budget = [130, 50, 300], [20, 50, 7], 2, 4, 128, 16, 40
+    pools, table, _ = make_cache(g, lengths, KH, D, page, torch.bfloat16, "joint", spare=12)
+    dev, k, v = views(pools, D)
+    wide = torch.randn(sum(rows), H, 3, D, generator=g).to(torch.bfloat16)
+    q = wide.to(DEV)[:, :, 1]
+    tables = torch.full((6, table.shape[1] + 3), 10_000, dtype=torch.int32)  # rows of a wider table, every other one
+    tables[::2, : table.shape[1]] = table
+    t = tables.to(DEV)[::2, : table.shape[1]]
+    free = sorted(set(range(1, pools[0].shape[0])) - set(table.flatten().tolist()))
+    to = torch.tensor(free[:9], dtype=torch.int32).view(3, 3)
+    wide_to = torch.full((3, 5), 10_000, dtype=torch.int32)
+    wide_to[:, :3] = to
+    big = torch.rand(3, 3 * KH, 310, generator=g)
+    dbig = big.to(DEV)
+    L = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0] + rows).cumsum(0).int()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = ops().paged_window_attention(q, k, v, cu.to(DEV), L, t, 50, 300, D ** -0.5, window=60, sinks=2)
+        kept, n, got = ops().evict_paged_context(k, v, L, t, dbig[:, 1:1 + KH, :300], budget, sinks=1, recent=5,
+                                                 out_block_table=wide_to.to(DEV)[:, :3])
+    side.synchronize()
+    assert error_word() == 0
+    want, mag, _ = O.window_attention(wide[:, :, 1], *cpu_views(pools, D), cu, lengths, table, D ** -0.5, 60, 2)
+    close(out, want, mag, "window")
+    rows_kept = O.evict(big[:, 1:1 + KH], lengths, budget, 1, 5)
+    assert kept.tolist() == rows_kept and n.tolist() == [40, 40, 40]
+    for r in range(3):
+        for h in range(KH):
+            assert torch.equal(got[r, h].cpu(), big[r, 1 + h, rows_kept[r][h]])
+    assert torch.equal(dev[0].view(torch.uint8).cpu(), evicted(pools, table, to, rows_kept, lengths, budget, page)[0])
