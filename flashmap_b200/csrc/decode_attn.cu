@@ -605,8 +605,12 @@ extern "C" fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_
     return set_error(FM_ERR_SHAPE, "paged_decode_attn: window and sinks must not be negative");
   if (cache->requests == 0) return FM_OK;
   if (!p->q || !p->out) return set_error(FM_ERR_INVALID, "paged_decode_attn: null pointer");
-  if ((uintptr_t)p->q % 4 || p->q_request_stride % 2 || p->q_head_stride % 2 || (uintptr_t)p->out % 8 ||
-      p->out_request_stride % 4 || p->out_head_stride % 4)
+  // one request or one head is not stepped through: its stride may be anything
+  a.q_rs = cache->requests == 1 ? 0 : p->q_request_stride;
+  a.q_hs = p->heads == 1 ? 0 : p->q_head_stride;
+  a.o_rs = cache->requests == 1 ? 0 : p->out_request_stride;
+  a.o_hs = p->heads == 1 ? 0 : p->out_head_stride;
+  if ((uintptr_t)p->q % 4 || a.q_rs % 2 || a.q_hs % 2 || (uintptr_t)p->out % 8 || a.o_rs % 4 || a.o_hs % 4)
     return set_error(FM_ERR_ALIGN, "paged_decode_attn: query rows must be 4-byte, output rows 8-byte aligned");
   const bool sums = p->weight_sums != nullptr;
   const DecodePlan pl = decode_plan(cache->requests, p->heads, cache->kv_heads, cache->head_dim, cache->max_length,
@@ -615,8 +619,6 @@ extern "C" fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_
     return set_error(FM_ERR_WORKSPACE, "paged_decode_attn: workspace %zu < %zu", p->workspace_bytes, pl.total);
   if ((uintptr_t)p->workspace % 16) return set_error(FM_ERR_ALIGN, "paged_decode_attn: workspace not 16-byte aligned");
   a.q = static_cast<const uint8_t*>(p->q);
-  a.q_rs = p->q_request_stride;
-  a.q_hs = p->q_head_stride;
   a.H = (int)p->heads;
   a.G = (int)(p->heads / cache->kv_heads);
   a.hgroups = pl.hgroups;
@@ -626,8 +628,6 @@ extern "C" fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_
   a.least = pl.least;
   a.chunks = pl.chunks;
   a.out = static_cast<__nv_bfloat16*>(p->out);
-  a.o_rs = p->out_request_stride;
-  a.o_hs = p->out_head_stride;
   a.sums = p->weight_sums;
   a.s_rs = p->sums_request_stride;
   a.s_hs = p->sums_head_stride;

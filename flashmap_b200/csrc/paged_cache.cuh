@@ -71,6 +71,10 @@ inline fm_status cache_ref(const fm_paged_cache* p, const char* who, CacheRef* c
                 p->page_table, p->page_table_stride, p->lengths, p->descales,
                 (int)p->page_size, (int)p->num_pages, 0, (int)p->requests, (int)p->kv_heads,
                 make_divider((uint32_t)p->page_size), false};
+  // what has one page, head or token is not stepped through: its stride may be anything
+  if (c->num_pages == 1) c->kps = c->vps = 0;
+  if (c->KH == 1) c->khs = c->vhs = 0;
+  if (c->page == 1) c->kts = c->vts = 0;
   c->same = c->kps == c->vps && c->khs == c->vhs && c->kts == c->vts;
   const long long cap = p->page_table_cols > p->max_length / p->page_size ? p->max_length
                                                                            : p->page_table_cols * p->page_size;

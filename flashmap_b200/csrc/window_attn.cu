@@ -1211,12 +1211,14 @@ extern "C" fm_status fm_paged_window_attn(const fm_paged_cache* cache, const fm_
     return set_error(FM_ERR_SHAPE, "paged_window_attn: too many query rows");
   if (cache->requests == 0 || p->rows == 0) return FM_OK;
   if (!p->q || !p->out || !p->cu_seqlens_q) return set_error(FM_ERR_INVALID, "paged_window_attn: null pointer");
-  if ((uintptr_t)p->q % 16 || p->q_token_stride % 8 || p->q_head_stride % 8 || (uintptr_t)p->out % 16 ||
-      p->out_token_stride % 8 || p->out_head_stride % 8)
+  // one row or one head is not stepped through: its stride may be anything
+  a.q_ts = p->rows == 1 ? 0 : p->q_token_stride;
+  a.q_hs = p->heads == 1 ? 0 : p->q_head_stride;
+  a.o_ts = p->rows == 1 ? 0 : p->out_token_stride;
+  a.o_hs = p->heads == 1 ? 0 : p->out_head_stride;
+  if ((uintptr_t)p->q % 16 || a.q_ts % 8 || a.q_hs % 8 || (uintptr_t)p->out % 16 || a.o_ts % 8 || a.o_hs % 8)
     return set_error(FM_ERR_ALIGN, "paged_window_attn: query and output rows must be 16-byte aligned");
   a.q = static_cast<const uint8_t*>(p->q);
-  a.q_ts = p->q_token_stride;
-  a.q_hs = p->q_head_stride;
   a.cu = p->cu_seqlens_q;
   a.T = (int)p->rows;
   a.H = (int)p->heads;
@@ -1226,8 +1228,6 @@ extern "C" fm_status fm_paged_window_attn(const fm_paged_cache* cache, const fm_
   a.window = p->window >= cache->max_length ? 0 : (int)p->window;  // so wide that it hides nothing
   a.sinks = (int)p->sinks;
   a.out = static_cast<__nv_bfloat16*>(p->out);
-  a.o_ts = p->out_token_stride;
-  a.o_hs = p->out_head_stride;
   a.err = p->err;
   const WindowPlan pl = window_plan(cache->requests, p->rows, p->heads, cache->kv_heads, cache->head_dim, p->max_q,
                                     cache->max_length, p->window, p->sinks);

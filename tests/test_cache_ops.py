@@ -147,3 +147,21 @@ def test_oracle_evict_rules():
     assert O.evict(sums, [8], 4, 2, 1) == [[[0, 1, 2, 7]]]
     assert O.evict(sums, [7], 6, 1, 1) == [[[0, 1, 2, 3, 5, 6]]]  # what is no number goes first
     assert O.evict(sums, [8], 3, 1, 2) == [[[0, 6, 7]]]
+
+
+def test_strides_of_dimensions_of_one_do_not_matter():
+    """A tensor may give a dimension of size 1 any stride, and nothing steps by it."""
+    for kw in (dict(num_pages=1, k_page_stride=4101, v_page_stride=3), dict(kv_heads=1, k_head_stride=7, v_head_stride=1),
+               dict(page_size=1, k_token_stride=5, v_token_stride=9)):
+        st, msg = _status("fm_paged_evict", _cache(**kw), _evict())
+        assert st == WORKSPACE, (kw, st, msg)  # the check that comes after the alignment
+    st, msg = _status("fm_paged_decode_attn", _cache(requests=1), _decode(q_request_stride=3, weight_sums=1 << 28))
+    assert st == WORKSPACE, (st, msg)
+    st, msg = _status("fm_paged_decode_attn", _cache(kv_heads=1), _decode(heads=1, q_head_stride=3, weight_sums=1 << 28))
+    assert st == WORKSPACE, (st, msg)
+    long = _cache(max_length=4096, page_table_cols=256)
+    st, msg = _status("fm_paged_window_attn", long, _window(rows=1, q_token_stride=5))
+    assert st == WORKSPACE, (st, msg)
+    long.kv_heads = 1
+    st, msg = _status("fm_paged_window_attn", long, _window(heads=1, q_head_stride=5))
+    assert st == WORKSPACE, (st, msg)

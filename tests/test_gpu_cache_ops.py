@@ -832,3 +832,22 @@ def test_window_and_eviction_of_strided_tensors_on_another_stream():
         for h in range(KH):
             assert torch.equal(got[r, h].cpu(), big[r, 1 + h, rows_kept[r][h]])
     assert torch.equal(dev[0].view(torch.uint8).cpu(), evicted(pools, table, to, rows_kept, lengths, budget, page)[0])
+
+
+def test_strides_of_dimensions_of_one():
+    g = torch.Generator().manual_seed(32)
+    D, page = 128, 48
+    pool = torch.randn(page * 2 * D + 16, generator=g).to(torch.bfloat16)
+    cache = pool.as_strided((1, 1, page, 2 * D), (5, 3, 2 * D, 1))
+    q = torch.randn(4 * D, generator=g).to(torch.bfloat16).as_strided((1, 4, D), (3, D, 1))
+    table, L, cu = torch.zeros(1, 1, dtype=torch.int32), torch.tensor([40], dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32)
+    dc = pool.to(DEV).as_strided((1, 1, page, 2 * D), (5, 3, 2 * D, 1))
+    dq = q.contiguous().to(DEV).as_strided((1, 4, D), (3, D, 1))
+    want, mag, _ = O.decode_attention(q, cache[..., :D], cache[..., D:], [40], table, D ** -0.5)
+    a = ops().paged_decode_attention(dq, dc[..., :D], dc[..., D:], L.to(DEV), table.to(DEV), 40, D ** -0.5)
+    b = ops().paged_window_attention(dq, dc[..., :D], dc[..., D:], cu.to(DEV), L.to(DEV), table.to(DEV), 1, 40, D ** -0.5)
+    close(a, want, mag, "decode")
+    close(b, want, mag, "window")
+    kept, n, _ = ops().evict_paged_context(dc[..., :D], dc[..., D:], L.to(DEV), table.to(DEV),
+                                           torch.arange(40.0, device=DEV).view(1, 1, 40), 20)
+    assert kept[0, 0].tolist() == list(range(20, 40)) and error_word() == 0
