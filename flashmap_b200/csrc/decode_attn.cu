@@ -651,7 +651,7 @@ extern "C" fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_
   const unsigned grid = (unsigned)(items * pl.chunks);
   st = cache->head_dim == 128 ? launch_decode_hd<128>(a, kv8, pl.ng, grid, s)
                               : launch_decode_hd<64>(a, kv8, pl.ng, grid, s);
-  if (st != FM_OK || (pl.chunks == 1 && !sums)) return st;
+  if (st != FM_OK || join == 0) return st;  // one chunk, and no sums or no positions
   const dim3 grid2((unsigned)join), block(nt);
   auto join_launch = [&](auto kernel) {
     return launch_kernel(kernel, grid2, block, 0, s, true, a, (int)row_blocks, (int)key_blocks);

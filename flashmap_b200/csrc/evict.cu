@@ -395,13 +395,13 @@ extern "C" fm_status fm_paged_evict(const fm_paged_cache* cache, const fm_evict*
       p->recent > p->budget - p->sinks)
     return set_error(FM_ERR_SHAPE, "paged_evict: sinks + recent must lie within the budget");
   if (cache->requests == 0) return FM_OK;
-  if (!p->weight_sums || !p->kept || !p->lengths || !p->out_sums)
+  if ((!p->weight_sums && cache->max_length > 0) || !p->kept || !p->lengths || !p->out_sums)
     return set_error(FM_ERR_INVALID, "paged_evict: null pointer");
   if (p->out_page_table && p->out_page_table_cols < (p->budget + cache->page_size - 1) / cache->page_size)
     return set_error(FM_ERR_SHAPE, "paged_evict: the new page table does not cover the budget");
   if (p->lengths == cache->lengths)
     return set_error(FM_ERR_INVALID, "paged_evict: the new lengths must not overwrite the old");
-  if (p->out_page_table == cache->page_table)
+  if (p->out_page_table && p->out_page_table == cache->page_table)
     return set_error(FM_ERR_INVALID, "paged_evict: pass no new page table to evict in place");
   const size_t need = fm_paged_evict_workspace_size(cache->requests, cache->kv_heads, p->budget);
   if (!p->workspace || p->workspace_bytes < need)

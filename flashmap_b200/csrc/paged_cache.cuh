@@ -63,7 +63,10 @@ inline fm_status cache_ref(const fm_paged_cache* p, const char* who, CacheRef* c
   if (p->dtype != FM_DT_BF16 && p->dtype != FM_DT_E4M3)
     return set_error(FM_ERR_INVALID, "%s: the cache is bf16 or e4m3", who);
   if (p->requests == 0) return FM_OK;
-  if (!p->k || !p->v || !p->page_table || !p->lengths) return set_error(FM_ERR_INVALID, "%s: null pointer", who);
+  // a cache without a page, a table column or a position has no address to give, and none is used
+  const bool holds = p->num_pages > 0 && p->page_table_cols > 0 && p->max_length > 0;
+  if (!p->lengths || (holds && (!p->k || !p->v || !p->page_table)))
+    return set_error(FM_ERR_INVALID, "%s: null pointer", who);
   const long long esz = p->dtype == FM_DT_E4M3 ? 1 : 2;
   *c = CacheRef{static_cast<uint8_t*>(p->k), static_cast<uint8_t*>(p->v),
                 p->k_page_stride * esz, p->k_head_stride * esz, p->k_token_stride * esz,
@@ -78,7 +81,7 @@ inline fm_status cache_ref(const fm_paged_cache* p, const char* who, CacheRef* c
   c->same = c->kps == c->vps && c->khs == c->vhs && c->kts == c->vts;
   const long long cap = p->page_table_cols > p->max_length / p->page_size ? p->max_length
                                                                            : p->page_table_cols * p->page_size;
-  c->max_len = (int)(p->max_length < cap ? p->max_length : cap);
+  c->max_len = !holds ? 0 : (int)(p->max_length < cap ? p->max_length : cap);
   if ((uintptr_t)c->k % 16 || (uintptr_t)c->v % 16 || c->kps % 16 || c->khs % 16 || c->kts % 16 || c->vps % 16 ||
       c->vhs % 16 || c->vts % 16)
     return set_error(FM_ERR_ALIGN, "%s: cache rows must be 16-byte aligned", who);

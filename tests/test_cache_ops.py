@@ -165,3 +165,15 @@ def test_strides_of_dimensions_of_one_do_not_matter():
     long.kv_heads = 1
     st, msg = _status("fm_paged_window_attn", long, _window(heads=1, q_head_stride=5))
     assert st == WORKSPACE, (st, msg)
+
+
+def test_caches_that_hold_nothing():
+    """Empty tensors have no address: no pages, no table columns, no positions are no error."""
+    for kw in (dict(num_pages=0, k=None, v=None), dict(page_table_cols=0, page_table=None), dict(max_length=0, k=None),
+               dict(max_length=0, page_table_cols=0, page_table=None, num_pages=0, k=None, v=None)):
+        st, msg = _status("fm_paged_evict", _cache(**kw), _evict())
+        assert st == WORKSPACE, (kw, st, msg)  # the check that comes after the addresses
+    st, msg = _status("fm_paged_evict", _cache(max_length=0), _evict(weight_sums=None))
+    assert st == WORKSPACE, (st, msg)
+    assert _status("fm_paged_evict", _cache(num_pages=0, lengths=None), _evict())[0] == INVALID
+    assert _status("fm_paged_evict", _cache(), _evict(weight_sums=None))[0] == INVALID

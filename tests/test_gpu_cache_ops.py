@@ -851,3 +851,27 @@ def test_strides_of_dimensions_of_one():
     kept, n, _ = ops().evict_paged_context(dc[..., :D], dc[..., D:], L.to(DEV), table.to(DEV),
                                            torch.arange(40.0, device=DEV).view(1, 1, 40), 20)
     assert kept[0, 0].tolist() == list(range(20, 40)) and error_word() == 0
+
+
+@pytest.mark.parametrize("dt", ["bf16", "e4m3"])
+def test_caches_that_hold_nothing(dt):
+    """Requests without a position yet: empty tables, sums and pools; their rows see nothing and are zero."""
+    KH, H, D, page, R = 2, 4, 64, 16, 3
+    L = torch.zeros(R, dtype=torch.int32, device=DEV)
+    q = torch.randn(R, H, D, device=DEV).to(torch.bfloat16)
+    cu = torch.arange(R + 1, dtype=torch.int32, device=DEV)
+    for pages, cols in ((4, 0), (0, 0), (0, 2)):
+        cache = torch.zeros(pages, KH, page, 2 * D, dtype=torch.bfloat16, device=DEV)
+        cache = cache.to(FP8) if dt == "e4m3" else cache
+        k, v = cache[..., :D], cache[..., D:]
+        t = torch.zeros(R, cols, dtype=torch.int32, device=DEV)
+        for most in (0, 20):
+            sums = torch.zeros(R, KH, most, device=DEV)
+            for gather in (None, sums, torch.zeros(R, KH, 30, device=DEV)):
+                out = ops().paged_decode_attention(q, k, v, L, t, most, 0.1, weight_sums=gather)
+                assert out.shape == q.shape and float(out.float().abs().max()) == 0.0
+            out = ops().paged_window_attention(q, k, v, cu, L, t, 1, most, 0.1, window=5, sinks=1)
+            assert out.shape == q.shape and float(out.float().abs().max()) == 0.0
+            kept, n, got = ops().evict_paged_context(k, v, L, t, sums, 8, sinks=1)
+            assert int((kept != -1).sum()) == 0 and n.tolist() == [0] * R and float(got.abs().sum()) == 0.0
+    assert error_word() == 0
