@@ -170,7 +170,8 @@ def _err_word(device) -> int:
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_size(name: str, *sizes: int) -> int:
+def _workspace_size(name: str, device: torch.device, *sizes: int) -> int:
+    # `device`, the current one, is part of the key: a size may go by its number of SMs
     return getattr(_lib.load(), name)(*sizes)
 
 
@@ -210,7 +211,7 @@ def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     if cache.requests == 0:
         return out
     heads, qs, os = query.shape[1], query.stride(), out.stride()
-    need = _workspace_size("fm_paged_decode_attn_workspace_size", cache.requests, heads, cache.kv_heads, cache.head_dim,
+    need = _workspace_size("fm_paged_decode_attn_workspace_size", dev, cache.requests, heads, cache.kv_heads, cache.head_dim,
                            cache.max_length, window, sinks, int(weight_sums is not None))
     ws = seqused_k.new_empty(need // 4) if need else None  # sizes are multiples of 8
     _launch("fm_paged_decode_attn", cache,
@@ -246,7 +247,7 @@ def paged_window_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     if cache.requests == 0 or tokens == 0:
         return out
     qs, os = query.stride(), out.stride()
-    need = _workspace_size("fm_paged_window_attn_workspace_size", cache.requests, tokens, heads, cache.kv_heads,
+    need = _workspace_size("fm_paged_window_attn_workspace_size", dev, cache.requests, tokens, heads, cache.kv_heads,
                            cache.head_dim, int(max_seqlen_q), cache.max_length, window, sinks)
     ws = seqused_k.new_empty(need // 4) if need else None  # sizes are multiples of 8
     _launch("fm_paged_window_attn", cache,
@@ -294,7 +295,7 @@ def evict_paged_context(k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k:
         _need(out_block_table.shape[1] * cache.page_size >= budget, "out_block_table does not cover the budget")
         to, to_stride, to_cols = out_block_table.data_ptr(), out_block_table.stride(0), out_block_table.shape[1]
     if cache.requests:
-        need = _workspace_size("fm_paged_evict_workspace_size", cache.requests, cache.kv_heads, budget)
+        need = _workspace_size("fm_paged_evict_workspace_size", dev, cache.requests, cache.kv_heads, budget)
         ws = seqused_k.new_empty(need // 4)
         _launch("fm_paged_evict", cache,
                 _EVICT.pack(weight_sums.data_ptr(), weight_sums.stride(0), weight_sums.stride(1), budget, sinks, recent,

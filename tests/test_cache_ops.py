@@ -177,3 +177,21 @@ def test_caches_that_hold_nothing():
     assert st == WORKSPACE, (st, msg)
     assert _status("fm_paged_evict", _cache(num_pages=0, lengths=None), _evict())[0] == INVALID
     assert _status("fm_paged_evict", _cache(), _evict(weight_sums=None))[0] == INVALID
+
+
+def test_workspace_sizes_are_kept_by_device(monkeypatch):
+    """The chunk kernel's workspace goes by the device's number of SMs."""
+    from flashmap_b200 import cache_ops as C
+    device = [0]
+
+    class Library:
+        def fm_paged_window_attn_workspace_size(self, *sizes):
+            return sum(sizes) * (1 + device[0])
+
+    monkeypatch.setattr(C._lib, "load", lambda: Library())
+    C._workspace_size.cache_clear()
+    got = []
+    for device[0] in (0, 1, 0):
+        got.append(C._workspace_size("fm_paged_window_attn_workspace_size", torch.device("cuda", device[0]), 3, 4))
+    C._workspace_size.cache_clear()
+    assert got == [7, 14, 7]
