@@ -24,7 +24,10 @@ f16 for an e4m3 cache) for the product with the values, and the output to bf16.
 A row that sees no position is zero.  A position that no row of a request may
 see is never read.  Each call checks its arguments (``OpArgumentError``), runs
 on the current stream without a host synchronisation, and can be captured in a
-CUDA graph.  There is no fallback.
+CUDA graph.  The two attentions are registered operators
+(``flashmap_b200::paged_decode_attention``, ``::paged_window_attention``) to
+``torch.compile``; they have no gradient, and asking for one raises.  There is
+no fallback.
 """
 
 from __future__ import annotations
@@ -181,20 +184,8 @@ def _launch(name: str, cache: _Cache, args: bytes) -> None:
         _lib.check(status, name)
 
 
-def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
-                           seqused_k: torch.Tensor, block_table: torch.Tensor, max_seqlen_k: int,
-                           softmax_scale: float, *, window: int = 0, sinks: int = 0,
-                           descales: Optional[torch.Tensor] = None,
-                           weight_sums: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Attention of one new token per request, ``query (requests, heads,
-    head_dim)`` bf16, at position ``seqused_k - 1`` of its context (its own key
-    and value are in the cache already); ``(requests, heads, head_dim)`` bf16.
-
-    It sees every position, or with ``window > 0`` the last ``window`` and the
-    first ``sinks``.  ``weight_sums (requests, kv_heads, >= max_seqlen_k)`` fp32
-    is added to in place: position j of a kv head gathers the attention weights
-    of its query heads, which ``evict_paged_context`` goes by; no two of its rows
-    may share memory.  A request has at most ``max_seqlen_k`` positions."""
+def _decode(query, k_cache, v_cache, seqused_k, block_table, max_seqlen_k, softmax_scale, window, sinks, descales,
+            weight_sums) -> torch.Tensor:
     cache = _cache(k_cache, v_cache, seqused_k, block_table, descales, int(max_seqlen_k))
     dev = k_cache.device
     query = _query(query, cache, dev)
@@ -220,20 +211,8 @@ def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     return out
 
 
-def paged_window_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
-                           cu_seqlens_q: torch.Tensor, seqused_k: torch.Tensor, block_table: torch.Tensor,
-                           max_seqlen_q: int, max_seqlen_k: int, softmax_scale: float, *, window: int = 0,
-                           sinks: int = 0, descales: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Causal attention of chunks of query rows: rows ``cu_seqlens_q[r] ..
-    cu_seqlens_q[r + 1]`` of ``query (tokens, heads, head_dim)`` bf16 are the
-    last positions of request r's ``seqused_k[r]`` (their own keys and values
-    are in the cache already); ``(tokens, heads, head_dim)`` bf16.
-
-    The row at position p sees the positions j <= p; with ``window > 0`` of
-    those only p - j < ``window`` or j < ``sinks``.  A request has at most
-    ``max_seqlen_q`` rows and ``max_seqlen_k`` positions.  Values that some rows
-    of a chunk see and others do not must be finite.  Rows that ``cu_seqlens_q``
-    gives to no request are not written."""
+def _window(query, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, max_seqlen_q, max_seqlen_k, softmax_scale,
+            window, sinks, descales) -> torch.Tensor:
     cache = _cache(k_cache, v_cache, seqused_k, block_table, descales, int(max_seqlen_k))
     dev = k_cache.device
     query = _query(query, cache, dev)
@@ -255,6 +234,80 @@ def paged_window_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
                          softmax_scale, window, sinks, out.data_ptr(), os[0], os[1], ws.data_ptr() if need else 0, need,
                          _err_word(dev)))
     return out
+
+
+@torch.library.custom_op("flashmap_b200::paged_decode_attention", mutates_args=("weight_sums",))
+def _decode_op(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k: torch.Tensor,
+               block_table: torch.Tensor, max_seqlen_k: int, softmax_scale: float, window: int, sinks: int,
+               descales: Optional[torch.Tensor], weight_sums: Optional[torch.Tensor]) -> torch.Tensor:
+    return _decode(query, k_cache, v_cache, seqused_k, block_table, max_seqlen_k, softmax_scale, window, sinks, descales,
+                   weight_sums)
+
+
+@_decode_op.register_fake
+def _(query, k_cache, v_cache, seqused_k, block_table, max_seqlen_k, softmax_scale, window, sinks, descales, weight_sums):
+    return query.new_empty(query.shape)
+
+
+@torch.library.custom_op("flashmap_b200::paged_window_attention", mutates_args=())
+def _window_op(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, cu_seqlens_q: torch.Tensor,
+               seqused_k: torch.Tensor, block_table: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int,
+               softmax_scale: float, window: int, sinks: int, descales: Optional[torch.Tensor]) -> torch.Tensor:
+    return _window(query, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, max_seqlen_q, max_seqlen_k,
+                   softmax_scale, window, sinks, descales)
+
+
+@_window_op.register_fake
+def _(query, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, max_seqlen_q, max_seqlen_k, softmax_scale, window,
+      sinks, descales):
+    return query.new_empty(query.shape)
+
+
+def _by_op(query, k_cache, v_cache) -> bool:
+    """Whether a call goes through its registered operator: where it is traced,
+    and where a gradient would be asked of it (which that operator refuses).
+    Else it goes straight to the kernels, for a registered operator costs as
+    much host time as the rest of a short call."""
+    return torch.compiler.is_compiling() or torch.is_grad_enabled() and (
+        query.requires_grad or k_cache.requires_grad or v_cache.requires_grad)
+
+
+def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                           seqused_k: torch.Tensor, block_table: torch.Tensor, max_seqlen_k: int,
+                           softmax_scale: float, *, window: int = 0, sinks: int = 0,
+                           descales: Optional[torch.Tensor] = None,
+                           weight_sums: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per request, ``query (requests, heads,
+    head_dim)`` bf16, at position ``seqused_k - 1`` of its context (its own key
+    and value are in the cache already); ``(requests, heads, head_dim)`` bf16.
+
+    It sees every position, or with ``window > 0`` the last ``window`` and the
+    first ``sinks``.  ``weight_sums (requests, kv_heads, >= max_seqlen_k)`` fp32
+    is added to in place: position j of a kv head gathers the attention weights
+    of its query heads, which ``evict_paged_context`` goes by; no two of its rows
+    may share memory.  A request has at most ``max_seqlen_k`` positions."""
+    call = _decode_op if _by_op(query, k_cache, v_cache) else _decode
+    return call(query, k_cache, v_cache, seqused_k, block_table, max_seqlen_k, softmax_scale, window, sinks, descales,
+                weight_sums)
+
+
+def paged_window_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                           cu_seqlens_q: torch.Tensor, seqused_k: torch.Tensor, block_table: torch.Tensor,
+                           max_seqlen_q: int, max_seqlen_k: int, softmax_scale: float, *, window: int = 0,
+                           sinks: int = 0, descales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of chunks of query rows: rows ``cu_seqlens_q[r] ..
+    cu_seqlens_q[r + 1]`` of ``query (tokens, heads, head_dim)`` bf16 are the
+    last positions of request r's ``seqused_k[r]`` (their own keys and values
+    are in the cache already); ``(tokens, heads, head_dim)`` bf16.
+
+    The row at position p sees the positions j <= p; with ``window > 0`` of
+    those only p - j < ``window`` or j < ``sinks``.  A request has at most
+    ``max_seqlen_q`` rows and ``max_seqlen_k`` positions.  Values that some rows
+    of a chunk see and others do not must be finite.  Rows that ``cu_seqlens_q``
+    gives to no request are not written."""
+    call = _window_op if _by_op(query, k_cache, v_cache) else _window
+    return call(query, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, max_seqlen_q, max_seqlen_k, softmax_scale,
+                window, sinks, descales)
 
 
 def evict_paged_context(k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k: torch.Tensor,

@@ -195,3 +195,17 @@ def test_workspace_sizes_are_kept_by_device(monkeypatch):
         got.append(C._workspace_size("fm_paged_window_attn_workspace_size", torch.device("cuda", device[0]), 3, 4))
     C._workspace_size.cache_clear()
     assert got == [7, 14, 7]
+
+
+def test_attentions_are_registered_with_a_fake():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from flashmap_b200 import cache_ops  # noqa: F401
+    with FakeTensorMode():
+        k = torch.empty(4, 2, 16, 64, dtype=torch.bfloat16)
+        q, L = torch.empty(3, 4, 64, dtype=torch.bfloat16), torch.empty(3, dtype=torch.int32)
+        t, cu = torch.empty(3, 2, dtype=torch.int32), torch.empty(4, dtype=torch.int32)
+        a = torch.ops.flashmap_b200.paged_decode_attention(q, k, k, L, t, 20, 0.1, 0, 0, None, torch.empty(3, 2, 20))
+        b = torch.ops.flashmap_b200.paged_window_attention(q, k, k, cu, L, t, 1, 20, 0.1, 5, 1, None)
+        for x in (a, b):
+            assert x.shape == q.shape and x.dtype == q.dtype and x.is_contiguous()

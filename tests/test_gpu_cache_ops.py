@@ -875,3 +875,53 @@ def test_caches_that_hold_nothing(dt):
             kept, n, got = ops().evict_paged_context(k, v, L, t, sums, 8, sinks=1)
             assert int((kept != -1).sum()) == 0 and n.tolist() == [0] * R and float(got.abs().sum()) == 0.0
     assert error_word() == 0
+
+
+def attention_calls(KH=2, H=8, D=128, page=16, lengths=(90, 33)):
+    """(query, one call of each attention on it) over one small cache."""
+    g = torch.Generator().manual_seed(33)
+    pools, table, _ = make_cache(g, list(lengths), KH, D, page, torch.bfloat16, "joint")
+    _, k, v = views(pools, D)
+    L, t = torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV)
+    cu = torch.arange(len(lengths) + 1, dtype=torch.int32, device=DEV)
+    q = torch.randn(len(lengths), H, D, generator=g).to(torch.bfloat16).to(DEV)
+
+    def decode(q, sums=None, k=k):
+        return ops().paged_decode_attention(q, k, v, L, t, max(lengths), D ** -0.5, weight_sums=sums)
+
+    def chunk(q, sums=None, k=k):
+        return ops().paged_window_attention(q, k, v, cu, L, t, 1, max(lengths), D ** -0.5, window=50, sinks=2)
+
+    return q, k, (decode, chunk)
+
+
+def test_no_gradient_is_an_error_and_not_a_constant():
+    q, k, calls = attention_calls()
+    for call in calls:
+        plain = call(q)
+        assert not plain.requires_grad
+        for kw in (dict(q=q.clone().requires_grad_()), dict(q=q, k=k.detach().clone().requires_grad_())):
+            out = call(**kw)
+            assert torch.equal(out, plain) and out.requires_grad
+            with pytest.raises(RuntimeError):
+                out.float().sum().backward()
+            with torch.no_grad():
+                assert not call(**kw).requires_grad
+    a, b = torch.zeros(2, 2, 90, device=DEV), torch.zeros(2, 2, 90, device=DEV)
+    assert torch.equal(calls[0](q, a), calls[0](q.clone().requires_grad_(), b)) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_attentions_stay_whole_in_a_compiled_graph(backend):
+    q, _, calls = attention_calls()
+    for call in calls:
+        def layer(q, sums):
+            return call(q * 2, sums) + 1
+
+        compiled = torch.compile(layer, backend=backend, fullgraph=True)
+        for scale in (1.0, 0.5):
+            a, b = torch.zeros(2, 2, 90, device=DEV), torch.zeros(2, 2, 90, device=DEV)
+            with torch.no_grad():
+                assert torch.equal(compiled(q * scale, a), layer(q * scale, b))
+            assert torch.equal(a, b)
+    assert error_word() == 0
