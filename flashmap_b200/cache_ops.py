@@ -173,8 +173,8 @@ def _err_word(device) -> int:
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_size(name: str, device: torch.device, *sizes: int) -> int:
-    # `device`, the current one, is part of the key: a size may go by its number of SMs
+def _workspace_size(name: str, device: int, *sizes: int) -> int:
+    # the index of the current device is part of the key: a size may go by its number of SMs
     return getattr(_lib.load(), name)(*sizes)
 
 
@@ -189,9 +189,11 @@ def _decode(query, k_cache, v_cache, seqused_k, block_table, max_seqlen_k, softm
     cache = _cache(k_cache, v_cache, seqused_k, block_table, descales, int(max_seqlen_k))
     dev = k_cache.device
     query = _query(query, cache, dev)
-    _need(query.shape[0] == cache.requests, "one query row per request")
-    _visibility(window, sinks)
-    out = query.new_empty(query.shape)
+    shape = query.shape
+    if shape[0] != cache.requests or window < 0 or sinks < 0:
+        _need(shape[0] == cache.requests, "one query row per request")
+        _visibility(window, sinks)
+    out = query.new_empty(shape)
     sums, s0, s1 = 0, 0, 0
     if weight_sums is not None:
         _sums(weight_sums, cache, dev, cache.max_length)
@@ -201,13 +203,14 @@ def _decode(query, k_cache, v_cache, seqused_k, block_table, max_seqlen_k, softm
             _need(_apart(weight_sums), "rows of weight_sums must not share memory")
     if cache.requests == 0:
         return out
-    heads, qs, os = query.shape[1], query.stride(), out.stride()
-    need = _workspace_size("fm_paged_decode_attn_workspace_size", dev, cache.requests, heads, cache.kv_heads, cache.head_dim,
-                           cache.max_length, window, sinks, int(weight_sums is not None))
+    heads, qs = shape[1], query.stride()
+    need = _workspace_size("fm_paged_decode_attn_workspace_size", dev.index, cache.requests, heads, cache.kv_heads,
+                           cache.head_dim, cache.max_length, window, sinks, int(weight_sums is not None))
     ws = seqused_k.new_empty(need // 4) if need else None  # sizes are multiples of 8
     _launch("fm_paged_decode_attn", cache,
             _DECODE.pack(query.data_ptr(), qs[0], qs[1], heads, softmax_scale, window, sinks, sums, s0, s1,
-                         out.data_ptr(), os[0], os[1], ws.data_ptr() if need else 0, need, _err_word(dev)))
+                         out.data_ptr(), heads * cache.head_dim, cache.head_dim, ws.data_ptr() if need else 0, need,
+                         _err_word(dev)))
     return out
 
 
@@ -226,7 +229,7 @@ def _window(query, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, max_s
     if cache.requests == 0 or tokens == 0:
         return out
     qs, os = query.stride(), out.stride()
-    need = _workspace_size("fm_paged_window_attn_workspace_size", dev, cache.requests, tokens, heads, cache.kv_heads,
+    need = _workspace_size("fm_paged_window_attn_workspace_size", dev.index, cache.requests, tokens, heads, cache.kv_heads,
                            cache.head_dim, int(max_seqlen_q), cache.max_length, window, sinks)
     ws = seqused_k.new_empty(need // 4) if need else None  # sizes are multiples of 8
     _launch("fm_paged_window_attn", cache,
@@ -263,13 +266,11 @@ def _(query, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, max_seqlen_
     return query.new_empty(query.shape)
 
 
-def _by_op(query, k_cache, v_cache) -> bool:
-    """Whether a call goes through its registered operator: where it is traced,
-    and where a gradient would be asked of it (which that operator refuses).
-    Else it goes straight to the kernels, for a registered operator costs as
-    much host time as the rest of a short call."""
-    return torch.compiler.is_compiling() or torch.is_grad_enabled() and (
-        query.requires_grad or k_cache.requires_grad or v_cache.requires_grad)
+# A call goes through its registered operator where it is traced, and where a
+# gradient would be asked of it (which that operator refuses).  Else it goes
+# straight to the kernels: the operator's dispatch costs as much host time as
+# the rest of a short call.
+_tracing = torch.compiler.is_compiling
 
 
 def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -286,7 +287,9 @@ def paged_decode_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     is added to in place: position j of a kv head gathers the attention weights
     of its query heads, which ``evict_paged_context`` goes by; no two of its rows
     may share memory.  A request has at most ``max_seqlen_k`` positions."""
-    call = _decode_op if _by_op(query, k_cache, v_cache) else _decode
+    call = _decode
+    if _tracing() or (query.requires_grad or k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled():
+        call = _decode_op
     return call(query, k_cache, v_cache, seqused_k, block_table, max_seqlen_k, softmax_scale, window, sinks, descales,
                 weight_sums)
 
@@ -305,7 +308,9 @@ def paged_window_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     ``max_seqlen_q`` rows and ``max_seqlen_k`` positions.  Values that some rows
     of a chunk see and others do not must be finite.  Rows that ``cu_seqlens_q``
     gives to no request are not written."""
-    call = _window_op if _by_op(query, k_cache, v_cache) else _window
+    call = _window
+    if _tracing() or (query.requires_grad or k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled():
+        call = _window_op
     return call(query, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, max_seqlen_q, max_seqlen_k, softmax_scale,
                 window, sinks, descales)
 
@@ -348,7 +353,7 @@ def evict_paged_context(k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k:
         _need(out_block_table.shape[1] * cache.page_size >= budget, "out_block_table does not cover the budget")
         to, to_stride, to_cols = out_block_table.data_ptr(), out_block_table.stride(0), out_block_table.shape[1]
     if cache.requests:
-        need = _workspace_size("fm_paged_evict_workspace_size", dev, cache.requests, cache.kv_heads, budget)
+        need = _workspace_size("fm_paged_evict_workspace_size", dev.index, cache.requests, cache.kv_heads, budget)
         ws = seqused_k.new_empty(need // 4)
         _launch("fm_paged_evict", cache,
                 _EVICT.pack(weight_sums.data_ptr(), weight_sums.stride(0), weight_sums.stride(1), budget, sinks, recent,

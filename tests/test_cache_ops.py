@@ -192,7 +192,7 @@ def test_workspace_sizes_are_kept_by_device(monkeypatch):
     C._workspace_size.cache_clear()
     got = []
     for device[0] in (0, 1, 0):
-        got.append(C._workspace_size("fm_paged_window_attn_workspace_size", torch.device("cuda", device[0]), 3, 4))
+        got.append(C._workspace_size("fm_paged_window_attn_workspace_size", device[0], 3, 4))
     C._workspace_size.cache_clear()
     assert got == [7, 14, 7]
 
