@@ -3,13 +3,15 @@
     python examples/bounded_context.py --requests 4 --prompt 1500 --new 200 --budget 1024
 
 Each layer's prompt goes through the cache in chunks (``paged_window_attention``:
-a sliding window, the first tokens stay visible), then every new token attends
-to what its request holds (``paged_decode_attention``, which gathers each
-position's attention weight), and whenever a request holds ``--budget`` plus
-``--slack`` positions its cache is cut back to the budget
-(``evict_paged_context``).  Keys and values are written by the serving
-operators' ``write_context_kv``: a key is normed and rotated at the position
-its token has in the text, and keeps that rotation when its row moves.
+a sliding window, the first tokens stay visible), its last ``--look`` tokens and
+then every new token one at a time.  Each of those attends to what its request
+holds (``paged_decode_attention``, which gathers each position's attention
+weight), so that a prompt past the budget is cut by what its last tokens looked
+at.  Whenever a request holds ``--budget`` plus ``--slack`` positions its cache
+is cut back to the budget (``evict_paged_context``).  Keys and values are
+written by the serving operators' ``write_context_kv``: a key is normed and
+rotated at the position its token has in the text, and keeps that rotation when
+its row moves.
 
 The model is a stack of attention layers with random weights: what it computes
 is of no use, the calls are a serving loop's.
@@ -77,8 +79,8 @@ class PagedLayers:
         self.most = min(self.most, budget)
 
 
-def run(requests=4, prompt=1500, new=200, budget=1024, slack=64, window=512, sinks=4, chunk=512, layers=2, heads=16,
-        kv_heads=4, head_dim=128, seed=0):
+def run(requests=4, prompt=1500, new=200, budget=1024, slack=64, window=512, sinks=4, chunk=512, look=32, layers=2,
+        heads=16, kv_heads=4, head_dim=128, seed=0):
     """Runs the loop; returns the last step's output and the positions held after every step."""
     g = torch.Generator(device="cuda").manual_seed(seed)
     cache = PagedLayers(layers, requests, heads, kv_heads, head_dim, max(prompt, budget + slack) + 1)
@@ -92,9 +94,21 @@ def run(requests=4, prompt=1500, new=200, budget=1024, slack=64, window=512, sin
     def rotated(q, positions):
         return serving_ops.vllm_rms_norm_rope(q, cache.norm[0], cache.rope, positions.flatten(), 1e-6)
 
-    # the prompt, chunk by chunk
-    for begin in range(0, prompt, chunk):
-        rows = min(chunk, prompt - begin)
+    def token(position):  # one new token of every request, which gathers weights
+        q, kv = project(1)
+        positions = torch.full((requests, 1), position, device="cuda")
+        cache.append(kv, positions, 1)
+        x = rotated(q, positions)
+        for layer in range(layers):
+            x = cache_ops.paged_decode_attention(x, *cache.views(layer), cache.held, cache.table, cache.most, scale,
+                                                 weight_sums=cache.sums[layer])
+        return x
+
+    # the prompt: chunk by chunk up to its last tokens, whose weights the first eviction goes by
+    x = None
+    body = prompt - min(max(look, 0), prompt)
+    for begin in range(0, body, chunk):
+        rows = min(chunk, body - begin)
         q, kv = project(rows)
         positions = (begin + torch.arange(rows, device="cuda")).repeat(requests, 1)
         cache.append(kv, positions, rows)
@@ -103,18 +117,14 @@ def run(requests=4, prompt=1500, new=200, budget=1024, slack=64, window=512, sin
         for layer in range(layers):
             x = cache_ops.paged_window_attention(x, *cache.views(layer), cu, cache.held, cache.table, rows, cache.most,
                                                  scale, window=window, sinks=sinks)
+    for position in range(body, prompt):
+        x = token(position)
     # new tokens, one at a time
     held = []
     for step in range(new):
         if cache.most >= budget + slack:
             cache.evict(budget, sinks, recent=min(window, budget - sinks))
-        q, kv = project(1)
-        positions = torch.full((requests, 1), prompt + step, device="cuda")
-        cache.append(kv, positions, 1)
-        x = rotated(q, positions)
-        for layer in range(layers):
-            x = cache_ops.paged_decode_attention(x, *cache.views(layer), cache.held, cache.table, cache.most, scale,
-                                                 weight_sums=cache.sums[layer])
+        x = token(prompt + step)
         held.append(cache.most)
     return x, held
 
@@ -122,7 +132,7 @@ def run(requests=4, prompt=1500, new=200, budget=1024, slack=64, window=512, sin
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     for name, value in (("requests", 4), ("prompt", 1500), ("new", 200), ("budget", 1024), ("slack", 64), ("window", 512),
-                        ("sinks", 4), ("chunk", 512), ("layers", 2)):
+                        ("sinks", 4), ("chunk", 512), ("look", 32), ("layers", 2)):
         ap.add_argument(f"--{name}", type=int, default=value)
     args = ap.parse_args(argv)
     x, held = run(**vars(args))

@@ -49,3 +49,20 @@ def test_sums_follow_the_rows_that_stay():
             middle = before[r, h, 4:130].sort(descending=True).values[:76].sum()
             want = middle + before[r, h, :4].sum() + before[r, h, 130:150].sum()
             assert torch.allclose(kept[r, h].sum(), want, atol=1e-5)
+
+
+def test_the_first_eviction_has_weights_to_go_by(monkeypatch):
+    """A prompt past the budget is cut before the first new token: the weights of its own last tokens rank it."""
+    m = example()
+    seen = []
+    plain = m.PagedLayers.evict
+
+    def evict(cache, budget, sinks, recent):
+        seen.append([s[..., : cache.most].sum(-1) for s in cache.sums])
+        plain(cache, budget, sinks, recent)
+
+    monkeypatch.setattr(m.PagedLayers, "evict", evict)
+    _, held = m.run(requests=2, prompt=300, new=2, budget=128, slack=16, window=64, sinks=4, chunk=100, look=20)
+    assert held == [129, 130] and len(seen) == 1
+    for total in seen[0]:  # 20 tokens, 4 query heads to a kv head
+        assert torch.allclose(total, torch.full_like(total, 80.0), atol=1e-3)
