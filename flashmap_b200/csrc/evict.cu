@@ -369,11 +369,14 @@ __global__ void __launch_bounds__(256, 4) evict_move_kernel(EvictArgs a) {
   move_rows<IN_PLACE>(a, r, h, part, slice, begin, end, threadIdx.x);
 }
 
-// CTAs of a cluster: as many as leave three to an SM, with 2048 positions each at least
+// CTAs of a cluster: as many as run at once, two to an SM, with 2048 positions each at least
 // (1 request of 16000, 8 kv heads: 31.6 us against 36.1 us with 4096 and 31.4 us with 1024; 8 of 8000: 36.6, 38.1, 38.0).
+// With three to an SM, 5 requests of 16500 .. 33000 take 79 us against 65 us, 10 of 8200 .. 16000 65 us against 58 us,
+// 20 of 4200 .. 8000, where that means two CTAs against one, 91 us against 92 us.
 int evict_cluster(int64_t items, int64_t positions) {
+  const int64_t resident = 2 * num_sms();
   int cs = 1;
-  while (cs < 8 && items * cs * 2 <= 3 * 148 && positions >= 2048 * 2 * cs) cs *= 2;
+  while (cs < 8 && items * cs * 2 <= resident && positions >= 2048 * 2 * cs) cs *= 2;
   return cs;
 }
 
