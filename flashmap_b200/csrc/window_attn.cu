@@ -112,9 +112,18 @@ constexpr int WA_ITEM = 2;
 constexpr int WA_CUT = 2;
 constexpr int WA_SHARE = WA_ITEM + 4;  // the least length of a CTA's share
 //
-// Where items are too short to cut and there are enough of them, CTA b simply
-// takes items b, b + CTAs, .. from the last row tile on (the longest of a
-// prompt): no shares, no join (12 windowed prompts: 60 us, with shares 65 us).
+// Where there are as many items as CTAs and none has WA_LONG key tiles, CTA b
+// simply takes items b, b + CTAs, .. from the last row tile on (the longest of a
+// prompt): no shares, no join.  Whole items fill the CTAs unevenly, which costs
+// more the longer they are; shares cost their sums and the join.  Us one by one
+// and in shares, 32 heads on 8 of 128, requests of one length, 64 rows each:
+//   requests          500    900     1200     1600     2400     6000 positions
+//         20        37 41  51 51    59 55    71 63    94 77  199 136
+//         40        51 56  75 81    86 85   102 99  137 124  303 243
+//         80        80 93 120 138  137 151  166 169  225 220       -
+// Lengths spread over a factor of 8, and 17 rows each, part ways near there, too; 24
+// prompts of 500 .. 1400 take 289 us one by one, 364 us in shares.
+constexpr int WA_LONG = 14;
 struct WaBorder {
   int r, y, c, t;  // request, row tile, kv head, and the first tile after the border
 };
@@ -1158,7 +1167,7 @@ WindowPlan window_plan(int64_t R, int64_t T, int64_t H, int64_t KH, int64_t HD, 
   const int64_t per = WA_ROWS / (H / KH) + 2, tokens = max_q < per ? max_q : per;  // that a row tile touches
   if (window > 0 && window + tokens + sinks < span) span = window + tokens + sinks;
   const int64_t tiles = span / WA_KEYS + 3;
-  p.cuts = tiles >= (items >= sms ? 8 : 2 * WA_CUT);
+  p.cuts = tiles >= (items >= sms ? WA_LONG : 2 * WA_CUT);
   // an item that can be cut gives work to as many CTAs as it has tiles at most
   const int64_t most = p.cuts ? items * tiles : items;
   p.ctas = (int)(most < sms ? most : sms);

@@ -561,11 +561,14 @@ RUNS_OF_NOTHING = [
     # requests that hold nothing, or less than their rows, between chunks
     (16, 8, [2304, 0, 2304, 0, 2304], [800, 1, 900, 1, 1000]),
     (32, 8, [900, 30, 900, 25, 700], [700, 3000, 800, 4000, 600]),
+    # long enough for shares among many items, too
+    (8, 8, [171 * i % 890 + 911 if i % 8 == 3 else 0 for i in range(200)], [17] * 200),
+    (32, 8, [1900, 30, 1900, 25, 1700], [300, 3000, 400, 4000, 200]),
 ]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "e4m3"])
-@pytest.mark.parametrize("case", RUNS_OF_NOTHING, ids=["padded", "padded_shares", "between", "rows_before"])
+@pytest.mark.parametrize("case", RUNS_OF_NOTHING, ids=["padded", "padded_shares", "between", "rows_before", "padded_long", "rows_before_long"])
 def test_window_runs_of_items_that_see_nothing(case, dt):
     """Several items of a CTA in a row whose rows see no key, after one that has keys: what it still waits for
     must not be held back by them."""
@@ -925,3 +928,24 @@ def test_attentions_stay_whole_in_a_compiled_graph(backend):
                 assert torch.equal(compiled(q * scale, a), layer(q * scale, b))
             assert torch.equal(a, b)
     assert error_word() == 0
+
+
+@pytest.mark.parametrize("dt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("rows_most", [8, 40])
+def test_window_of_many_row_tiles_in_shares(dt, rows_most):
+    """More than 512 row tiles, some of them long enough that all are dealt out in shares."""
+    H, KH, D, page = 16, 1, 64, 16
+    lengths = [(53 * i) % 90 + 1 + (1900 if i % 61 == 7 else 0) for i in range(530)]
+    rows = [min(L, 1 + (7 * i) % rows_most) for i, L in enumerate(lengths)]
+    g = torch.Generator().manual_seed(34)
+    pools, table, descales = make_cache(g, lengths, KH, D, page, FP8 if dt == "e4m3" else torch.bfloat16, "joint")
+    cu = torch.tensor([0] + rows).cumsum(0).int()
+    q = torch.randn(int(cu[-1]), H, D, generator=g).to(torch.bfloat16)
+    _, k, v = views(pools, D)
+    for window, sinks in ((0, 0), (1700, 3)):
+        got = ops().paged_window_attention(
+            q.to(DEV), k, v, cu.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV), max(rows),
+            max(lengths), D ** -0.5, window=window, sinks=sinks, descales=None if descales is None else descales.to(DEV))
+        assert error_word() == 0
+        want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu, lengths, table, D ** -0.5, window, sinks, descales)
+        close(got, want, mag, "window", dt == "e4m3")
