@@ -122,8 +122,12 @@ constexpr int WA_SHARE = WA_ITEM + 4;  // the least length of a CTA's share
 //         40        51 56  75 81    86 85   102 99  137 124  303 243
 //         80        80 93 120 138  137 151  166 169  225 220       -
 // Lengths spread over a factor of 8, and 17 rows each, part ways near there, too; 24
-// prompts of 500 .. 1400 take 289 us one by one, 364 us in shares.
+// prompts of 500 .. 1400 take 289 us one by one, 364 us in shares.  An item taken by
+// itself is looked up among all requests, so above WA_MANY of them it is shares again
+// (17 rows on 100 .. 900 positions: 300 requests 214 and 286 us, 600 438 and 527, 1200
+// 1330 and 891).
 constexpr int WA_LONG = 14;
+constexpr int WA_MANY = 800;
 struct WaBorder {
   int r, y, c, t;  // request, row tile, kv head, and the first tile after the border
 };
@@ -1167,7 +1171,7 @@ WindowPlan window_plan(int64_t R, int64_t T, int64_t H, int64_t KH, int64_t HD, 
   const int64_t per = WA_ROWS / (H / KH) + 2, tokens = max_q < per ? max_q : per;  // that a row tile touches
   if (window > 0 && window + tokens + sinks < span) span = window + tokens + sinks;
   const int64_t tiles = span / WA_KEYS + 3;
-  p.cuts = tiles >= (items >= sms ? WA_LONG : 2 * WA_CUT);
+  p.cuts = tiles >= (items >= sms && R <= WA_MANY ? WA_LONG : 2 * WA_CUT);
   // an item that can be cut gives work to as many CTAs as it has tiles at most
   const int64_t most = p.cuts ? items * tiles : items;
   p.ctas = (int)(most < sms ? most : sms);

@@ -949,3 +949,22 @@ def test_window_of_many_row_tiles_in_shares(dt, rows_most):
         assert error_word() == 0
         want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu, lengths, table, D ** -0.5, window, sinks, descales)
         close(got, want, mag, "window", dt == "e4m3")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "e4m3"])
+def test_window_of_many_requests(dt):
+    """So many requests that their short items are dealt out in shares; some have no rows, some no positions."""
+    H, KH, D, page = 4, 2, 64, 16
+    lengths = [(53 * i) % 90 + (400 if i % 61 == 7 else 0) for i in range(1100)]
+    rows = [min(L + i % 2, (7 * i) % 6) for i, L in enumerate(lengths)]
+    g = torch.Generator().manual_seed(35)
+    pools, table, descales = make_cache(g, lengths, KH, D, page, FP8 if dt == "e4m3" else torch.bfloat16, "joint")
+    cu = torch.tensor([0] + rows).cumsum(0).int()
+    q = torch.randn(int(cu[-1]), H, D, generator=g).to(torch.bfloat16)
+    _, k, v = views(pools, D)
+    got = ops().paged_window_attention(
+        q.to(DEV), k, v, cu.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV), table.to(DEV), max(rows),
+        max(lengths), D ** -0.5, descales=None if descales is None else descales.to(DEV))
+    assert error_word() == 0
+    want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu, lengths, table, D ** -0.5, descales=descales)
+    close(got, want, mag, "window", dt == "e4m3")
