@@ -22,12 +22,14 @@ Query head h reads kv head ``h // (heads / kv_heads)``.  Scores, softmax sums
 and outputs are held in fp32; the softmax numerators are rounded to bf16 (to
 f16 for an e4m3 cache) for the product with the values, and the output to bf16.
 A row that sees no position is zero.  A position that no row of a request may
-see is never read.  Each call checks its arguments (``OpArgumentError``), runs
-on the current stream without a host synchronisation, and can be captured in a
-CUDA graph.  The two attentions are registered operators
-(``flashmap_b200::paged_decode_attention``, ``::paged_window_attention``) to
-``torch.compile``; they have no gradient, and asking for one raises.  There is
-no fallback.
+see is never read.  Each call checks its arguments (``OpArgumentError``; the
+alignment of addresses and strides and the limits of sizes are the library's to
+check, ``FlashMapError``), records lengths, bounds and page ids out of range
+for ``check_device_errors``, runs on the current stream without a host
+synchronisation, and can be captured in a CUDA graph.  The two attentions are
+registered operators (``flashmap_b200::paged_decode_attention``,
+``::paged_window_attention``) to ``torch.compile``; they have no gradient, and
+asking for one raises.  There is no fallback.
 """
 
 from __future__ import annotations
@@ -41,7 +43,8 @@ import torch
 from . import _lib
 from .serving_ops import OpArgumentError, _err, _need
 
-__all__ = ["OpArgumentError", "paged_decode_attention", "paged_window_attention", "evict_paged_context"]
+__all__ = ["OpArgumentError", "paged_decode_attention", "paged_window_attention", "evict_paged_context",
+           "check_device_errors"]
 
 _FP8 = torch.float8_e4m3fn
 
@@ -170,6 +173,18 @@ def _err_word(device) -> int:
     if err is None:
         err = _ERR_WORDS[device.index] = _err(device).data_ptr()
     return err
+
+
+def check_device_errors(device=None) -> None:
+    """Raises ``FlashMapError`` for what kernels of this process have recorded
+    on `device` (the current one by default) since the last check, an index out
+    of range or a wait that ran out, and clears it.  Waits for the device's
+    current stream; the calls themselves wait for nothing and go on past both."""
+    word = _err(torch.device("cuda") if device is None else device)
+    code = int(word.item())
+    if code:
+        word.zero_()
+        raise _lib.FlashMapError(f"a FlashMap kernel reported device error {code} (index or wait)")
 
 
 @functools.lru_cache(maxsize=1024)

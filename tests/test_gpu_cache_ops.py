@@ -968,3 +968,18 @@ def test_window_of_many_requests(dt):
     assert error_word() == 0
     want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu, lengths, table, D ** -0.5, descales=descales)
     close(got, want, mag, "window", dt == "e4m3")
+
+
+def test_recorded_errors_are_raised_once():
+    from flashmap_b200._lib import FlashMapError
+    _, k, (decode, _) = attention_calls()
+    c = ops()
+    q = torch.zeros(2, 8, 128, dtype=torch.bfloat16, device=DEV)
+    c.check_device_errors()
+    decode(q)
+    c.check_device_errors()
+    bad = torch.full((1, 1), 10_000, dtype=torch.int32, device=DEV)
+    c.paged_decode_attention(q[:1], k, k, torch.tensor([5], dtype=torch.int32, device=DEV), bad, 5, 1.0)
+    with pytest.raises(FlashMapError, match="device error 4"):
+        c.check_device_errors(torch.device("cuda", torch.cuda.current_device()))
+    c.check_device_errors()
