@@ -455,7 +455,8 @@ FM_API fm_status fm_paged_decode_attn(const fm_paged_cache* cache, const fm_deco
 /* Causal attention of query rows cu_seqlens_q[r] .. cu_seqlens_q[r + 1] of q
  * (rows, heads, head_dim) bf16, which are request r's last positions: row i of
  * n stands at p = lengths[r] - n + i and sees the positions j <= p with no
- * window, p - j < window or j < sinks.  A row that sees nothing is zero. */
+ * window, p - j < window or j < sinks.  A row that sees nothing is zero.  At
+ * most 16384 requests. */
 typedef struct fm_window_attn {
   const void* q;
   int64_t q_token_stride, q_head_stride;
