@@ -983,3 +983,27 @@ def test_recorded_errors_are_raised_once():
     with pytest.raises(FlashMapError, match="device error 4"):
         c.check_device_errors(torch.device("cuda", torch.cuda.current_device()))
     c.check_device_errors()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("H,KH", [(300, 1), (514, 2)])
+def test_head_groups_wider_than_a_row_tile(H, KH, dt):
+    D, page, lengths, rows = 64, 16, [150, 1, 0, 700], [5, 1, 2, 3]
+    g = torch.Generator().manual_seed(36)
+    pools, table, descales = make_cache(g, lengths, KH, D, page, FP8 if dt == "e4m3" else torch.bfloat16, "joint")
+    cu = torch.tensor([0] + rows).cumsum(0).int()
+    q = torch.randn(int(cu[-1]), H, D, generator=g).to(torch.bfloat16)
+    _, k, v = views(pools, D)
+    L, dd = torch.tensor(lengths, dtype=torch.int32, device=DEV), None if descales is None else descales.to(DEV)
+    got = ops().paged_window_attention(q.to(DEV), k, v, cu.to(DEV), L, table.to(DEV), max(rows), max(lengths), D ** -0.5,
+                                       window=200, sinks=3, descales=dd)
+    want, mag, _ = O.window_attention(q, *cpu_views(pools, D), cu, lengths, table, D ** -0.5, 200, 3, descales)
+    close(got, want, mag, "window", dt == "e4m3")
+    sums = torch.zeros(4, KH, 700, device=DEV)
+    got = ops().paged_decode_attention(q[:4].to(DEV), k, v, L, table.to(DEV), max(lengths), D ** -0.5, descales=dd,
+                                       weight_sums=sums)
+    want, mag, w = O.decode_attention(q[:4], *cpu_views(pools, D), lengths, table, D ** -0.5, descales=descales)
+    close(got, want, mag, "decode", dt == "e4m3")
+    for r, n in enumerate(lengths):
+        assert ((sums[r, :, :n].double().cpu() - w[r]).abs() <= (2.0 ** -16 + 2.0 ** -20) * w[r]).all()
+    assert error_word() == 0
