@@ -72,7 +72,8 @@ class ExtendIO(ctypes.Structure):
                 ("batch", c_int32)]
 
 
-FM_DT_BF16, FM_DT_F32, FM_DT_E4M3, FM_DT_I32, FM_DT_I64 = 0, 1, 2, 3, 4
+FM_DT_BF16, FM_DT_F32, FM_DT_E4M3, FM_DT_I32, FM_DT_I64, FM_DT_E2M1 = 0, 1, 2, 3, 4, 5
+FM_TOKEN_LOGPROBS_MAX_TOP = 32
 FM_NORM_DIT, FM_NORM_FUSED = 0, 1
 
 
@@ -138,6 +139,22 @@ class Evict(ctypes.Structure):
                 ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("err", c_void_p)]
 
 
+class BlockScales(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p),
+                ("k_page_stride", c_int64), ("k_head_stride", c_int64), ("k_token_stride", c_int64),
+                ("v_page_stride", c_int64), ("v_head_stride", c_int64), ("v_token_stride", c_int64)]
+
+
+class Append(ctypes.Structure):
+    _fields_ = [("key", c_void_p), ("value", c_void_p), ("k_token_stride", c_int64), ("k_head_stride", c_int64),
+                ("v_token_stride", c_int64), ("v_head_stride", c_int64),
+                ("query", c_void_p), ("q_token_stride", c_int64), ("q_head_stride", c_int64), ("heads", c_int64),
+                ("out", c_void_p), ("out_token_stride", c_int64), ("out_head_stride", c_int64), ("tokens", c_int64),
+                ("cu_seqlens_q", c_void_p), ("positions", c_void_p), ("positions_dtype", c_int32),
+                ("rope", c_void_p), ("rope_rows", c_int64), ("rotary_dim", c_int64), ("interleaved", c_int32),
+                ("err", c_void_p)]
+
+
 _SIGNATURES = {
     "fm_last_error": (ctypes.c_char_p, []),
     "fm_version": (c_int, []),
@@ -178,6 +195,10 @@ _SIGNATURES = {
     "fm_paged_window_attn": (c_int, [c_void_p, c_void_p, c_void_p]),  # PagedCache, WindowAttn
     "fm_paged_evict_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
     "fm_paged_evict": (c_int, [c_void_p, c_void_p, c_void_p]),  # PagedCache, Evict
+    "fm_paged_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),  # PagedCache, BlockScales or NULL, Append
+    "fm_token_logprobs_workspace_size": (c_size_t, [c_int64, c_int64, c_int32, c_int64]),
+    "fm_token_logprobs": (c_int, [c_void_p, c_int32, c_int64, c_void_p, c_int64, c_int64, c_float, c_int64, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "fm_tree_build": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
     "fm_tree_commit": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

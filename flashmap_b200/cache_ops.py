@@ -44,7 +44,7 @@ from . import _lib
 from .serving_ops import OpArgumentError, _err, _need
 
 __all__ = ["OpArgumentError", "paged_decode_attention", "paged_window_attention", "evict_paged_context",
-           "check_device_errors"]
+           "append_paged_context", "check_device_errors"]
 
 _FP8 = torch.float8_e4m3fn
 
@@ -55,11 +55,25 @@ _CACHE = struct.Struct("@PPiqqqqqqqqPqqPqqqqP")
 _DECODE = struct.Struct("@PqqqfqqPqqPqqPNP")
 _WINDOW = struct.Struct("@PqqqqPqfqqPqqPNP")
 _EVICT = struct.Struct("@PqqqqqPqqPPPPNP")
+_SCALES = struct.Struct("@PPqqqqqq")
+_APPEND = struct.Struct("@PPqqqqPqqqPqqqPPiPqqiP")
 
 
 class _Cache(NamedTuple):
     """A checked cache: its packed fm_paged_cache and the sizes that calls go by."""
     packed: bytes
+    device: torch.device
+    requests: int
+    kv_heads: int
+    page_size: int
+    head_dim: int
+    max_length: int
+
+
+class _Cache4(NamedTuple):
+    """A checked 4-bit cache: ``_Cache`` and its factors' packed fm_block_scales."""
+    packed: bytes
+    scales: bytes
     device: torch.device
     requests: int
     kv_heads: int
@@ -124,6 +138,66 @@ def _cache(k_cache, v_cache, lengths, block_table, descales, max_len: int) -> _C
                               ts[0], table[1], lengths.data_ptr(), max_len, table[0], shape[1], shape[3],
                               0 if descales is None else descales.data_ptr()),
                   dev, table[0], shape[1], shape[2], shape[3], max_len)
+
+
+def _refuse_cache4(k_cache, v_cache, k_scales, v_scales, lengths, block_table, descales, max_len: int) -> None:
+    """Raises for the argument that ``_cache4`` could not take."""
+    _need(k_cache.is_cuda, "k_cache must be a CUDA tensor")
+    dev = k_cache.device
+    _need(dev.index == torch.cuda.current_device(), f"the cache is on {dev}, which is not the current device")
+    _need(k_scales is not None and v_scales is not None, "a 4-bit cache needs k_scales and v_scales")
+    for t, name in ((v_cache, "v_cache"), (k_scales, "k_scales"), (v_scales, "v_scales"), (lengths, "the lengths"),
+                    (block_table, "block_table")):
+        _on(t, name, dev)
+    _need(k_cache.dtype == torch.uint8 and v_cache.dtype == torch.uint8, f"a 4-bit cache is uint8, got {k_cache.dtype}")
+    _need(k_cache.dim() == 4 and v_cache.shape == k_cache.shape,
+          "k_cache and v_cache must both be (pages, kv_heads, page_size, head_dim / 2)")
+    _need(k_cache.shape[3] in (32, 64), f"head_dim must be 64 or 128, got {2 * k_cache.shape[3]}")
+    _need(k_cache.shape[1] > 0 and k_cache.shape[2] > 0, "the cache needs a kv head and a token to a page")
+    _need(k_scales.dtype == _FP8 and v_scales.dtype == _FP8, f"k_scales and v_scales must be e4m3, got {k_scales.dtype}")
+    rows = (*k_cache.shape[:3], k_cache.shape[3] // 8)
+    _need(k_scales.shape == rows and v_scales.shape == rows,
+          "k_scales and v_scales must both be (pages, kv_heads, page_size, head_dim / 16)")
+    _need(k_cache.stride(3) == 1 and v_cache.stride(3) == 1 and k_scales.stride(3) == 1 and v_scales.stride(3) == 1,
+          "cache rows must be contiguous")
+    _need(lengths.dtype == torch.int32 and lengths.dim() == 1 and lengths.is_contiguous(),
+          "the lengths must be contiguous int32 (requests,)")
+    _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == lengths.shape[0],
+          "block_table must be int32 (requests, pages)")
+    _need(block_table.shape[1] <= 1 or block_table.stride(1) == 1, "block_table rows must be contiguous")
+    _need(max_len >= 0, "the largest length must not be negative")
+    if descales is not None:
+        _on(descales, "descales", dev)
+        _need(descales.dtype == torch.float32 and descales.is_contiguous()
+              and descales.shape == (2, lengths.shape[0], k_cache.shape[1]),
+              "descales must be contiguous float32 (2, requests, kv_heads)")
+
+
+def _cache4(k_cache, v_cache, k_scales, v_scales, lengths, block_table, descales, max_len: int) -> _Cache4:
+    dev, u8 = k_cache.device, torch.uint8
+    if k_scales is None or v_scales is None:
+        _refuse_cache4(k_cache, v_cache, k_scales, v_scales, lengths, block_table, descales, max_len)
+    shape, ks, vs, ts, table = k_cache.shape, k_cache.stride(), v_cache.stride(), block_table.stride(), block_table.shape
+    fk, fv = k_scales.stride(), v_scales.stride()
+    if not (dev.type == "cuda" and dev.index == torch._C._cuda_getDevice() and v_cache.device == dev
+            and k_scales.device == dev and v_scales.device == dev and lengths.device == dev and block_table.device == dev
+            and k_cache.dtype == u8 and v_cache.dtype == u8 and k_scales.dtype == _FP8 and v_scales.dtype == _FP8
+            and len(shape) == 4 and v_cache.shape == shape and shape[3] in (32, 64) and shape[1] > 0 and shape[2] > 0
+            and k_scales.shape == (shape[0], shape[1], shape[2], shape[3] // 8) and v_scales.shape == k_scales.shape
+            and ks[3] == 1 and vs[3] == 1 and fk[3] == 1 and fv[3] == 1
+            and lengths.dtype == torch.int32 and block_table.dtype == torch.int32
+            and lengths.dim() == 1 and lengths.is_contiguous() and len(table) == 2 and table[0] == lengths.shape[0]
+            and (table[1] <= 1 or ts[1] == 1) and max_len >= 0
+            and (descales is None or descales.device == dev and descales.dtype == torch.float32
+                 and descales.is_contiguous() and descales.shape == (2, table[0], shape[1]))):
+        _refuse_cache4(k_cache, v_cache, k_scales, v_scales, lengths, block_table, descales, max_len)
+        raise OpArgumentError("the cache's tensors do not go together")
+    return _Cache4(_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), _lib.FM_DT_E2M1, ks[0], ks[1], ks[2],
+                               vs[0], vs[1], vs[2], shape[2], shape[0], block_table.data_ptr(), ts[0], table[1],
+                               lengths.data_ptr(), max_len, table[0], shape[1], 2 * shape[3],
+                               0 if descales is None else descales.data_ptr()),
+                   _SCALES.pack(k_scales.data_ptr(), v_scales.data_ptr(), fk[0], fk[1], fk[2], fv[0], fv[1], fv[2]),
+                   dev, table[0], shape[1], shape[2], 2 * shape[3], max_len)
 
 
 def _query(query, cache: _Cache, device) -> torch.Tensor:
@@ -375,3 +449,102 @@ def evict_paged_context(k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k:
                             to, to_stride, to_cols, kept.data_ptr(), lengths.data_ptr(), sums.data_ptr(), ws.data_ptr(),
                             need, _err_word(dev)))
     return kept, lengths, sums
+
+
+def _rows(x, name: str, heads: int, cache, tokens: int):
+    """``x (tokens, heads, head_dim)`` bf16 with rows that the kernels can read 16 bytes at a time."""
+    shape, stride = x.shape, x.stride()
+    if not (x.device == cache.device and x.dtype == torch.bfloat16 and shape == (tokens, heads, cache.head_dim)):
+        _on(x, name, cache.device)
+        raise OpArgumentError(f"{name} must be bf16 ({tokens}, {heads}, {cache.head_dim}), got {x.dtype} {tuple(shape)}")
+    if stride[2] != 1 or stride[0] % 8 or stride[1] % 8 or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:  # a contiguous view that starts between two 16-byte lines
+            x = x.clone()
+    return x
+
+
+def append_paged_context(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         seqused_k: torch.Tensor, block_table: torch.Tensor, *,
+                         cu_seqlens_q: Optional[torch.Tensor] = None, query: Optional[torch.Tensor] = None,
+                         rope: Optional[torch.Tensor] = None, interleaved: bool = False,
+                         positions: Optional[torch.Tensor] = None, k_scales: Optional[torch.Tensor] = None,
+                         v_scales: Optional[torch.Tensor] = None,
+                         descales: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Writes new tokens' ``key`` and ``value (tokens, kv_heads, head_dim)`` bf16 into the cache, in place: rows
+    ``cu_seqlens_q[r] .. cu_seqlens_q[r + 1]`` become the last positions of request r's ``seqused_k[r]``, which
+    counts them already; without ``cu_seqlens_q`` every request has one new token.
+
+    ``rope (positions, rotary_dim / 2, 2)`` fp32, the cosines and sines of ``serving_ops.rope_table``, rotates keys
+    and ``query (tokens, heads, head_dim)`` bf16 on the way: the pairs (i, i + rotary_dim / 2) of the first
+    ``rotary_dim`` values (a multiple of 16), or (2 i, 2 i + 1) when ``interleaved``.  A token stands at
+    ``positions (tokens,)`` int32 or int64, or where those are not given at its place in the cache (a context that was
+    cut holds fewer positions than its text).  Returns the rotated queries ``(tokens, heads, head_dim)``, or None.
+
+    A bf16 cache takes the rotated values rounded; an e4m3 cache rounded and cut to +-448; a 4-bit cache (uint8, with
+    ``k_scales`` and ``v_scales``) as e2m1 codes with one e4m3 factor for 16 values, their largest magnitude / 6.  The
+    last two divide by ``descales`` first.
+
+    A row without a place (a request of length 0, more rows than positions) writes nothing and its query comes back
+    zero; so does, recorded for ``check_device_errors``, one whose request is longer than its table or whose position
+    lies outside ``rope``.  A bad page id is recorded and not written to.  Rows that ``cu_seqlens_q`` gives to no request
+    are not touched.  No two requests may append to the same page's slot."""
+    most = block_table.shape[1] * k_cache.shape[2] if block_table.dim() == 2 and k_cache.dim() == 4 else 0
+    most = min(most, 0x7ffffff0)
+    scales = None
+    if k_cache.dtype == torch.uint8:
+        cache = _cache4(k_cache, v_cache, k_scales, v_scales, seqused_k, block_table, descales, most)
+        scales = cache.scales
+    else:
+        _need(k_scales is None and v_scales is None, "k_scales and v_scales go with a 4-bit cache")
+        cache = _cache(k_cache, v_cache, seqused_k, block_table, descales, most)
+    dev = cache.device
+    for t in (key, value, query):
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise OpArgumentError("append_paged_context has no gradient: detach the rows")
+    tokens = key.shape[0] if key.dim() == 3 else -1
+    key = _rows(key, "key", cache.kv_heads, cache, tokens)
+    value = _rows(value, "value", cache.kv_heads, cache, tokens)
+    cu = 0
+    if cu_seqlens_q is not None:
+        _on(cu_seqlens_q, "cu_seqlens_q", dev)
+        _need(cu_seqlens_q.dtype is torch.int32 and cu_seqlens_q.shape == (cache.requests + 1,)
+              and cu_seqlens_q.is_contiguous(), "cu_seqlens_q must be contiguous int32 (requests + 1,)")
+        cu = cu_seqlens_q.data_ptr()
+    else:
+        _need(tokens == cache.requests, "one new token per request without cu_seqlens_q")
+    table, rows, rotary = 0, 0, 0
+    if rope is not None:
+        _on(rope, "rope", dev)
+        _need(rope.dtype is torch.float32 and rope.dim() == 3 and rope.shape[2] == 2 and rope.is_contiguous(),
+              "rope must be contiguous float32 (positions, rotary_dim / 2, 2)")
+        rows, rotary = rope.shape[0], 2 * rope.shape[1]
+        _need(rotary >= 16 and rotary % 16 == 0 and rotary <= cache.head_dim,
+              f"rotary_dim must be a multiple of 16 up to head_dim, got {rotary}")
+        table = rope.data_ptr()
+    at, at_dtype = 0, _lib.FM_DT_I32
+    if positions is not None:
+        _need(rope is not None, "positions go with a rope table")
+        _on(positions, "positions", dev)
+        _need(positions.dtype in (torch.int32, torch.int64) and positions.shape == (tokens,)
+              and positions.is_contiguous(), "positions must be contiguous int32 or int64 (tokens,)")
+        at, at_dtype = positions.data_ptr(), _lib.FM_DT_I32 if positions.dtype == torch.int32 else _lib.FM_DT_I64
+    out, q, q0, q1, heads, to, o0, o1 = None, 0, 0, 0, 0, 0, 0, 0
+    if query is not None:
+        _need(rope is not None, "queries are taken to be rotated: they go with a rope table")
+        heads = query.shape[1] if query.dim() == 3 else 0
+        _need(heads > 0 and heads % cache.kv_heads == 0, f"{heads} query heads are no multiple of {cache.kv_heads} kv heads")
+        query = _rows(query, "query", heads, cache, tokens)
+        out = query.new_empty(query.shape)
+        q, q0, q1, to = query.data_ptr(), query.stride(0), query.stride(1), out.data_ptr()
+        o0, o1 = heads * cache.head_dim, cache.head_dim
+    if cache.requests and tokens:
+        status = _lib.load().fm_paged_append(
+            cache.packed, scales,
+            _APPEND.pack(key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), value.stride(0), value.stride(1),
+                         q, q0, q1, heads, to, o0, o1, tokens, cu, at, at_dtype, table, rows, rotary, interleaved,
+                         _err_word(dev)),
+            torch._C._cuda_getCurrentRawStream(dev.index))
+        if status:
+            _lib.check(status, "fm_paged_append")
+    return out

@@ -1,0 +1,272 @@
+// New tokens' keys and values into a paged cache, rotated on the way, and
+// their queries rotated.
+//
+// With (c, s) the cosine and sine of a pair at the token's position:
+//   (a, b) -> (a c - b s, b c + a s)
+// in fp32, each product and sum rounded, then one rounding to the cache's type.
+// A 4-bit row's 16 values share the factor f = e4m3(max |x| / 6) and become the
+// e2m1 codes of x / f, both to nearest even.
+//
+// Every value is read and written once; the bytes bound it, and a few tokens
+// the latency of table, position and row.
+#include "paged_cache.cuh"
+
+namespace fm {
+namespace {
+
+enum { AP_BF16 = 0, AP_E4M3 = 1, AP_FP4 = 2 };
+enum { AP_PLAIN = 0, AP_HALVES = 1, AP_PAIRS = 2 };
+
+struct AppendArgs {
+  CacheRef c;
+  ScaleRef f;
+  const __nv_bfloat16 *k, *v, *q;
+  long long k_ts, k_hs, v_ts, v_hs, q_ts, q_hs;
+  __nv_bfloat16* out;
+  long long o_ts, o_hs;
+  int T, H;  // H: query heads, 0 without queries
+  const int* cu;
+  const void* pos;
+  bool pos64;
+  const float2* rope;
+  long long rope_rows;
+  int rot;
+  int* err;
+};
+
+// NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+  uint16_t y;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+// eight values as e2m1 codes, the first in the lowest four bits
+__device__ __forceinline__ uint32_t to_e2m1x8(const float* x) {
+  uint32_t y;
+  asm("{.reg .b8 a, b, c, d; cvt.rn.satfinite.e2m1x2.f32 a, %2, %1; cvt.rn.satfinite.e2m1x2.f32 b, %4, %3; "
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5; cvt.rn.satfinite.e2m1x2.f32 d, %8, %7; mov.b32 %0, {a, b, c, d};}"
+      : "=r"(y)
+      : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
+  return y;
+}
+__device__ __forceinline__ void unpack8(const uint4& u, float* x) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+// Request of token t, or -1; by one warp.
+__device__ __forceinline__ int append_request(const AppendArgs& a, int t) {
+  if (a.cu == nullptr) return t;
+  const int lane = threadIdx.x & 31;
+  for (int r0 = 0; r0 < a.c.R; r0 += 32) {
+    const unsigned hit = __ballot_sync(0xffffffffu, r0 + lane < a.c.R && a.cu[r0 + lane + 1] > t);
+    if (hit) return r0 + __ffs(hit) - 1;
+  }
+  return -1;
+}
+
+// Eight values to a thread; block (t, y) has rows y * 256 / LPR .. of token t:
+// its query heads, then keys, then values.
+template <int HD, int KIND, int ROPE>
+__global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
+  constexpr int LPR = HD / 8;
+  pdl_wait();
+  const int t = blockIdx.x, at = threadIdx.x % LPR, d0 = at * 8;
+  const int row = blockIdx.y * (256 / LPR) + threadIdx.x / LPR;
+  if (a.cu != nullptr && t == 0 && blockIdx.y == 0)  // one block looks at all bounds: those that run back give rows to nobody
+    for (int i = threadIdx.x; i < a.c.R; i += 256)
+      if (a.cu[i + 1] < a.cu[i]) record_error(a.err, DEV_BAD_INDEX);
+  const int r = append_request(a, t);
+  if (r < 0 || row >= a.H + 2 * a.c.KH) return;
+  int j, n = 1;  // place in the cache
+  bool ok = true;
+  const int len = a.c.lengths[r];
+  j = len - 1;
+  if (a.cu != nullptr) {
+    const int q0 = a.cu[r];
+    n = a.cu[r + 1] - q0;
+    ok = q0 >= 0 && n <= a.T - q0 && t >= q0;
+    j = len - n + (t - q0);
+  }
+  ok = ok && len >= 0 && len <= a.c.max_len;
+  bool bad = !ok;
+  ok = ok && j >= 0;
+  const bool is_q = row < a.H, is_k = !is_q && row < a.H + a.c.KH;
+  const int h = is_q ? row : is_k ? row - a.H : row - a.H - a.c.KH;
+  long long p = j;
+  if (ROPE != AP_PLAIN && ok) {
+    if (a.pos != nullptr) p = a.pos64 ? static_cast<const long long*>(a.pos)[t] : static_cast<const int*>(a.pos)[t];
+    if (p < 0 || p >= a.rope_rows) {
+      bad = true;
+      ok = false;
+    }
+  }
+  if (bad && threadIdx.x == 0 && blockIdx.y == 0) record_error(a.err, DEV_BAD_INDEX);
+  if (!ok) {
+    if (is_q) *reinterpret_cast<uint4*>(a.out + t * a.o_ts + h * a.o_hs + d0) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const __nv_bfloat16* src = is_q   ? a.q + t * a.q_ts + h * a.q_hs
+                             : is_k ? a.k + t * a.k_ts + h * a.k_hs
+                                    : a.v + t * a.v_ts + h * a.v_hs;
+  float x[8];
+  unpack8(*reinterpret_cast<const uint4*>(src + d0), x);
+  if (ROPE != AP_PLAIN && (is_q || is_k) && d0 < a.rot) {
+    const float2* cs = a.rope + p * (a.rot / 2);
+    if constexpr (ROPE == AP_HALVES) {
+      const int half = a.rot / 2;
+      const bool first = d0 < half;
+      float y[8];
+      unpack8(*reinterpret_cast<const uint4*>(src + (first ? d0 + half : d0 - half)), y);
+      const float4* c4 = reinterpret_cast<const float4*>(cs + (first ? d0 : d0 - half));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 w = c4[i];
+        const float u0 = __fmul_rn(y[2 * i], w.y), u1 = __fmul_rn(y[2 * i + 1], w.w);
+        x[2 * i] = __fadd_rn(__fmul_rn(x[2 * i], w.x), first ? -u0 : u0);
+        x[2 * i + 1] = __fadd_rn(__fmul_rn(x[2 * i + 1], w.z), first ? -u1 : u1);
+      }
+    } else {
+      const float4* c4 = reinterpret_cast<const float4*>(cs + d0 / 2);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float4 w = c4[i];
+        float* z = x + 4 * i;
+        const float a0 = z[0], a1 = z[2];
+        z[0] = __fsub_rn(__fmul_rn(a0, w.x), __fmul_rn(z[1], w.y));
+        z[1] = __fadd_rn(__fmul_rn(z[1], w.x), __fmul_rn(a0, w.y));
+        z[2] = __fsub_rn(__fmul_rn(a1, w.z), __fmul_rn(z[3], w.w));
+        z[3] = __fadd_rn(__fmul_rn(z[3], w.z), __fmul_rn(a1, w.w));
+      }
+    }
+  }
+  if (is_q) {
+    *reinterpret_cast<uint4*>(a.out + t * a.o_ts + h * a.o_hs + d0) =
+        make_uint4(pack16(x[0], x[1], false), pack16(x[2], x[3], false), pack16(x[4], x[5], false), pack16(x[6], x[7], false));
+    return;
+  }
+  if (KIND != AP_BF16 && a.c.descales != nullptr) {
+    const float d = a.c.descales[(long long)(is_k ? r : a.c.R + r) * a.c.KH + h];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __fdiv_rn(x[i], d);
+  }
+  uint32_t factor = 0;
+  if constexpr (KIND == AP_FP4) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
+    // the row's lanes go through here together, whichever of the warp's rows return above
+    const unsigned pair = 3u << (threadIdx.x & 30);
+    top = max_nan(top, __shfl_xor_sync(pair, top, 1));
+    factor = to_e4m3x2(__fdiv_rn(top, 6.0f), 0.0f);
+    const __half2 f2 = [&] {
+      const uint32_t b = e4m3x2_h(factor);
+      return *reinterpret_cast<const __half2*>(&b);
+    }();
+    const float f = __low2float(f2);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = f == 0.0f ? copysignf(0.0f, x[i]) : __fdiv_rn(x[i], f);
+  }
+  const int pg = a.c.by_page.div(j), tok = j - pg * a.c.page;
+  const int page = a.c.table[(long long)r * a.c.tstride + pg];
+  if (page < 0 || page >= a.c.num_pages) {
+    record_error(a.err, DEV_BAD_INDEX);
+    return;
+  }
+  uint8_t* dst = is_k ? a.c.k + page * a.c.kps + h * a.c.khs + tok * a.c.kts
+                      : a.c.v + page * a.c.vps + h * a.c.vhs + tok * a.c.vts;
+  if constexpr (KIND == AP_BF16) {
+    *reinterpret_cast<uint4*>(dst + d0 * 2) =
+        make_uint4(pack16(x[0], x[1], false), pack16(x[2], x[3], false), pack16(x[4], x[5], false), pack16(x[6], x[7], false));
+  } else if constexpr (KIND == AP_E4M3) {
+    *reinterpret_cast<uint2*>(dst + d0) = make_uint2(to_e4m3x2(x[0], x[1]) | to_e4m3x2(x[2], x[3]) << 16,
+                                                     to_e4m3x2(x[4], x[5]) | to_e4m3x2(x[6], x[7]) << 16);
+  } else {
+    *reinterpret_cast<uint32_t*>(dst + d0 / 2) = to_e2m1x8(x);
+    uint8_t* fd = is_k ? a.f.k + page * a.f.kps + h * a.f.khs + tok * a.f.kts
+                       : a.f.v + page * a.f.vps + h * a.f.vhs + tok * a.f.vts;
+    if ((at & 1) == 0) fd[at >> 1] = (uint8_t)factor;
+  }
+}
+
+template <int HD, int KIND>
+fm_status launch_append(const AppendArgs& a, int rope, cudaStream_t s) {
+  constexpr int RPB = 256 / (HD / 8);
+  const dim3 grid((unsigned)a.T, (unsigned)((a.H + 2 * a.c.KH + RPB - 1) / RPB));
+  auto go = [&](auto kernel) { return launch_kernel(kernel, grid, dim3(256), 0, s, true, a); };
+  return rope == AP_PLAIN    ? go(append_kernel<HD, KIND, AP_PLAIN>)
+         : rope == AP_HALVES ? go(append_kernel<HD, KIND, AP_HALVES>)
+                             : go(append_kernel<HD, KIND, AP_PAIRS>);
+}
+
+}  // namespace
+}  // namespace fm
+
+using namespace fm;
+
+extern "C" fm_status fm_paged_append(const fm_paged_cache* cache, const fm_block_scales* scales, const fm_append* p,
+                                     fm_stream stream) {
+  AppendArgs a{};
+  const bool fp4 = cache && cache->dtype == FM_DT_E2M1;
+  fm_status st = cache_ref(cache, "paged_append", &a.c, fp4);
+  if (st != FM_OK) return st;
+  if (fp4 && (st = scale_ref(cache, scales, "paged_append", &a.f)) != FM_OK) return st;
+  if (!p) return set_error(FM_ERR_INVALID, "paged_append: null arguments");
+  if (p->tokens < 0 || p->tokens > 0x7fffffff || (p->query && (p->heads < 1 || p->heads > 65535)))
+    return set_error(FM_ERR_SHAPE, "paged_append: bad shape");
+  if (!p->cu_seqlens_q && p->tokens != cache->requests)
+    return set_error(FM_ERR_SHAPE, "paged_append: without row bounds there is one token to a request");
+  if (p->rope && (p->rotary_dim < 16 || p->rotary_dim % 16 || p->rotary_dim > cache->head_dim || p->rope_rows < 0))
+    return set_error(FM_ERR_SHAPE, "paged_append: rotary_dim must be a multiple of 16 up to head_dim");
+  if (p->query && !p->rope) return set_error(FM_ERR_INVALID, "paged_append: queries are taken to be rotated");
+  if (p->positions && p->positions_dtype != FM_DT_I32 && p->positions_dtype != FM_DT_I64)
+    return set_error(FM_ERR_INVALID, "paged_append: positions are int32 or int64");
+  if (cache->dtype == FM_DT_BF16 && cache->descales)
+    return set_error(FM_ERR_INVALID, "paged_append: descales go with an e4m3 or 4-bit cache");
+  if (cache->requests == 0 || p->tokens == 0) return FM_OK;
+  if (!p->key || !p->value || (p->query && !p->out)) return set_error(FM_ERR_INVALID, "paged_append: null pointer");
+  // one token or one head is not stepped through: its stride may be anything
+  const bool one = p->tokens == 1, lone = cache->kv_heads == 1;
+  a.k_ts = one ? 0 : p->k_token_stride;
+  a.v_ts = one ? 0 : p->v_token_stride;
+  a.k_hs = lone ? 0 : p->k_head_stride;
+  a.v_hs = lone ? 0 : p->v_head_stride;
+  if (p->query) {
+    a.q_ts = one ? 0 : p->q_token_stride;
+    a.o_ts = one ? 0 : p->out_token_stride;
+    a.q_hs = p->heads == 1 ? 0 : p->q_head_stride;
+    a.o_hs = p->heads == 1 ? 0 : p->out_head_stride;
+  }
+  if ((uintptr_t)p->key % 16 || (uintptr_t)p->value % 16 || a.k_ts % 8 || a.k_hs % 8 || a.v_ts % 8 || a.v_hs % 8 ||
+      (p->query && ((uintptr_t)p->query % 16 || (uintptr_t)p->out % 16 || a.q_ts % 8 || a.q_hs % 8 || a.o_ts % 8 || a.o_hs % 8)) ||
+      (uintptr_t)p->rope % 16)
+    return set_error(FM_ERR_ALIGN, "paged_append: rows must be 16-byte aligned");
+  a.k = static_cast<const __nv_bfloat16*>(p->key);
+  a.v = static_cast<const __nv_bfloat16*>(p->value);
+  a.q = static_cast<const __nv_bfloat16*>(p->query);
+  a.out = static_cast<__nv_bfloat16*>(p->out);
+  a.T = (int)p->tokens;
+  a.H = p->query ? (int)p->heads : 0;
+  a.cu = p->cu_seqlens_q;
+  a.pos = p->positions;
+  a.pos64 = p->positions_dtype == FM_DT_I64;
+  a.rope = reinterpret_cast<const float2*>(p->rope);
+  a.rope_rows = p->rope_rows;
+  a.rot = (int)p->rotary_dim;
+  a.err = p->err;
+  const int rope = !p->rope ? AP_PLAIN : p->interleaved ? AP_PAIRS : AP_HALVES;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool wide = cache->head_dim == 128;
+  if (cache->dtype == FM_DT_BF16) return wide ? launch_append<128, AP_BF16>(a, rope, s) : launch_append<64, AP_BF16>(a, rope, s);
+  if (cache->dtype == FM_DT_E4M3) return wide ? launch_append<128, AP_E4M3>(a, rope, s) : launch_append<64, AP_E4M3>(a, rope, s);
+  return wide ? launch_append<128, AP_FP4>(a, rope, s) : launch_append<64, AP_FP4>(a, rope, s);
+}

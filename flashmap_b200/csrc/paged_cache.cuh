@@ -50,8 +50,16 @@ __device__ __forceinline__ int cache_length(const CacheRef& c, int r, int* err, 
   return len < 0 ? 0 : c.max_len;
 }
 
-// fm_paged_cache -> CacheRef; FM_OK or the error of the first bad field.
-inline fm_status cache_ref(const fm_paged_cache* p, const char* who, CacheRef* c) {
+// Factors of a 4-bit cache; strides in bytes.
+struct ScaleRef {
+  uint8_t* k;
+  uint8_t* v;
+  long long kps, khs, kts, vps, vhs, vts;
+};
+
+// fm_paged_cache -> CacheRef; FM_OK or the error of the first bad field.  A
+// 4-bit cache is one where `fp4` says that the caller takes its factors.
+inline fm_status cache_ref(const fm_paged_cache* p, const char* who, CacheRef* c, bool fp4 = false) {
   if (!p) return set_error(FM_ERR_INVALID, "%s: null cache", who);
   if (p->requests < 0 || p->kv_heads < 1 || p->page_size < 1 || p->num_pages < 0 || p->page_table_cols < 0 ||
       p->max_length < 0)
@@ -60,14 +68,14 @@ inline fm_status cache_ref(const fm_paged_cache* p, const char* who, CacheRef* c
       p->max_length > 0x7ffffff0)
     return set_error(FM_ERR_SHAPE, "%s: cache too large", who);
   if (p->head_dim != 64 && p->head_dim != 128) return set_error(FM_ERR_UNSUPPORTED, "%s: head_dim 64 or 128", who);
-  if (p->dtype != FM_DT_BF16 && p->dtype != FM_DT_E4M3)
-    return set_error(FM_ERR_INVALID, "%s: the cache is bf16 or e4m3", who);
+  if (fp4 ? p->dtype != FM_DT_E2M1 : p->dtype != FM_DT_BF16 && p->dtype != FM_DT_E4M3)
+    return set_error(FM_ERR_INVALID, "%s: the cache is %s", who, fp4 ? "e2m1" : "bf16 or e4m3");
   if (p->requests == 0) return FM_OK;
   // a cache without a page, a table column or a position has no address to give, and none is used
   const bool holds = p->num_pages > 0 && p->page_table_cols > 0 && p->max_length > 0;
   if (!p->lengths || (holds && (!p->k || !p->v || !p->page_table)))
     return set_error(FM_ERR_INVALID, "%s: null pointer", who);
-  const long long esz = p->dtype == FM_DT_E4M3 ? 1 : 2;
+  const long long esz = p->dtype == FM_DT_BF16 ? 2 : 1;
   *c = CacheRef{static_cast<uint8_t*>(p->k), static_cast<uint8_t*>(p->v),
                 p->k_page_stride * esz, p->k_head_stride * esz, p->k_token_stride * esz,
                 p->v_page_stride * esz, p->v_head_stride * esz, p->v_token_stride * esz,
@@ -85,6 +93,24 @@ inline fm_status cache_ref(const fm_paged_cache* p, const char* who, CacheRef* c
   if ((uintptr_t)c->k % 16 || (uintptr_t)c->v % 16 || c->kps % 16 || c->khs % 16 || c->kts % 16 || c->vps % 16 ||
       c->vhs % 16 || c->vts % 16)
     return set_error(FM_ERR_ALIGN, "%s: cache rows must be 16-byte aligned", who);
+  return FM_OK;
+}
+
+// fm_block_scales -> ScaleRef, of a cache that cache_ref has accepted.
+inline fm_status scale_ref(const fm_paged_cache* p, const fm_block_scales* f, const char* who, ScaleRef* s) {
+  if (!f) return set_error(FM_ERR_INVALID, "%s: a 4-bit cache needs its factors", who);
+  if (p->requests == 0) return FM_OK;
+  if (p->num_pages > 0 && p->page_table_cols > 0 && p->max_length > 0 && (!f->k || !f->v))
+    return set_error(FM_ERR_INVALID, "%s: null pointer", who);
+  *s = ScaleRef{static_cast<uint8_t*>(f->k), static_cast<uint8_t*>(f->v),
+                f->k_page_stride, f->k_head_stride, f->k_token_stride, f->v_page_stride, f->v_head_stride, f->v_token_stride};
+  if (p->num_pages == 1) s->kps = s->vps = 0;
+  if (p->kv_heads == 1) s->khs = s->vhs = 0;
+  if (p->page_size == 1) s->kts = s->vts = 0;
+  const long long n = p->head_dim / 16;
+  if ((uintptr_t)s->k % n || (uintptr_t)s->v % n || s->kps % n || s->khs % n || s->kts % n || s->vps % n || s->vhs % n ||
+      s->vts % n)
+    return set_error(FM_ERR_ALIGN, "%s: rows of factors must be aligned to their %d bytes", who, (int)n);
   return FM_OK;
 }
 
@@ -168,6 +194,24 @@ __device__ __forceinline__ void e4m3x4_h(uint32_t four, uint32_t& lo, uint32_t& 
   asm("{.reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b;}"
       : "=r"(lo), "=r"(hi)
       : "r"(four));
+}
+// four bytes of two e2m1 codes each (low half first) as f16x2
+__device__ __forceinline__ void e2m1x8_h(uint32_t bytes, uint32_t* h) {
+  asm("{.reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4; cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b; "
+      "cvt.rn.f16x2.e2m1x2 %2, c; cvt.rn.f16x2.e2m1x2 %3, d;}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(bytes));
+}
+// two e4m3 values (low byte first) as f16x2
+__device__ __forceinline__ uint32_t e4m3x2_h(uint32_t two) {
+  uint32_t y;
+  asm("{.reg .b16 a, b; mov.b32 {a, b}, %1; cvt.rn.f16x2.e4m3x2 %0, a;}" : "=r"(y) : "r"(two));
+  return y;
+}
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
 }
 // 2^x; results under 2^-126 are zero
 __device__ __forceinline__ float ex2(float x) {

@@ -8,7 +8,9 @@ instead, runs on the current CUDA stream, and returns new tensors.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+from typing import NamedTuple
 
 import torch
 
@@ -24,6 +26,23 @@ def _p(t):
 
 def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+_ERR_WORDS: dict = {}
+
+
+def error_word(device) -> torch.Tensor:
+    """The device's error word (int32, zero until a kernel records an index or
+    timeout code; the first code sticks), allocated once per device so that a
+    call launches no fill kernel for it."""
+    key = torch.device(device)
+    if key.index is None:
+        key = torch.device(key.type, torch.cuda.current_device())
+    w = _ERR_WORDS.get(key)
+    if w is None:
+        w = torch.zeros(1, dtype=torch.int32, device=key)
+        _ERR_WORDS[key] = w
+    return w
 
 
 def _logits_dtype(t) -> int:
@@ -178,6 +197,64 @@ def accept_rejection(target_logits, draft, q, temperature: float, seed: int, off
     _lib.call("fm_accept_rejection", _p(target_logits), dt, _p(draft), _p(q), B, K1 - 1, V, float(temperature),
               int(seed), int(offset), _p(acc), _p(bonus), _p(ws), wsb, _stream())
     return acc, bonus
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` says of each row: fp32 ``logprobs`` and ``entropy`` (rows...), int64 ``top_ids`` and fp32
+    ``top_logprobs`` (rows..., top_k)."""
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+@functools.lru_cache(maxsize=1024)
+def _logprobs_workspace(device: int, rows: int, V: int, dtype: int, top_k: int) -> int:
+    # the index of the current device is part of the key: the size goes by its number of SMs
+    return _lib.load().fm_token_logprobs_workspace_size(rows, V, dtype, top_k)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, temperature: float = 1.0) -> TokenLogprobs:
+    """Log probabilities of ``tokens (...)`` int64 under ``softmax(logits / temperature)`` of ``logits (..., V)`` bf16 or
+    fp32, the softmax's entropy (in nats) and the ``top_k`` (at most 32) likeliest ids with theirs, equal logits by the
+    lowest id; in one pass over the logits and without writing probabilities (``fm_token_logprobs``).
+
+    A row's values are contiguous, rows may lie further apart (a vocabulary padded in memory); more than one leading
+    dimension is flattened, with a copy where its strides do not allow a view.  An id outside the vocabulary has
+    log probability -inf and is recorded for ``cache_ops.check_device_errors``.  A row of -inf alone has -inf and entropy 0,
+    one with a NaN or +inf NaN throughout.  Runs on the current stream without a host synchronisation and can be
+    captured in a CUDA graph; there is no gradient."""
+    if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() < 1:
+        raise ValueError(f"logits must be a CUDA bf16 or fp32 tensor, got {logits.dtype} on {logits.device}")
+    dev, shape = logits.device, logits.shape[:-1]
+    if dev.index != torch._C._cuda_getDevice():
+        raise ValueError(f"the logits are on {dev}, which is not the current device")
+    if tokens.device != dev or tokens.dtype != torch.int64 or tokens.shape != shape or not tokens.is_contiguous():
+        raise ValueError(f"tokens must be contiguous int64 {tuple(shape)} on {dev}, "
+                         f"got {tokens.dtype} {tuple(tokens.shape)} on {tokens.device}")
+    if logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError("token_logprobs has no gradient: detach the logits")
+    V = logits.shape[-1]
+    if not 0 <= top_k <= min(V, _lib.FM_TOKEN_LOGPROBS_MAX_TOP):
+        raise ValueError(f"top_k must lie in 0 .. {min(V, _lib.FM_TOKEN_LOGPROBS_MAX_TOP)}, got {top_k}")
+    if not 0.0 < temperature < math.inf:
+        raise ValueError(f"the temperature must be positive, got {temperature}")
+    if V > 1 and logits.stride(-1) != 1:
+        raise ValueError("a row of logits must be contiguous")
+    if len(shape) != 1:
+        logits = logits.reshape(-1, V)
+    rows = logits.shape[0]
+    out = logits.new_empty((2,) + shape, dtype=torch.float32)
+    ids = tokens.new_empty(shape + (top_k,))
+    top = logits.new_empty(shape + (top_k,), dtype=torch.float32)
+    if rows:
+        dt = 0 if logits.dtype == torch.bfloat16 else 1
+        need = _logprobs_workspace(dev.index, rows, V, dt, top_k)
+        ws = tokens.new_empty(need // 8) if need else None  # sizes are multiples of 16
+        _lib.call("fm_token_logprobs", logits.data_ptr(), dt, logits.stride(0), tokens.data_ptr(), rows, V, temperature,
+                  top_k, out.data_ptr(), out.data_ptr() + 4 * rows, ids.data_ptr(), top.data_ptr(),
+                  ws.data_ptr() if need else None, need, error_word(dev).data_ptr(), torch._C._cuda_getCurrentRawStream(dev.index))
+    return TokenLogprobs(out[0], out[1], ids, top)
 
 
 def transpose(x):

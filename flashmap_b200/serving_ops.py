@@ -35,6 +35,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
+from .ops import error_word as _err
 
 __all__ = [
     "OpArgumentError", "rope_table", "rope_freqs", "vllm_rms_norm", "vllm_rms_norm_rope",
@@ -98,23 +99,6 @@ def _half_table(cos_sin: torch.Tensor, head_dim: int) -> _lib.RopeView:
           and cos_sin.shape[1] == head_dim, f"cos_sin must be contiguous float32 (positions, {head_dim})")
     return _lib.RopeView(cos_sin.data_ptr(), cos_sin.data_ptr() + 4 * (head_dim // 2), head_dim, 1,
                          cos_sin.shape[0])
-
-
-_ERR_WORDS: dict = {}
-
-
-def _err(device) -> torch.Tensor:
-    """The device's error word (int32, zero until a kernel records an index or
-    timeout code; the first code sticks), allocated once per device so that a
-    call launches no fill kernel for it."""
-    key = torch.device(device)
-    if key.index is None:
-        key = torch.device(key.type, torch.cuda.current_device())
-    w = _ERR_WORDS.get(key)
-    if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=key)
-        _ERR_WORDS[key] = w
-    return w
 
 
 def _bf16_weight(w: torch.Tensor, name: str) -> torch.Tensor:

@@ -271,7 +271,7 @@ FM_API fm_status fm_cross_attn(const void* q, const void* cache, void* out, cons
  * ------------------------------------------------------------------------ */
 
 /* Element types of operator arguments. */
-enum { FM_DT_BF16 = 0, FM_DT_F32 = 1, FM_DT_E4M3 = 2, FM_DT_I32 = 3, FM_DT_I64 = 4 };
+enum { FM_DT_BF16 = 0, FM_DT_F32 = 1, FM_DT_E4M3 = 2, FM_DT_I32 = 3, FM_DT_I64 = 4, FM_DT_E2M1 = 5 };
 
 /* RMSNorm rounding: FM_NORM_DIT is the DiT's x * bf16(w * rsqrt(mean(x^2) + eps))
  * (modeling_flashmap.py:69-80, vllm/kernels.py:38-46); FM_NORM_FUSED is
@@ -563,6 +563,77 @@ FM_API fm_status fm_time_sinusoid(void* out, int64_t dim, float s, float t, floa
                                   fm_stream stream);
 FM_API fm_status fm_silu(const void* x, void* y, int64_t n, fm_stream stream);
 FM_API fm_status fm_add(const void* a, const void* b, void* y, int64_t n, fm_stream stream);
+
+/* What an emitted token's row of logits says of it, without probabilities
+ * being written.  logits: rows of V values, row_stride elements apart, bf16
+ * (FM_DT_BF16) or fp32 (FM_DT_F32).  With p = softmax(logits / temperature):
+ *   logprobs[r] = ln p[tokens[r]] (an id outside the row: -inf, DEV_BAD_INDEX),
+ *   entropy[r] = -sum p ln p,
+ *   top_ids, top_logprobs (rows, top_k): the top_k largest, equal logits by the
+ *   lowest id; top_k at most FM_TOKEN_LOGPROBS_MAX_TOP and V.
+ * A row of -inf alone has logprobs -inf and entropy 0.  One that holds a NaN or
+ * +inf has NaN for all (in the order of top_ids a NaN stands where -inf does).
+ * The workspace need not be initialised. */
+enum { FM_TOKEN_LOGPROBS_MAX_TOP = 32 };
+FM_API size_t fm_token_logprobs_workspace_size(int64_t rows, int64_t V, int32_t dtype, int64_t top_k);
+FM_API fm_status fm_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, const int64_t* tokens,
+                                   int64_t rows, int64_t V, float temperature, int64_t top_k, float* logprobs,
+                                   float* entropy, int64_t* top_ids, float* top_logprobs, void* workspace,
+                                   size_t workspace_bytes, int32_t* err, fm_stream stream);
+
+/* ------------------------------------------------------------------------
+ * The same cache held in 4 bits, and appending to it.
+ * ------------------------------------------------------------------------ */
+
+/* Where the factors of a 4-bit cache (fm_paged_cache.dtype FM_DT_E2M1) lie.  A
+ * row of head_dim values is head_dim / 2 bytes of e2m1 codes (value 2 i in the
+ * low half of byte i), 16-byte aligned, the strides of fm_paged_cache counted
+ * in bytes; and head_dim / 16 e4m3 factors, one for each 16 values, at page *
+ * page_stride + kv_head * head_stride + token * token_stride bytes, aligned to
+ * their number.  A value is code * factor (* descale). */
+typedef struct fm_block_scales {
+  void* k;
+  void* v;
+  int64_t k_page_stride, k_head_stride, k_token_stride;
+  int64_t v_page_stride, v_head_stride, v_token_stride;
+} fm_block_scales;
+
+/* New tokens' keys and values (tokens, kv_heads, head_dim) bf16 go to the last
+ * positions of their request's lengths[r]: rows cu_seqlens_q[r] ..
+ * cu_seqlens_q[r + 1], or row r where cu_seqlens_q is NULL (then tokens ==
+ * requests).  With `rope`, (rope_rows, rotary_dim / 2, 2) fp32 cosines and sines
+ * of a position, keys and queries (tokens, heads, head_dim) are rotated on the
+ * way: pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when interleaved, of the
+ * first rotary_dim values (a multiple of 16), at positions[token] or, where
+ * positions is NULL, at the token's place in the cache.  Rotation is fp32,
+ * each product and sum rounded; then one rounding to the cache's type (values
+ * divided by the descales first; a 4-bit row's factor is its 16 values'
+ * largest magnitude / 6 as e4m3).  out (tokens, heads, head_dim) bf16 are the
+ * rotated queries.  A row without a place (a request without positions, more
+ * rows than positions) writes nothing and its query comes back zero; so does,
+ * with DEV_BAD_INDEX recorded, one whose length passes the table, or whose
+ * position passes the rope's rows; one whose page id is out of range writes
+ * nothing.  Rows that cu_seqlens_q gives to no request are not written. */
+typedef struct fm_append {
+  const void* key;
+  const void* value;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  const void* query; /* or NULL */
+  int64_t q_token_stride, q_head_stride, heads;
+  void* out;
+  int64_t out_token_stride, out_head_stride;
+  int64_t tokens;
+  const int32_t* cu_seqlens_q; /* or NULL */
+  const void* positions;       /* or NULL */
+  int32_t positions_dtype;     /* FM_DT_I32 or FM_DT_I64 */
+  const float* rope;           /* or NULL */
+  int64_t rope_rows, rotary_dim;
+  int32_t interleaved;
+  int32_t* err;
+} fm_append;
+/* scales: of a 4-bit cache; NULL otherwise. */
+FM_API fm_status fm_paged_append(const fm_paged_cache* cache, const fm_block_scales* scales, const fm_append* args,
+                                 fm_stream stream);
 
 /* ------------------------------------------------------------------------
  * The whole drafter: a plan over caller-owned weights and buffers.

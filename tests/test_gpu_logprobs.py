@@ -1,0 +1,174 @@
+"""``token_logprobs`` against 64 bits.
+
+Tolerances.  A thread adds up to V / 256 exponentials one after the other, and
+about 40 sums are joined after that, each addition off by 2^-24; an exponential
+is off by 2^-22 and by 2^-24 of its exponent d, a join's factor likewise.  So S
+is off by (V / 256 + 300) 2^-24 and by 2^-22 of the mean |d|, which is under
+log2 V + 2 for the rows here or carries no weight.  A log probability adds 2^-22
+of itself and of log S (the constants' and the result's roundings); the entropy
+sum |p d| is off by the same share of its own size.
+"""
+
+import math
+
+import pytest
+import torch
+
+from oracle import serving_step as O
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def call(*a, **k):
+    from flashmap_b200 import ops
+    return ops.token_logprobs(*a, **k)
+
+
+def error_word():
+    from flashmap_b200.ops import error_word as word
+    torch.cuda.synchronize()
+    w = word(torch.device("cuda", torch.cuda.current_device()))
+    code = int(w)
+    w.zero_()
+    return code
+
+
+def check(got, logits, tokens, k, T):
+    V = logits.shape[-1]
+    lp, ent, ids, top = O.token_logprobs(logits.cpu(), tokens.cpu().tolist(), k, T)
+    tol = (V / 256 + 300) * 2.0 ** -24 + 2.0 ** -22 * (math.log2(V) + 2)
+    assert torch.equal(got.top_ids.cpu(), ids)
+    for a, b, more in ((got.logprobs, lp, 0.0), (got.top_logprobs, top, 0.0), (got.entropy, ent, tol * math.log2(V))):
+        a = a.double().cpu()
+        live = torch.isfinite(b)
+        assert torch.equal(a[~live], b[~live]) and torch.isfinite(a[live]).all()
+        err, lim = (a - b).abs()[live], tol + more + 2.0 ** -21 * (b.abs()[live] + math.log(V))
+        assert (err <= lim).all(), (err / lim).max().item()
+
+
+CASES = [
+    # rows, V, pitch, dtype, top_k, temperature
+    (1, 1, 1, torch.float32, 1, 1.0),
+    (3, 2, 9, torch.bfloat16, 2, 0.5),
+    (5, 33, 33, torch.bfloat16, 32, 1.0),
+    (2, 255, 256, torch.float32, 0, 1.7),
+    (7, 1000, 1003, torch.bfloat16, 20, 1.0),
+    (4, 4097, 4100, torch.float32, 5, 0.3),
+    (1, 32003, 32064, torch.float32, 32, 1.0),
+    (37, 32003, 32003, torch.bfloat16, 1, 2.0),
+    (2, 151936, 151936, torch.bfloat16, 20, 1.0),
+    (700, 5001, 5001, torch.bfloat16, 7, 0.8),
+    (1, 1500001, 1500001, torch.bfloat16, 32, 1.0),
+    (2, 700001, 700001, torch.float32, 3, 1.0),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_logprobs(case):
+    n, V, pitch, dtype, k, T = case
+    g = torch.Generator().manual_seed(41)
+    x = torch.full((n, pitch), math.nan)
+    x[:, :V] = 3.0 * torch.randn(n, V, generator=g)
+    x[:, V // 2] += 8.0
+    x = x.to(dtype).to(DEV)[:, :V]
+    tokens = torch.randint(0, V, (n,), generator=g).to(DEV)
+    tokens[0] = V - 1
+    check(call(x, tokens, top_k=k, temperature=T), x, tokens, k, T)
+    assert error_word() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_ties_masks_and_empty_rows(dtype):
+    """All values equal (more ties than are sorted at once), few that differ, all but some -inf, -inf alone, -0 and 0."""
+    V = 9000
+    x = torch.zeros(7, V)
+    x[1, 4000:] = 1.0
+    x[2] = -math.inf
+    x[2, [8999, 17, 4096]] = torch.tensor([1.0, 2.0, 1.0])
+    x[3] = -math.inf
+    x[4, ::2] = -0.0
+    x[5] = torch.arange(V) % 3
+    x[6] = -1e4
+    x[6, 5000] = 1e4
+    x = x.to(dtype).to(DEV)
+    tokens = torch.tensor([5, 4000, 0, 3, 1, 2, 1], device=DEV)
+    for k in (0, 4, 32):
+        got = call(x, tokens, top_k=k)
+        check(got, x, tokens, k, 1.0)
+        assert float(got.logprobs[3]) == -math.inf and float(got.entropy[3]) == 0.0 and float(got.logprobs[2]) == -math.inf
+    assert error_word() == 0
+
+
+def test_nan_and_infinity():
+    V = 5000
+    x = torch.randn(4, V, generator=torch.Generator().manual_seed(42))
+    x[0, 100] = math.nan
+    x[1, 4999] = math.inf
+    x[2] = math.nan
+    got = call(x.to(DEV), torch.zeros(4, dtype=torch.int64, device=DEV), top_k=3)
+    for t in (got.logprobs, got.entropy, got.top_logprobs):
+        assert torch.isnan(t[:3]).all() and torch.isfinite(t[3]).all()
+    assert ((got.top_ids >= 0) & (got.top_ids < V)).all()
+    want = torch.where(torch.isnan(x[0]), -math.inf, x[0]).topk(3).indices
+    assert torch.equal(got.top_ids[0].cpu(), want) and int(got.top_ids[1, 0]) == 4999
+    assert got.top_ids[2].tolist() == [0, 1, 2]
+
+
+def test_ids_outside_the_vocabulary():
+    x = torch.randn(3, 100, device=DEV)
+    got = call(x, torch.tensor([-1, 100, 5], device=DEV))
+    assert got.logprobs[:2].tolist() == [-math.inf] * 2 and math.isfinite(float(got.logprobs[2]))
+    assert error_word() == 4
+
+
+def test_shapes_streams_graphs_and_repeats():
+    g = torch.Generator().manual_seed(43)
+    x = (2.0 * torch.randn(3, 5, 3003, generator=g)).to(torch.bfloat16).to(DEV)
+    tokens = torch.randint(0, 3003, (3, 5), generator=g).to(DEV)
+    a = call(x, tokens, top_k=4)
+    assert a.logprobs.shape == (3, 5) and a.top_ids.shape == (3, 5, 4)
+    check(type(a)(*[t.flatten(0, 1) for t in a]), x.flatten(0, 1), tokens.flatten(), 4, 1.0)
+    one = call(x[1, 2], tokens[1, 2], top_k=4)
+    assert one.logprobs.shape == () and torch.equal(one.top_ids, a.top_ids[1, 2])
+    strided = call(x.transpose(0, 1)[:, :, 1:], (tokens.T - 1).clamp(min=0).contiguous(), top_k=2)
+    check(type(a)(*[t.flatten(0, 1) for t in strided]), x.transpose(0, 1)[:, :, 1:].reshape(15, 3002),
+          (tokens.T - 1).clamp(min=0).flatten(), 2, 1.0)
+    empty = call(x[:0], tokens[:0], top_k=3)
+    assert empty.top_logprobs.shape == (0, 5, 3)
+    row = (2.0 * torch.randn(1, 100003, generator=g)).to(DEV)
+    t = torch.tensor([77], device=DEV)
+    runs = [call(row, t, top_k=9) for _ in range(3)]
+    assert all(torch.equal(p, q) for r in runs[1:] for p, q in zip(runs[0], r))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = call(row, t, top_k=9)
+    side.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(runs[0], other))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call(row, t, top_k=9)
+    row.copy_(2.0 * torch.randn(1, 100003, generator=g))
+    graph.replay()
+    check(held, row, t, 9, 1.0)
+
+
+def test_rows_past_32_bit_offsets():
+    V, stride = 500, 2_200_000_000
+    pool = torch.empty(stride + V, dtype=torch.bfloat16, device=DEV)
+    x = pool.as_strided((2, V), (stride, 1))
+    x.copy_(torch.randn(2, V, generator=torch.Generator().manual_seed(44)))
+    t = torch.tensor([3, 4], device=DEV)
+    check(call(x, t, top_k=5), x.contiguous(), t, 5, 1.0)
+
+
+def test_refusals():
+    x, t = torch.randn(2, 50, device=DEV), torch.zeros(2, dtype=torch.int64, device=DEV)
+    for a, k in (((x.half(), t), {}), ((x.cpu(), t), {}), ((x, t.int()), {}), ((x, t[:1]), {}), ((x, t.cpu()), {}),
+                 ((x, t), dict(top_k=33)), ((x, t), dict(top_k=-1)), ((x[:, :3], t), dict(top_k=4)), ((x, t), dict(temperature=0.0)),
+                 ((x, t), dict(temperature=math.nan)), ((x, t), dict(temperature=math.inf)), ((x[:, ::2], t), {}),
+                 ((x.clone().requires_grad_(), t), {}), ((x[:, :0], t), {})):
+        with pytest.raises((ValueError, RuntimeError)):
+            call(*a, **k)
