@@ -196,6 +196,9 @@ _SIGNATURES = {
     "fm_paged_evict_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
     "fm_paged_evict": (c_int, [c_void_p, c_void_p, c_void_p]),  # PagedCache, Evict
     "fm_paged_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),  # PagedCache, BlockScales or NULL, Append
+    "fm_paged_decode_attn_fp4_workspace_size": (c_size_t, [c_int64] * 7),
+    "fm_paged_decode_attn_fp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),  # PagedCache, BlockScales, DecodeAttn
+    "fm_paged_window_attn_fp4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p]),  # PagedCache, BlockScales, WindowAttn
     "fm_token_logprobs_workspace_size": (c_size_t, [c_int64, c_int64, c_int32, c_int64]),
     "fm_token_logprobs": (c_int, [c_void_p, c_int32, c_int64, c_void_p, c_int64, c_int64, c_float, c_int64, c_void_p,
                                   c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),

@@ -44,7 +44,7 @@ from . import _lib
 from .serving_ops import OpArgumentError, _err, _need
 
 __all__ = ["OpArgumentError", "paged_decode_attention", "paged_window_attention", "evict_paged_context",
-           "append_paged_context", "check_device_errors"]
+           "append_paged_context", "paged_decode_attention_fp4", "paged_window_attention_fp4", "check_device_errors"]
 
 _FP8 = torch.float8_e4m3fn
 
@@ -328,6 +328,60 @@ def _window(query, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, max_s
     return out
 
 
+def _launch4(name: str, cache: _Cache4, args: bytes) -> None:
+    status = getattr(_lib.load(), name)(cache.packed, cache.scales, args,
+                                        torch._C._cuda_getCurrentRawStream(cache.device.index))
+    if status:
+        _lib.check(status, name)
+
+
+def _decode4(query, k_cache, v_cache, k_scales, v_scales, seqused_k, block_table, max_seqlen_k, softmax_scale, window,
+             sinks, descales) -> torch.Tensor:
+    cache = _cache4(k_cache, v_cache, k_scales, v_scales, seqused_k, block_table, descales, int(max_seqlen_k))
+    dev = cache.device
+    query = _query(query, cache, dev)
+    shape = query.shape
+    if shape[0] != cache.requests or window < 0 or sinks < 0:
+        _need(shape[0] == cache.requests, "one query row per request")
+        _visibility(window, sinks)
+    out = query.new_empty(shape)
+    if cache.requests == 0:
+        return out
+    heads, qs = shape[1], query.stride()
+    need = _workspace_size("fm_paged_decode_attn_fp4_workspace_size", dev.index, cache.requests, heads, cache.kv_heads,
+                           cache.head_dim, cache.max_length, window, sinks)
+    ws = seqused_k.new_empty(need // 4) if need else None  # sizes are multiples of 8
+    _launch4("fm_paged_decode_attn_fp4", cache,
+             _DECODE.pack(query.data_ptr(), qs[0], qs[1], heads, softmax_scale, window, sinks, 0, 0, 0, out.data_ptr(),
+                          heads * cache.head_dim, cache.head_dim, ws.data_ptr() if need else 0, need, _err_word(dev)))
+    return out
+
+
+def _window4(query, k_cache, v_cache, k_scales, v_scales, cu_seqlens_q, seqused_k, block_table, max_seqlen_q,
+             max_seqlen_k, softmax_scale, window, sinks, descales) -> torch.Tensor:
+    cache = _cache4(k_cache, v_cache, k_scales, v_scales, seqused_k, block_table, descales, int(max_seqlen_k))
+    dev = cache.device
+    query = _query(query, cache, dev)
+    _on(cu_seqlens_q, "cu_seqlens_q", dev)
+    _need(cu_seqlens_q.dtype is torch.int32 and cu_seqlens_q.shape == (cache.requests + 1,)
+          and cu_seqlens_q.is_contiguous(), "cu_seqlens_q must be contiguous int32 (requests + 1,)")
+    _need(max_seqlen_q >= 0, "max_seqlen_q must not be negative")
+    _visibility(window, sinks)
+    out = query.new_empty(query.shape)
+    tokens, heads = query.shape[0], query.shape[1]
+    if cache.requests == 0 or tokens == 0:
+        return out
+    qs, os = query.stride(), out.stride()
+    need = _workspace_size("fm_paged_window_attn_workspace_size", dev.index, cache.requests, tokens, heads, cache.kv_heads,
+                           cache.head_dim, int(max_seqlen_q), cache.max_length, window, sinks)
+    ws = seqused_k.new_empty(need // 4) if need else None  # sizes are multiples of 8
+    _launch4("fm_paged_window_attn_fp4", cache,
+             _WINDOW.pack(query.data_ptr(), qs[0], qs[1], tokens, heads, cu_seqlens_q.data_ptr(), int(max_seqlen_q),
+                          softmax_scale, window, sinks, out.data_ptr(), os[0], os[1], ws.data_ptr() if need else 0, need,
+                          _err_word(dev)))
+    return out
+
+
 @torch.library.custom_op("flashmap_b200::paged_decode_attention", mutates_args=("weight_sums",))
 def _decode_op(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k: torch.Tensor,
                block_table: torch.Tensor, max_seqlen_k: int, softmax_scale: float, window: int, sinks: int,
@@ -352,6 +406,35 @@ def _window_op(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
 @_window_op.register_fake
 def _(query, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, max_seqlen_q, max_seqlen_k, softmax_scale, window,
       sinks, descales):
+    return query.new_empty(query.shape)
+
+
+@torch.library.custom_op("flashmap_b200::paged_decode_attention_fp4", mutates_args=())
+def _decode4_op(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor,
+                v_scales: torch.Tensor, seqused_k: torch.Tensor, block_table: torch.Tensor, max_seqlen_k: int,
+                softmax_scale: float, window: int, sinks: int, descales: Optional[torch.Tensor]) -> torch.Tensor:
+    return _decode4(query, k_cache, v_cache, k_scales, v_scales, seqused_k, block_table, max_seqlen_k, softmax_scale,
+                    window, sinks, descales)
+
+
+@_decode4_op.register_fake
+def _(query, k_cache, v_cache, k_scales, v_scales, seqused_k, block_table, max_seqlen_k, softmax_scale, window, sinks,
+      descales):
+    return query.new_empty(query.shape)
+
+
+@torch.library.custom_op("flashmap_b200::paged_window_attention_fp4", mutates_args=())
+def _window4_op(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scales: torch.Tensor,
+                v_scales: torch.Tensor, cu_seqlens_q: torch.Tensor, seqused_k: torch.Tensor, block_table: torch.Tensor,
+                max_seqlen_q: int, max_seqlen_k: int, softmax_scale: float, window: int, sinks: int,
+                descales: Optional[torch.Tensor]) -> torch.Tensor:
+    return _window4(query, k_cache, v_cache, k_scales, v_scales, cu_seqlens_q, seqused_k, block_table, max_seqlen_q,
+                    max_seqlen_k, softmax_scale, window, sinks, descales)
+
+
+@_window4_op.register_fake
+def _(query, k_cache, v_cache, k_scales, v_scales, cu_seqlens_q, seqused_k, block_table, max_seqlen_q, max_seqlen_k,
+      softmax_scale, window, sinks, descales):
     return query.new_empty(query.shape)
 
 
@@ -402,6 +485,33 @@ def paged_window_attention(query: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         call = _window_op
     return call(query, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, max_seqlen_q, max_seqlen_k, softmax_scale,
                 window, sinks, descales)
+
+
+def paged_decode_attention_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                               k_scales: torch.Tensor, v_scales: torch.Tensor, seqused_k: torch.Tensor,
+                               block_table: torch.Tensor, max_seqlen_k: int, softmax_scale: float, *, window: int = 0,
+                               sinks: int = 0, descales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_decode_attention`` on a 4-bit cache: ``k_cache`` and ``v_cache (pages, kv_heads, page_size, head_dim / 2)``
+    uint8 with ``k_scales`` and ``v_scales (pages, kv_heads, page_size, head_dim / 16)`` e4m3, as
+    ``append_paged_context`` writes them; ``descales (2, requests, kv_heads)`` go on top.  It gathers no weights."""
+    call = _decode4
+    if _tracing() or query.requires_grad and torch.is_grad_enabled():
+        call = _decode4_op
+    return call(query, k_cache, v_cache, k_scales, v_scales, seqused_k, block_table, max_seqlen_k, softmax_scale, window,
+                sinks, descales)
+
+
+def paged_window_attention_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                               k_scales: torch.Tensor, v_scales: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                               seqused_k: torch.Tensor, block_table: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int,
+                               softmax_scale: float, *, window: int = 0, sinks: int = 0,
+                               descales: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``paged_window_attention`` on a 4-bit cache, given as to ``paged_decode_attention_fp4``."""
+    call = _window4
+    if _tracing() or query.requires_grad and torch.is_grad_enabled():
+        call = _window4_op
+    return call(query, k_cache, v_cache, k_scales, v_scales, cu_seqlens_q, seqused_k, block_table, max_seqlen_q,
+                max_seqlen_k, softmax_scale, window, sinks, descales)
 
 
 def evict_paged_context(k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k: torch.Tensor,

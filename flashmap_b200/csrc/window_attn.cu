@@ -50,6 +50,7 @@ struct WindowArgs {
   WaCutItem* cuts;  // [CTAs], or null: items are not cut
   int row_tiles;    // no fewer than there are
   int* err;
+  ScaleRef f;       // of a 4-bit cache
 };
 
 // The key tiles that rows row0 .. of request r see: those of the first tokens,
@@ -298,12 +299,16 @@ struct WaCtrl {
 // products run, and join their halves at the end (24 x 17 rows on 512 .. 4096
 // positions: 70 us with one warpgroup, 64 us with both; in the same kernel as
 // the rest it costs that 4 percent).
-template <int HD, bool KV8, bool DUO>
+//
+// BITS: of a cache value (16, 8 or 4).  8 and 4 bits go through the loading
+// warps' registers and on as f16, which holds them exactly.
+template <int HD, int BITS, bool DUO>
 __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
+  constexpr bool KV8 = BITS < 16;
   using Lay = WaLayout<HD>;
   constexpr int TILE = Lay::TILE, SLOTS = Lay::SLOTS;
   constexpr int CPR = HD / 8;  // 16-byte chunks of a 16-bit row
-  // registers: 2 x 184 + 64 + 80, or 2 x 176 + 96 + 64 where e4m3 rows pass
+  // registers: 2 x 184 + 64 + 80, or 2 x 176 + 96 + 64 where narrow rows pass
   // through the loading warps, is what 4 x 128 threads are launched with
   extern __shared__ __align__(1024) uint8_t wa_smem[];
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -704,7 +709,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
     bool ok = true;
     int slot = 0, tiles = 0;
     uint32_t phase = 1;  // an empty slot's first wait succeeds at once
-    constexpr int RC = HD * (KV8 ? 1 : 2) / 16, RPI = 32 / RC, U = 32 / RPI;  // 16-byte chunks of a cache row, rows at a time
+    constexpr int RC = HD * BITS / 128, RPI = 32 / RC, U = 32 / RPI;  // 16-byte chunks of a cache row, rows at a time
     const int ch = lane % RC, sub = lane / RC;
     auto advance = [&]() {
       if (++slot == SLOTS) {
@@ -743,7 +748,66 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
         return page < 0 ? -1ll : page * a.c.vps + (long long)w.c * a.c.vhs + tok * a.c.vts;
       };
       int tok_next = 0, page_next = lookup(0, &tok_next);
-      if constexpr (KV8) {
+      if constexpr (BITS == 4) {
+        // codes and factors come into registers, one tile ahead: 32 values and two factors to a lane
+        uint4 xk[U], xv[U];
+        uint32_t fk[U], fv[U];
+        auto fetch = [&](uint4* x, uint32_t* fx, const uint8_t* from, long long off, const uint8_t* scales, long long foff) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const long long o = __shfl_sync(0xffffffffu, off, u * RPI + sub);
+            const long long fo = __shfl_sync(0xffffffffu, foff, u * RPI + sub);
+            x[u] = o < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(from + o + ch * 16);
+            fx[u] = o < 0 ? 0u : *reinterpret_cast<const uint16_t*>(scales + fo + ch * 2);
+          }
+        };
+        auto kf_off = [&](int page, int tok) {
+          return page < 0 ? 0ll : page * a.f.kps + (long long)w.c * a.f.khs + tok * a.f.kts;
+        };
+        auto vf_off = [&](int page, int tok) {
+          return page < 0 ? 0ll : page * a.f.vps + (long long)w.c * a.f.vhs + tok * a.f.vts;
+        };
+        auto widen = [&](const uint4* x, const uint32_t* fx) {
+          if (!mbar_wait(&ctl->empty[slot], phase, abort)) {
+            ok = false;
+            return;
+          }
+          // a lane's 32 values are half of a 64-column block; which quarter first: no two lanes of two rows share a bank
+          uint8_t* dst = sKV + slot * TILE + (ch >> 1) * 16384 + (lw * 32 + sub) * 128;
+          const int c0 = (ch & 1) * 4, turn = ch & 2;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int sw = (u * RPI + sub) & 7;
+            const uint32_t f2 = e4m3x2_h(fx[u]), f_lo = __byte_perm(f2, 0, 0x1010), f_hi = __byte_perm(f2, 0, 0x3232);
+            const uint32_t words[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t h[4];
+              // with `turn` the quarters 2, 3 come first
+              e2m1x8_h(turn ? words[q ^ 2] : words[q], h);
+              const uint32_t f = (q < 2) == (turn == 0) ? f_lo : f_hi;
+              *reinterpret_cast<uint4*>(dst + u * RPI * 128 + (((c0 + (q ^ turn)) ^ sw) << 4)) =
+                  make_uint4(mul_h2(h[0], f), mul_h2(h[1], f), mul_h2(h[2], f), mul_h2(h[3], f));
+            }
+          }
+          fence_async_smem();
+          mbar_arrive(&ctl->full[slot]);
+          advance();
+        };
+        int page = page_next, tok = tok_next;
+        if (w.n > 0) fetch(xk, fk, a.c.k, k_off(page, tok), a.f.k, kf_off(page, tok));
+        for (int j = 0; j < w.n && ok; ++j, ++tiles) {
+          page_next = lookup(j + 1, &tok_next);
+          const uint32_t good = __ballot_sync(0xffffffffu, page != -2);
+          if (lane == 0) ctl->valid[tiles & 7][lw] = good;
+          fetch(xv, fv, a.c.v, v_off(page, tok), a.f.v, vf_off(page, tok));
+          widen(xk, fk);
+          page = page_next;
+          tok = tok_next;
+          if (j + 1 < w.n) fetch(xk, fk, a.c.k, k_off(page, tok), a.f.k, kf_off(page, tok));
+          if (ok) widen(xv, fv);
+        }
+      } else if constexpr (KV8) {
         // e4m3 rows come into registers, one tile ahead, and go on as f16, which holds them exactly
         uint4 xk[U], xv[U];
         auto fetch = [&](uint4* x, const uint8_t* from, long long off) {
@@ -1181,20 +1245,66 @@ WindowPlan window_plan(int64_t R, int64_t T, int64_t H, int64_t KH, int64_t HD, 
   return p;
 }
 
-template <int HD, bool KV8, bool DUO>
+template <int HD, int BITS, bool DUO>
 fm_status launch_window(const WindowArgs& a, const WindowPlan& pl, cudaStream_t s) {
   constexpr int smem = WaLayout<HD>::SMEM;
   static_assert(sizeof(WaCtrl) <= 3072 && smem <= 232448, "shared memory");
-  fm_status st = allow_smem<window_attn_kernel<HD, KV8, DUO>>(smem, "paged_window_attn");
+  fm_status st = allow_smem<window_attn_kernel<HD, BITS, DUO>>(smem, "paged_window_attn");
   if (st != FM_OK) return st;
-  st = launch_kernel(window_attn_kernel<HD, KV8, DUO>, dim3((unsigned)pl.ctas), dim3(512), smem, s, true, a);
+  st = launch_kernel(window_attn_kernel<HD, BITS, DUO>, dim3((unsigned)pl.ctas), dim3(512), smem, s, true, a);
   if (st != FM_OK || !pl.cuts) return st;
   return launch_kernel(window_join_kernel<HD>, dim3((unsigned)pl.ctas, HD / 16), dim3(WA_ROWS), 0, s, true, a, pl.ctas);
 }
 
-template <int HD, bool KV8>
+template <int HD, int BITS>
 fm_status launch_window(const WindowArgs& a, const WindowPlan& pl, bool duo, cudaStream_t s) {
-  return duo ? launch_window<HD, KV8, true>(a, pl, s) : launch_window<HD, KV8, false>(a, pl, s);
+  return duo ? launch_window<HD, BITS, true>(a, pl, s) : launch_window<HD, BITS, false>(a, pl, s);
+}
+
+// The arguments of a call on a cache that cache_ref has accepted.
+fm_status window_args(const fm_paged_cache* cache, const fm_window_attn* p, const char* who, WindowArgs* out,
+                      WindowPlan* plan) {
+  WindowArgs& a = *out;
+  if (!p) return set_error(FM_ERR_INVALID, "%s: null arguments", who);
+  if (p->heads < 1 || p->heads % cache->kv_heads || p->heads > 65535)
+    return set_error(FM_ERR_SHAPE, "%s: query heads must be a multiple of the kv heads", who);
+  if (p->window < 0 || p->sinks < 0 || p->window > 0x7ffffff0 || p->sinks > 0x7ffffff0)
+    return set_error(FM_ERR_SHAPE, "%s: window and sinks must not be negative", who);
+  if (p->rows < 0 || p->rows > 0x7ffffff0 || p->rows * p->heads > 0x7ffffff0)
+    return set_error(FM_ERR_SHAPE, "%s: too many query rows", who);
+  if (cache->requests == 0 || p->rows == 0) return FM_OK;  // the caller stops here, too
+  if (!p->q || !p->out || !p->cu_seqlens_q) return set_error(FM_ERR_INVALID, "%s: null pointer", who);
+  // one row or one head is not stepped through: its stride may be anything
+  a.q_ts = p->rows == 1 ? 0 : p->q_token_stride;
+  a.q_hs = p->heads == 1 ? 0 : p->q_head_stride;
+  a.o_ts = p->rows == 1 ? 0 : p->out_token_stride;
+  a.o_hs = p->heads == 1 ? 0 : p->out_head_stride;
+  if ((uintptr_t)p->q % 16 || a.q_ts % 8 || a.q_hs % 8 || (uintptr_t)p->out % 16 || a.o_ts % 8 || a.o_hs % 8)
+    return set_error(FM_ERR_ALIGN, "%s: query and output rows must be 16-byte aligned", who);
+  a.q = static_cast<const uint8_t*>(p->q);
+  a.cu = p->cu_seqlens_q;
+  a.T = (int)p->rows;
+  a.H = (int)p->heads;
+  a.G = (int)(p->heads / cache->kv_heads);
+  a.by_g = make_divider((uint32_t)a.G);
+  a.scale = p->softmax_scale * kLog2e;
+  a.window = p->window >= cache->max_length ? 0 : (int)p->window;  // so wide that it hides nothing
+  a.sinks = (int)p->sinks;
+  a.out = static_cast<__nv_bfloat16*>(p->out);
+  a.err = p->err;
+  const WindowPlan pl = *plan = window_plan(cache->requests, p->rows, p->heads, cache->kv_heads, cache->head_dim, p->max_q,
+                                    cache->max_length, p->window, p->sinks);
+  if (pl.total > p->workspace_bytes || (pl.total && !p->workspace))
+    return set_error(FM_ERR_WORKSPACE, "%s: workspace %zu < %zu", who, p->workspace_bytes, pl.total);
+  if ((uintptr_t)p->workspace % 16) return set_error(FM_ERR_ALIGN, "%s: workspace not 16-byte aligned", who);
+  if (cache->requests > WA_REQUESTS || p->rows * a.G / WA_ROWS + cache->requests > WA_ROW_TILES)
+    return set_error(FM_ERR_SHAPE, "%s: more than %d requests or %d row tiles", who, WA_REQUESTS, WA_ROW_TILES);
+  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
+  a.part = reinterpret_cast<float*>(ws);
+  a.stats = reinterpret_cast<float2*>(ws + pl.part);
+  a.cuts = pl.cuts ? reinterpret_cast<WaCutItem*>(ws + pl.part + pl.stats) : nullptr;
+  a.row_tiles = (int)(p->rows * a.G / WA_ROWS + cache->requests);
+  return FM_OK;
 }
 
 }  // namespace
@@ -1213,49 +1323,26 @@ extern "C" size_t fm_paged_window_attn_workspace_size(int64_t requests, int64_t 
 
 extern "C" fm_status fm_paged_window_attn(const fm_paged_cache* cache, const fm_window_attn* p, fm_stream stream) {
   WindowArgs a{};
+  WindowPlan pl{};
   fm_status st = cache_ref(cache, "paged_window_attn", &a.c);
-  if (st != FM_OK) return st;
-  if (!p) return set_error(FM_ERR_INVALID, "paged_window_attn: null arguments");
-  if (p->heads < 1 || p->heads % cache->kv_heads || p->heads > 65535)
-    return set_error(FM_ERR_SHAPE, "paged_window_attn: query heads must be a multiple of the kv heads");
-  if (p->window < 0 || p->sinks < 0 || p->window > 0x7ffffff0 || p->sinks > 0x7ffffff0)
-    return set_error(FM_ERR_SHAPE, "paged_window_attn: window and sinks must not be negative");
-  if (p->rows < 0 || p->rows > 0x7ffffff0 || p->rows * p->heads > 0x7ffffff0)
-    return set_error(FM_ERR_SHAPE, "paged_window_attn: too many query rows");
-  if (cache->requests == 0 || p->rows == 0) return FM_OK;
-  if (!p->q || !p->out || !p->cu_seqlens_q) return set_error(FM_ERR_INVALID, "paged_window_attn: null pointer");
-  // one row or one head is not stepped through: its stride may be anything
-  a.q_ts = p->rows == 1 ? 0 : p->q_token_stride;
-  a.q_hs = p->heads == 1 ? 0 : p->q_head_stride;
-  a.o_ts = p->rows == 1 ? 0 : p->out_token_stride;
-  a.o_hs = p->heads == 1 ? 0 : p->out_head_stride;
-  if ((uintptr_t)p->q % 16 || a.q_ts % 8 || a.q_hs % 8 || (uintptr_t)p->out % 16 || a.o_ts % 8 || a.o_hs % 8)
-    return set_error(FM_ERR_ALIGN, "paged_window_attn: query and output rows must be 16-byte aligned");
-  a.q = static_cast<const uint8_t*>(p->q);
-  a.cu = p->cu_seqlens_q;
-  a.T = (int)p->rows;
-  a.H = (int)p->heads;
-  a.G = (int)(p->heads / cache->kv_heads);
-  a.by_g = make_divider((uint32_t)a.G);
-  a.scale = p->softmax_scale * kLog2e;
-  a.window = p->window >= cache->max_length ? 0 : (int)p->window;  // so wide that it hides nothing
-  a.sinks = (int)p->sinks;
-  a.out = static_cast<__nv_bfloat16*>(p->out);
-  a.err = p->err;
-  const WindowPlan pl = window_plan(cache->requests, p->rows, p->heads, cache->kv_heads, cache->head_dim, p->max_q,
-                                    cache->max_length, p->window, p->sinks);
-  if (pl.total > p->workspace_bytes || (pl.total && !p->workspace))
-    return set_error(FM_ERR_WORKSPACE, "paged_window_attn: workspace %zu < %zu", p->workspace_bytes, pl.total);
-  if ((uintptr_t)p->workspace % 16) return set_error(FM_ERR_ALIGN, "paged_window_attn: workspace not 16-byte aligned");
-  if (cache->requests > WA_REQUESTS || p->rows * a.G / WA_ROWS + cache->requests > WA_ROW_TILES)
-    return set_error(FM_ERR_SHAPE, "paged_window_attn: more than %d requests or %d row tiles", WA_REQUESTS, WA_ROW_TILES);
-  uint8_t* ws = static_cast<uint8_t*>(p->workspace);
-  a.part = reinterpret_cast<float*>(ws);
-  a.stats = reinterpret_cast<float2*>(ws + pl.part);
-  a.cuts = pl.cuts ? reinterpret_cast<WaCutItem*>(ws + pl.part + pl.stats) : nullptr;
-  a.row_tiles = (int)(p->rows * a.G / WA_ROWS + cache->requests);
+  if (st == FM_OK) st = window_args(cache, p, "paged_window_attn", &a, &pl);
+  if (st != FM_OK || cache->requests == 0 || p->rows == 0) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool kv8 = cache->dtype == FM_DT_E4M3, duo = p->max_q * a.G <= 128;
-  if (cache->head_dim == 128) return kv8 ? launch_window<128, true>(a, pl, duo, s) : launch_window<128, false>(a, pl, duo, s);
-  return kv8 ? launch_window<64, true>(a, pl, duo, s) : launch_window<64, false>(a, pl, duo, s);
+  if (cache->head_dim == 128) return kv8 ? launch_window<128, 8>(a, pl, duo, s) : launch_window<128, 16>(a, pl, duo, s);
+  return kv8 ? launch_window<64, 8>(a, pl, duo, s) : launch_window<64, 16>(a, pl, duo, s);
+}
+
+extern "C" fm_status fm_paged_window_attn_fp4(const fm_paged_cache* cache, const fm_block_scales* scales,
+                                              const fm_window_attn* p, fm_stream stream) {
+  const char* who = "paged_window_attn_fp4";
+  WindowArgs a{};
+  WindowPlan pl{};
+  fm_status st = cache_ref(cache, who, &a.c, true);
+  if (st == FM_OK) st = scale_ref(cache, scales, who, &a.f);
+  if (st == FM_OK) st = window_args(cache, p, who, &a, &pl);
+  if (st != FM_OK || cache->requests == 0 || p->rows == 0) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool duo = p->max_q * a.G <= 128;
+  return cache->head_dim == 128 ? launch_window<128, 4>(a, pl, duo, s) : launch_window<64, 4>(a, pl, duo, s);
 }

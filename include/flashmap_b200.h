@@ -635,6 +635,18 @@ typedef struct fm_append {
 FM_API fm_status fm_paged_append(const fm_paged_cache* cache, const fm_block_scales* scales, const fm_append* args,
                                  fm_stream stream);
 
+/* fm_paged_decode_attn (weight_sums must be NULL) and fm_paged_window_attn on a
+ * 4-bit cache, whose values f16 holds exactly: only the softmax numerators, to
+ * f16, and the output are rounded.  The second's workspace is that of
+ * fm_paged_window_attn. */
+FM_API size_t fm_paged_decode_attn_fp4_workspace_size(int64_t requests, int64_t heads, int64_t kv_heads,
+                                                      int64_t head_dim, int64_t max_length, int64_t window,
+                                                      int64_t sinks);
+FM_API fm_status fm_paged_decode_attn_fp4(const fm_paged_cache* cache, const fm_block_scales* scales,
+                                          const fm_decode_attn* args, fm_stream stream);
+FM_API fm_status fm_paged_window_attn_fp4(const fm_paged_cache* cache, const fm_block_scales* scales,
+                                          const fm_window_attn* args, fm_stream stream);
+
 /* ------------------------------------------------------------------------
  * The whole drafter: a plan over caller-owned weights and buffers.
  * ------------------------------------------------------------------------ */
