@@ -74,138 +74,162 @@ __device__ __forceinline__ int append_request(const AppendArgs& a, int t) {
   return -1;
 }
 
-// Eight values to a thread; block (t, y) has rows y * 256 / LPR .. of token t:
-// its query heads, then keys, then values.
-template <int HD, int KIND, int ROPE>
-__global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
-  constexpr int LPR = HD / 8;
-  pdl_wait();
+// Eight values to a thread, P rows to a thread: block (t, y) has rows y * P *
+// 256 / LPR .. of token t, its query heads, then keys, then values.  The rows are
+// read before it is known whose they are: what a token waits for is the chain
+// from the row bounds to its position's cosines and its page.
+template <int HD, int KIND, int ROPE, int P>
+__global__ void __launch_bounds__(256, 4) append_kernel(AppendArgs a) {
+  constexpr int LPR = HD / 8, RPP = 256 / LPR;
   const int t = blockIdx.x, at = threadIdx.x % LPR, d0 = at * 8;
-  const int row = blockIdx.y * (256 / LPR) + threadIdx.x / LPR;
+  const int row0 = blockIdx.y * P * RPP + threadIdx.x / LPR, rows = a.H + 2 * a.c.KH;
+  const bool turned = ROPE != AP_PLAIN && d0 < a.rot;
+  const int half = a.rot / 2;
+  const bool first = d0 < half;  // of the two halves that are rotated into one another
+  pdl_wait();
+  uint4 own[P], mate[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int row = row0 + p * RPP;
+    if (row >= rows) break;
+    const __nv_bfloat16* src = row < a.H            ? a.q + t * a.q_ts + row * a.q_hs
+                               : row < a.H + a.c.KH ? a.k + t * a.k_ts + (row - a.H) * a.k_hs
+                                                    : a.v + t * a.v_ts + (row - a.H - a.c.KH) * a.v_hs;
+    own[p] = *reinterpret_cast<const uint4*>(src + d0);
+    if (ROPE == AP_HALVES && turned && row < a.H + a.c.KH)
+      mate[p] = *reinterpret_cast<const uint4*>(src + (first ? d0 + half : d0 - half));
+  }
   if (a.cu != nullptr && t == 0 && blockIdx.y == 0)  // one block looks at all bounds: those that run back give rows to nobody
     for (int i = threadIdx.x; i < a.c.R; i += 256)
       if (a.cu[i + 1] < a.cu[i]) record_error(a.err, DEV_BAD_INDEX);
   const int r = append_request(a, t);
-  if (r < 0 || row >= a.H + 2 * a.c.KH) return;
-  int j, n = 1;  // place in the cache
-  bool ok = true;
+  if (r < 0 || row0 >= rows) return;
   const int len = a.c.lengths[r];
-  j = len - 1;
+  int j = len - 1;  // place in the cache
+  bool ok = true;
   if (a.cu != nullptr) {
-    const int q0 = a.cu[r];
-    n = a.cu[r + 1] - q0;
+    const int q0 = a.cu[r], n = a.cu[r + 1] - q0;
     ok = q0 >= 0 && n <= a.T - q0 && t >= q0;
     j = len - n + (t - q0);
   }
   ok = ok && len >= 0 && len <= a.c.max_len;
   bool bad = !ok;
   ok = ok && j >= 0;
-  const bool is_q = row < a.H, is_k = !is_q && row < a.H + a.c.KH;
-  const int h = is_q ? row : is_k ? row - a.H : row - a.H - a.c.KH;
-  long long p = j;
+  long long pos = j;
   if (ROPE != AP_PLAIN && ok) {
-    if (a.pos != nullptr) p = a.pos64 ? static_cast<const long long*>(a.pos)[t] : static_cast<const int*>(a.pos)[t];
-    if (p < 0 || p >= a.rope_rows) {
+    if (a.pos != nullptr) pos = a.pos64 ? static_cast<const long long*>(a.pos)[t] : static_cast<const int*>(a.pos)[t];
+    if (pos < 0 || pos >= a.rope_rows) {
       bad = true;
       ok = false;
     }
   }
   if (bad && threadIdx.x == 0 && blockIdx.y == 0) record_error(a.err, DEV_BAD_INDEX);
   if (!ok) {
-    if (is_q) *reinterpret_cast<uint4*>(a.out + t * a.o_ts + h * a.o_hs + d0) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      if (row0 + p * RPP < a.H)
+        *reinterpret_cast<uint4*>(a.out + t * a.o_ts + (row0 + p * RPP) * a.o_hs + d0) = make_uint4(0, 0, 0, 0);
     return;
-  }
-  const __nv_bfloat16* src = is_q   ? a.q + t * a.q_ts + h * a.q_hs
-                             : is_k ? a.k + t * a.k_ts + h * a.k_hs
-                                    : a.v + t * a.v_ts + h * a.v_hs;
-  float x[8];
-  unpack8(*reinterpret_cast<const uint4*>(src + d0), x);
-  if (ROPE != AP_PLAIN && (is_q || is_k) && d0 < a.rot) {
-    const float2* cs = a.rope + p * (a.rot / 2);
-    if constexpr (ROPE == AP_HALVES) {
-      const int half = a.rot / 2;
-      const bool first = d0 < half;
-      float y[8];
-      unpack8(*reinterpret_cast<const uint4*>(src + (first ? d0 + half : d0 - half)), y);
-      const float4* c4 = reinterpret_cast<const float4*>(cs + (first ? d0 : d0 - half));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 w = c4[i];
-        const float u0 = __fmul_rn(y[2 * i], w.y), u1 = __fmul_rn(y[2 * i + 1], w.w);
-        x[2 * i] = __fadd_rn(__fmul_rn(x[2 * i], w.x), first ? -u0 : u0);
-        x[2 * i + 1] = __fadd_rn(__fmul_rn(x[2 * i + 1], w.z), first ? -u1 : u1);
-      }
-    } else {
-      const float4* c4 = reinterpret_cast<const float4*>(cs + d0 / 2);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float4 w = c4[i];
-        float* z = x + 4 * i;
-        const float a0 = z[0], a1 = z[2];
-        z[0] = __fsub_rn(__fmul_rn(a0, w.x), __fmul_rn(z[1], w.y));
-        z[1] = __fadd_rn(__fmul_rn(z[1], w.x), __fmul_rn(a0, w.y));
-        z[2] = __fsub_rn(__fmul_rn(a1, w.z), __fmul_rn(z[3], w.w));
-        z[3] = __fadd_rn(__fmul_rn(z[3], w.z), __fmul_rn(a1, w.w));
-      }
-    }
-  }
-  if (is_q) {
-    *reinterpret_cast<uint4*>(a.out + t * a.o_ts + h * a.o_hs + d0) =
-        make_uint4(pack16(x[0], x[1], false), pack16(x[2], x[3], false), pack16(x[4], x[5], false), pack16(x[6], x[7], false));
-    return;
-  }
-  if (KIND != AP_BF16 && a.c.descales != nullptr) {
-    const float d = a.c.descales[(long long)(is_k ? r : a.c.R + r) * a.c.KH + h];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __fdiv_rn(x[i], d);
-  }
-  uint32_t factor = 0;
-  if constexpr (KIND == AP_FP4) {
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
-    // the row's lanes go through here together, whichever of the warp's rows return above
-    const unsigned pair = 3u << (threadIdx.x & 30);
-    top = max_nan(top, __shfl_xor_sync(pair, top, 1));
-    factor = to_e4m3x2(__fdiv_rn(top, 6.0f), 0.0f);
-    const __half2 f2 = [&] {
-      const uint32_t b = e4m3x2_h(factor);
-      return *reinterpret_cast<const __half2*>(&b);
-    }();
-    const float f = __low2float(f2);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = f == 0.0f ? copysignf(0.0f, x[i]) : __fdiv_rn(x[i], f);
   }
   const int pg = a.c.by_page.div(j), tok = j - pg * a.c.page;
   const int page = a.c.table[(long long)r * a.c.tstride + pg];
-  if (page < 0 || page >= a.c.num_pages) {
-    record_error(a.err, DEV_BAD_INDEX);
-    return;
+  constexpr int PAIRS = ROPE == AP_HALVES ? 8 : 4;  // of this thread's values
+  float4 cs[PAIRS / 2];
+  if (turned) {
+    const float4* c4 = reinterpret_cast<const float4*>(a.rope + pos * half + (ROPE == AP_PAIRS ? d0 / 2 : first ? d0 : d0 - half));
+#pragma unroll
+    for (int i = 0; i < PAIRS / 2; ++i) cs[i] = c4[i];
   }
-  uint8_t* dst = is_k ? a.c.k + page * a.c.kps + h * a.c.khs + tok * a.c.kts
-                      : a.c.v + page * a.c.vps + h * a.c.vhs + tok * a.c.vts;
-  if constexpr (KIND == AP_BF16) {
-    *reinterpret_cast<uint4*>(dst + d0 * 2) =
-        make_uint4(pack16(x[0], x[1], false), pack16(x[2], x[3], false), pack16(x[4], x[5], false), pack16(x[6], x[7], false));
-  } else if constexpr (KIND == AP_E4M3) {
-    *reinterpret_cast<uint2*>(dst + d0) = make_uint2(to_e4m3x2(x[0], x[1]) | to_e4m3x2(x[2], x[3]) << 16,
-                                                     to_e4m3x2(x[4], x[5]) | to_e4m3x2(x[6], x[7]) << 16);
-  } else {
-    *reinterpret_cast<uint32_t*>(dst + d0 / 2) = to_e2m1x8(x);
-    uint8_t* fd = is_k ? a.f.k + page * a.f.kps + h * a.f.khs + tok * a.f.kts
-                       : a.f.v + page * a.f.vps + h * a.f.vhs + tok * a.f.vts;
-    if ((at & 1) == 0) fd[at >> 1] = (uint8_t)factor;
+  const bool there = page >= 0 && page < a.c.num_pages;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int row = row0 + p * RPP;
+    if (row >= rows) return;
+    const bool is_q = row < a.H, is_k = !is_q && row < a.H + a.c.KH;
+    const int h = is_q ? row : is_k ? row - a.H : row - a.H - a.c.KH;
+    float x[8];
+    unpack8(own[p], x);
+    if (turned && (is_q || is_k)) {
+      if constexpr (ROPE == AP_HALVES) {
+        float y[8];
+        unpack8(mate[p], y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float u0 = __fmul_rn(y[2 * i], cs[i].y), u1 = __fmul_rn(y[2 * i + 1], cs[i].w);
+          x[2 * i] = __fadd_rn(__fmul_rn(x[2 * i], cs[i].x), first ? -u0 : u0);
+          x[2 * i + 1] = __fadd_rn(__fmul_rn(x[2 * i + 1], cs[i].z), first ? -u1 : u1);
+        }
+      } else if constexpr (ROPE == AP_PAIRS) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float* z = x + 4 * i;
+          const float a0 = z[0], a1 = z[2];
+          z[0] = __fsub_rn(__fmul_rn(a0, cs[i].x), __fmul_rn(z[1], cs[i].y));
+          z[1] = __fadd_rn(__fmul_rn(z[1], cs[i].x), __fmul_rn(a0, cs[i].y));
+          z[2] = __fsub_rn(__fmul_rn(a1, cs[i].z), __fmul_rn(z[3], cs[i].w));
+          z[3] = __fadd_rn(__fmul_rn(z[3], cs[i].z), __fmul_rn(a1, cs[i].w));
+        }
+      }
+    }
+    if (is_q) {
+      *reinterpret_cast<uint4*>(a.out + t * a.o_ts + h * a.o_hs + d0) =
+          make_uint4(pack16(x[0], x[1], false), pack16(x[2], x[3], false), pack16(x[4], x[5], false), pack16(x[6], x[7], false));
+      continue;
+    }
+    if (KIND != AP_BF16 && a.c.descales != nullptr) {
+      const float d = a.c.descales[(long long)(is_k ? r : a.c.R + r) * a.c.KH + h];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __fdiv_rn(x[i], d);
+    }
+    uint32_t factor = 0;
+    if constexpr (KIND == AP_FP4) {
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
+      // both lanes of sixteen values come here together, whatever the warp's other rows do
+      const unsigned pair = 3u << (threadIdx.x & 30);
+      top = max_nan(top, __shfl_xor_sync(pair, top, 1));
+      factor = to_e4m3x2(__fdiv_rn(top, 6.0f), 0.0f);
+      const uint32_t f2 = e4m3x2_h(factor);
+      const float f = __half2float(__ushort_as_half((unsigned short)(f2 & 0xffffu)));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = f == 0.0f ? copysignf(0.0f, x[i]) : __fdiv_rn(x[i], f);
+    }
+    if (!there) {
+      record_error(a.err, DEV_BAD_INDEX);
+      continue;
+    }
+    uint8_t* dst = is_k ? a.c.k + page * a.c.kps + h * a.c.khs + tok * a.c.kts
+                        : a.c.v + page * a.c.vps + h * a.c.vhs + tok * a.c.vts;
+    if constexpr (KIND == AP_BF16) {
+      *reinterpret_cast<uint4*>(dst + d0 * 2) =
+          make_uint4(pack16(x[0], x[1], false), pack16(x[2], x[3], false), pack16(x[4], x[5], false), pack16(x[6], x[7], false));
+    } else if constexpr (KIND == AP_E4M3) {
+      *reinterpret_cast<uint2*>(dst + d0) = make_uint2(to_e4m3x2(x[0], x[1]) | to_e4m3x2(x[2], x[3]) << 16,
+                                                       to_e4m3x2(x[4], x[5]) | to_e4m3x2(x[6], x[7]) << 16);
+    } else {
+      *reinterpret_cast<uint32_t*>(dst + d0 / 2) = to_e2m1x8(x);
+      uint8_t* fd = is_k ? a.f.k + page * a.f.kps + h * a.f.khs + tok * a.f.kts
+                         : a.f.v + page * a.f.vps + h * a.f.vhs + tok * a.f.vts;
+      if ((at & 1) == 0) fd[at >> 1] = (uint8_t)factor;
+    }
   }
 }
 
+template <int HD, int KIND, int ROPE>
+fm_status launch_append(const AppendArgs& a, cudaStream_t s) {
+  constexpr int RPP = 256 / (HD / 8), P = HD == 128 ? 3 : 2;
+  const unsigned passes = (unsigned)((a.H + 2 * a.c.KH + RPP - 1) / RPP);
+  // few tokens: a row to a thread, so that more blocks share the work; many: one chain of loads for P rows
+  if ((long long)a.T * passes <= 148 * 8)
+    return launch_kernel(append_kernel<HD, KIND, ROPE, 1>, dim3((unsigned)a.T, passes), dim3(256), 0, s, true, a);
+  return launch_kernel(append_kernel<HD, KIND, ROPE, P>, dim3((unsigned)a.T, (passes + P - 1) / P), dim3(256), 0, s, true, a);
+}
 template <int HD, int KIND>
 fm_status launch_append(const AppendArgs& a, int rope, cudaStream_t s) {
-  constexpr int RPB = 256 / (HD / 8);
-  const dim3 grid((unsigned)a.T, (unsigned)((a.H + 2 * a.c.KH + RPB - 1) / RPB));
-  auto go = [&](auto kernel) { return launch_kernel(kernel, grid, dim3(256), 0, s, true, a); };
-  return rope == AP_PLAIN    ? go(append_kernel<HD, KIND, AP_PLAIN>)
-         : rope == AP_HALVES ? go(append_kernel<HD, KIND, AP_HALVES>)
-                             : go(append_kernel<HD, KIND, AP_PAIRS>);
+  return rope == AP_PLAIN    ? launch_append<HD, KIND, AP_PLAIN>(a, s)
+         : rope == AP_HALVES ? launch_append<HD, KIND, AP_HALVES>(a, s)
+                             : launch_append<HD, KIND, AP_PAIRS>(a, s);
 }
 
 }  // namespace

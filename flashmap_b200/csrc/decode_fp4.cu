@@ -79,9 +79,16 @@ __device__ __forceinline__ uint32_t d4_transpose(uint32_t x) {
   return y;
 }
 
-// NG: groups of 8 query heads (1 or 2).
-template <int HD, int NG, int STAGES>
-__global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef f) {
+// Strides in units of 16 bytes (codes) and of a row (factors), for caches
+// whose offsets in them fit 32 bits.
+struct D4Narrow {
+  uint32_t kp, kt, vp, vt, kfp, kft, vfp, vft;
+  bool same;  // one offset serves keys and values, and one their factors
+};
+
+// NG: groups of 8 query heads (1 or 2).  WIDE: offsets past what D4Narrow holds.
+template <int HD, int NG, int STAGES, bool WIDE>
+__global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef f, D4Narrow nr) {
   using Lay = D4Layout<HD, STAGES>;
   constexpr int RB = Lay::RB, SB = Lay::SB;
   constexpr int KW = HD / 32, VW = HD / 64;  // words of a thread's piece of a key, of a value
@@ -115,6 +122,7 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
   }
 
   // Query operand: head h0 + gid (and + 8), d = HD / 4 tig .. as a key's piece holds them; f16 times a power of two.
+  const float scale = a.scale * kd;
   uint32_t qb[NG][KS][2];
   float sscale[NG][2];  // of heads 2 tig, 2 tig + 1
 #pragma unroll
@@ -133,14 +141,15 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
       }
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const float up = half_row_scale(amax);
+    const float up = half_row_scale(amax), sign = scale < 0.0f ? -up : scale == 0.0f ? 0.0f : up;
 #pragma unroll
     for (int i = 0; i < KS; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        qb[n][i][e] = pack16(__uint_as_float(qb[n][i][e] << 16) * up, __uint_as_float(qb[n][i][e] & 0xffff0000u) * up, true);
-    sscale[n][0] = a.scale * kd / __shfl_sync(0xffffffffu, up, tig * 8);
-    sscale[n][1] = a.scale * kd / __shfl_sync(0xffffffffu, up, tig * 8 + 4);
+        qb[n][i][e] = pack16(__uint_as_float(qb[n][i][e] << 16) * sign, __uint_as_float(qb[n][i][e] & 0xffff0000u) * sign, true);
+    // |scale| goes with the scores, its sign (or a zero) with the queries
+    sscale[n][0] = (scale == 0.0f ? 1.0f : fabsf(scale)) / __shfl_sync(0xffffffffu, up, tig * 8);
+    sscale[n][1] = (scale == 0.0f ? 1.0f : fabsf(scale)) / __shfl_sync(0xffffffffu, up, tig * 8 + 4);
   }
 
   const uint32_t wbase = smem_u32(d4_smem_buf) + warp * Lay::WARP;
@@ -172,21 +181,33 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
       const int st = t % STAGES;
       const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
       if (lane == 0) wok[st] = ok;
-      const uint32_t sbase = wbase + st * Lay::STAGE;
-      // rows that no position stands for are zero: what the cache holds there may be no number
+      const uint32_t sbase = wbase + st * Lay::STAGE, dst = sbase + d4_sw<RB>(sub, ch);
+      // Codes are numbers whatever they are, so rows that no position stands for may be any row; their factors are zero.
       const uint32_t own = page >= 0 ? SB : 0u;
-      d4_cp_async(sbase + Lay::KF + lane * SB, page >= 0 ? kfbase + page * f.kps + tok * f.kts : kfbase, own, SB == 8);
-      d4_cp_async(sbase + Lay::VF + lane * SB, page >= 0 ? vfbase + page * f.vps + tok * f.vts : vfbase, own, SB == 8);
-      const long long koff = page >= 0 ? page * a.c.kps + tok * a.c.kts : 0;
-      const long long voff = page >= 0 ? page * a.c.vps + tok * a.c.vts : 0;
-      const uint32_t mine = ok >> sub;
+      if constexpr (WIDE) {
+        const long long koff = page >= 0 ? page * a.c.kps + tok * a.c.kts : 0;
+        const long long voff = page >= 0 ? page * a.c.vps + tok * a.c.vts : 0;
+        d4_cp_async(sbase + Lay::KF + lane * SB, page >= 0 ? kfbase + page * f.kps + tok * f.kts : kfbase, own, SB == 8);
+        d4_cp_async(sbase + Lay::VF + lane * SB, page >= 0 ? vfbase + page * f.vps + tok * f.vts : vfbase, own, SB == 8);
 #pragma unroll
-      for (int u = 0; u < D4_TILE / RPI; ++u) {
-        const long long o = __shfl_sync(0xffffffffu, koff, u * RPI + sub);
-        const long long w = a.c.same ? o : __shfl_sync(0xffffffffu, voff, u * RPI + sub);
-        const uint32_t dst = sbase + d4_sw<RB>(u * RPI + sub, ch), n = (mine >> (u * RPI)) & 1u ? 16u : 0u;
-        pc_cp_async16(dst, kbase + o, n);
-        pc_cp_async16(dst + Lay::V, vbase + w, n);
+        for (int u = 0; u < D4_TILE / RPI; ++u) {
+          const long long o = __shfl_sync(0xffffffffu, koff, u * RPI + sub), w = __shfl_sync(0xffffffffu, voff, u * RPI + sub);
+          pc_cp_async16(dst + u * RPI * RB, kbase + o, 16u);
+          pc_cp_async16(dst + Lay::V + u * RPI * RB, vbase + w, 16u);
+        }
+      } else {
+        const uint32_t pg = page >= 0 ? page : 0, tk = page >= 0 ? tok : 0;
+        const uint32_t koff = pg * nr.kp + tk * nr.kt, kfoff = pg * nr.kfp + tk * nr.kft;
+        const uint32_t voff = nr.same ? koff : pg * nr.vp + tk * nr.vt, vfoff = nr.same ? kfoff : pg * nr.vfp + tk * nr.vft;
+        d4_cp_async(sbase + Lay::KF + lane * SB, kfbase + (unsigned long long)kfoff * SB, own, SB == 8);
+        d4_cp_async(sbase + Lay::VF + lane * SB, vfbase + (unsigned long long)vfoff * SB, own, SB == 8);
+#pragma unroll
+        for (int u = 0; u < D4_TILE / RPI; ++u) {
+          const uint32_t o = __shfl_sync(0xffffffffu, koff, u * RPI + sub);
+          const uint32_t w = nr.same ? o : __shfl_sync(0xffffffffu, voff, u * RPI + sub);
+          pc_cp_async16(dst + u * RPI * RB, kbase + (unsigned long long)o * 16, 16u);
+          pc_cp_async16(dst + Lay::V + u * RPI * RB, vbase + (unsigned long long)w * 16, 16u);
+        }
       }
     }
     pc_cp_commit();
@@ -210,7 +231,8 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
   const uint32_t k_at = d4_sw<RB>(krow, tig * KB / 16) + (tig * KB) % 16;
   const uint32_t va_at = d4_sw<RB>(va, gid * VB / 16) + (gid * VB) % 16;
   const uint32_t vb_at = d4_sw<RB>(vb, gid * VB / 16) + (gid * VB) % 16;
-  const int vf = gid * HD / 128;  // the factor of a value's piece
+  const uint32_t kf_at = Lay::KF + krow * SB + tig * (SB / 4);
+  const uint32_t vfa_at = Lay::VF + va * SB + gid * HD / 128, vfb_at = Lay::VF + vb * SB + gid * HD / 128;
 
   for (int t = 0; t < ntiles; ++t) {
     issue(t + STAGES - 1);
@@ -218,24 +240,24 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
     __syncwarp();
     const uint32_t sb = wbase + (t % STAGES) * Lay::STAGE;
     const uint32_t ok = wok[t % STAGES];
+    float sc[2][NG][4];  // of 16 keys each: keys gid, gid, gid + 8, gid + 8 of heads 2 tig, 2 tig + 1
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {  // 16 keys each
-      float sc[NG][4];  // keys gid, gid, gid + 8, gid + 8 of heads 2 tig, 2 tig + 1
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-      for (int n = 0; n < NG; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+      for (int n = 0; n < NG; ++n) sc[half][n][0] = sc[half][n][1] = sc[half][n][2] = sc[half][n][3] = 0.0f;
       uint32_t ka[KW], kb[KW], fa[2], fb[2];
       d4_lds<KW>(sb + k_at + half * 16 * RB, ka);
       d4_lds<KW>(sb + k_at + (half * 16 + 8) * RB, kb);
       if constexpr (HD == 128) {  // two factors to a piece
-        const uint32_t ea = e4m3x2_h(d4_lds16(sb + Lay::KF + (half * 16 + krow) * SB + 2 * tig));
-        const uint32_t eb = e4m3x2_h(d4_lds16(sb + Lay::KF + (half * 16 + 8 + krow) * SB + 2 * tig));
+        const uint32_t ea = e4m3x2_h(d4_lds16(sb + kf_at + half * 16 * SB));
+        const uint32_t eb = e4m3x2_h(d4_lds16(sb + kf_at + (half * 16 + 8) * SB));
         fa[0] = __byte_perm(ea, 0, 0x1010);
         fa[1] = __byte_perm(ea, 0, 0x3232);
         fb[0] = __byte_perm(eb, 0, 0x1010);
         fb[1] = __byte_perm(eb, 0, 0x3232);
       } else {
-        fa[0] = fa[1] = e4m3x2_h(d4_lds8(sb + Lay::KF + (half * 16 + krow) * SB + tig) * 0x101u);
-        fb[0] = fb[1] = e4m3x2_h(d4_lds8(sb + Lay::KF + (half * 16 + 8 + krow) * SB + tig) * 0x101u);
+        fa[0] = fa[1] = e4m3x2_h(d4_lds8(sb + kf_at + half * 16 * SB) * 0x101u);
+        fb[0] = fb[1] = e4m3x2_h(d4_lds8(sb + kf_at + (half * 16 + 8) * SB) * 0x101u);
       }
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
@@ -251,49 +273,64 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
         for (int e = 0; e < 2; ++e)
 #pragma unroll
           for (int n = 0; n < NG; ++n)
-            mma16816<true>(sc[n], xa[2 * e], xb[2 * e], xa[2 * e + 1], xb[2 * e + 1], qb[n][2 * w + e][0], qb[n][2 * w + e][1]);
+            mma16816<true>(sc[half][n], xa[2 * e], xb[2 * e], xa[2 * e + 1], xb[2 * e + 1], qb[n][2 * w + e][0],
+                           qb[n][2 * w + e][1]);
       }
-      const uint32_t seen = ok >> (half * 16 + krow);
-      uint32_t pb[NG][2];
+    }
+    if (ok != 0xffffffffu) {
+      const uint32_t seen = ok >> krow;
 #pragma unroll
-      for (int n = 0; n < NG; ++n) {
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[n][e] = (seen >> (e & 2 ? 8 : 0)) & 1u ? sc[n][e] * sscale[n][e & 1] : -INFINITY;
-        const float top0 = fmaxf(sc[n][0], sc[n][2]), top1 = fmaxf(sc[n][1], sc[n][3]);
-        // m is the maximum less the lift, and moves when a score outgrows it by the lag
-        if (__any_sync(0xffffffffu, top0 > m[n][0] + (D4_LIFT + D4_LAG) || top1 > m[n][1] + (D4_LIFT + D4_LAG))) {
+        for (int n = 0; n < NG; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float mx = e ? top1 : top0;
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float mn = fmaxf(m[n][e], mx - D4_LIFT);
-            const float al = mn == -INFINITY ? 1.0f : ex2(m[n][e] - mn);
-            m[n][e] = mn;
-            l[n][e] *= al;
+          for (int e = 0; e < 4; ++e)
+            sc[half][n][e] = (seen >> (half * 16 + (e & 2) * 4)) & 1u ? sc[half][n][e] : -INFINITY;
+    }
+    uint32_t pb[2][NG][2];
 #pragma unroll
-            for (int i = 0; i < KS; ++i) {
-              o[n][i][e] *= al;
-              o[n][i][2 + e] *= al;
-            }
+    for (int n = 0; n < NG; ++n) {
+      const float top0 = fmaxf(fmaxf(sc[0][n][0], sc[0][n][2]), fmaxf(sc[1][n][0], sc[1][n][2])) * sscale[n][0];
+      const float top1 = fmaxf(fmaxf(sc[0][n][1], sc[0][n][3]), fmaxf(sc[1][n][1], sc[1][n][3])) * sscale[n][1];
+      // m is the maximum less the lift, and moves when a score outgrows it by the lag
+      if (__any_sync(0xffffffffu, top0 > m[n][0] + (D4_LIFT + D4_LAG) || top1 > m[n][1] + (D4_LIFT + D4_LAG))) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = e ? top1 : top0;
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float mn = fmaxf(m[n][e], mx - D4_LIFT);
+          const float al = mn == -INFINITY ? 1.0f : ex2(m[n][e] - mn);
+          m[n][e] = mn;
+          l[n][e] *= al;
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            o[n][i][e] *= al;
+            o[n][i][2 + e] *= al;
           }
         }
-        const float u0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], u1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];
-        const float p0 = ex2(sc[n][0] - u0), p1 = ex2(sc[n][1] - u1), p2 = ex2(sc[n][2] - u0), p3 = ex2(sc[n][3] - u1);
+      }
+      const float u0 = m[n][0] == -INFINITY ? 0.0f : -m[n][0], u1 = m[n][1] == -INFINITY ? 0.0f : -m[n][1];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float p0 = ex2(fmaf(sc[half][n][0], sscale[n][0], u0)), p1 = ex2(fmaf(sc[half][n][1], sscale[n][1], u1));
+        const float p2 = ex2(fmaf(sc[half][n][2], sscale[n][0], u0)), p3 = ex2(fmaf(sc[half][n][3], sscale[n][1], u1));
         l[n][0] += p0 + p2;
         l[n][1] += p1 + p3;
-        pb[n][0] = d4_transpose(pack16(p0, p1, true));  // keys 2 tig, 2 tig + 1 of head gid
-        pb[n][1] = d4_transpose(pack16(p2, p3, true));
+        pb[half][n][0] = d4_transpose(pack16(p0, p1, true));  // keys 2 tig, 2 tig + 1 of head gid
+        pb[half][n][1] = d4_transpose(pack16(p2, p3, true));
       }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
       uint32_t x[2][4 * VW], y[2][4 * VW];  // values 2 i, and 2 i + 1, of a pair of keys
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         uint32_t wa[VW], wb[VW];
         d4_lds<VW>(sb + Lay::V + va_at + (half * 16 + q * 8) * RB, wa);
         d4_lds<VW>(sb + Lay::V + vb_at + (half * 16 + q * 8) * RB, wb);
-        const uint32_t s2 = e4m3x2_h(d4_lds8(sb + Lay::VF + (half * 16 + q * 8 + va) * SB + vf) |
-                                     d4_lds8(sb + Lay::VF + (half * 16 + q * 8 + vb) * SB + vf) << 8);
+        const uint32_t s2 = e4m3x2_h(d4_lds8(sb + vfa_at + (half * 16 + q * 8) * SB) | d4_lds8(sb + vfb_at + (half * 16 + q * 8) * SB) << 8);
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
           e2m1x8_h((wa[w] & 0x0f0f0f0fu) | ((wb[w] << 4) & 0xf0f0f0f0u), &x[q][4 * w]);
@@ -308,7 +345,7 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll
-        for (int n = 0; n < NG; ++n) mma16816<true>(o[n][i], x[0][i], y[0][i], x[1][i], y[1][i], pb[n][0], pb[n][1]);
+        for (int n = 0; n < NG; ++n) mma16816<true>(o[n][i], x[0][i], y[0][i], x[1][i], y[1][i], pb[half][n][0], pb[half][n][1]);
     }
     __syncwarp();  // the stage may be refilled from here on
   }
@@ -376,12 +413,25 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
   }
 }
 
-template <int HD, int NG>
-fm_status launch_decode_fp4(const DecodeArgs& a, const ScaleRef& f, unsigned grid, cudaStream_t s) {
+template <int HD, int NG, bool WIDE>
+fm_status launch_decode_fp4(const DecodeArgs& a, const ScaleRef& f, const D4Narrow& nr, unsigned grid, cudaStream_t s) {
   constexpr int STAGES = 2, smem = d4_smem<HD, NG, STAGES>();
-  const fm_status st = allow_smem<decode_fp4_kernel<HD, NG, STAGES>>(smem, "paged_decode_attn_fp4");
+  const fm_status st = allow_smem<decode_fp4_kernel<HD, NG, STAGES, WIDE>>(smem, "paged_decode_attn_fp4");
   if (st != FM_OK) return st;
-  return launch_kernel(decode_fp4_kernel<HD, NG, STAGES>, dim3(grid), dim3(128), smem, s, true, a, f);
+  return launch_kernel(decode_fp4_kernel<HD, NG, STAGES, WIDE>, dim3(grid), dim3(128), smem, s, true, a, f, nr);
+}
+template <int HD, bool WIDE>
+fm_status launch_decode_fp4(const DecodeArgs& a, const ScaleRef& f, const D4Narrow& nr, int ng, unsigned grid, cudaStream_t s) {
+  return ng == 2 ? launch_decode_fp4<HD, 2, WIDE>(a, f, nr, grid, s) : launch_decode_fp4<HD, 1, WIDE>(a, f, nr, grid, s);
+}
+
+// Whether pages' and tokens' offsets in units of `unit` bytes fit 32 bits.
+bool d4_fits(const CacheRef& c, long long ps, long long ts, long long unit, uint32_t* p, uint32_t* t) {
+  if (ps < 0 || ts < 0 || ps / unit > 0xffffffffll || ts / unit > 0xffffffffll) return false;
+  const double most = (double)(c.num_pages > 0 ? c.num_pages - 1 : 0) * (double)ps + (double)(c.page - 1) * (double)ts;
+  *p = (uint32_t)(ps / unit);
+  *t = (uint32_t)(ts / unit);
+  return most / (double)unit < 4.0e9;
 }
 
 }  // namespace
@@ -415,9 +465,14 @@ extern "C" fm_status fm_paged_decode_attn_fp4(const fm_paged_cache* cache, const
   if (items * pl.chunks > 0x7fffffff || join.blocks > 0x7fffffff) return set_error(FM_ERR_SHAPE, "%s: grid too large", who);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const unsigned grid = (unsigned)(items * pl.chunks);
+  const long long row = cache->head_dim / 16;
+  D4Narrow nr{};
+  const bool narrow = d4_fits(a.c, a.c.kps, a.c.kts, 16, &nr.kp, &nr.kt) && d4_fits(a.c, a.c.vps, a.c.vts, 16, &nr.vp, &nr.vt) &&
+                      d4_fits(a.c, f.kps, f.kts, row, &nr.kfp, &nr.kft) && d4_fits(a.c, f.vps, f.vts, row, &nr.vfp, &nr.vft);
+  nr.same = nr.kp == nr.vp && nr.kt == nr.vt && nr.kfp == nr.vfp && nr.kft == nr.vft;
   if (cache->head_dim == 128)
-    st = pl.ng == 2 ? launch_decode_fp4<128, 2>(a, f, grid, s) : launch_decode_fp4<128, 1>(a, f, grid, s);
+    st = narrow ? launch_decode_fp4<128, false>(a, f, nr, pl.ng, grid, s) : launch_decode_fp4<128, true>(a, f, nr, pl.ng, grid, s);
   else
-    st = pl.ng == 2 ? launch_decode_fp4<64, 2>(a, f, grid, s) : launch_decode_fp4<64, 1>(a, f, grid, s);
+    st = narrow ? launch_decode_fp4<64, false>(a, f, nr, pl.ng, grid, s) : launch_decode_fp4<64, true>(a, f, nr, pl.ng, grid, s);
   return st != FM_OK ? st : launch_decode_join(a, join, cache->head_dim, s);
 }

@@ -10,13 +10,15 @@
 // d is formed with one rounding and every m is the same rounded product
 // wherever it is used, so that the rounding of m cancels.
 //
-// Alternatives.  The pass also leaves the maximum of every group of GM warp
-// loads (512 bytes each).  The k largest values, equal ones by the lowest id, lie in the
+// Alternatives.  The pass also leaves the maximum of every group of one or more
+// warp loads (512 bytes each).  The k largest values, equal ones by the lowest id, lie in the
 // k groups that come first by (maximum, lowest group): an element of another
 // group is preceded by the k maxima of those.  Those groups are read once more
 // (from L2), what reaches the k-th maximum is kept, and sorted.
 //
 // The row's bytes bound it (one exponential, and five other operations to a value).
+#include <type_traits>
+
 #include "common.cuh"
 #include "launch.cuh"
 
@@ -35,7 +37,7 @@ struct LogprobArgs {
   int V, rows;
   const long long* tokens;
   float c;         // log2(e) / T
-  int k, gm;       // gm: warp loads of a group
+  int k, gs;       // 2^gs warp loads make a group
   int groups;      // room for a row's group maxima
   int slices, per; // CTAs of a row, warp loads of each
   float* logprob;
@@ -95,14 +97,17 @@ __device__ __forceinline__ void lp_unpack(const uint4& u, float* x) {
     }
   }
 }
+// the largest and the least of a piece, NaN left out
 template <typename T>
-__device__ __forceinline__ float lp_max(const uint4& u) {  // the largest, NaN left out
+__device__ __forceinline__ float2 lp_range(const uint4& u) {
   if constexpr (sizeof(T) == 2) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
     const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-    return fmaxf(__low2float(m), __high2float(m));
+    const __nv_bfloat162 l = __hmin2(__hmin2(h[0], h[1]), __hmin2(h[2], h[3]));
+    return make_float2(fmaxf(__low2float(m), __high2float(m)), fminf(__low2float(l), __high2float(l)));
   } else {
-    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+    const float x[4] = {__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w)};
+    return make_float2(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fminf(fminf(x[0], x[1]), fminf(x[2], x[3])));
   }
 }
 
@@ -148,9 +153,10 @@ __device__ __forceinline__ float lp_key_value(unsigned long long key) {
 __device__ __forceinline__ unsigned long long lp_key(float v, uint32_t i) { return argmax_key(v != v ? -INFINITY : v, i); }
 
 struct LpShared {
-  unsigned long long keys[LP_LIST];  // groups first, then candidates
+  unsigned long long keys[LP_LIST];  // the warps' first groups, then candidates
   float gmax[LP_GROUPS];
   int chosen[32];
+  float least;
   LpSum warp[LP_T / 32];
   unsigned long long best[LP_T / 32];
   int count;
@@ -175,20 +181,47 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
     a.entropy[row] = none ? 0.0f : LP_LN2 * (log_s - all.u / all.s);
   }
   if (a.k == 0) return;
-  const int loads = (x.pieces + 31) / 32, groups = (loads + a.gm - 1) / a.gm;
-  int n = 2;
-  while (n < groups) n <<= 1;
-  for (int g = tid; g < n; g += LP_T) sh.keys[g] = g < groups ? lp_key(gmax[g], (uint32_t)g) : 0ull;
-  lp_sort(sh.keys, n);
+  const int loads = (x.pieces + 31) / 32, groups = (loads + (1 << a.gs) - 1) >> a.gs;
+  // Every warp draws the k first of its 128 groups, four to a lane; of those the k first stand behind fewer than k others.
+  constexpr int W = LP_T / 32, PER = LP_GROUPS / LP_T;
+  uint32_t mine[PER];  // orderable maxima of groups (warp * PER + j) * 32 + lane; 0: none
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int g = (warp * PER + j) * 32 + lane;
+    mine[j] = g < groups ? (uint32_t)(lp_key(gmax[g], 0) >> 32) : 0u;
+  }
+  for (int i = 0; i < a.k; ++i) {
+    uint32_t best = mine[0];
+#pragma unroll
+    for (int j = 1; j < PER; ++j) best = max(best, mine[j]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    uint32_t at = 0xffffffffu;
+#pragma unroll
+    for (int j = PER - 1; j >= 0; --j) at = mine[j] == best ? (uint32_t)((warp * PER + j) * 32 + lane) : at;
+    at = __reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (at == (uint32_t)((warp * PER + j) * 32 + lane)) mine[j] = 0u;
+    if (lane == 0) sh.keys[warp * a.k + i] = best ? (unsigned long long)best << 32 | (0xffffffffu - at) : 0ull;
+  }
+  __syncthreads();
   const int take = min(a.k, groups);
-  const float least = take < a.k ? -INFINITY : lp_key_value(sh.keys[take - 1]);
-  if (tid < take) sh.chosen[tid] = (int)argmax_key_index(sh.keys[tid]);
+  for (int i = tid; i < W * a.k; i += LP_T) {
+    const unsigned long long key = sh.keys[i];
+    int before = 0;
+    for (int j = 0; j < W * a.k; ++j) before += sh.keys[j] > key;
+    if (key && before < take) {
+      sh.chosen[before] = (int)argmax_key_index(key);
+      if (before == take - 1) sh.least = lp_key_value(key);
+    }
+  }
   if (tid == 0) sh.count = 0;
   __syncthreads();
+  const float least = take < a.k ? -INFINITY : sh.least;
   // the chosen groups once more: values that reach the k-th maximum
   auto each = [&](auto&& f) {
-    for (int i = warp; i < take * a.gm; i += LP_T / 32) {
-      const int p = (sh.chosen[i / a.gm] * a.gm + i % a.gm) * 32 + lane;
+    for (int i = warp; i < take << a.gs; i += LP_T / 32) {
+      const int p = ((sh.chosen[i >> a.gs] << a.gs) + (i & ((1 << a.gs) - 1))) * 32 + lane;
       if (p >= x.pieces) continue;
       float v[LpRow<T>::N];
       lp_unpack<T>(x.load(p), v);
@@ -206,8 +239,18 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
   });
   __syncthreads();
   const int count = sh.count;
+  if (count <= LP_T) {  // as a rule: a candidate to a thread, which counts those before it
+    const unsigned long long key = tid < count ? sh.keys[tid] : 0ull;
+    int before = 0;
+    for (int j = 0; j < count; ++j) before += sh.keys[j] > key;
+    if (tid < count && before < a.k) {
+      a.ids[(long long)row * a.k + before] = argmax_key_index(key);
+      a.top[(long long)row * a.k + before] = logprob(lp_key_value(key));
+    }
+    return;
+  }
   if (count <= LP_LIST) {
-    n = 2;
+    int n = 2;
     while (n < count) n <<= 1;
     for (int i = count + tid; i < n; i += LP_T) sh.keys[i] = 0ull;
     lp_sort(sh.keys, n);
@@ -258,9 +301,10 @@ __device__ __forceinline__ LpSum lp_block_join(LpSum v, LpShared& sh) {
   return v;
 }
 
-// Block (row, slice): warp loads slice * per .. of the row.
-template <typename T>
-__global__ void __launch_bounds__(LP_T) logprob_scan_kernel(LogprobArgs a) {
+// Block (row, slice): warp loads slice * per .. of the row.  ONE: a warp load is
+// a group of its own.
+template <typename T, bool TOP, bool ONE>
+__global__ void __launch_bounds__(LP_T, 4) logprob_scan_kernel(LogprobArgs a) {
   __shared__ LpShared sh;
   pdl_wait();
   const int row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
@@ -268,53 +312,103 @@ __global__ void __launch_bounds__(LP_T) logprob_scan_kernel(LogprobArgs a) {
   const LpRow<T> x(a, row);
   constexpr int N = LpRow<T>::N;
   const int loads = (x.pieces + 31) / 32, end = min(loads, (slice + 1) * a.per);
-  const int span = max(LP_LOADS, a.gm);  // a warp's loads at a time hold whole groups
+  const int span = ONE ? LP_LOADS : max(LP_LOADS, 1 << a.gs);  // a warp's loads at a time hold whole groups
   float* gmax = a.slices == 1 ? sh.gmax : a.gmax + (long long)row * a.groups;
   const uint4 nothing = sizeof(T) == 2 ? make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u)
                                        : make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
-  LpSum v{-INFINITY, 0.0f, 0.0f};
-  for (int l0 = slice * a.per + warp * span; l0 < end; l0 += LP_T / 32 * span) {
-    float gm = -INFINITY;
-    for (int l1 = l0; l1 < l0 + span; l1 += LP_LOADS) {  // past the row's end there is nothing, but a group is still closed
-      uint4 u[LP_LOADS];
+  const int whole = x.shift ? 1 : 0, whole_end = (a.V + x.shift) / N;  // pieces that lie in the row altogether
+  const uint4* base = reinterpret_cast<const uint4*>(x.x - x.shift) + lane;
+  auto fetch = [&](uint4* u, int l1) {
+    if (l1 * 32 >= whole && (l1 + LP_LOADS) * 32 <= whole_end) {
+#pragma unroll
+      for (int q = 0; q < LP_LOADS; ++q) u[q] = __ldcs(base + (l1 + q) * 32);
+    } else {
 #pragma unroll
       for (int q = 0; q < LP_LOADS; ++q) {
         const int p = (l1 + q) * 32 + lane;
         u[q] = p < x.pieces ? x.load(p) : nothing;
       }
-      float mx[LP_LOADS], top = -INFINITY;
+    }
+  };
+  // the warp's batches: LP_LOADS loads each, span after span
+  auto after = [&](int l1) { return ((l1 + LP_LOADS) & (span - 1)) ? l1 + LP_LOADS : l1 + LP_LOADS + (LP_T / 32 - 1) * span; };
+  LpSum v{-INFINITY, 0.0f, 0.0f};
+  const float2 c2 = make_float2(a.c, a.c);
+  uint4 next[LP_LOADS];
+  float gm = -INFINITY;
+  // A span is gone through to its end: behind the row there is nothing, but a group is still closed.
+  const int stop = (end + span - 1) & ~(span - 1);
+  int l1 = slice * a.per + warp * span;
+  if (l1 < stop) fetch(next, l1);
+  while (l1 < stop) {
+    uint4 u[LP_LOADS];
 #pragma unroll
-      for (int q = 0; q < LP_LOADS; ++q) top = fmaxf(top, mx[q] = lp_max<T>(u[q]));
-      top *= a.c;
-      if (top > v.m) {
-        if (v.m != -INFINITY) {
-          const float d = fmaxf(v.m - top, -1000.0f), f = lp_ex2(d);
-          v.u = f * (v.u + d * v.s);
-          v.s *= f;
-        }
-        v.m = top;
+    for (int q = 0; q < LP_LOADS; ++q) u[q] = next[q];
+    const int l2 = after(l1);
+    if (l2 < stop) fetch(next, l2);
+    float mx[LP_LOADS], top = -INFINITY, low = INFINITY;
+#pragma unroll
+    for (int q = 0; q < LP_LOADS; ++q) {
+      const float2 range = lp_range<T>(u[q]);
+      mx[q] = range.x;
+      top = fmaxf(top, range.x);
+      low = fminf(low, range.y);
+    }
+    top *= a.c;
+    if (top > v.m) {
+      if (v.m != -INFINITY) {
+        const float d = fmaxf(v.m - top, -1000.0f), f = lp_ex2(d);
+        v.u = f * (v.u + d * v.s);
+        v.s *= f;
       }
-      const float off = v.m == -INFINITY ? 0.0f : v.m;
+      v.m = top;
+    }
+    const float off = v.m == -INFINITY ? 0.0f : v.m;
+    // 2^d d is 0 where d is -inf; where no value is so low that d could be, it needs no guard
+    const bool guard = __any_sync(0xffffffffu, !(low * a.c - off > -1e30f));
+    float2 s2 = make_float2(v.s, 0.0f), u2 = make_float2(v.u, 0.0f);
+    const float2 o2 = make_float2(-off, -off);
+    auto add = [&](auto guarded) {
 #pragma unroll
       for (int q = 0; q < LP_LOADS; ++q) {
         float y[N];
         lp_unpack<T>(u[q], y);
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float d = fmaf(y[e], a.c, -off), p = lp_ex2(d);
-          v.s += p;
-          v.u = fmaf(p, fmaxf(d, -1000.0f), v.u);
+        for (int e = 0; e < N; e += 2) {
+          float2 d = __ffma2_rn(make_float2(y[e], y[e + 1]), c2, o2);
+          const float2 p = make_float2(lp_ex2(d.x), lp_ex2(d.y));
+          s2 = __fadd2_rn(s2, p);
+          if constexpr (decltype(guarded)::value) d = make_float2(fmaxf(d.x, -1000.0f), fmaxf(d.y, -1000.0f));
+          u2 = __ffma2_rn(p, d, u2);
         }
-        if (a.k) {
-          gm = fmaxf(gm, mx[q]);
-          if (((l1 + q + 1) & (a.gm - 1)) == 0) {
-            const float g = lp_warp_max(gm);
-            if (lane == 0 && l1 + q - (a.gm - 1) < loads) gmax[(l1 + q) / a.gm] = g;
-            gm = -INFINITY;
-          }
+      }
+    };
+    if (guard)
+      add(std::true_type{});
+    else
+      add(std::false_type{});
+    v.s = s2.x + s2.y;
+    v.u = u2.x + u2.y;
+    if constexpr (TOP && ONE) {
+      float mine = lp_warp_max(mx[0]);
+#pragma unroll
+      for (int q = 1; q < LP_LOADS; ++q) {
+        const float g = lp_warp_max(mx[q]);
+        mine = lane == q ? g : mine;
+      }
+      if (lane < LP_LOADS && l1 + lane < loads) gmax[l1 + lane] = mine;
+    } else if constexpr (TOP) {
+#pragma unroll
+      for (int q = 0; q < LP_LOADS; ++q) {
+        gm = fmaxf(gm, mx[q]);
+        if (((l1 + q + 1) & ((1 << a.gs) - 1)) == 0) {
+          const float g = lp_warp_max(gm);
+          if (lane == 0 && l1 + q + 1 - (1 << a.gs) < loads) gmax[(l1 + q) >> a.gs] = g;
+          gm = -INFINITY;
         }
       }
     }
+    l1 = l2;
   }
   v = lp_block_join(v, sh);
   if (a.slices > 1) {
@@ -339,16 +433,15 @@ __global__ void __launch_bounds__(LP_T) logprob_join_kernel(LogprobArgs a) {
 }
 
 struct LogprobPlan {
-  int gm, groups, slices, per;
+  int gs, groups, slices, per;
   size_t part, total;
 };
 LogprobPlan logprob_plan(int64_t rows, int64_t V, int64_t esz, int64_t k) {
   LogprobPlan p{};
   const int64_t load = 512 / esz, loads = (V + 16 / esz - 1 + load - 1) / load + 1;
-  p.gm = 1;
-  while ((loads + p.gm - 1) / p.gm > LP_GROUPS) p.gm <<= 1;
-  p.groups = (int)((loads + p.gm - 1) / p.gm);
-  const int64_t span = p.gm > LP_LOADS ? p.gm : LP_LOADS, least = span * (LP_T / 32);
+  while (((loads - 1) >> p.gs) + 1 > LP_GROUPS) ++p.gs;
+  p.groups = (int)(((loads - 1) >> p.gs) + 1);
+  const int64_t span = 1 << p.gs > LP_LOADS ? 1 << p.gs : LP_LOADS, least = span * (LP_T / 32);
   int64_t slices = (4 * num_sms() + rows - 1) / rows;
   const int64_t most = (loads + least - 1) / least;
   if (slices > most) slices = most;
@@ -361,7 +454,8 @@ LogprobPlan logprob_plan(int64_t rows, int64_t V, int64_t esz, int64_t k) {
 
 template <typename T>
 fm_status launch_logprobs(const LogprobArgs& a, cudaStream_t s) {
-  const fm_status st = launch_kernel(logprob_scan_kernel<T>, dim3((unsigned)(a.rows * (int64_t)a.slices)), dim3(LP_T), 0, s, true, a);
+  auto kernel = a.k == 0 ? logprob_scan_kernel<T, false, true> : a.gs == 0 ? logprob_scan_kernel<T, true, true> : logprob_scan_kernel<T, true, false>;
+  const fm_status st = launch_kernel(kernel, dim3((unsigned)(a.rows * (int64_t)a.slices)), dim3(LP_T), 0, s, true, a);
   if (st != FM_OK || a.slices == 1) return st;
   return launch_kernel(logprob_join_kernel<T>, dim3((unsigned)a.rows), dim3(LP_T), 0, s, true, a);
 }
@@ -406,7 +500,7 @@ extern "C" fm_status fm_token_logprobs(const void* logits, int32_t dtype, int64_
   a.tokens = reinterpret_cast<const long long*>(tokens);
   a.c = LP_LOG2E / temperature;
   a.k = (int)top_k;
-  a.gm = pl.gm;
+  a.gs = pl.gs;
   a.groups = pl.groups;
   a.slices = pl.slices;
   a.per = pl.per;

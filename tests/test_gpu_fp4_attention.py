@@ -279,12 +279,22 @@ def test_strides_streams_graphs_and_far_pages():
         close(a, want, mag, "decode")
         if min(lengths):
             close(b, want, mag, "window")
-    # pages, and pages of factors, whose offset passes 32 bits
+    assert error_word() == 0
+
+
+@pytest.mark.parametrize("reach", [2_200_000_000, 8_600_000_000])  # offsets past 32 bits in bytes, and in rows of factors
+def test_far_pages(reach):
+    g = torch.Generator().manual_seed(57)
+    D, KH, page = 64, 2, 16
+    cache = Cache(g, [130, 50], KH, D, page, "joint")
+    wide = torch.randn(2, 4, 3, D, generator=g).to(torch.bfloat16)
+    q = wide.to(DEV)[:, :, 1]
+    cu = torch.arange(3, dtype=torch.int32, device=DEV)
     stride = 2_200_000_000
-    pool = torch.zeros(2 * stride + KH * page * D, dtype=torch.uint8, device=DEV)
+    pool = torch.empty(2 * stride + KH * page * D, dtype=torch.uint8, device=DEV)
     far = pool.as_strided((3, KH, page, D), (stride, page * D, D, 1))
-    factors = torch.zeros(2 * stride + KH * page * D // 8, dtype=torch.uint8, device=DEV)
-    far_f = factors.as_strided((3, KH, page, D // 8), (stride, page * D // 8, D // 8, 1))
+    factors = torch.empty(2 * reach + KH * page * D // 8, dtype=torch.uint8, device=DEV)
+    far_f = factors.as_strided((3, KH, page, D // 8), (reach, page * D // 8, D // 8, 1))
     used = cache.table[1, :3].long().to(DEV)
     far.copy_(cache.dev[0][0][used])
     far_f.copy_(cache.dev[0][1].view(torch.uint8)[used])
