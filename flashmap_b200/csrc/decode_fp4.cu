@@ -13,12 +13,25 @@
 // (in S) and of d (in O) may be chosen: a thread takes 16 consecutive
 // bytes of a key, and 8 of a value, as they lie.  Values of two keys
 // are paired for V^T by exchanging half bytes before the conversion.
+#include <type_traits>
+
 #include "decode_parts.cuh"
 
 namespace fm {
 namespace {
 
 constexpr int D4_TILE = 32;  // keys of a warp's tile
+// A CTA's first copies and its merge weigh more against 4-bit keys: one long
+// request is cut into as many chunks as CTAs are resident (100003 positions,
+// 8 kv heads: 34 us, and 40 us in three times as many), and a batch into chunks
+// of 2048 keys (128 requests of 1024 .. 8192: 163 us; of 1024 keys 173 us, of 4096 170 us).
+#ifndef RL
+#define RL 1536
+#endif
+#ifndef RM
+#define RM 2048
+#endif
+constexpr DecodeRule D4_RULE{148 * 4, 128, RL, RM, 148 * 32};
 
 // P goes to f16 times 2^11, and the subtracted maximum may lag behind the true
 // one by a factor 2^4: numerators stay below 2^15, and only those under 2^-25 of
@@ -115,42 +128,6 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
   }
   const int begin = chunk * size, end = min(sp.n, begin + size);
 
-  float kd = 1.0f, vd = 1.0f;
-  if (a.c.descales) {
-    kd = a.c.descales[(long long)r * a.c.KH + c];
-    vd = a.c.descales[(long long)(a.c.R + r) * a.c.KH + c];
-  }
-
-  // Query operand: head h0 + gid (and + 8), d = HD / 4 tig .. as a key's piece holds them; f16 times a power of two.
-  const float scale = a.scale * kd;
-  uint32_t qb[NG][KS][2];
-  float sscale[NG][2];  // of heads 2 tig, 2 tig + 1
-#pragma unroll
-  for (int n = 0; n < NG; ++n) {
-    const bool live = gid + 8 * n < nh;
-    const __nv_bfloat16* row = reinterpret_cast<const __nv_bfloat16*>(a.q) + (long long)r * a.q_rs +
-                               (long long)(h0 + (live ? gid + 8 * n : 0)) * a.q_hs + tig * (HD / 4);
-    float amax = 0.0f;
-#pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t w = live ? *reinterpret_cast<const uint32_t*>(row + 4 * i + 2 * e) : 0u;
-        qb[n][i][e] = w;
-        amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u))));
-      }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const float up = half_row_scale(amax), sign = scale < 0.0f ? -up : scale == 0.0f ? 0.0f : up;
-#pragma unroll
-    for (int i = 0; i < KS; ++i)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        qb[n][i][e] = pack16(__uint_as_float(qb[n][i][e] << 16) * sign, __uint_as_float(qb[n][i][e] & 0xffff0000u) * sign, true);
-    // |scale| goes with the scores, its sign (or a zero) with the queries
-    sscale[n][0] = (scale == 0.0f ? 1.0f : fabsf(scale)) / __shfl_sync(0xffffffffu, up, tig * 8);
-    sscale[n][1] = (scale == 0.0f ? 1.0f : fabsf(scale)) / __shfl_sync(0xffffffffu, up, tig * 8 + 4);
-  }
 
   const uint32_t wbase = smem_u32(d4_smem_buf) + warp * Lay::WARP;
   uint32_t* wok = reinterpret_cast<uint32_t*>(d4_smem_buf + d4_smem<HD, NG, STAGES>() - 4 * STAGES * 4) + warp * STAGES;
@@ -174,11 +151,10 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
   const uint8_t* vbase = a.c.v + (long long)c * a.c.vhs + ch * 16;
   const uint8_t* kfbase = f.k + (long long)c * f.khs;
   const uint8_t* vfbase = f.v + (long long)c * f.vhs;
-  auto issue = [&](int t) {
+  auto issue = [&](int t, int st) {
     if (t < ntiles) {
       const int page = page_next, tok = tok_next;
       page_next = lookup(t + 1, &tok_next);
-      const int st = t % STAGES;
       const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
       if (lane == 0) wok[st] = ok;
       const uint32_t sbase = wbase + st * Lay::STAGE, dst = sbase + d4_sw<RB>(sub, ch);
@@ -213,7 +189,44 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
     pc_cp_commit();
   };
 #pragma unroll
-  for (int t = 0; t < STAGES - 1; ++t) issue(t);
+  for (int t = 0; t < STAGES - 1; ++t) issue(t, t);
+
+  // while the first tile is on its way
+  float kd = 1.0f, vd = 1.0f;
+  if (a.c.descales) {
+    kd = a.c.descales[(long long)r * a.c.KH + c];
+    vd = a.c.descales[(long long)(a.c.R + r) * a.c.KH + c];
+  }
+  // Query operand: head h0 + gid (and + 8), d = HD / 4 tig .. as a key's piece holds them; f16 times a power of two.
+  const float scale = a.scale * kd;
+  uint32_t qb[NG][KS][2];
+  float sscale[NG][2];  // of heads 2 tig, 2 tig + 1
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    const bool live = gid + 8 * n < nh;
+    const __nv_bfloat16* row = reinterpret_cast<const __nv_bfloat16*>(a.q) + (long long)r * a.q_rs +
+                               (long long)(h0 + (live ? gid + 8 * n : 0)) * a.q_hs + tig * (HD / 4);
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t w = live ? *reinterpret_cast<const uint32_t*>(row + 4 * i + 2 * e) : 0u;
+        qb[n][i][e] = w;
+        amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u))));
+      }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const float up = half_row_scale(amax), sign = scale < 0.0f ? -up : scale == 0.0f ? 0.0f : up;
+#pragma unroll
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        qb[n][i][e] = pack16(__uint_as_float(qb[n][i][e] << 16) * sign, __uint_as_float(qb[n][i][e] & 0xffff0000u) * sign, true);
+    // |scale| goes with the scores, its sign (or a zero) with the queries
+    sscale[n][0] = (scale == 0.0f ? 1.0f : fabsf(scale)) / __shfl_sync(0xffffffffu, up, tig * 8);
+    sscale[n][1] = (scale == 0.0f ? 1.0f : fabsf(scale)) / __shfl_sync(0xffffffffu, up, tig * 8 + 4);
+  }
 
   float o[NG][KS][4];
   float m[NG][2], l[NG][2];  // of heads 2 tig, 2 tig + 1: the reference and, of this lane's keys, the sum
@@ -234,12 +247,13 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
   const uint32_t kf_at = Lay::KF + krow * SB + tig * (SB / 4);
   const uint32_t vfa_at = Lay::VF + va * SB + gid * HD / 128, vfb_at = Lay::VF + vb * SB + gid * HD / 128;
 
-  for (int t = 0; t < ntiles; ++t) {
-    issue(t + STAGES - 1);
+  auto tile = [&](int t, auto stage_at) {
+    constexpr int stage = decltype(stage_at)::value;
+    issue(t + STAGES - 1, (stage + STAGES - 1) % STAGES);
     pc_cp_wait<STAGES - 1>();
     __syncwarp();
-    const uint32_t sb = wbase + (t % STAGES) * Lay::STAGE;
-    const uint32_t ok = wok[t % STAGES];
+    const uint32_t sb = wbase + stage * Lay::STAGE;
+    const uint32_t ok = wok[stage];
     float sc[2][NG][4];  // of 16 keys each: keys gid, gid, gid + 8, gid + 8 of heads 2 tig, 2 tig + 1
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -348,6 +362,11 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
         for (int n = 0; n < NG; ++n) mma16816<true>(o[n][i], x[0][i], y[0][i], x[1][i], y[1][i], pb[half][n][0], pb[half][n][1]);
     }
     __syncwarp();  // the stage may be refilled from here on
+  };
+  static_assert(STAGES == 2, "the loop goes by twos");
+  for (int t = 0; t < ntiles; t += 2) {
+    tile(t, std::integral_constant<int, 0>{});
+    if (t + 1 < ntiles) tile(t + 1, std::integral_constant<int, 1>{});
   }
   pc_cp_wait<0>();
   __syncthreads();  // every warp's pipeline is drained: its shared memory is free
@@ -445,7 +464,7 @@ extern "C" size_t fm_paged_decode_attn_fp4_workspace_size(int64_t requests, int6
   if (requests < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || head_dim < 1 || max_length < 0 ||
       max_length > 0x7ffffff0 || window < 0 || window > 0x7ffffff0 || sinks < 0 || sinks > 0x7ffffff0)
     return 0;
-  return decode_plan(requests, heads, kv_heads, head_dim, max_length, window, false, sinks).total;
+  return decode_plan(requests, heads, kv_heads, head_dim, max_length, window, false, sinks, D4_RULE).total;
 }
 
 extern "C" fm_status fm_paged_decode_attn_fp4(const fm_paged_cache* cache, const fm_block_scales* scales,
@@ -456,7 +475,7 @@ extern "C" fm_status fm_paged_decode_attn_fp4(const fm_paged_cache* cache, const
   fm_status st = cache_ref(cache, who, &a.c, true);
   if (st == FM_OK) st = scale_ref(cache, scales, who, &f);
   DecodePlan pl{};
-  if (st == FM_OK) st = decode_args(cache, p, who, &a, &pl);
+  if (st == FM_OK) st = decode_args(cache, p, who, &a, &pl, D4_RULE);
   if (st != FM_OK) return st;
   if (p->weight_sums) return set_error(FM_ERR_UNSUPPORTED, "%s: a 4-bit cache gathers no weights", who);
   if (cache->requests == 0) return FM_OK;

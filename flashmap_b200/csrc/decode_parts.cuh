@@ -3,6 +3,8 @@
 // launch that joins the chunks.
 #pragma once
 
+#include <algorithm>
+
 #include "paged_cache.cuh"
 
 namespace fm {
@@ -198,16 +200,27 @@ constexpr int DA_CTAS = 148 * 12;
 constexpr int DA_CHUNK = 128;
 constexpr int DA_ENOUGH = 1536;
 
+struct DecodeRule {
+  int64_t ctas, chunk, enough;  // as above
+  int64_t most, cap;            // keys of a chunk at most where that takes no more than `cap` CTAs; 0: no such bound
+};
+constexpr DecodeRule DA_RULE{DA_CTAS, DA_CHUNK, DA_ENOUGH, 0, 0};
+
 DecodePlan decode_plan(int64_t R, int64_t H, int64_t KH, int64_t HD, int64_t max_len, int64_t window, bool sums,
-                       int64_t sinks) {
+                       int64_t sinks, const DecodeRule& rule = DA_RULE) {
   DecodePlan p{};
   const int64_t G = H / KH;
   p.ng = G > 8 ? 2 : 1;
   p.hgroups = (int)((G + 8 * p.ng - 1) / (8 * p.ng));
   const int64_t span = visible_span((int)max_len, (int)window, (int)sinks).n;
-  const int64_t items = R * KH * p.hgroups, cut = (DA_CTAS + items - 1) / items;
-  int64_t least = DA_ENOUGH * items / (3 * 148) / 64 * 64;
-  least = least < DA_CHUNK ? DA_CHUNK : least > DA_ENOUGH ? DA_ENOUGH : least;
+  const int64_t items = R * KH * p.hgroups;
+  int64_t cut = (rule.ctas + items - 1) / items;
+  if (rule.most) {
+    const int64_t fine = (span + rule.most - 1) / rule.most, room = rule.cap / items;
+    cut = std::max(cut, std::min(fine, room));
+  }
+  int64_t least = rule.enough * items / (3 * 148) / 64 * 64;
+  least = least < rule.chunk ? rule.chunk : least > rule.enough ? rule.enough : least;
   p.least = (int)least;
   const int64_t most = span <= DA_WHOLE ? 1 : (span + least - 1) / least;
   p.chunks = (int)(cut < most ? cut : most);
@@ -224,7 +237,7 @@ DecodePlan decode_plan(int64_t R, int64_t H, int64_t KH, int64_t HD, int64_t max
 
 // The arguments of a call on a cache that cache_ref has accepted.
 inline fm_status decode_args(const fm_paged_cache* cache, const fm_decode_attn* p, const char* who, DecodeArgs* out,
-                             DecodePlan* plan) {
+                             DecodePlan* plan, const DecodeRule& rule = DA_RULE) {
   DecodeArgs& a = *out;
   if (!p) return set_error(FM_ERR_INVALID, "%s: null arguments", who);
   if (p->heads < 1 || p->heads % cache->kv_heads || p->heads > 65535)
@@ -242,7 +255,7 @@ inline fm_status decode_args(const fm_paged_cache* cache, const fm_decode_attn* 
     return set_error(FM_ERR_ALIGN, "%s: query rows must be 4-byte, output rows 8-byte aligned", who);
   const bool sums = p->weight_sums != nullptr;
   *plan = decode_plan(cache->requests, p->heads, cache->kv_heads, cache->head_dim, cache->max_length,
-                                    p->window, sums, p->sinks);
+                      p->window, sums, p->sinks, rule);
   const DecodePlan& pl = *plan;
   if (pl.total > p->workspace_bytes || (pl.total && !p->workspace))
     return set_error(FM_ERR_WORKSPACE, "%s: workspace %zu < %zu", who, p->workspace_bytes, pl.total);

@@ -195,11 +195,12 @@ __device__ __forceinline__ void e4m3x4_h(uint32_t four, uint32_t& lo, uint32_t& 
       : "=r"(lo), "=r"(hi)
       : "r"(four));
 }
-// four bytes of two e2m1 codes each (low half first) as f16x2
+// four bytes of two e2m1 codes each (low half first) as f16x2; the conversion
+// takes a half's low byte, so one shift brings the other two into place
 __device__ __forceinline__ void e2m1x8_h(uint32_t bytes, uint32_t* h) {
-  asm("{.reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4; cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b; "
-      "cvt.rn.f16x2.e2m1x2 %2, c; cvt.rn.f16x2.e2m1x2 %3, d;}"
-      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+  asm("{.reg .b8 a, b, c, d; .reg .b32 u; mov.b32 {a, b, c, d}, %4; cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %2, c; "
+      "shr.u32 u, %4, 8; mov.b32 {a, b, c, d}, u; cvt.rn.f16x2.e2m1x2 %1, a; cvt.rn.f16x2.e2m1x2 %3, c;}"
+      : "=&r"(h[0]), "=r"(h[1]), "=&r"(h[2]), "=r"(h[3])
       : "r"(bytes));
 }
 // two e4m3 values (low byte first) as f16x2
