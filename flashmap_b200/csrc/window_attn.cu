@@ -205,6 +205,17 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32
       "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(WA_DESC_HI)
       : "memory");
 }
+__device__ __forceinline__ void wa_cp_async4(uint32_t dst, const void* src, uint32_t src_bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+}
+// (loads and stores of one thread's own place or of a tile that a barrier hands over: no compiler fence between them)
+__device__ __forceinline__ void wa_lds8(uint32_t at, uint32_t* v) {
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(at));
+}
+__device__ __forceinline__ void wa_lds4(uint32_t at, uint32_t* v) { asm volatile("ld.shared.u32 %0, [%1];" : "=r"(*v) : "r"(at)); }
+__device__ __forceinline__ void wa_sts16(uint32_t at, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 // Low descriptor words.  K-major (Q, K): the leading offset is unused.  A B
 // operand stored key by key (V, 64 columns of N to a 128-byte row): the next 64
 // columns follow 16384 bytes on.
@@ -240,12 +251,18 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // Shared memory: two row tiles of Q and a ring of K and V tiles (16-bit,
-// 128-byte swizzled in blocks of 64 columns).
-template <int HD>
+// 128-byte swizzled in blocks of 64 columns).  Rows of 4 bits arrive in a ring of
+// their own, AHEAD tiles of K or V (a tile's codes and factors for each loading
+// lane) that are in flight beside the one that is widened.
+template <int HD, int BITS, bool DUO>
 struct WaLayout {
   static constexpr int TILE = 128 * HD * 2;  // Q, K or V tile
-  static constexpr int SLOTS = HD == 64 ? 8 : 5;
-  static constexpr int CTRL = 2 * TILE + SLOTS * TILE;
+  static constexpr int QT = BITS == 4 && DUO ? 1 : 2;  // calls of 128 rows have one row tile
+  static constexpr int SLOTS = HD == 64 ? 8 : BITS == 4 && !DUO ? 4 : 5;
+  static constexpr int AHEAD = BITS == 4 ? 3 : 0;
+  static constexpr int RAW = 128 * (HD / 32) * 20;  // 16 bytes of codes and 4 of factors for each of a lane's rows
+  static constexpr int RING = QT * TILE + SLOTS * TILE;
+  static constexpr int CTRL = RING + AHEAD * RAW;
   static constexpr int SMEM = CTRL + 3072;  // 227 KB at head_dim 128: all that a CTA may have
 };
 
@@ -305,7 +322,7 @@ struct WaCtrl {
 template <int HD, int BITS, bool DUO>
 __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
   constexpr bool KV8 = BITS < 16;
-  using Lay = WaLayout<HD>;
+  using Lay = WaLayout<HD, BITS, DUO>;
   constexpr int TILE = Lay::TILE, SLOTS = Lay::SLOTS;
   constexpr int CPR = HD / 8;  // 16-byte chunks of a 16-bit row
   // registers: 2 x 184 + 64 + 80, or 2 x 176 + 96 + 64 where narrow rows pass
@@ -313,7 +330,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
   extern __shared__ __align__(1024) uint8_t wa_smem[];
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   uint8_t* sQ = wa_smem;
-  uint8_t* sKV = wa_smem + 2 * TILE;
+  uint8_t* sKV = wa_smem + Lay::QT * TILE;
   WaCtrl* ctl = reinterpret_cast<WaCtrl*>(wa_smem + Lay::CTRL);
   if (smem_u32(wa_smem) & 1023) {  // the swizzled tiles need the alignment that the declaration asks for
     pdl_wait();
@@ -724,6 +741,124 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       oldest = oldest + 1 == SLOTS ? 0 : oldest + 1;
       --behind;
     };
+    if constexpr (BITS == 4) {
+      // A stream of tiles, K and V in turn, item after item: copies run AHEAD tiles before the widening.
+      constexpr int AHEAD = Lay::AHEAD;
+      const uint32_t raw = smem_u32(wa_smem) + Lay::RING + (lw * 32 + lane) * 16;  // [tile][row][lane], codes and then factors
+      constexpr int CODES = 128 * 16;                                              // of a row of all lanes
+      const int half = (ch & 1) * 16;  // where in a word of four factors this lane's two are
+      const int turn = (ch >> 1) & 1;
+      const uint32_t near = turn ? 0x3232u : 0x1010u, far = 0x4242u - near;  // the factors of the half that goes first, second
+      const uint32_t dst0 = smem_u32(sKV) + (ch >> 1) * 16384 + (lw * 32 + sub) * 128;
+      uint32_t quarter[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) quarter[q] = (uint32_t)((((ch & 1) * 4 + (q ^ (turn * 2))) ^ (sub & 7)) << 4);
+      WaItem w;
+      w.n = 0;
+      int k = 0, j = 0, staged = 0, in = 0, out = 0;  // next item, key tile of w, tiles in flight, places in the ring
+      bool is_v = false, more = true;
+      int page = -1, tok = 0, page_next = -1, tok_next = 0;  // of this key tile and the next
+      auto lookup = [&](int t, int* at) {  // page of this lane's key of tile t; -1: none, -2: a bad one
+        if (t >= w.n) return -1;
+        const int key = w.key0(t) + lw * 32 + lane;
+        if (key > w.p_hi || !(key >= w.lo || key < a.sinks)) return -1;
+        const int pg = a.c.by_page.div(key);
+        *at = key - pg * a.c.page;
+        const int id = a.c.table[(long long)w.r * a.c.tstride + pg];
+        if (id >= 0 && id < a.c.num_pages) return id;
+        record_error(a.err, DEV_BAD_INDEX);
+        return -2;
+      };
+      auto fetch = [&]() {  // the tile's copies; what the cache holds of rows that are not seen may be no number
+        if (!is_v) {
+          page = page_next;
+          tok = tok_next;
+          page_next = lookup(j + 1, &tok_next);
+          const uint32_t good = __ballot_sync(0xffffffffu, page != -2);
+          if (lane == 0) ctl->valid[tiles & 7][lw] = good;
+        }
+        const unsigned long long off = page < 0 ? 0ull
+                                       : is_v   ? page * a.c.vps + tok * a.c.vts
+                                                : page * a.c.kps + tok * a.c.kts;
+        const unsigned long long foff = page < 0 ? 0ull
+                                        : is_v   ? page * a.f.vps + tok * a.f.vts
+                                                 : page * a.f.kps + tok * a.f.kts;
+        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) >> sub;
+        const uint8_t* codes = is_v ? a.c.v + w.c * a.c.vhs + ch * 16 : a.c.k + w.c * a.c.khs + ch * 16;
+        const uint8_t* factors = is_v ? a.f.v + w.c * a.f.vhs + (ch >> 1) * 4 : a.f.k + w.c * a.f.khs + (ch >> 1) * 4;
+        const uint32_t dst = raw + in * Lay::RAW, fdst = dst + U * CODES - (lw * 32 + lane) * 12;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          // codes are numbers whatever they are: of a row that is not seen the first row's are as good, its factors are zero
+          const unsigned long long o = __shfl_sync(0xffffffffu, off, u * RPI + sub), fo = __shfl_sync(0xffffffffu, foff, u * RPI + sub);
+          pc_cp_async16(dst + u * CODES, codes + o, 16u);
+          wa_cp_async4(fdst + u * 512, factors + fo, (there >> (u * RPI)) & 1u ? 4u : 0u);
+        }
+        pc_cp_commit();
+        in = in + 1 == AHEAD ? 0 : in + 1;
+        ++staged;
+        if (is_v) {
+          ++j;
+          ++tiles;
+        }
+        is_v = !is_v;
+      };
+      while (ok) {
+        while (more && staged < AHEAD) {
+          if (j >= w.n) {  // the next item; tiles that are in flight are handed on before this warp waits for one
+            if (staged > 0 && !__all_sync(0xffffffffu, mbar_try_wait(&ctl->item_full[k % WA_ITEMS], (k / WA_ITEMS) & 1))) break;
+            w = take(k++);
+            if (w.r < 0) {
+              more = false;
+              break;
+            }
+            j = 0;
+            page_next = lookup(0, &tok_next);
+            continue;
+          }
+          fetch();
+        }
+        if (staged == 0) {
+          if (!more) break;
+          continue;
+        }
+        if (staged == AHEAD)
+          pc_cp_wait<AHEAD - 1>();
+        else
+          pc_cp_wait<0>();
+        if (!mbar_wait(&ctl->empty[slot], phase, abort)) {
+          ok = false;
+          break;
+        }
+        // A lane's 32 values are half of a 64-column block; which of its halves goes first (`turn`): no two lanes of two
+        // rows share a bank then.
+        uint32_t words[U][4], factor[U];
+        const uint32_t src = raw + out * Lay::RAW;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          wa_lds8(src + u * CODES + turn * 8, words[u]);
+          wa_lds8(src + u * CODES + 8 - turn * 8, words[u] + 2);
+          wa_lds4(src + U * CODES - (lw * 32 + lane) * 12 + u * 512, factor + u);
+        }
+        const uint32_t dst = dst0 + slot * TILE;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const uint32_t f2 = e4m3x2_h(factor[u] >> half), f[2] = {__byte_perm(f2, 0, near), __byte_perm(f2, 0, far)};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t h[4];
+            e2m1x8_h(words[u][q], h);
+            wa_sts16(dst + u * RPI * 128 + quarter[q], mul_h2(h[0], f[q >> 1]), mul_h2(h[1], f[q >> 1]), mul_h2(h[2], f[q >> 1]),
+                     mul_h2(h[3], f[q >> 1]));
+          }
+        }
+        fence_async_smem();
+        mbar_arrive(&ctl->full[slot]);
+        advance();
+        out = out + 1 == AHEAD ? 0 : out + 1;
+        --staged;
+      }
+    } else
     for (int k = 0; ok; ++k) {
       const WaItem w = take(k);
       if (w.r < 0) break;
@@ -748,66 +883,7 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
         return page < 0 ? -1ll : page * a.c.vps + (long long)w.c * a.c.vhs + tok * a.c.vts;
       };
       int tok_next = 0, page_next = lookup(0, &tok_next);
-      if constexpr (BITS == 4) {
-        // codes and factors come into registers, one tile ahead: 32 values and two factors to a lane
-        uint4 xk[U], xv[U];
-        uint32_t fk[U], fv[U];
-        auto fetch = [&](uint4* x, uint32_t* fx, const uint8_t* from, long long off, const uint8_t* scales, long long foff) {
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const long long o = __shfl_sync(0xffffffffu, off, u * RPI + sub);
-            const long long fo = __shfl_sync(0xffffffffu, foff, u * RPI + sub);
-            x[u] = o < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(from + o + ch * 16);
-            fx[u] = o < 0 ? 0u : *reinterpret_cast<const uint16_t*>(scales + fo + ch * 2);
-          }
-        };
-        auto kf_off = [&](int page, int tok) {
-          return page < 0 ? 0ll : page * a.f.kps + (long long)w.c * a.f.khs + tok * a.f.kts;
-        };
-        auto vf_off = [&](int page, int tok) {
-          return page < 0 ? 0ll : page * a.f.vps + (long long)w.c * a.f.vhs + tok * a.f.vts;
-        };
-        auto widen = [&](const uint4* x, const uint32_t* fx) {
-          if (!mbar_wait(&ctl->empty[slot], phase, abort)) {
-            ok = false;
-            return;
-          }
-          // a lane's 32 values are half of a 64-column block; which quarter first: no two lanes of two rows share a bank
-          uint8_t* dst = sKV + slot * TILE + (ch >> 1) * 16384 + (lw * 32 + sub) * 128;
-          const int c0 = (ch & 1) * 4, turn = ch & 2;
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const int sw = (u * RPI + sub) & 7;
-            const uint32_t f2 = e4m3x2_h(fx[u]), f_lo = __byte_perm(f2, 0, 0x1010), f_hi = __byte_perm(f2, 0, 0x3232);
-            const uint32_t words[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t h[4];
-              // with `turn` the quarters 2, 3 come first
-              e2m1x8_h(turn ? words[q ^ 2] : words[q], h);
-              const uint32_t f = (q < 2) == (turn == 0) ? f_lo : f_hi;
-              *reinterpret_cast<uint4*>(dst + u * RPI * 128 + (((c0 + (q ^ turn)) ^ sw) << 4)) =
-                  make_uint4(mul_h2(h[0], f), mul_h2(h[1], f), mul_h2(h[2], f), mul_h2(h[3], f));
-            }
-          }
-          fence_async_smem();
-          mbar_arrive(&ctl->full[slot]);
-          advance();
-        };
-        int page = page_next, tok = tok_next;
-        if (w.n > 0) fetch(xk, fk, a.c.k, k_off(page, tok), a.f.k, kf_off(page, tok));
-        for (int j = 0; j < w.n && ok; ++j, ++tiles) {
-          page_next = lookup(j + 1, &tok_next);
-          const uint32_t good = __ballot_sync(0xffffffffu, page != -2);
-          if (lane == 0) ctl->valid[tiles & 7][lw] = good;
-          fetch(xv, fv, a.c.v, v_off(page, tok), a.f.v, vf_off(page, tok));
-          widen(xk, fk);
-          page = page_next;
-          tok = tok_next;
-          if (j + 1 < w.n) fetch(xk, fk, a.c.k, k_off(page, tok), a.f.k, kf_off(page, tok));
-          if (ok) widen(xv, fv);
-        }
-      } else if constexpr (KV8) {
+      if constexpr (KV8) {
         // e4m3 rows come into registers, one tile ahead, and go on as f16, which holds them exactly
         uint4 xk[U], xv[U];
         auto fetch = [&](uint4* x, const uint8_t* from, long long off) {
@@ -1247,7 +1323,7 @@ WindowPlan window_plan(int64_t R, int64_t T, int64_t H, int64_t KH, int64_t HD, 
 
 template <int HD, int BITS, bool DUO>
 fm_status launch_window(const WindowArgs& a, const WindowPlan& pl, cudaStream_t s) {
-  constexpr int smem = WaLayout<HD>::SMEM;
+  constexpr int smem = WaLayout<HD, BITS, DUO>::SMEM;
   static_assert(sizeof(WaCtrl) <= 3072 && smem <= 232448, "shared memory");
   fm_status st = allow_smem<window_attn_kernel<HD, BITS, DUO>>(smem, "paged_window_attn");
   if (st != FM_OK) return st;
