@@ -9,6 +9,9 @@
 //
 // Every value is read and written once; the bytes bound it, and a few tokens
 // the latency of table, position and row.
+#include <algorithm>
+#include <type_traits>
+
 #include "paged_cache.cuh"
 
 namespace fm {
@@ -31,6 +34,7 @@ struct AppendArgs {
   const float2* rope;
   long long rope_rows;
   int rot;
+  int per, chunks;  // slots of a warp, warps of a token
   int* err;
 };
 
@@ -74,36 +78,39 @@ __device__ __forceinline__ int append_request(const AppendArgs& a, int t) {
   return -1;
 }
 
-// Eight values to a thread, P rows to a thread: block (t, y) has rows y * P *
-// 256 / LPR .. of token t, its query heads, then keys, then values.  The rows are
-// read before it is known whose they are: what a token waits for is the chain
-// from the row bounds to its position's cosines and its page.
-template <int HD, int KIND, int ROPE, int P>
+// x / d to the last bit where neither is out of range, r = 1 / d rounded: the
+// rounded product is off by at most an ulp, and one step with the exact
+// remainder rounds to nearest (Markstein).  inf and NaN do not come through.
+__device__ __forceinline__ float ap_divide(float x, float d, float r) {
+  const float q = __fmul_rn(x, r);
+  return __fmaf_rn(__fmaf_rn(-q, d, x), r, q);
+}
+__device__ __forceinline__ uint4 ap_bf16x8(const float* x) {
+  return make_uint4(pack16(x[0], x[1], false), pack16(x[2], x[3], false), pack16(x[4], x[5], false), pack16(x[6], x[7], false));
+}
+
+// Eight values to a thread, RPW rows to a warp at a time (a slot: rows of one
+// kind, the last of a kind may be fewer).  A warp takes `per` slots of one token,
+// its queries, then keys, then values: the token's request, place and cosines are
+// found once for all of them, and addresses step from slot to slot.
+template <int HD, int KIND, int ROPE>
 __global__ void __launch_bounds__(256, 4) append_kernel(AppendArgs a) {
-  constexpr int LPR = HD / 8, RPP = 256 / LPR;
-  const int t = blockIdx.x, at = threadIdx.x % LPR, d0 = at * 8;
-  const int row0 = blockIdx.y * P * RPP + threadIdx.x / LPR, rows = a.H + 2 * a.c.KH;
+  constexpr int LPR = HD / 8, RPW = 32 / LPR, U = 2;  // U: slots whose rows are read at a time
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+  const int at = lane % LPR, sub = lane / LPR, d0 = at * 8;
+  const int QW = (a.H + RPW - 1) / RPW, KW = (a.c.KH + RPW - 1) / RPW, slots = QW + 2 * KW;
+  const long long item = (long long)blockIdx.x * 8 + warp;
+  const int t = (int)(item / a.chunks), s0 = (int)(item - (long long)t * a.chunks) * a.per, s1 = min(slots, s0 + a.per);
   const bool turned = ROPE != AP_PLAIN && d0 < a.rot;
   const int half = a.rot / 2;
   const bool first = d0 < half;  // of the two halves that are rotated into one another
   pdl_wait();
-  uint4 own[P], mate[P];
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int row = row0 + p * RPP;
-    if (row >= rows) break;
-    const __nv_bfloat16* src = row < a.H            ? a.q + t * a.q_ts + row * a.q_hs
-                               : row < a.H + a.c.KH ? a.k + t * a.k_ts + (row - a.H) * a.k_hs
-                                                    : a.v + t * a.v_ts + (row - a.H - a.c.KH) * a.v_hs;
-    own[p] = *reinterpret_cast<const uint4*>(src + d0);
-    if (ROPE == AP_HALVES && turned && row < a.H + a.c.KH)
-      mate[p] = *reinterpret_cast<const uint4*>(src + (first ? d0 + half : d0 - half));
-  }
-  if (a.cu != nullptr && t == 0 && blockIdx.y == 0)  // one block looks at all bounds: those that run back give rows to nobody
+  if (a.cu != nullptr && blockIdx.x == 0)  // one block looks at all bounds: those that run back give rows to nobody
     for (int i = threadIdx.x; i < a.c.R; i += 256)
       if (a.cu[i + 1] < a.cu[i]) record_error(a.err, DEV_BAD_INDEX);
+  if (t >= a.T) return;
   const int r = append_request(a, t);
-  if (r < 0 || row0 >= rows) return;
+  if (r < 0) return;
   const int len = a.c.lengths[r];
   int j = len - 1;  // place in the cache
   bool ok = true;
@@ -123,12 +130,11 @@ __global__ void __launch_bounds__(256, 4) append_kernel(AppendArgs a) {
       ok = false;
     }
   }
-  if (bad && threadIdx.x == 0 && blockIdx.y == 0) record_error(a.err, DEV_BAD_INDEX);
+  if (bad && lane == 0) record_error(a.err, DEV_BAD_INDEX);
   if (!ok) {
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-      if (row0 + p * RPP < a.H)
-        *reinterpret_cast<uint4*>(a.out + t * a.o_ts + (row0 + p * RPP) * a.o_hs + d0) = make_uint4(0, 0, 0, 0);
+    for (int s = s0; s < min(s1, QW); ++s)
+      if (s * RPW + sub < a.H)
+        *reinterpret_cast<uint4*>(a.out + t * a.o_ts + (s * RPW + sub) * a.o_hs + d0) = make_uint4(0, 0, 0, 0);
     return;
   }
   const int pg = a.c.by_page.div(j), tok = j - pg * a.c.page;
@@ -138,92 +144,130 @@ __global__ void __launch_bounds__(256, 4) append_kernel(AppendArgs a) {
   if (turned) {
     const float4* c4 = reinterpret_cast<const float4*>(a.rope + pos * half + (ROPE == AP_PAIRS ? d0 / 2 : first ? d0 : d0 - half));
 #pragma unroll
-    for (int i = 0; i < PAIRS / 2; ++i) cs[i] = c4[i];
-  }
-  const bool there = page >= 0 && page < a.c.num_pages;
-#pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int row = row0 + p * RPP;
-    if (row >= rows) return;
-    const bool is_q = row < a.H, is_k = !is_q && row < a.H + a.c.KH;
-    const int h = is_q ? row : is_k ? row - a.H : row - a.H - a.c.KH;
-    float x[8];
-    unpack8(own[p], x);
-    if (turned && (is_q || is_k)) {
-      if constexpr (ROPE == AP_HALVES) {
-        float y[8];
-        unpack8(mate[p], y);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float u0 = __fmul_rn(y[2 * i], cs[i].y), u1 = __fmul_rn(y[2 * i + 1], cs[i].w);
-          x[2 * i] = __fadd_rn(__fmul_rn(x[2 * i], cs[i].x), first ? -u0 : u0);
-          x[2 * i + 1] = __fadd_rn(__fmul_rn(x[2 * i + 1], cs[i].z), first ? -u1 : u1);
-        }
-      } else if constexpr (ROPE == AP_PAIRS) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float* z = x + 4 * i;
-          const float a0 = z[0], a1 = z[2];
-          z[0] = __fsub_rn(__fmul_rn(a0, cs[i].x), __fmul_rn(z[1], cs[i].y));
-          z[1] = __fadd_rn(__fmul_rn(z[1], cs[i].x), __fmul_rn(a0, cs[i].y));
-          z[2] = __fsub_rn(__fmul_rn(a1, cs[i].z), __fmul_rn(z[3], cs[i].w));
-          z[3] = __fadd_rn(__fmul_rn(z[3], cs[i].z), __fmul_rn(a1, cs[i].w));
-        }
+    for (int i = 0; i < PAIRS / 2; ++i) {
+      cs[i] = c4[i];
+      if (ROPE == AP_HALVES && first) {  // a c - b s as a c + b (-s): the same bits
+        cs[i].y = -cs[i].y;
+        cs[i].w = -cs[i].w;
       }
     }
-    if (is_q) {
-      *reinterpret_cast<uint4*>(a.out + t * a.o_ts + h * a.o_hs + d0) =
-          make_uint4(pack16(x[0], x[1], false), pack16(x[2], x[3], false), pack16(x[4], x[5], false), pack16(x[6], x[7], false));
-      continue;
+  }
+  auto rotate = [&](float* x, const uint4& mate) {
+    if (!turned) return;
+    if constexpr (ROPE == AP_HALVES) {
+      float y[8];
+      unpack8(mate, y);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __fadd_rn(__fmul_rn(x[2 * i], cs[i].x), __fmul_rn(y[2 * i], cs[i].y));
+        x[2 * i + 1] = __fadd_rn(__fmul_rn(x[2 * i + 1], cs[i].z), __fmul_rn(y[2 * i + 1], cs[i].w));
+      }
+    } else if constexpr (ROPE == AP_PAIRS) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float* z = x + 4 * i;
+        const float a0 = z[0], a1 = z[2];
+        z[0] = __fsub_rn(__fmul_rn(a0, cs[i].x), __fmul_rn(z[1], cs[i].y));
+        z[1] = __fadd_rn(__fmul_rn(z[1], cs[i].x), __fmul_rn(a0, cs[i].y));
+        z[2] = __fsub_rn(__fmul_rn(a1, cs[i].z), __fmul_rn(z[3], cs[i].w));
+        z[3] = __fadd_rn(__fmul_rn(z[3], cs[i].z), __fmul_rn(a1, cs[i].w));
+      }
     }
-    if (KIND != AP_BF16 && a.c.descales != nullptr) {
-      const float d = a.c.descales[(long long)(is_k ? r : a.c.R + r) * a.c.KH + h];
+  };
+  const int to_mate = first ? half : -half;
+  // rows s .. of a kind with `heads` heads, U slots at a time: f(x, head) for each, the last slot's lanes without a row left out
+  auto rows = [&](const __nv_bfloat16* src, long long hs, int from, int to, int heads, auto with_mate, auto&& f) {
+    const __nv_bfloat16* row = src + (from * RPW + sub) * hs + d0;
+    const long long step = RPW * hs;
+    for (int s = from; s < to; s += U) {
+      uint4 own[U], mate[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (s + u < to && (s + u) * RPW + sub < heads) {
+          own[u] = *reinterpret_cast<const uint4*>(row);
+          if (decltype(with_mate)::value && ROPE == AP_HALVES && turned) mate[u] = *reinterpret_cast<const uint4*>(row + to_mate);
+        }
+        row += step;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (s + u >= to) break;
+        float x[8];
+        unpack8(own[u], x);
+        if (decltype(with_mate)::value) rotate(x, mate[u]);
+        f(x, (s + u) * RPW + sub);
+      }
+    }
+  };
+  if (s0 < QW)
+    rows(a.q + t * a.q_ts, a.q_hs, s0, min(s1, QW), a.H, std::true_type{}, [&](const float* x, int h) {
+      if (h < a.H) *reinterpret_cast<uint4*>(a.out + t * a.o_ts + h * a.o_hs + d0) = ap_bf16x8(x);
+    });
+  if (s1 <= QW) return;
+  if (page < 0 || page >= a.c.num_pages) {
+    if (lane == 0) record_error(a.err, DEV_BAD_INDEX);
+    return;
+  }
+  // a key or value row as the cache holds it
+  auto put = [&](float* x, int h, uint8_t* to, long long hs, uint8_t* factors, long long fhs, const float* descales) {
+    if (KIND != AP_BF16 && descales != nullptr) {
+      const float d = descales[min(h, a.c.KH - 1)];
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = __fdiv_rn(x[i], d);
     }
-    uint32_t factor = 0;
-    if constexpr (KIND == AP_FP4) {
-      float top = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
-      // both lanes of sixteen values come here together, whatever the warp's other rows do
-      const unsigned pair = 3u << (threadIdx.x & 30);
-      top = max_nan(top, __shfl_xor_sync(pair, top, 1));
-      factor = to_e4m3x2(__fdiv_rn(top, 6.0f), 0.0f);
-      const uint32_t f2 = e4m3x2_h(factor);
-      const float f = __half2float(__ushort_as_half((unsigned short)(f2 & 0xffffu)));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = f == 0.0f ? copysignf(0.0f, x[i]) : __fdiv_rn(x[i], f);
-    }
-    if (!there) {
-      record_error(a.err, DEV_BAD_INDEX);
-      continue;
-    }
-    uint8_t* dst = is_k ? a.c.k + page * a.c.kps + h * a.c.khs + tok * a.c.kts
-                        : a.c.v + page * a.c.vps + h * a.c.vhs + tok * a.c.vts;
+    const bool live = h < a.c.KH;
+    uint8_t* dst = to + h * hs;
     if constexpr (KIND == AP_BF16) {
-      *reinterpret_cast<uint4*>(dst + d0 * 2) =
-          make_uint4(pack16(x[0], x[1], false), pack16(x[2], x[3], false), pack16(x[4], x[5], false), pack16(x[6], x[7], false));
+      if (live) *reinterpret_cast<uint4*>(dst + d0 * 2) = ap_bf16x8(x);
     } else if constexpr (KIND == AP_E4M3) {
-      *reinterpret_cast<uint2*>(dst + d0) = make_uint2(to_e4m3x2(x[0], x[1]) | to_e4m3x2(x[2], x[3]) << 16,
-                                                       to_e4m3x2(x[4], x[5]) | to_e4m3x2(x[6], x[7]) << 16);
+      if (live)
+        *reinterpret_cast<uint2*>(dst + d0) = make_uint2(to_e4m3x2(x[0], x[1]) | to_e4m3x2(x[2], x[3]) << 16,
+                                                         to_e4m3x2(x[4], x[5]) | to_e4m3x2(x[6], x[7]) << 16);
     } else {
-      *reinterpret_cast<uint32_t*>(dst + d0 / 2) = to_e2m1x8(x);
-      uint8_t* fd = is_k ? a.f.k + page * a.f.kps + h * a.f.khs + tok * a.f.kts
-                         : a.f.v + page * a.f.vps + h * a.f.vhs + tok * a.f.vts;
-      if ((at & 1) == 0) fd[at >> 1] = (uint8_t)factor;
+      float top = fabsf(x[0]);
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
+      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      constexpr float FINITE = 3.40282347e38f, SIXTH = 1.0f / 6.0f;
+      if (top > FINITE) {  // an infinity counts as the largest finite value: both end at the largest factor and code
+        top = FINITE;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = fminf(fmaxf(x[i], -FINITE), FINITE);
+      }
+      const uint32_t factor = to_e4m3x2(ap_divide(top, 6.0f, SIXTH), 0.0f);
+      const float f = __half2float(__ushort_as_half((unsigned short)(e4m3x2_h(factor) & 0xffffu)));
+      const float inverse = f == 0.0f ? 0.0f : __frcp_rn(f);  // a factor of zero: codes of zero, with their sign
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = ap_divide(x[i], f, inverse);
+      if (live) {
+        *reinterpret_cast<uint32_t*>(dst + d0 / 2) = to_e2m1x8(x);
+        if ((at & 1) == 0) factors[h * fhs + (at >> 1)] = (uint8_t)factor;
+      }
     }
-  }
+  };
+  const float* descales = KIND != AP_BF16 && a.c.descales ? a.c.descales + (long long)r * a.c.KH : nullptr;
+  if (s0 < QW + KW)
+    rows(a.k + t * a.k_ts, a.k_hs, max(s0 - QW, 0), min(s1 - QW, KW), a.c.KH, std::true_type{}, [&](float* x, int h) {
+      put(x, h, a.c.k + page * a.c.kps + tok * a.c.kts, a.c.khs, a.f.k + page * a.f.kps + tok * a.f.kts, a.f.khs, descales);
+    });
+  if (s1 > QW + KW)
+    rows(a.v + t * a.v_ts, a.v_hs, max(s0 - QW - KW, 0), s1 - QW - KW, a.c.KH, std::false_type{}, [&](float* x, int h) {
+      put(x, h, a.c.v + page * a.c.vps + tok * a.c.vts, a.c.vhs, a.f.v + page * a.f.vps + tok * a.f.vts, a.f.vhs,
+          descales ? descales + (long long)a.c.R * a.c.KH : nullptr);
+    });
 }
 
 template <int HD, int KIND, int ROPE>
-fm_status launch_append(const AppendArgs& a, cudaStream_t s) {
-  constexpr int RPP = 256 / (HD / 8), P = HD == 128 ? 3 : 2;
-  const unsigned passes = (unsigned)((a.H + 2 * a.c.KH + RPP - 1) / RPP);
-  // few tokens: a row to a thread, so that more blocks share the work; many: one chain of loads for P rows
-  if ((long long)a.T * passes <= 148 * 8)
-    return launch_kernel(append_kernel<HD, KIND, ROPE, 1>, dim3((unsigned)a.T, passes), dim3(256), 0, s, true, a);
-  return launch_kernel(append_kernel<HD, KIND, ROPE, P>, dim3((unsigned)a.T, (passes + P - 1) / P), dim3(256), 0, s, true, a);
+fm_status launch_append(AppendArgs a, cudaStream_t s) {
+  constexpr int RPW = 32 / (HD / 8);
+  const int slots = (a.H + RPW - 1) / RPW + 2 * ((a.c.KH + RPW - 1) / RPW);
+  // as many slots to a warp as leave every SM 32 warps
+  const long long room = 148ll * 32 / a.T;
+  const int chunks = (int)std::max(1ll, std::min<long long>(slots, room));
+  a.per = (slots + chunks - 1) / chunks;
+  a.chunks = (slots + a.per - 1) / a.per;
+  const long long blocks = ((long long)a.T * a.chunks + 7) / 8;
+  return launch_kernel(append_kernel<HD, KIND, ROPE>, dim3((unsigned)blocks), dim3(256), 0, s, true, a);
 }
 template <int HD, int KIND>
 fm_status launch_append(const AppendArgs& a, int rope, cudaStream_t s) {

@@ -1,14 +1,16 @@
 // Log probabilities of given tokens, the entropy and the largest alternatives
 // of rows of logits, without writing probabilities.
 //
-// With c = log2(e) / T, m = c max x (rounded) and d_i = c x_i - m:
+// With c = log2(e) / T, m near max x and d_i = c (x_i - m):
 //   S = sum 2^d,  U = sum 2^d d,  log p_i = ln 2 (d_i - log2 S),
 //   entropy = ln 2 (log2 S - U / S).
-// One pass over the row: every thread keeps (m, S, U) of what it has seen and
-// rescales when its maximum grows,
-//   d' = d + a, a = m - m':  S' = 2^a S,  U' = 2^a (U + a S).
-// d is formed with one rounding and every m is the same rounded product
-// wherever it is used, so that the rounding of m cancels.
+// One pass over the row: every thread keeps (m, S, U) of what it has seen, m
+// any value near the maximum, and rescales when m moves,
+//   d' = d + a, a = c (m - m'):  S' = 2^a S,  U' = 2^a (U + a S).
+// d is formed as c x - round(c m), one multiplication and addition, and c (m - m')
+// as the difference of the same rounded products, so that their rounding
+// cancels; only where c m is no ordinary number (rows of a type's lowest value,
+// tiny T) as c (x - m).
 //
 // Alternatives.  The pass also leaves the maximum of every group of one or more
 // warp loads (512 bytes each).  The k largest values, equal ones by the lowest id, lie in the
@@ -27,7 +29,7 @@ namespace {
 
 constexpr int LP_T = 256;
 constexpr int LP_LOADS = 4;        // warp loads in flight
-constexpr int LP_GROUPS = 1024;    // groups of a row at most
+constexpr int LP_GROUPS = 256;     // groups of a row at most: one to a thread
 constexpr int LP_LIST = 2048;      // candidates that are sorted at once
 constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
 
@@ -36,7 +38,7 @@ struct LogprobArgs {
   long long ld;  // elements between rows
   int V, rows;
   const long long* tokens;
-  float c;         // log2(e) / T
+  float c, lag;    // log2(e) / T, 8 / c
   int k, gs;       // 2^gs warp loads make a group
   int groups;      // room for a row's group maxima
   int slices, per; // CTAs of a row, warp loads of each
@@ -60,6 +62,27 @@ __device__ __forceinline__ float lp_warp_max(float x) {
   return y;
 }
 
+// Eight bf16 or four fp32 values from x[i0] on, -inf where the row has none.
+template <typename T>
+__device__ __noinline__ uint4 lp_edge(const T* x, int i0, int V) {
+  constexpr int N = 16 / (int)sizeof(T);
+  uint32_t w[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (sizeof(T) == 2) {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
+      const int i = i0 + 2 * q;
+      const uint32_t lo = i >= 0 && i < V ? h[i] : 0xff80u, hi = i + 1 >= 0 && i + 1 < V ? h[i + 1] : 0xff80u;
+      w[q] = lo | hi << 16;
+    } else {
+      const int i = i0 + q;
+      w[q] = i >= 0 && i < V ? reinterpret_cast<const uint32_t*>(x)[i] : 0xff800000u;
+    }
+  }
+  static_assert(N == 8 || N == 4, "bf16 or fp32");
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // A row as 16-byte pieces: piece v has values v * N - shift .. of the row
 // (shift: how far the row starts behind a 16-byte boundary).
 template <typename T>
@@ -76,12 +99,9 @@ struct LpRow {
   __device__ __forceinline__ int first(int piece) const { return piece * N - shift; }
   // piece `p` as it lies in memory; values outside the row are -inf
   __device__ __forceinline__ uint4 load(int p) const {
-    const int i0 = first(p);
+    const int i0 = min(first(p), V);
     if (i0 >= 0 && i0 + N <= V) return __ldg(reinterpret_cast<const uint4*>(x + i0));
-    T v[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = i0 + e >= 0 && i0 + e < V ? x[i0 + e] : (T)(-INFINITY);
-    return *reinterpret_cast<const uint4*>(v);
+    return lp_edge(x, i0, V);
   }
 };
 template <typename T>
@@ -114,14 +134,19 @@ __device__ __forceinline__ float2 lp_range(const uint4& u) {
 struct LpSum {
   float m, s, u;
 };
+// c (x - m); `fast` where c m is an ordinary number
+__device__ __forceinline__ bool lp_fast(float m, float c) { return fabsf(m * c) < 1e30f; }
+__device__ __forceinline__ float lp_diff(float x, float m, float c) {
+  return lp_fast(m, c) && lp_fast(x, c) ? __fsub_rn(__fmul_rn(x, c), __fmul_rn(m, c)) : (x - m) * c;
+}
 // both of one row
-__device__ __forceinline__ LpSum lp_join(const LpSum& a, const LpSum& b) {
+__device__ __forceinline__ LpSum lp_join(const LpSum& a, const LpSum& b, float c) {
   const float m = fmaxf(a.m, b.m);
   if (m == -INFINITY) return LpSum{m, a.s + b.s, a.u + b.u};  // sums of nothing, or NaN
   LpSum r{m, 0.0f, 0.0f};
   auto add = [&](const LpSum& v) {
     if (v.m == -INFINITY && v.s == 0.0f) return;  // saw nothing
-    const float d = fmaxf(v.m - m, -1000.0f), f = lp_ex2(d);
+    const float d = v.m == m ? 0.0f : fmaxf(lp_diff(v.m, m, c), -1000.0f), f = lp_ex2(d);
     r.s += f * v.s;
     r.u += f * (v.u + d * v.s);
   };
@@ -152,9 +177,9 @@ __device__ __forceinline__ float lp_key_value(unsigned long long key) {
 }
 __device__ __forceinline__ unsigned long long lp_key(float v, uint32_t i) { return argmax_key(v != v ? -INFINITY : v, i); }
 
+template <bool TOP>
 struct LpShared {
-  unsigned long long keys[LP_LIST];  // the warps' first groups, then candidates
-  float gmax[LP_GROUPS];
+  unsigned long long keys[TOP ? LP_LIST : 1];  // the warps' first groups, then candidates
   int chosen[32];
   float least;
   LpSum warp[LP_T / 32];
@@ -163,13 +188,13 @@ struct LpShared {
 };
 
 // What a row's sums and group maxima say; by one block.
-template <typename T>
-__device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const float* gmax, LpShared& sh) {
+template <typename T, bool TOP>
+__device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const float* gmax, LpShared<TOP>& sh) {
   const LpRow<T> x(a, row);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float log_s = log2f(all.s);
   const bool none = all.m == -INFINITY && all.s == 0.0f;  // -inf alone
-  auto logprob = [&](float v) { return none ? -INFINITY : LP_LN2 * (fmaf(v, a.c, -all.m) - log_s); };
+  auto logprob = [&](float v) { return none ? -INFINITY : LP_LN2 * ((lp_fast(all.m, a.c) ? fmaf(v, a.c, -__fmul_rn(all.m, a.c)) : (v - all.m) * a.c) - log_s); };
   if (tid == 0) {
     const long long t = a.tokens[row];
     float lp = -INFINITY;
@@ -180,36 +205,28 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
     a.logprob[row] = lp;
     a.entropy[row] = none ? 0.0f : LP_LN2 * (log_s - all.u / all.s);
   }
-  if (a.k == 0) return;
+  if (!TOP || a.k == 0) return;
   const int loads = (x.pieces + 31) / 32, groups = (loads + (1 << a.gs) - 1) >> a.gs;
-  // Every warp draws the k first of its 128 groups, four to a lane; of those the k first stand behind fewer than k others.
-  constexpr int W = LP_T / 32, PER = LP_GROUPS / LP_T;
-  uint32_t mine[PER];  // orderable maxima of groups (warp * PER + j) * 32 + lane; 0: none
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int g = (warp * PER + j) * 32 + lane;
-    mine[j] = g < groups ? (uint32_t)(lp_key(gmax[g], 0) >> 32) : 0u;
-  }
-  for (int i = 0; i < a.k; ++i) {
-    uint32_t best = mine[0];
-#pragma unroll
-    for (int j = 1; j < PER; ++j) best = max(best, mine[j]);
-    best = __reduce_max_sync(0xffffffffu, best);
-    uint32_t at = 0xffffffffu;
-#pragma unroll
-    for (int j = PER - 1; j >= 0; --j) at = mine[j] == best ? (uint32_t)((warp * PER + j) * 32 + lane) : at;
-    at = __reduce_min_sync(0xffffffffu, at);
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (at == (uint32_t)((warp * PER + j) * 32 + lane)) mine[j] = 0u;
-    if (lane == 0) sh.keys[warp * a.k + i] = best ? (unsigned long long)best << 32 | (0xffffffffu - at) : 0ull;
+  // Every warp draws the k first of its groups, one to a lane; of those the k first stand behind fewer than k others.
+  const int drawn = (groups + 31) / 32 * a.k;  // by the warps that have groups
+  if (warp * 32 < groups) {
+    uint32_t mine = tid < groups ? (uint32_t)(lp_key(gmax[tid], 0) >> 32) : 0u;  // orderable; 0: none, or drawn
+    for (int i = 0; i < a.k; ++i) {
+      const uint32_t best = __reduce_max_sync(0xffffffffu, mine);
+      const int at = __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1;  // the lowest of equal ones
+      if (lane == at) {
+        sh.keys[warp * a.k + i] = best ? (unsigned long long)best << 32 | (0xffffffffu - tid) : 0ull;
+        mine = 0u;
+      }
+    }
   }
   __syncthreads();
   const int take = min(a.k, groups);
-  for (int i = tid; i < W * a.k; i += LP_T) {
+  for (int i = tid; i < drawn; i += LP_T) {
     const unsigned long long key = sh.keys[i];
     int before = 0;
-    for (int j = 0; j < W * a.k; ++j) before += sh.keys[j] > key;
+#pragma unroll 4
+    for (int j = 0; j < drawn; ++j) before += sh.keys[j] > key;
     if (key && before < take) {
       sh.chosen[before] = (int)argmax_key_index(key);
       if (before == take - 1) sh.least = lp_key_value(key);
@@ -219,19 +236,32 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
   __syncthreads();
   const float least = take < a.k ? -INFINITY : sh.least;
   // the chosen groups once more: values that reach the k-th maximum
-  auto each = [&](auto&& f) {
-    for (int i = warp; i < take << a.gs; i += LP_T / 32) {
-      const int p = ((sh.chosen[i >> a.gs] << a.gs) + (i & ((1 << a.gs) - 1))) * 32 + lane;
-      if (p >= x.pieces) continue;
-      float v[LpRow<T>::N];
-      lp_unpack<T>(x.load(p), v);
-      const int i0 = x.first(p);
+  const int again = take << a.gs;  // warp loads
+  auto each = [&](float from, auto&& f) {
+    constexpr int U = 4, W = LP_T / 32;
+    for (int i0 = warp; i0 < again; i0 += U * W) {
+      uint4 u[U];
 #pragma unroll
-      for (int e = 0; e < LpRow<T>::N; ++e)
-        if (i0 + e >= 0 && i0 + e < a.V) f(v[e] != v[e] ? -INFINITY : v[e], i0 + e);
+      for (int q = 0; q < U; ++q) {
+        const int i = min(i0 + q * W, again - 1);
+        u[q] = x.load(((sh.chosen[i >> a.gs] << a.gs) + (i & ((1 << a.gs) - 1))) * 32 + lane);
+      }
+#pragma unroll 1
+      for (int q = 0; q < U; ++q) {
+        const int i = i0 + q * W;
+        const uint4 now = u[0];
+        u[0] = u[1], u[1] = u[2], u[2] = u[3];
+        if (i >= again || (!(lp_range<T>(now).x >= from) && from > -INFINITY)) continue;  // as a rule
+        const int first = x.first(((sh.chosen[i >> a.gs] << a.gs) + (i & ((1 << a.gs) - 1))) * 32 + lane);
+        float v[LpRow<T>::N];
+        lp_unpack<T>(now, v);
+#pragma unroll
+        for (int e = 0; e < LpRow<T>::N; ++e)
+          if (first + e >= 0 && first + e < a.V) f(v[e] != v[e] ? -INFINITY : v[e], first + e);
+      }
     }
   };
-  each([&](float v, int i) {
+  each(least, [&](float v, int i) {
     if (v >= least) {
       const int at = atomicAdd(&sh.count, 1);
       if (at < LP_LIST) sh.keys[at] = lp_key(v, (uint32_t)i);
@@ -240,10 +270,12 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
   __syncthreads();
   const int count = sh.count;
   if (count <= LP_T) {  // as a rule: a candidate to a thread, which counts those before it
-    const unsigned long long key = tid < count ? sh.keys[tid] : 0ull;
+    if (tid >= count) return;
+    const unsigned long long key = sh.keys[tid];
     int before = 0;
+#pragma unroll 4
     for (int j = 0; j < count; ++j) before += sh.keys[j] > key;
-    if (tid < count && before < a.k) {
+    if (before < a.k) {
       a.ids[(long long)row * a.k + before] = argmax_key_index(key);
       a.top[(long long)row * a.k + before] = logprob(lp_key_value(key));
     }
@@ -265,7 +297,7 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
   unsigned long long last = ~0ull;
   for (int j = 0; j < a.k; ++j) {
     unsigned long long best = 0;
-    each([&](float v, int i) {
+    each(-INFINITY, [&](float v, int i) {
       const unsigned long long key = lp_key(v, (uint32_t)i);
       if (key < last && key > best) best = key;
     });
@@ -286,66 +318,49 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
   }
 }
 
-__device__ __forceinline__ LpSum lp_block_join(LpSum v, LpShared& sh) {
+// The sum of all lanes', in every lane.
+__device__ __forceinline__ LpSum lp_warp_join(LpSum v, float c) {
+  const float m = lp_warp_max(v.m);
+  if (m != -INFINITY) {  // a lane that saw nothing gets a factor of 0, one with NaN keeps it
+    const float d = v.m == m ? 0.0f : fmaxf(lp_diff(v.m, m, c), -1000.0f), f = lp_ex2(d);
+    v.u = f * (v.u + d * v.s);
+    v.s *= f;
+  }
+  v.m = m;
 #pragma unroll
   for (int off = 16; off; off >>= 1) {
-    const LpSum o{__shfl_xor_sync(0xffffffffu, v.m, off), __shfl_xor_sync(0xffffffffu, v.s, off),
-                  __shfl_xor_sync(0xffffffffu, v.u, off)};
-    // the lower lane's first, so that both get the same bits
-    v = (threadIdx.x & off) ? lp_join(o, v) : lp_join(v, o);
+    v.s += __shfl_xor_sync(0xffffffffu, v.s, off);
+    v.u += __shfl_xor_sync(0xffffffffu, v.u, off);
   }
-  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = sh.warp[0];
-  for (int w = 1; w < LP_T / 32; ++w) v = lp_join(v, sh.warp[w]);
   return v;
 }
+template <bool TOP>
+__device__ __forceinline__ LpSum lp_block_join(LpSum v, float c, LpShared<TOP>& sh) {
+  const int lane = threadIdx.x & 31;
+  v = lp_warp_join(v, c);
+  if (lane == 0) sh.warp[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return lp_warp_join(lane < LP_T / 32 ? sh.warp[lane] : LpSum{-INFINITY, 0.0f, 0.0f}, c);
+}
 
-// Block (row, slice): warp loads slice * per .. of the row.  ONE: a warp load is
-// a group of its own.
-template <typename T, bool TOP, bool ONE>
+// Block (row, slice): warp loads slice * per .. of the row, LP_LOADS of them at a
+// time to a warp (a batch), the next batch on its way meanwhile.  Batches that
+// do not lie in the row altogether come last.
+// LONG: groups of more than a batch.
+template <typename T, bool TOP, bool LONG>
 __global__ void __launch_bounds__(LP_T, 4) logprob_scan_kernel(LogprobArgs a) {
-  __shared__ LpShared sh;
+  __shared__ LpShared<false> sh;
   pdl_wait();
   const int row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const LpRow<T> x(a, row);
-  constexpr int N = LpRow<T>::N;
+  constexpr int N = LpRow<T>::N, W = LP_T / 32;
   const int loads = (x.pieces + 31) / 32, end = min(loads, (slice + 1) * a.per);
-  const int span = ONE ? LP_LOADS : max(LP_LOADS, 1 << a.gs);  // a warp's loads at a time hold whole groups
-  float* gmax = a.slices == 1 ? sh.gmax : a.gmax + (long long)row * a.groups;
-  const uint4 nothing = sizeof(T) == 2 ? make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u)
-                                       : make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
-  const int whole = x.shift ? 1 : 0, whole_end = (a.V + x.shift) / N;  // pieces that lie in the row altogether
-  const uint4* base = reinterpret_cast<const uint4*>(x.x - x.shift) + lane;
-  auto fetch = [&](uint4* u, int l1) {
-    if (l1 * 32 >= whole && (l1 + LP_LOADS) * 32 <= whole_end) {
-#pragma unroll
-      for (int q = 0; q < LP_LOADS; ++q) u[q] = __ldcs(base + (l1 + q) * 32);
-    } else {
-#pragma unroll
-      for (int q = 0; q < LP_LOADS; ++q) {
-        const int p = (l1 + q) * 32 + lane;
-        u[q] = p < x.pieces ? x.load(p) : nothing;
-      }
-    }
-  };
-  // the warp's batches: LP_LOADS loads each, span after span
-  auto after = [&](int l1) { return ((l1 + LP_LOADS) & (span - 1)) ? l1 + LP_LOADS : l1 + LP_LOADS + (LP_T / 32 - 1) * span; };
+  float* gmax = a.gmax + (long long)row * a.groups;
   LpSum v{-INFINITY, 0.0f, 0.0f};
   const float2 c2 = make_float2(a.c, a.c);
-  uint4 next[LP_LOADS];
-  float gm = -INFINITY;
-  // A span is gone through to its end: behind the row there is nothing, but a group is still closed.
-  const int stop = (end + span - 1) & ~(span - 1);
-  int l1 = slice * a.per + warp * span;
-  if (l1 < stop) fetch(next, l1);
-  while (l1 < stop) {
-    uint4 u[LP_LOADS];
-#pragma unroll
-    for (int q = 0; q < LP_LOADS; ++q) u[q] = next[q];
-    const int l2 = after(l1);
-    if (l2 < stop) fetch(next, l2);
+
+  auto add = [&](const uint4* u, int l1) {
     float mx[LP_LOADS], top = -INFINITY, low = INFINITY;
 #pragma unroll
     for (int q = 0; q < LP_LOADS; ++q) {
@@ -354,82 +369,140 @@ __global__ void __launch_bounds__(LP_T, 4) logprob_scan_kernel(LogprobArgs a) {
       top = fmaxf(top, range.x);
       low = fminf(low, range.y);
     }
-    top *= a.c;
-    if (top > v.m) {
+    // m need not be the maximum: it follows when that is 2^8 ahead of it
+    if (top > v.m && (v.m == -INFINITY || top > v.m + a.lag)) {
       if (v.m != -INFINITY) {
-        const float d = fmaxf(v.m - top, -1000.0f), f = lp_ex2(d);
+        const float d = fmaxf(lp_diff(v.m, top, a.c), -1000.0f), f = lp_ex2(d);
         v.u = f * (v.u + d * v.s);
         v.s *= f;
       }
       v.m = top;
     }
-    const float off = v.m == -INFINITY ? 0.0f : v.m;
-    // 2^d d is 0 where d is -inf; where no value is so low that d could be, it needs no guard
-    const bool guard = __any_sync(0xffffffffu, !(low * a.c - off > -1e30f));
+    const float off = v.m == -INFINITY ? 0.0f : __fmul_rn(v.m, a.c);
     float2 s2 = make_float2(v.s, 0.0f), u2 = make_float2(v.u, 0.0f);
-    const float2 o2 = make_float2(-off, -off);
-    auto add = [&](auto guarded) {
+    // 2^d d is 0 where d is -inf; where no value is so low that d could be, and c m is an ordinary number, nothing is guarded
+    if (__any_sync(0xffffffffu, !(fabsf(off) < 1e30f && low * a.c > -1e30f))) {
+      const bool fast = fabsf(off) < 1e30f;
+      const float m = v.m == -INFINITY ? 0.0f : v.m;
+#pragma unroll
+      for (int q = 0; q < LP_LOADS; ++q) {
+        float y[N];
+        lp_unpack<T>(u[q], y);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float d = fast ? fmaf(y[e], a.c, -off) : (y[e] - m) * a.c, p = lp_ex2(d);
+          s2.x += p;
+          u2.x = fmaf(p, fmaxf(d, -1000.0f), u2.x);
+        }
+      }
+    } else {
+      const float2 o2 = make_float2(-off, -off);
 #pragma unroll
       for (int q = 0; q < LP_LOADS; ++q) {
         float y[N];
         lp_unpack<T>(u[q], y);
 #pragma unroll
         for (int e = 0; e < N; e += 2) {
-          float2 d = __ffma2_rn(make_float2(y[e], y[e + 1]), c2, o2);
+          const float2 d = __ffma2_rn(make_float2(y[e], y[e + 1]), c2, o2);
           const float2 p = make_float2(lp_ex2(d.x), lp_ex2(d.y));
           s2 = __fadd2_rn(s2, p);
-          if constexpr (decltype(guarded)::value) d = make_float2(fmaxf(d.x, -1000.0f), fmaxf(d.y, -1000.0f));
           u2 = __ffma2_rn(p, d, u2);
         }
       }
-    };
-    if (guard)
-      add(std::true_type{});
-    else
-      add(std::false_type{});
+    }
     v.s = s2.x + s2.y;
     v.u = u2.x + u2.y;
-    if constexpr (TOP && ONE) {
-      float mine = lp_warp_max(mx[0]);
-#pragma unroll
-      for (int q = 1; q < LP_LOADS; ++q) {
-        const float g = lp_warp_max(mx[q]);
-        mine = lane == q ? g : mine;
-      }
-      if (lane < LP_LOADS && l1 + lane < loads) gmax[l1 + lane] = mine;
-    } else if constexpr (TOP) {
-#pragma unroll
-      for (int q = 0; q < LP_LOADS; ++q) {
-        gm = fmaxf(gm, mx[q]);
-        if (((l1 + q + 1) & ((1 << a.gs) - 1)) == 0) {
-          const float g = lp_warp_max(gm);
-          if (lane == 0 && l1 + q + 1 - (1 << a.gs) < loads) gmax[(l1 + q) >> a.gs] = g;
-          gm = -INFINITY;
+    if constexpr (TOP) {
+      if constexpr (!LONG) {  // groups of one, two or four loads
+        if (a.gs == 1) {
+          mx[0] = fmaxf(mx[0], mx[1]);
+          mx[1] = fmaxf(mx[2], mx[3]);
+        } else if (a.gs == 2) {
+          mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        }
+        float mine = lp_warp_max(mx[0]);
+        if (a.gs < 2) {
+          const float g = lp_warp_max(mx[1]);
+          mine = lane == 1 ? g : mine;
+        }
+        if (a.gs < 1) {
+          const float g = lp_warp_max(mx[2]), h = lp_warp_max(mx[3]);
+          mine = lane == 2 ? g : lane == 3 ? h : mine;
+        }
+        const int g0 = (l1 >> a.gs) + lane;
+        if (lane < LP_LOADS >> a.gs && g0 << a.gs < loads) gmax[g0] = mine;
+      } else {  // a group is one warp's, batch after batch
+        const float g = lp_warp_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        if (lane == 0) {
+          float* at = gmax + (l1 >> a.gs);
+          *at = (l1 & ((1 << a.gs) - 1)) == 0 ? g : fmaxf(*at, g);
         }
       }
     }
-    l1 = l2;
+  };
+  const uint4* base = reinterpret_cast<const uint4*>(x.x - x.shift) + lane;
+  auto fetch = [&](uint4* u, int l1) {
+#pragma unroll
+    for (int q = 0; q < LP_LOADS; ++q) u[q] = __ldcs(base + (l1 + q) * 32);
+  };
+  // Batches of the warp: span after span, so that a group is one warp's.
+  const int span = LONG ? 1 << a.gs : LP_LOADS;
+  auto after = [&](int l1) {
+    if constexpr (!LONG) return l1 + W * LP_LOADS;
+    return ((l1 + LP_LOADS) & (span - 1)) ? l1 + LP_LOADS : l1 + LP_LOADS + (W - 1) * span;
+  };
+  const int first = slice * a.per + warp * span;
+  const int whole_end = (a.V + x.shift) / N / (32 * LP_LOADS) * LP_LOADS;  // batches below this one are whole, but for
+  const bool ragged = x.shift != 0 && first == 0;                          // the row's first where it starts between two pieces
+  auto edge = [&](int l1) {
+    uint4 u[LP_LOADS];
+#pragma unroll
+    for (int q = 0; q < LP_LOADS; ++q) u[q] = x.load((l1 + q) * 32 + lane);
+    add(u, l1);
+  };
+  int l1 = first;
+  if (ragged && l1 < end) {
+    edge(l1);
+    l1 = after(l1);
   }
-  v = lp_block_join(v, sh);
-  if (a.slices > 1) {
+  const int stop = min(end, whole_end);
+  if (l1 < stop) {
+    uint4 u[LP_LOADS], w[LP_LOADS];
+    fetch(u, l1);
+    while (true) {
+      const int l2 = after(l1);
+      if (l2 < stop) fetch(w, l2);
+      add(u, l1);
+      l1 = l2;
+      if (l1 >= stop) break;
+      const int l3 = after(l1);
+      if (l3 < stop) fetch(u, l3);
+      add(w, l1);
+      l1 = l3;
+      if (l1 >= stop) break;
+    }
+  }
+  for (; l1 < end; l1 = after(l1)) edge(l1);
+  v = lp_block_join(v, a.c, sh);
+  if (a.part != nullptr) {
     if (threadIdx.x == 0) a.part[(long long)row * a.slices + slice] = make_float4(v.m, v.s, v.u, 0.0f);
     return;
   }
-  lp_finish<T>(a, row, v, sh.gmax, sh);
+  lp_finish<T, false>(a, row, v, nullptr, sh);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(LP_T) logprob_join_kernel(LogprobArgs a) {
-  __shared__ LpShared sh;
+  __shared__ LpShared<true> sh;
   pdl_wait();
   const int row = blockIdx.x;
   LpSum v{-INFINITY, 0.0f, 0.0f};
   for (int s = threadIdx.x; s < a.slices; s += LP_T) {
     const float4 p = a.part[(long long)row * a.slices + s];
-    v = lp_join(v, LpSum{p.x, p.y, p.z});
+    v = lp_join(v, LpSum{p.x, p.y, p.z}, a.c);
   }
-  v = lp_block_join(v, sh);
-  lp_finish<T>(a, row, v, a.gmax + (long long)row * a.groups, sh);
+  v = lp_block_join(v, a.c, sh);
+  lp_finish<T, true>(a, row, v, a.gmax + (long long)row * a.groups, sh);
 }
 
 struct LogprobPlan {
@@ -439,24 +512,30 @@ struct LogprobPlan {
 LogprobPlan logprob_plan(int64_t rows, int64_t V, int64_t esz, int64_t k) {
   LogprobPlan p{};
   const int64_t load = 512 / esz, loads = (V + 16 / esz - 1 + load - 1) / load + 1;
+  p.gs = 1;  // of two loads or more: what is read again is little, and there are fewer to draw from
   while (((loads - 1) >> p.gs) + 1 > LP_GROUPS) ++p.gs;
   p.groups = (int)(((loads - 1) >> p.gs) + 1);
   const int64_t span = 1 << p.gs > LP_LOADS ? 1 << p.gs : LP_LOADS, least = span * (LP_T / 32);
-  int64_t slices = (4 * num_sms() + rows - 1) / rows;
+#ifndef SLM
+#define SLM 4
+#endif
+  int64_t slices = (SLM * num_sms() + rows - 1) / rows;
   const int64_t most = (loads + least - 1) / least;
   if (slices > most) slices = most;
   p.per = (int)(((loads + slices - 1) / slices + span - 1) / span * span);
   p.slices = (int)((loads + p.per - 1) / p.per);
-  p.part = p.slices > 1 ? (size_t)rows * p.slices * sizeof(float4) : 0;
-  p.total = p.part + (p.slices > 1 && k ? ((size_t)rows * p.groups * 4 + 15) / 16 * 16 : 0);
+  p.part = p.slices > 1 || k ? (size_t)rows * p.slices * sizeof(float4) : 0;
+  p.total = p.part + (k ? ((size_t)rows * p.groups * 4 + 15) / 16 * 16 : 0);
   return p;
 }
 
 template <typename T>
 fm_status launch_logprobs(const LogprobArgs& a, cudaStream_t s) {
-  auto kernel = a.k == 0 ? logprob_scan_kernel<T, false, true> : a.gs == 0 ? logprob_scan_kernel<T, true, true> : logprob_scan_kernel<T, true, false>;
+  auto kernel = a.k == 0      ? logprob_scan_kernel<T, false, false>
+                : a.gs <= 2 ? logprob_scan_kernel<T, true, false>
+                            : logprob_scan_kernel<T, true, true>;
   const fm_status st = launch_kernel(kernel, dim3((unsigned)(a.rows * (int64_t)a.slices)), dim3(LP_T), 0, s, true, a);
-  if (st != FM_OK || a.slices == 1) return st;
+  if (st != FM_OK || a.part == nullptr) return st;
   return launch_kernel(logprob_join_kernel<T>, dim3((unsigned)a.rows), dim3(LP_T), 0, s, true, a);
 }
 
@@ -499,6 +578,7 @@ extern "C" fm_status fm_token_logprobs(const void* logits, int32_t dtype, int64_
   a.rows = (int)rows;
   a.tokens = reinterpret_cast<const long long*>(tokens);
   a.c = LP_LOG2E / temperature;
+  a.lag = 8.0f / a.c;
   a.k = (int)top_k;
   a.gs = pl.gs;
   a.groups = pl.groups;
@@ -508,7 +588,7 @@ extern "C" fm_status fm_token_logprobs(const void* logits, int32_t dtype, int64_
   a.entropy = entropy;
   a.ids = reinterpret_cast<long long*>(top_ids);
   a.top = top_logprobs;
-  a.part = static_cast<float4*>(workspace);
+  a.part = pl.part ? static_cast<float4*>(workspace) : nullptr;
   a.gmax = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.part);
   a.err = err;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -59,7 +59,8 @@ def token_logprobs(logits: torch.Tensor, tokens, top_k: int, temperature: float)
         if (row == -math.inf).all():
             lp, ent = torch.full_like(row, -math.inf), torch.zeros((), dtype=torch.float64)
         else:
-            lp = row - torch.logsumexp(row, 0)
+            d = row - row.max()  # first: rows of 1e38 leave no place for a logarithm
+            lp = d - d.exp().sum().log()
             ent = -torch.where(lp == -math.inf, 0.0, lp.exp() * lp).sum()
         lps.append(lp[t] if 0 <= t < row.numel() else torch.tensor(-math.inf, dtype=torch.float64))
         ents.append(ent)

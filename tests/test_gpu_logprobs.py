@@ -41,7 +41,7 @@ def check(got, logits, tokens, k, T):
     tol = (V / 256 + 300) * 2.0 ** -24 + 2.0 ** -22 * (math.log2(V) + 2)
     assert torch.equal(got.top_ids.cpu(), ids)
     for a, b, more in ((got.logprobs, lp, 0.0), (got.top_logprobs, top, 0.0), (got.entropy, ent, tol * math.log2(V))):
-        a = a.double().cpu()
+        a, b = a.double().cpu(), b.float().double()  # past fp32's range (3e38 above -3e38): -inf
         live = torch.isfinite(b)
         assert torch.equal(a[~live], b[~live]) and torch.isfinite(a[live]).all()
         err, lim = (a - b).abs()[live], tol + more + 2.0 ** -21 * (b.abs()[live] + math.log(V))
@@ -99,6 +99,31 @@ def test_ties_masks_and_empty_rows(dtype):
         check(got, x, tokens, k, 1.0)
         assert float(got.logprobs[3]) == -math.inf and float(got.entropy[3]) == 0.0 and float(got.logprobs[2]) == -math.inf
     assert error_word() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_lowest_values_and_temperatures(dtype):
+    """Masks of the type's lowest value (alone in a row, beside -inf, beside logits), logits at both ends, tiny and huge T."""
+    V, low = 3001, torch.finfo(dtype).min
+    x = 2.0 * torch.randn(8, V, generator=torch.Generator().manual_seed(45))
+    x[0] = low
+    x[1] = -math.inf
+    x[1, 100:300] = low
+    x[2, ::2] = low
+    x[3] = -math.inf
+    x[3, 7], x[3, 8] = 3e38, low
+    x[4] *= 1e35
+    x[5, 5] = 1e30
+    x = x.to(dtype).to(DEV)
+    tokens = torch.tensor([0, 150, 1, 7, 3, 5, 6, 3000], device=DEV)
+    check(call(x, tokens, top_k=6), x, tokens, 6, 1.0)
+    y, t = x[6:], tokens[6:]
+    check(call(y, t, top_k=3, temperature=1e6), y, t, 3, 1e6)
+    lp, ent, ids, top = O.token_logprobs(y.cpu(), t.cpu().tolist(), 3, 1e-30)  # numbers of 1e30: by their share
+    got = call(y, t, top_k=3, temperature=1e-30)
+    assert torch.equal(got.top_ids.cpu(), ids) and torch.equal(got.entropy.double().cpu(), ent)
+    assert ((got.logprobs.double().cpu() - lp).abs() <= 2.0 ** -21 * lp.abs()).all()
+    assert ((got.top_logprobs.double().cpu() - top).abs() <= 2.0 ** -21 * top.abs()).all()
 
 
 def test_nan_and_infinity():
