@@ -561,17 +561,19 @@ def evict_paged_context(k_cache: torch.Tensor, v_cache: torch.Tensor, seqused_k:
     return kept, lengths, sums
 
 
-def _rows(x, name: str, heads: int, cache, tokens: int):
-    """``x (tokens, heads, head_dim)`` bf16 with rows that the kernels can read 16 bytes at a time."""
-    shape, stride = x.shape, x.stride()
-    if not (x.device == cache.device and x.dtype == torch.bfloat16 and shape == (tokens, heads, cache.head_dim)):
-        _on(x, name, cache.device)
-        raise OpArgumentError(f"{name} must be bf16 ({tokens}, {heads}, {cache.head_dim}), got {x.dtype} {tuple(shape)}")
-    if stride[2] != 1 or stride[0] % 8 or stride[1] % 8 or x.data_ptr() % 16:
+def _rows(x, name: str, shape, device):
+    """``x`` of ``shape (tokens, heads, head_dim)``, bf16, and its token and head stride, with rows that the kernels can
+    read 16 bytes at a time."""
+    if not (x.shape == shape and x.dtype == torch.bfloat16 and x.device == device):
+        _on(x, name, device)
+        raise OpArgumentError(f"{name} must be bf16 {tuple(shape)}, got {x.dtype} {tuple(x.shape)}")
+    s0, s1, s2 = x.stride()
+    if s2 != 1 or s0 % 8 or s1 % 8 or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:  # a contiguous view that starts between two 16-byte lines
             x = x.clone()
-    return x
+        s0, s1, s2 = x.stride()
+    return x, s0, s1
 
 
 def append_paged_context(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -599,39 +601,44 @@ def append_paged_context(key: torch.Tensor, value: torch.Tensor, k_cache: torch.
     zero; so does, recorded for ``check_device_errors``, one whose request is longer than its table or whose position
     lies outside ``rope``.  A bad page id is recorded and not written to.  Rows that ``cu_seqlens_q`` gives to no request
     are not touched.  No two requests may append to the same page's slot."""
-    most = block_table.shape[1] * k_cache.shape[2] if block_table.dim() == 2 and k_cache.dim() == 4 else 0
-    most = min(most, 0x7ffffff0)
+    table, pool = block_table.shape, k_cache.shape
+    most = min(table[1] * pool[2], 0x7ffffff0) if len(table) == 2 and len(pool) == 4 else 0
     scales = None
     if k_cache.dtype == torch.uint8:
         cache = _cache4(k_cache, v_cache, k_scales, v_scales, seqused_k, block_table, descales, most)
         scales = cache.scales
     else:
-        _need(k_scales is None and v_scales is None, "k_scales and v_scales go with a 4-bit cache")
+        if k_scales is not None or v_scales is not None:
+            raise OpArgumentError("k_scales and v_scales go with a 4-bit cache")
         cache = _cache(k_cache, v_cache, seqused_k, block_table, descales, most)
-    dev = cache.device
-    for t in (key, value, query):
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise OpArgumentError("append_paged_context has no gradient: detach the rows")
+    dev, requests, kv_heads, head_dim = cache.device, cache.requests, cache.kv_heads, cache.head_dim
+    if (key.requires_grad or value.requires_grad or query is not None and query.requires_grad) and torch.is_grad_enabled():
+        raise OpArgumentError("append_paged_context has no gradient: detach the rows")
     tokens = key.shape[0] if key.dim() == 3 else -1
-    key = _rows(key, "key", cache.kv_heads, cache, tokens)
-    value = _rows(value, "value", cache.kv_heads, cache, tokens)
+    shape = (tokens, kv_heads, head_dim)
+    key, k0, k1 = _rows(key, "key", shape, dev)
+    value, v0, v1 = _rows(value, "value", shape, dev)
     cu = 0
     if cu_seqlens_q is not None:
         _on(cu_seqlens_q, "cu_seqlens_q", dev)
-        _need(cu_seqlens_q.dtype is torch.int32 and cu_seqlens_q.shape == (cache.requests + 1,)
-              and cu_seqlens_q.is_contiguous(), "cu_seqlens_q must be contiguous int32 (requests + 1,)")
+        _need(cu_seqlens_q.dtype is torch.int32 and cu_seqlens_q.shape == (requests + 1,) and cu_seqlens_q.is_contiguous(),
+              "cu_seqlens_q must be contiguous int32 (requests + 1,)")
         cu = cu_seqlens_q.data_ptr()
-    else:
-        _need(tokens == cache.requests, "one new token per request without cu_seqlens_q")
-    table, rows, rotary = 0, 0, 0
+    elif tokens != requests:
+        raise OpArgumentError("one new token per request without cu_seqlens_q")
+    angles, rows, rotary = 0, 0, 0
     if rope is not None:
-        _on(rope, "rope", dev)
-        _need(rope.dtype is torch.float32 and rope.dim() == 3 and rope.shape[2] == 2 and rope.is_contiguous(),
-              "rope must be contiguous float32 (positions, rotary_dim / 2, 2)")
-        rows, rotary = rope.shape[0], 2 * rope.shape[1]
-        _need(rotary >= 16 and rotary % 16 == 0 and rotary <= cache.head_dim,
-              f"rotary_dim must be a multiple of 16 up to head_dim, got {rotary}")
-        table = rope.data_ptr()
+        turns = rope.shape
+        if not (rope.device == dev and rope.dtype is torch.float32 and len(turns) == 3 and turns[2] == 2
+                and rope.is_contiguous() and turns[1] >= 8 and turns[1] % 8 == 0 and 2 * turns[1] <= head_dim):
+            _on(rope, "rope", dev)
+            _need(rope.dtype is torch.float32 and rope.dim() == 3 and turns[2] == 2 and rope.is_contiguous(),
+                  "rope must be contiguous float32 (positions, rotary_dim / 2, 2)")
+            raise OpArgumentError(f"rotary_dim must be a multiple of 16 up to head_dim, got {2 * turns[1]}")
+        angles, rows, rotary = rope.data_ptr(), turns[0], 2 * turns[1]
+        if angles % 16:
+            rope = rope.clone()
+            angles = rope.data_ptr()
     at, at_dtype = 0, _lib.FM_DT_I32
     if positions is not None:
         _need(rope is not None, "positions go with a rope table")
@@ -641,19 +648,18 @@ def append_paged_context(key: torch.Tensor, value: torch.Tensor, k_cache: torch.
         at, at_dtype = positions.data_ptr(), _lib.FM_DT_I32 if positions.dtype == torch.int32 else _lib.FM_DT_I64
     out, q, q0, q1, heads, to, o0, o1 = None, 0, 0, 0, 0, 0, 0, 0
     if query is not None:
-        _need(rope is not None, "queries are taken to be rotated: they go with a rope table")
         heads = query.shape[1] if query.dim() == 3 else 0
-        _need(heads > 0 and heads % cache.kv_heads == 0, f"{heads} query heads are no multiple of {cache.kv_heads} kv heads")
-        query = _rows(query, "query", heads, cache, tokens)
-        out = query.new_empty(query.shape)
-        q, q0, q1, to = query.data_ptr(), query.stride(0), query.stride(1), out.data_ptr()
-        o0, o1 = heads * cache.head_dim, cache.head_dim
-    if cache.requests and tokens:
+        if rope is None or heads <= 0 or heads % kv_heads:
+            _need(rope is not None, "queries are taken to be rotated: they go with a rope table")
+            raise OpArgumentError(f"{heads} query heads are no multiple of {kv_heads} kv heads")
+        query, q0, q1 = _rows(query, "query", (tokens, heads, head_dim), dev)
+        out = query.new_empty((tokens, heads, head_dim))
+        q, to, o0, o1 = query.data_ptr(), out.data_ptr(), heads * head_dim, head_dim
+    if requests and tokens:
         status = _lib.load().fm_paged_append(
             cache.packed, scales,
-            _APPEND.pack(key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), value.stride(0), value.stride(1),
-                         q, q0, q1, heads, to, o0, o1, tokens, cu, at, at_dtype, table, rows, rotary, interleaved,
-                         _err_word(dev)),
+            _APPEND.pack(key.data_ptr(), value.data_ptr(), k0, k1, v0, v1, q, q0, q1, heads, to, o0, o1, tokens, cu, at,
+                         at_dtype, angles, rows, rotary, interleaved, _err_word(dev)),
             torch._C._cuda_getCurrentRawStream(dev.index))
         if status:
             _lib.check(status, "fm_paged_append")

@@ -30,6 +30,7 @@ namespace {
 constexpr int LP_T = 256;
 constexpr int LP_LOADS = 4;        // warp loads in flight
 constexpr int LP_GROUPS = 256;     // groups of a row at most: one to a thread
+constexpr int LP_HITS = 512;
 constexpr int LP_LIST = 2048;      // candidates that are sorted at once
 constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
 
@@ -179,9 +180,12 @@ __device__ __forceinline__ unsigned long long lp_key(float v, uint32_t i) { retu
 
 template <bool TOP>
 struct LpShared {
-  unsigned long long keys[TOP ? LP_LIST : 1];  // the warps' first groups, then candidates
+  alignas(16) unsigned long long keys[TOP ? LP_LIST : 2];  // candidates
+  alignas(16) uint32_t group[TOP ? LP_GROUPS : 4];  // orderable maxima
+  int hit[TOP ? LP_HITS : 1];  // pieces that hold a candidate
   int chosen[32];
-  float least;
+  int hits;
+  uint32_t least;
   LpSum warp[LP_T / 32];
   unsigned long long best[LP_T / 32];
   int count;
@@ -207,66 +211,69 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
   }
   if (!TOP || a.k == 0) return;
   const int loads = (x.pieces + 31) / 32, groups = (loads + (1 << a.gs) - 1) >> a.gs;
-  // Every warp draws the k first of its groups, one to a lane; of those the k first stand behind fewer than k others.
-  const int drawn = (groups + 31) / 32 * a.k;  // by the warps that have groups
-  if (warp * 32 < groups) {
-    uint32_t mine = tid < groups ? (uint32_t)(lp_key(gmax[tid], 0) >> 32) : 0u;  // orderable; 0: none, or drawn
-    for (int i = 0; i < a.k; ++i) {
-      const uint32_t best = __reduce_max_sync(0xffffffffu, mine);
-      const int at = __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1;  // the lowest of equal ones
-      if (lane == at) {
-        sh.keys[warp * a.k + i] = best ? (unsigned long long)best << 32 | (0xffffffffu - tid) : 0ull;
-        mine = 0u;
-      }
+  // The groups that stand behind fewer than k others.
+  static_assert(LP_GROUPS == LP_T, "a group to a thread");
+  if (tid < LP_GROUPS) sh.group[tid] = tid < groups ? (uint32_t)(lp_key(gmax[tid], 0) >> 32) : 0u;
+  if (tid == 0) {
+    sh.count = sh.hits = 0;
+    sh.least = 0xffffffffu;
+  }
+  __syncthreads();
+  if (tid < groups) {
+    const uint32_t mine = sh.group[tid];  // 1 at least
+    int before = 0;
+#pragma unroll 4
+    for (int j = 0; j < groups; j += 4) {
+      const uint4 g = *reinterpret_cast<const uint4*>(sh.group + j);
+      before += (g.x > mine - (j < tid)) + (g.y > mine - (j + 1 < tid)) + (g.z > mine - (j + 2 < tid)) + (g.w > mine - (j + 3 < tid));
+    }
+    if (before < a.k) {
+      sh.chosen[before] = tid;
+      atomicMin(&sh.least, mine);
     }
   }
   __syncthreads();
   const int take = min(a.k, groups);
-  for (int i = tid; i < drawn; i += LP_T) {
-    const unsigned long long key = sh.keys[i];
-    int before = 0;
-#pragma unroll 4
-    for (int j = 0; j < drawn; ++j) before += sh.keys[j] > key;
-    if (key && before < take) {
-      sh.chosen[before] = (int)argmax_key_index(key);
-      if (before == take - 1) sh.least = lp_key_value(key);
-    }
-  }
-  if (tid == 0) sh.count = 0;
-  __syncthreads();
-  const float least = take < a.k ? -INFINITY : sh.least;
+  const float least = take < a.k ? -INFINITY : lp_key_value((unsigned long long)sh.least << 32);
   // the chosen groups once more: values that reach the k-th maximum
   const int again = take << a.gs;  // warp loads
-  auto each = [&](float from, auto&& f) {
-    constexpr int U = 4, W = LP_T / 32;
+  auto piece = [&](int i) { return ((sh.chosen[i >> a.gs] << a.gs) + (i & ((1 << a.gs) - 1))) * 32 + lane; };
+  auto values = [&](int p, const uint4& u, auto&& f) {  // those of a piece, NaN as -inf
+    const int first = x.first(p);
+    float v[LpRow<T>::N];
+    lp_unpack<T>(u, v);
+#pragma unroll
+    for (int e = 0; e < LpRow<T>::N; ++e)
+      if (first + e >= 0 && first + e < a.V) f(v[e] != v[e] ? -INFINITY : v[e], first + e);
+  };
+  constexpr int W = LP_T / 32;
+  {
+    constexpr int U = 5;
     for (int i0 = warp; i0 < again; i0 += U * W) {
       uint4 u[U];
 #pragma unroll
-      for (int q = 0; q < U; ++q) {
-        const int i = min(i0 + q * W, again - 1);
-        u[q] = x.load(((sh.chosen[i >> a.gs] << a.gs) + (i & ((1 << a.gs) - 1))) * 32 + lane);
-      }
-#pragma unroll 1
-      for (int q = 0; q < U; ++q) {
-        const int i = i0 + q * W;
-        const uint4 now = u[0];
-        u[0] = u[1], u[1] = u[2], u[2] = u[3];
-        if (i >= again || (!(lp_range<T>(now).x >= from) && from > -INFINITY)) continue;  // as a rule
-        const int first = x.first(((sh.chosen[i >> a.gs] << a.gs) + (i & ((1 << a.gs) - 1))) * 32 + lane);
-        float v[LpRow<T>::N];
-        lp_unpack<T>(now, v);
+      for (int q = 0; q < U; ++q) u[q] = x.load(piece(min(i0 + q * W, again - 1)));
 #pragma unroll
-        for (int e = 0; e < LpRow<T>::N; ++e)
-          if (first + e >= 0 && first + e < a.V) f(v[e] != v[e] ? -INFINITY : v[e], first + e);
-      }
+      for (int q = 0; q < U; ++q)
+        if (i0 + q * W < again && !(lp_range<T>(u[q]).x < least)) {
+          const int at = atomicAdd(&sh.hits, 1);
+          if (at < LP_HITS) sh.hit[at] = piece(i0 + q * W);
+        }
     }
-  };
-  each(least, [&](float v, int i) {
-    if (v >= least) {
-      const int at = atomicAdd(&sh.count, 1);
-      if (at < LP_LIST) sh.keys[at] = lp_key(v, (uint32_t)i);
-    }
-  });
+  }
+  __syncthreads();
+  const int hits = sh.hits;
+  if (hits <= LP_HITS) {  // as a rule: the few pieces that hold such a value, one to a thread
+    for (int i = tid; i < hits; i += LP_T)
+      values(sh.hit[i], x.load(sh.hit[i]), [&](float v, int id) {
+        if (v >= least) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < LP_LIST) sh.keys[at] = lp_key(v, (uint32_t)id);
+        }
+      });
+  } else if (tid == 0) {
+    sh.count = LP_LIST + 1;
+  }
   __syncthreads();
   const int count = sh.count;
   if (count <= LP_T) {  // as a rule: a candidate to a thread, which counts those before it
@@ -274,7 +281,11 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
     const unsigned long long key = sh.keys[tid];
     int before = 0;
 #pragma unroll 4
-    for (int j = 0; j < count; ++j) before += sh.keys[j] > key;
+    for (int j = 0; j + 1 < count; j += 2) {
+      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(sh.keys + j);
+      before += (two.x > key) + (two.y > key);
+    }
+    if (count & 1) before += sh.keys[count - 1] > key;
     if (before < a.k) {
       a.ids[(long long)row * a.k + before] = argmax_key_index(key);
       a.top[(long long)row * a.k + before] = logprob(lp_key_value(key));
@@ -297,10 +308,11 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
   unsigned long long last = ~0ull;
   for (int j = 0; j < a.k; ++j) {
     unsigned long long best = 0;
-    each(-INFINITY, [&](float v, int i) {
-      const unsigned long long key = lp_key(v, (uint32_t)i);
-      if (key < last && key > best) best = key;
-    });
+    for (int i = warp; i < again; i += W)
+      values(piece(i), x.load(piece(i)), [&](float v, int id) {
+        const unsigned long long key = lp_key(v, (uint32_t)id);
+        if (key < last && key > best) best = key;
+      });
 #pragma unroll
     for (int off = 16; off; off >>= 1) {
       const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, off);
@@ -309,7 +321,7 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
     __syncthreads();
     if (lane == 0) sh.best[warp] = best;
     __syncthreads();
-    for (int w = 0; w < LP_T / 32; ++w) best = sh.best[w] > best ? sh.best[w] : best;
+    for (int w = 0; w < W; ++w) best = sh.best[w] > best ? sh.best[w] : best;
     last = best;
     if (tid == 0) {
       a.ids[(long long)row * a.k + j] = argmax_key_index(best);
@@ -492,7 +504,7 @@ __global__ void __launch_bounds__(LP_T, 4) logprob_scan_kernel(LogprobArgs a) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(LP_T) logprob_join_kernel(LogprobArgs a) {
+__global__ void __launch_bounds__(LP_T, 6) logprob_join_kernel(LogprobArgs a) {
   __shared__ LpShared<true> sh;
   pdl_wait();
   const int row = blockIdx.x;
@@ -516,10 +528,7 @@ LogprobPlan logprob_plan(int64_t rows, int64_t V, int64_t esz, int64_t k) {
   while (((loads - 1) >> p.gs) + 1 > LP_GROUPS) ++p.gs;
   p.groups = (int)(((loads - 1) >> p.gs) + 1);
   const int64_t span = 1 << p.gs > LP_LOADS ? 1 << p.gs : LP_LOADS, least = span * (LP_T / 32);
-#ifndef SLM
-#define SLM 4
-#endif
-  int64_t slices = (SLM * num_sms() + rows - 1) / rows;
+  int64_t slices = (4 * num_sms() + rows - 1) / rows;
   const int64_t most = (loads + least - 1) / least;
   if (slices > most) slices = most;
   p.per = (int)(((loads + slices - 1) / slices + span - 1) / span * span);

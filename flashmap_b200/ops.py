@@ -244,17 +244,22 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, t
     if len(shape) != 1:
         logits = logits.reshape(-1, V)
     rows = logits.shape[0]
-    out = logits.new_empty((2,) + shape, dtype=torch.float32)
+    f32 = torch.float32
+    out = logits.new_empty((2,) + shape, dtype=f32)
     ids = tokens.new_empty(shape + (top_k,))
-    top = logits.new_empty(shape + (top_k,), dtype=torch.float32)
+    top = logits.new_empty(shape + (top_k,), dtype=f32)
     if rows:
         dt = 0 if logits.dtype == torch.bfloat16 else 1
         need = _logprobs_workspace(dev.index, rows, V, dt, top_k)
         ws = tokens.new_empty(need // 8) if need else None  # sizes are multiples of 16
-        _lib.call("fm_token_logprobs", logits.data_ptr(), dt, logits.stride(0), tokens.data_ptr(), rows, V, temperature,
-                  top_k, out.data_ptr(), out.data_ptr() + 4 * rows, ids.data_ptr(), top.data_ptr(),
-                  ws.data_ptr() if need else None, need, error_word(dev).data_ptr(), torch._C._cuda_getCurrentRawStream(dev.index))
-    return TokenLogprobs(out[0], out[1], ids, top)
+        status = _lib.load().fm_token_logprobs(
+            logits.data_ptr(), dt, logits.stride(0), tokens.data_ptr(), rows, V, temperature, top_k, out.data_ptr(),
+            out.data_ptr() + 4 * rows, ids.data_ptr(), top.data_ptr(), ws.data_ptr() if need else None, need,
+            error_word(dev).data_ptr(), torch._C._cuda_getCurrentRawStream(dev.index))
+        if status:
+            _lib.check(status, "fm_token_logprobs")
+    logprobs, entropy = out.unbind(0)
+    return TokenLogprobs(logprobs, entropy, ids, top)
 
 
 def transpose(x):
