@@ -92,16 +92,9 @@ __device__ __forceinline__ uint32_t d4_transpose(uint32_t x) {
   return y;
 }
 
-// Strides in units of 16 bytes (codes) and of a row (factors), for caches
-// whose offsets in them fit 32 bits.
-struct D4Narrow {
-  uint32_t kp, kt, vp, vt, kfp, kft, vfp, vft;
-  bool same;  // one offset serves keys and values, and one their factors
-};
-
-// NG: groups of 8 query heads (1 or 2).  WIDE: offsets past what D4Narrow holds.
+// NG: groups of 8 query heads (1 or 2).  WIDE: offsets past 32 bits in NarrowRef's units.
 template <int HD, int NG, int STAGES, bool WIDE>
-__global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef f, D4Narrow nr) {
+__global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef f, NarrowRef nr) {
   using Lay = D4Layout<HD, STAGES>;
   constexpr int RB = Lay::RB, SB = Lay::SB;
   constexpr int KW = HD / 32, VW = HD / 64;  // words of a thread's piece of a key, of a value
@@ -433,24 +426,15 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
 }
 
 template <int HD, int NG, bool WIDE>
-fm_status launch_decode_fp4(const DecodeArgs& a, const ScaleRef& f, const D4Narrow& nr, unsigned grid, cudaStream_t s) {
+fm_status launch_decode_fp4(const DecodeArgs& a, const ScaleRef& f, const NarrowRef& nr, unsigned grid, cudaStream_t s) {
   constexpr int STAGES = 2, smem = d4_smem<HD, NG, STAGES>();
   const fm_status st = allow_smem<decode_fp4_kernel<HD, NG, STAGES, WIDE>>(smem, "paged_decode_attn_fp4");
   if (st != FM_OK) return st;
   return launch_kernel(decode_fp4_kernel<HD, NG, STAGES, WIDE>, dim3(grid), dim3(128), smem, s, true, a, f, nr);
 }
 template <int HD, bool WIDE>
-fm_status launch_decode_fp4(const DecodeArgs& a, const ScaleRef& f, const D4Narrow& nr, int ng, unsigned grid, cudaStream_t s) {
+fm_status launch_decode_fp4(const DecodeArgs& a, const ScaleRef& f, const NarrowRef& nr, int ng, unsigned grid, cudaStream_t s) {
   return ng == 2 ? launch_decode_fp4<HD, 2, WIDE>(a, f, nr, grid, s) : launch_decode_fp4<HD, 1, WIDE>(a, f, nr, grid, s);
-}
-
-// Whether pages' and tokens' offsets in units of `unit` bytes fit 32 bits.
-bool d4_fits(const CacheRef& c, long long ps, long long ts, long long unit, uint32_t* p, uint32_t* t) {
-  if (ps < 0 || ts < 0 || ps / unit > 0xffffffffll || ts / unit > 0xffffffffll) return false;
-  const double most = (double)(c.num_pages > 0 ? c.num_pages - 1 : 0) * (double)ps + (double)(c.page - 1) * (double)ts;
-  *p = (uint32_t)(ps / unit);
-  *t = (uint32_t)(ts / unit);
-  return most / (double)unit < 4.0e9;
 }
 
 }  // namespace
@@ -484,14 +468,10 @@ extern "C" fm_status fm_paged_decode_attn_fp4(const fm_paged_cache* cache, const
   if (items * pl.chunks > 0x7fffffff || join.blocks > 0x7fffffff) return set_error(FM_ERR_SHAPE, "%s: grid too large", who);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const unsigned grid = (unsigned)(items * pl.chunks);
-  const long long row = cache->head_dim / 16;
-  D4Narrow nr{};
-  const bool narrow = d4_fits(a.c, a.c.kps, a.c.kts, 16, &nr.kp, &nr.kt) && d4_fits(a.c, a.c.vps, a.c.vts, 16, &nr.vp, &nr.vt) &&
-                      d4_fits(a.c, f.kps, f.kts, row, &nr.kfp, &nr.kft) && d4_fits(a.c, f.vps, f.vts, row, &nr.vfp, &nr.vft);
-  nr.same = nr.kp == nr.vp && nr.kt == nr.vt && nr.kfp == nr.vfp && nr.kft == nr.vft;
+  const NarrowRef nr = narrow_ref(a.c, f, cache->head_dim);
   if (cache->head_dim == 128)
-    st = narrow ? launch_decode_fp4<128, false>(a, f, nr, pl.ng, grid, s) : launch_decode_fp4<128, true>(a, f, nr, pl.ng, grid, s);
+    st = nr.fits ? launch_decode_fp4<128, false>(a, f, nr, pl.ng, grid, s) : launch_decode_fp4<128, true>(a, f, nr, pl.ng, grid, s);
   else
-    st = narrow ? launch_decode_fp4<64, false>(a, f, nr, pl.ng, grid, s) : launch_decode_fp4<64, true>(a, f, nr, pl.ng, grid, s);
+    st = nr.fits ? launch_decode_fp4<64, false>(a, f, nr, pl.ng, grid, s) : launch_decode_fp4<64, true>(a, f, nr, pl.ng, grid, s);
   return st != FM_OK ? st : launch_decode_join(a, join, cache->head_dim, s);
 }

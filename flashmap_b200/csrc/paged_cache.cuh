@@ -114,6 +114,29 @@ inline fm_status scale_ref(const fm_paged_cache* p, const fm_block_scales* f, co
   return FM_OK;
 }
 
+// Page and token strides of a 4-bit cache in units of 16 bytes (codes) and of a
+// row (factors): where offsets in these units fit 32 bits.
+struct NarrowRef {
+  uint32_t kp, kt, vp, vt, kfp, kft, vfp, vft;
+  bool fits;
+  bool same;  // one offset serves keys and values, and one their factors
+};
+inline NarrowRef narrow_ref(const CacheRef& c, const ScaleRef& f, long long head_dim) {
+  NarrowRef n{};
+  auto fits = [&](long long ps, long long ts, long long unit, uint32_t* p, uint32_t* t) {
+    if (ps < 0 || ts < 0 || ps / unit > 0xffffffffll || ts / unit > 0xffffffffll) return false;
+    const double most = (double)(c.num_pages > 0 ? c.num_pages - 1 : 0) * (double)ps + (double)(c.page - 1) * (double)ts;
+    *p = (uint32_t)(ps / unit);
+    *t = (uint32_t)(ts / unit);
+    return most / (double)unit < 4.0e9;
+  };
+  const long long row = head_dim / 16;
+  n.fits = fits(c.kps, c.kts, 16, &n.kp, &n.kt) && fits(c.vps, c.vts, 16, &n.vp, &n.vt) && fits(f.kps, f.kts, row, &n.kfp, &n.kft) &&
+           fits(f.vps, f.vts, row, &n.vfp, &n.vft);
+  n.same = n.kp == n.vp && n.kt == n.vt && n.kfp == n.vfp && n.kft == n.vft;
+  return n;
+}
+
 // Lets kernel K have `bytes` of dynamic shared memory, once per device.
 template <auto K>
 inline fm_status allow_smem(int bytes, const char* who) {

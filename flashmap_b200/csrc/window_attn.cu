@@ -51,6 +51,7 @@ struct WindowArgs {
   int row_tiles;    // no fewer than there are
   int* err;
   ScaleRef f;       // of a 4-bit cache
+  NarrowRef nr;
 };
 
 // The key tiles that rows row0 .. of request r see: those of the first tokens,
@@ -758,6 +759,8 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
       int k = 0, j = 0, staged = 0, in = 0, out = 0;  // next item, key tile of w, tiles in flight, places in the ring
       bool is_v = false, more = true;
       int page = -1, tok = 0, page_next = -1, tok_next = 0;  // of this key tile and the next
+      const uint8_t *kcodes = nullptr, *vcodes = nullptr, *kfactors = nullptr, *vfactors = nullptr;  // of w's head, this lane's piece
+      uint32_t at[U] = {}, fat[U] = {}, there = 0;  // where this lane's rows are, in NarrowRef's units
       auto lookup = [&](int t, int* at) {  // page of this lane's key of tile t; -1: none, -2: a bad one
         if (t >= w.n) return -1;
         const int key = w.key0(t) + lw * 32 + lane;
@@ -777,22 +780,41 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
           const uint32_t good = __ballot_sync(0xffffffffu, page != -2);
           if (lane == 0) ctl->valid[tiles & 7][lw] = good;
         }
-        const unsigned long long off = page < 0 ? 0ull
-                                       : is_v   ? page * a.c.vps + tok * a.c.vts
-                                                : page * a.c.kps + tok * a.c.kts;
-        const unsigned long long foff = page < 0 ? 0ull
-                                        : is_v   ? page * a.f.vps + tok * a.f.vts
-                                                 : page * a.f.kps + tok * a.f.kts;
-        const uint32_t there = __ballot_sync(0xffffffffu, page >= 0) >> sub;
-        const uint8_t* codes = is_v ? a.c.v + w.c * a.c.vhs + ch * 16 : a.c.k + w.c * a.c.khs + ch * 16;
-        const uint8_t* factors = is_v ? a.f.v + w.c * a.f.vhs + (ch >> 1) * 4 : a.f.k + w.c * a.f.khs + (ch >> 1) * 4;
+        // codes are numbers whatever they are: of a row that is not seen the first row's are as good, its factors are zero
         const uint32_t dst = raw + in * Lay::RAW, fdst = dst + U * CODES - (lw * 32 + lane) * 12;
+        if (a.nr.fits) {
+          if (!is_v || !a.nr.same) {
+            const uint32_t pg = max(page, 0), tk = page < 0 ? 0 : tok;
+            const uint32_t o = is_v ? pg * a.nr.vp + tk * a.nr.vt : pg * a.nr.kp + tk * a.nr.kt;
+            const uint32_t f = is_v ? pg * a.nr.vfp + tk * a.nr.vft : pg * a.nr.kfp + tk * a.nr.kft;
+            there = __ballot_sync(0xffffffffu, page >= 0) >> sub;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          // codes are numbers whatever they are: of a row that is not seen the first row's are as good, its factors are zero
-          const unsigned long long o = __shfl_sync(0xffffffffu, off, u * RPI + sub), fo = __shfl_sync(0xffffffffu, foff, u * RPI + sub);
-          pc_cp_async16(dst + u * CODES, codes + o, 16u);
-          wa_cp_async4(fdst + u * 512, factors + fo, (there >> (u * RPI)) & 1u ? 4u : 0u);
+            for (int u = 0; u < U; ++u) {
+              at[u] = __shfl_sync(0xffffffffu, o, u * RPI + sub);
+              fat[u] = __shfl_sync(0xffffffffu, f, u * RPI + sub);
+            }
+          }
+          const uint8_t* codes = is_v ? vcodes : kcodes;
+          const uint8_t* factors = is_v ? vfactors : kfactors;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            pc_cp_async16(dst + u * CODES, codes + (unsigned long long)at[u] * 16, 16u);
+            wa_cp_async4(fdst + u * 512, factors + (unsigned long long)fat[u] * (HD / 16), (there >> (u * RPI)) & 1u ? 4u : 0u);
+          }
+        } else {
+          const unsigned long long off = page < 0 ? 0ull
+                                         : is_v   ? page * a.c.vps + tok * a.c.vts
+                                                  : page * a.c.kps + tok * a.c.kts;
+          const unsigned long long foff = page < 0 ? 0ull
+                                          : is_v   ? page * a.f.vps + tok * a.f.vts
+                                                   : page * a.f.kps + tok * a.f.kts;
+          const uint32_t some = __ballot_sync(0xffffffffu, page >= 0) >> sub;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const unsigned long long o = __shfl_sync(0xffffffffu, off, u * RPI + sub), fo = __shfl_sync(0xffffffffu, foff, u * RPI + sub);
+            pc_cp_async16(dst + u * CODES, (is_v ? vcodes : kcodes) + o, 16u);
+            wa_cp_async4(fdst + u * 512, (is_v ? vfactors : kfactors) + fo, (some >> (u * RPI)) & 1u ? 4u : 0u);
+          }
         }
         pc_cp_commit();
         in = in + 1 == AHEAD ? 0 : in + 1;
@@ -813,6 +835,10 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
               break;
             }
             j = 0;
+            kcodes = a.c.k + w.c * a.c.khs + ch * 16;
+            vcodes = a.c.v + w.c * a.c.vhs + ch * 16;
+            kfactors = a.f.k + w.c * a.f.khs + (ch >> 1) * 4;
+            vfactors = a.f.v + w.c * a.f.vhs + (ch >> 1) * 4;
             page_next = lookup(0, &tok_next);
             continue;
           }
@@ -1418,6 +1444,7 @@ extern "C" fm_status fm_paged_window_attn_fp4(const fm_paged_cache* cache, const
   if (st == FM_OK) st = scale_ref(cache, scales, who, &a.f);
   if (st == FM_OK) st = window_args(cache, p, who, &a, &pl);
   if (st != FM_OK || cache->requests == 0 || p->rows == 0) return st;
+  a.nr = narrow_ref(a.c, a.f, cache->head_dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool duo = p->max_q * a.G <= 128;
   return cache->head_dim == 128 ? launch_window<128, 4>(a, pl, duo, s) : launch_window<64, 4>(a, pl, duo, s);
