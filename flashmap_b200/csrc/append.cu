@@ -67,15 +67,22 @@ __device__ __forceinline__ void unpack8(const uint4& u, float* x) {
   }
 }
 
-// Request of token t, or -1; by one warp.
+// Request of token t (the first whose rows end behind it), or -1; by one warp,
+// which narrows the requests down to a 32nd at a time.
 __device__ __forceinline__ int append_request(const AppendArgs& a, int t) {
   if (a.cu == nullptr) return t;
   const int lane = threadIdx.x & 31;
-  for (int r0 = 0; r0 < a.c.R; r0 += 32) {
-    const unsigned hit = __ballot_sync(0xffffffffu, r0 + lane < a.c.R && a.cu[r0 + lane + 1] > t);
-    if (hit) return r0 + __ffs(hit) - 1;
+  int lo = 0, hi = a.c.R;  // it is one of lo .. hi - 1, or none
+  while (hi - lo > 32) {
+    const int step = (hi - lo + 31) / 32, last = min(lo + (lane + 1) * step, hi) - 1;
+    const unsigned hit = __ballot_sync(0xffffffffu, a.cu[last + 1] > t);
+    if (!hit) return -1;
+    const int w = __ffs(hit) - 1;
+    hi = min(lo + (w + 1) * step, hi);
+    lo = lo + w * step;
   }
-  return -1;
+  const unsigned hit = __ballot_sync(0xffffffffu, lo + lane < hi && a.cu[lo + lane + 1] > t);
+  return hit ? lo + __ffs(hit) - 1 : -1;
 }
 
 // x / d to the last bit where neither is out of range, r = 1 / d rounded: the
@@ -116,7 +123,7 @@ __global__ void __launch_bounds__(256, 4) append_kernel(AppendArgs a) {
   bool ok = true;
   if (a.cu != nullptr) {
     const int q0 = a.cu[r], n = a.cu[r + 1] - q0;
-    ok = q0 >= 0 && n <= a.T - q0 && t >= q0;
+    ok = q0 >= 0 && n <= a.T - q0 && t >= q0 && t < q0 + n;
     j = len - n + (t - q0);
   }
   ok = ok && len >= 0 && len <= a.c.max_len;

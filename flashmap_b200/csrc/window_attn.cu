@@ -1195,6 +1195,10 @@ __global__ void __launch_bounds__(512, 1) window_attn_kernel(WindowArgs a) {
               w.q0 = a.cu[cur.r];
               w.row0 = row0;
               w.rows = min(WA_ROWS, nq * a.G - row0);
+              if (Lay::QT == 1 && w.rows > 128) {  // more rows than the call was sized for: there is no room for their queries
+                if (lane == 0) record_error(a.err, DEV_BAD_INDEX);
+                w.rows = 128;
+              }
               w.pos0 = keys.pos0;
               w.p_hi = keys.p_hi;
               w.lo = keys.lo;

@@ -267,6 +267,22 @@ def test_rows_without_a_place():
         assert error_word() == 4, bounds
 
 
+def test_many_requests():
+    """Rows found among more requests than a warp has lanes, and than its square; some without rows."""
+    g = torch.Generator().manual_seed(38)
+    for n in (33, 700, 1500):
+        rows = [int(x) for x in torch.randint(0, 3, (n,), generator=g)]
+        rows[0], rows[-1] = 0, 2
+        lengths = [r + int(x) for r, x in zip(rows, torch.randint(0, 4, (n,), generator=g))]
+        cache = Cache(g, lengths, 1, 64, 4, "fp4", "joint")
+        T = sum(rows)
+        k, v = (torch.randn(T + 3, 1, 64, generator=g).to(torch.bfloat16) for _ in range(2))
+        expect(cache, k, v, rows)
+        (kc, vc, L, table), kw = cache.args()
+        ops().append_paged_context(k.to(DEV), v.to(DEV), kc, vc, L, table, cu_seqlens_q=torch.tensor([0] + rows).cumsum(0).int().to(DEV), **kw)
+        assert cache.same() and error_word() == 0
+
+
 def test_strides_streams_graphs_and_far_pages():
     g = torch.Generator().manual_seed(35)
     H, KH, D, page = 4, 2, 64, 16

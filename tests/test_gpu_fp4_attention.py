@@ -246,6 +246,19 @@ def test_bad_indices_are_reported_and_not_seen():
     assert float(cache.decode(q, top=60).abs().max()) == 0.0 and error_word() == 4
 
 
+def test_more_rows_than_the_call_is_sized_for():
+    """max_seqlen_q says 10 rows of 4 heads (one row tile), a request has 50: recorded; the other request is as it should be."""
+    g = torch.Generator().manual_seed(60)
+    cache = Cache(g, [300, 200], 1, 128, 16, "joint")
+    q = torch.randn(60, 4, 128, generator=g).to(torch.bfloat16)
+    L, table = cache.rest()
+    cu = torch.tensor([0, 50, 60], dtype=torch.int32)
+    got = ops().paged_window_attention_fp4(q.to(DEV), *cache.tensors(), cu.to(DEV), L, table, 10, 300, 128 ** -0.5)
+    want, mag, _ = C.window_attention(q, *cache.host(), cu, cache.lengths, cache.table, 128 ** -0.5)
+    assert error_word() == 4
+    close(got[50:], want[50:], mag[50:], "window")
+
+
 def test_strides_streams_graphs_and_far_pages():
     g = torch.Generator().manual_seed(57)
     D, KH, page = 64, 2, 16
