@@ -45,6 +45,16 @@ def error_word(device) -> torch.Tensor:
     return w
 
 
+_ERR_ADDRESSES: dict = {}  # device index -> address of its error word, which lives as long as the process
+
+
+def _error_address(device) -> int:
+    at = _ERR_ADDRESSES.get(device.index)
+    if at is None:
+        at = _ERR_ADDRESSES[device.index] = error_word(device).data_ptr()
+    return at
+
+
 def _logits_dtype(t) -> int:
     if not t.is_cuda or not t.is_contiguous() or t.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"logits must be a contiguous CUDA bf16 or fp32 tensor, got {t.dtype} on {t.device}")
@@ -239,13 +249,14 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, t
         raise ValueError(f"top_k must lie in 0 .. {min(V, _lib.FM_TOKEN_LOGPROBS_MAX_TOP)}, got {top_k}")
     if not 0.0 < temperature < math.inf:
         raise ValueError(f"the temperature must be positive, got {temperature}")
-    if V > 1 and logits.stride(-1) != 1:
+    if V > 1 and logits.stride()[-1] != 1:
         raise ValueError("a row of logits must be contiguous")
     if len(shape) != 1:
         logits = logits.reshape(-1, V)
     rows = logits.shape[0]
     f32 = torch.float32
-    out = logits.new_empty((2,) + shape, dtype=f32)
+    logprobs = logits.new_empty(shape, dtype=f32)
+    entropy = torch.empty_like(logprobs)
     ids = tokens.new_empty(shape + (top_k,))
     top = logits.new_empty(shape + (top_k,), dtype=f32)
     if rows:
@@ -253,12 +264,11 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, t
         need = _logprobs_workspace(dev.index, rows, V, dt, top_k)
         ws = tokens.new_empty(need // 8) if need else None  # sizes are multiples of 16
         status = _lib.load().fm_token_logprobs(
-            logits.data_ptr(), dt, logits.stride(0), tokens.data_ptr(), rows, V, temperature, top_k, out.data_ptr(),
-            out.data_ptr() + 4 * rows, ids.data_ptr(), top.data_ptr(), ws.data_ptr() if need else None, need,
-            error_word(dev).data_ptr(), torch._C._cuda_getCurrentRawStream(dev.index))
+            logits.data_ptr(), dt, logits.stride()[0], tokens.data_ptr(), rows, V, temperature, top_k, logprobs.data_ptr(),
+            entropy.data_ptr(), ids.data_ptr(), top.data_ptr(), ws.data_ptr() if need else None, need, _error_address(dev),
+            torch._C._cuda_getCurrentRawStream(dev.index))
         if status:
             _lib.check(status, "fm_token_logprobs")
-    logprobs, entropy = out.unbind(0)
     return TokenLogprobs(logprobs, entropy, ids, top)
 
 
