@@ -102,7 +102,7 @@ __device__ __forceinline__ uint4 ap_bf16x8(const float* x) {
 // found once for all of them, and addresses step from slot to slot.
 template <int HD, int KIND, int ROPE>
 __global__ void __launch_bounds__(256, 4) append_kernel(AppendArgs a) {
-  constexpr int LPR = HD / 8, RPW = 32 / LPR, U = 2;  // U: slots whose rows are read at a time
+  constexpr int LPR = HD / 8, RPW = 32 / LPR, U = 4;  // U: slots whose rows are read at a time
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const int at = lane % LPR, sub = lane / LPR, d0 = at * 8;
   const int QW = (a.H + RPW - 1) / RPW, KW = (a.c.KH + RPW - 1) / RPW, slots = QW + 2 * KW;
@@ -181,19 +181,16 @@ __global__ void __launch_bounds__(256, 4) append_kernel(AppendArgs a) {
       }
     }
   };
-  const int to_mate = first ? half : -half;
+  const int mate_lane = ROPE == AP_HALVES && turned ? lane + (first ? half : -half) / 8 : lane;  // holds the values that this lane's are rotated with
   // rows s .. of a kind with `heads` heads, U slots at a time: f(x, head) for each, the last slot's lanes without a row left out
   auto rows = [&](const __nv_bfloat16* src, long long hs, int from, int to, int heads, auto with_mate, auto&& f) {
     const __nv_bfloat16* row = src + (from * RPW + sub) * hs + d0;
     const long long step = RPW * hs;
     for (int s = from; s < to; s += U) {
-      uint4 own[U], mate[U];
+      uint4 own[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (s + u < to && (s + u) * RPW + sub < heads) {
-          own[u] = *reinterpret_cast<const uint4*>(row);
-          if (decltype(with_mate)::value && ROPE == AP_HALVES && turned) mate[u] = *reinterpret_cast<const uint4*>(row + to_mate);
-        }
+        if (s + u < to && (s + u) * RPW + sub < heads) own[u] = *reinterpret_cast<const uint4*>(row);
         row += step;
       }
 #pragma unroll
@@ -201,7 +198,16 @@ __global__ void __launch_bounds__(256, 4) append_kernel(AppendArgs a) {
         if (s + u >= to) break;
         float x[8];
         unpack8(own[u], x);
-        if (decltype(with_mate)::value) rotate(x, mate[u]);
+        if constexpr (decltype(with_mate)::value) {
+          uint4 mate = own[u];
+          if constexpr (ROPE == AP_HALVES) {
+            mate.x = __shfl_sync(0xffffffffu, own[u].x, mate_lane);
+            mate.y = __shfl_sync(0xffffffffu, own[u].y, mate_lane);
+            mate.z = __shfl_sync(0xffffffffu, own[u].z, mate_lane);
+            mate.w = __shfl_sync(0xffffffffu, own[u].w, mate_lane);
+          }
+          rotate(x, mate);
+        }
         f(x, (s + u) * RPW + sub);
       }
     }

@@ -453,9 +453,12 @@ __global__ void __launch_bounds__(LP_T, 4) logprob_scan_kernel(LogprobArgs a) {
     }
   };
   const uint4* base = reinterpret_cast<const uint4*>(x.x - x.shift) + lane;
+  const uint4* at = base;  // of the batch that comes next
   auto fetch = [&](uint4* u, int l1) {
+    if constexpr (LONG) at = base + l1 * 32;
 #pragma unroll
-    for (int q = 0; q < LP_LOADS; ++q) u[q] = __ldcs(base + (l1 + q) * 32);
+    for (int q = 0; q < LP_LOADS; ++q) u[q] = __ldcs(at + q * 32);
+    at += W * LP_LOADS * 32;
   };
   // Batches of the warp: span after span, so that a group is one warp's.
   const int span = LONG ? 1 << a.gs : LP_LOADS;
@@ -480,6 +483,7 @@ __global__ void __launch_bounds__(LP_T, 4) logprob_scan_kernel(LogprobArgs a) {
   const int stop = min(end, whole_end);
   if (l1 < stop) {
     uint4 u[LP_LOADS], w[LP_LOADS];
+    at = base + l1 * 32;
     fetch(u, l1);
     while (true) {
       const int l2 = after(l1);
