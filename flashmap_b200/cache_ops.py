@@ -7,7 +7,11 @@
   prompt, a drafted block to verify) with a sliding window and first tokens
   that stay visible;
 * ``evict_paged_context``: cuts contexts to a budget of positions, those that
-  gathered the most attention weight among them.
+  gathered the most attention weight among them;
+* ``append_paged_context``: writes new tokens' keys and values, rotated on the
+  way, and rotates their queries;
+* ``paged_decode_attention_fp4`` and ``paged_window_attention_fp4``: the two
+  attentions on a cache held in 4 bits.
 
 The cache is given by two views ``k_cache`` and ``v_cache (pages, kv_heads,
 page_size, head_dim)``, bf16 or e4m3, whose rows are contiguous and 16-byte
@@ -18,17 +22,24 @@ size of 1.  Token i of request r is token ``i % page_size`` of page
 ``block_table[r, i // page_size]``.  An e4m3 cache takes ``descales (2,
 requests, kv_heads)``, the factors of keys and values.
 
+A 4-bit cache is ``k_cache`` and ``v_cache (pages, kv_heads, page_size, head_dim
+/ 2)`` uint8, e2m1 codes of 0, .5, 1, 1.5, 2, 3, 4, 6 and a sign bit, value 2 i in
+the low half of byte i, with ``k_scales`` and ``v_scales (pages, kv_heads,
+page_size, head_dim / 16)`` e4m3, the factor of each 16 values (rows of factors
+aligned to their 4 or 8 bytes): 0.5625 bytes a value.  ``append_paged_context``
+writes it, and f16 holds its values exactly.
+
 Query head h reads kv head ``h // (heads / kv_heads)``.  Scores, softmax sums
 and outputs are held in fp32; the softmax numerators are rounded to bf16 (to
-f16 for an e4m3 cache) for the product with the values, and the output to bf16.
+f16 for an e4m3 or 4-bit cache) for the product with the values, and the output to bf16.
 A row that sees no position is zero.  A position that no row of a request may
 see is never read.  Each call checks its arguments (``OpArgumentError``; the
 alignment of addresses and strides and the limits of sizes are the library's to
 check, ``FlashMapError``), records lengths, bounds and page ids out of range
 for ``check_device_errors``, runs on the current stream without a host
 synchronisation, and can be captured in a CUDA graph.  The two attentions are
-registered operators (``flashmap_b200::paged_decode_attention``,
-``::paged_window_attention``) to ``torch.compile``; they have no gradient, and
+registered operators (``flashmap_b200::paged_decode_attention[_fp4]``,
+``::paged_window_attention[_fp4]``) to ``torch.compile``; they have no gradient, and
 asking for one raises.  There is no fallback.
 """
 

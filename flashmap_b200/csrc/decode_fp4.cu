@@ -13,6 +13,12 @@
 // (in S) and of d (in O) may be chosen: a thread takes 16 consecutive
 // bytes of a key, and 8 of a value, as they lie.  Values of two keys
 // are paired for V^T by exchanging half bytes before the conversion.
+//
+// Measured, 32 heads on 8 of 128: 128 requests of 1024 .. 8192, 165 us (4.1 TB/s);
+// 1 request of 100003, 34 us (3.4 TB/s, of which 7 us are the join); 201
+// positions, 4.8 us.  No unit is full: the arithmetic pipe that converts is at 53
+// percent and issue slots at 59, with four warps to a scheduler (registers);
+// five, and a third stage of copies, measured the same, six spill.
 #include <type_traits>
 
 #include "decode_parts.cuh"

@@ -18,7 +18,10 @@
 // group is preceded by the k maxima of those.  Those groups are read once more
 // (from L2), what reaches the k-th maximum is kept, and sorted.
 //
-// The row's bytes bound it (one exponential, and five other operations to a value).
+// The row's bytes bound it, and beside them one exponential and about eight other
+// instructions to a value: 1088 bf16 rows of 151936, 56 us (5.9 TB/s), 81 us with
+// 20 alternatives, whose own launch is bound by instructions (13 million);
+// 1999 fp32 rows of 32003, half of it -inf, 44 us (5.8 TB/s); one row, 8 us for two launches.
 #include <type_traits>
 
 #include "common.cuh"
