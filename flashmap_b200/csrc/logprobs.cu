@@ -21,8 +21,9 @@
 // The row's bytes bound it, and beside them one exponential and about eight other
 // instructions to a value: 1088 bf16 rows of 151936, 56 us (5.9 TB/s), 81 us with
 // 20 alternatives, whose own launch is bound by instructions (13 million);
-// 1999 fp32 rows of 32003, half of it -inf, 44 us (5.8 TB/s); one row, 8 us for two launches.
-#include <type_traits>
+// 1999 fp32 rows of 32003, half of it -inf, 44 us (5.8 TB/s);
+// one bf16 row of 151936, 8.4 us with 5 alternatives, 10 us with 20.
+#include <algorithm>
 
 #include "common.cuh"
 #include "launch.cuh"
@@ -31,6 +32,7 @@ namespace fm {
 namespace {
 
 constexpr int LP_T = 256;
+constexpr int LP_SLICES = 8;       // of a row at most: a cluster
 constexpr int LP_LOADS = 4;        // warp loads in flight
 constexpr int LP_GROUPS = 256;     // groups of a row at most: one to a thread
 constexpr int LP_HITS = 512;
@@ -50,7 +52,7 @@ struct LogprobArgs {
   float* entropy;
   long long* ids;
   float* top;
-  float4* part;  // [rows][slices] (m, S, U)
+  float4* part;  // [rows] (m, S, U)
   float* gmax;   // [rows][groups]
   int* err;
 };
@@ -143,20 +145,9 @@ __device__ __forceinline__ bool lp_fast(float m, float c) { return fabsf(m * c) 
 __device__ __forceinline__ float lp_diff(float x, float m, float c) {
   return lp_fast(m, c) && lp_fast(x, c) ? __fsub_rn(__fmul_rn(x, c), __fmul_rn(m, c)) : (x - m) * c;
 }
-// both of one row
-__device__ __forceinline__ LpSum lp_join(const LpSum& a, const LpSum& b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return LpSum{m, a.s + b.s, a.u + b.u};  // sums of nothing, or NaN
-  LpSum r{m, 0.0f, 0.0f};
-  auto add = [&](const LpSum& v) {
-    if (v.m == -INFINITY && v.s == 0.0f) return;  // saw nothing
-    const float d = v.m == m ? 0.0f : fmaxf(lp_diff(v.m, m, c), -1000.0f), f = lp_ex2(d);
-    r.s += f * v.s;
-    r.u += f * (v.u + d * v.s);
-  };
-  add(a);
-  add(b);
-  return r;
+// to the same place in the first CTA of the cluster
+__device__ __forceinline__ void lp_store_first(const float* at, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(at), 0)), "f"(v) : "memory");
 }
 
 template <typename K>
@@ -361,17 +352,21 @@ __device__ __forceinline__ LpSum lp_block_join(LpSum v, float c, LpShared<TOP>& 
 // Block (row, slice): warp loads slice * per .. of the row, LP_LOADS of them at a
 // time to a warp (a batch), the next batch on its way meanwhile.  Batches that
 // do not lie in the row altogether come last.
-// LONG: groups of more than a batch.
-template <typename T, bool TOP, bool LONG>
+// LONG: groups of more than a batch.  CLUSTER: a row's slices are a cluster of
+// CTAs, which hand their sums and maxima to the first, and that finishes the row.
+template <typename T, bool TOP, bool LONG, bool CLUSTER>
 __global__ void __launch_bounds__(LP_T, 4) logprob_scan_kernel(LogprobArgs a) {
-  __shared__ LpShared<false> sh;
+  __shared__ LpShared<CLUSTER && TOP> sh;
+  __shared__ float row_gmax[CLUSTER && TOP ? LP_GROUPS : 1];
+  __shared__ LpSum row_part[CLUSTER ? LP_SLICES : 1];
+  if constexpr (CLUSTER) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_wait();
   const int row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
   const LpRow<T> x(a, row);
   constexpr int N = LpRow<T>::N, W = LP_T / 32;
   const int loads = (x.pieces + 31) / 32, end = min(loads, (slice + 1) * a.per);
-  float* gmax = a.gmax + (long long)row * a.groups;
+  float* gmax = CLUSTER ? row_gmax : a.gmax + (long long)row * a.groups;
   LpSum v{-INFINITY, 0.0f, 0.0f};
   const float2 c2 = make_float2(a.c, a.c);
 
@@ -503,11 +498,27 @@ __global__ void __launch_bounds__(LP_T, 4) logprob_scan_kernel(LogprobArgs a) {
   }
   for (; l1 < end; l1 = after(l1)) edge(l1);
   v = lp_block_join(v, a.c, sh);
-  if (a.part != nullptr) {
-    if (threadIdx.x == 0) a.part[(long long)row * a.slices + slice] = make_float4(v.m, v.s, v.u, 0.0f);
-    return;
+  if constexpr (CLUSTER) {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // all have begun: their shared memory is there
+    if (TOP && slice > 0) {
+      const int g1 = min((loads + (1 << a.gs) - 1) >> a.gs, ((slice + 1) * a.per) >> a.gs);
+      for (int g = ((slice * a.per) >> a.gs) + (int)threadIdx.x; g < g1; g += LP_T) lp_store_first(&row_gmax[g], row_gmax[g]);
+    }
+    if (threadIdx.x == 0) {
+      lp_store_first(&row_part[slice].m, v.m);
+      lp_store_first(&row_part[slice].s, v.s);
+      lp_store_first(&row_part[slice].u, v.u);
+    }
+    cluster_sync();
+    if (slice > 0) return;
+    v = lp_warp_join(lane < a.slices ? row_part[lane] : LpSum{-INFINITY, 0.0f, 0.0f}, a.c);
+    lp_finish<T, TOP>(a, row, v, row_gmax, sh);
+  } else if (TOP) {
+    if (threadIdx.x == 0) a.part[row] = make_float4(v.m, v.s, v.u, 0.0f);
+  } else {
+    lp_finish<T, false>(a, row, v, nullptr, sh);
   }
-  lp_finish<T, false>(a, row, v, nullptr, sh);
 }
 
 template <typename T>
@@ -515,44 +526,67 @@ __global__ void __launch_bounds__(LP_T, 6) logprob_join_kernel(LogprobArgs a) {
   __shared__ LpShared<true> sh;
   pdl_wait();
   const int row = blockIdx.x;
-  LpSum v{-INFINITY, 0.0f, 0.0f};
-  for (int s = threadIdx.x; s < a.slices; s += LP_T) {
-    const float4 p = a.part[(long long)row * a.slices + s];
-    v = lp_join(v, LpSum{p.x, p.y, p.z}, a.c);
-  }
-  v = lp_block_join(v, a.c, sh);
+  const float4 p = a.part[row];
+  const LpSum v{p.x, p.y, p.z};
   lp_finish<T, true>(a, row, v, a.gmax + (long long)row * a.groups, sh);
 }
 
+// Rows for four blocks to an SM: a block to a row, and where alternatives are
+// wanted a second launch for them (1088 rows, 20 alternatives: 81 us; in the same
+// launch 83 us, since all blocks come to that at once).  Fewer rows are cut into up
+// to eight slices, a cluster to a row, in one launch: as fast on the device as with
+// partial sums in memory and a second launch (1 row 8.4 and 8.2 us, 32 rows with
+// 20 alternatives 11.4 and 12.2), and a call costs the host 4 us less.  As many
+// slices as are at work at once, no more (200 rows: 2 slices 22 us, 3 slices 24 us;
+// 300 rows of 32003: 1 slice 13 us, 2 slices 18 us).
 struct LogprobPlan {
   int gs, groups, slices, per;
+  bool cluster;
   size_t part, total;
 };
 LogprobPlan logprob_plan(int64_t rows, int64_t V, int64_t esz, int64_t k) {
   LogprobPlan p{};
-  const int64_t load = 512 / esz, loads = (V + 16 / esz - 1 + load - 1) / load + 1;
+  const int64_t load = 512 / esz, loads = (V + 16 / esz - 1 + load - 1) / load + 1, fill = 4 * num_sms();
   p.gs = 1;  // of two loads or more: what is read again is little, and there are fewer to draw from
   while (((loads - 1) >> p.gs) + 1 > LP_GROUPS) ++p.gs;
   p.groups = (int)(((loads - 1) >> p.gs) + 1);
   const int64_t span = 1 << p.gs > LP_LOADS ? 1 << p.gs : LP_LOADS, least = span * (LP_T / 32);
-  int64_t slices = (4 * num_sms() + rows - 1) / rows;
-  const int64_t most = (loads + least - 1) / least;
-  if (slices > most) slices = most;
+  p.cluster = rows < fill;
+  int64_t slices = std::max<int64_t>(fill / rows, 1);
+  slices = std::min<int64_t>(std::min<int64_t>(slices, LP_SLICES), (loads + least - 1) / least);
   p.per = (int)(((loads + slices - 1) / slices + span - 1) / span * span);
   p.slices = (int)((loads + p.per - 1) / p.per);
-  p.part = p.slices > 1 || k ? (size_t)rows * p.slices * sizeof(float4) : 0;
-  p.total = p.part + (k ? ((size_t)rows * p.groups * 4 + 15) / 16 * 16 : 0);
+  p.part = !p.cluster && k ? (size_t)rows * sizeof(float4) : 0;
+  p.total = p.part + (p.part ? ((size_t)rows * p.groups * 4 + 15) / 16 * 16 : 0);
   return p;
 }
 
-template <typename T>
+template <typename T, bool CLUSTER>
 fm_status launch_logprobs(const LogprobArgs& a, cudaStream_t s) {
-  auto kernel = a.k == 0      ? logprob_scan_kernel<T, false, false>
-                : a.gs <= 2 ? logprob_scan_kernel<T, true, false>
-                            : logprob_scan_kernel<T, true, true>;
-  const fm_status st = launch_kernel(kernel, dim3((unsigned)(a.rows * (int64_t)a.slices)), dim3(LP_T), 0, s, true, a);
-  if (st != FM_OK || a.part == nullptr) return st;
+  auto kernel = a.k == 0      ? logprob_scan_kernel<T, false, false, CLUSTER>
+                : a.gs <= 2 ? logprob_scan_kernel<T, true, false, CLUSTER>
+                            : logprob_scan_kernel<T, true, true, CLUSTER>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(a.rows * (int64_t)a.slices));
+  cfg.blockDim = dim3(LP_T);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)a.slices;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CLUSTER ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e != cudaSuccess) return set_error(FM_ERR_LAUNCH, "token_logprobs: launch failed: %s", cudaGetErrorString(e));
+  ++launch_counter();
+  if (CLUSTER || a.k == 0) return FM_OK;
   return launch_kernel(logprob_join_kernel<T>, dim3((unsigned)a.rows), dim3(LP_T), 0, s, true, a);
+}
+template <typename T>
+fm_status launch_logprobs(const LogprobArgs& a, bool cluster, cudaStream_t s) {
+  return cluster ? launch_logprobs<T, true>(a, s) : launch_logprobs<T, false>(a, s);
 }
 
 bool logprob_sizes(int64_t rows, int64_t V, int32_t dtype, int64_t k) {
@@ -604,9 +638,9 @@ extern "C" fm_status fm_token_logprobs(const void* logits, int32_t dtype, int64_
   a.entropy = entropy;
   a.ids = reinterpret_cast<long long*>(top_ids);
   a.top = top_logprobs;
-  a.part = pl.part ? static_cast<float4*>(workspace) : nullptr;
+  a.part = static_cast<float4*>(workspace);
   a.gmax = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.part);
   a.err = err;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == FM_DT_F32 ? launch_logprobs<float>(a, s) : launch_logprobs<__nv_bfloat16>(a, s);
+  return dtype == FM_DT_F32 ? launch_logprobs<float>(a, pl.cluster, s) : launch_logprobs<__nv_bfloat16>(a, pl.cluster, s);
 }

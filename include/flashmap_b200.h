@@ -573,7 +573,7 @@ FM_API fm_status fm_add(const void* a, const void* b, void* y, int64_t n, fm_str
  *   lowest id; top_k at most FM_TOKEN_LOGPROBS_MAX_TOP and V.
  * A row of -inf alone has logprobs -inf and entropy 0.  One that holds a NaN or
  * +inf has NaN for all (in the order of top_ids a NaN stands where -inf does).
- * The workspace need not be initialised. */
+ * The workspace need not be initialised; calls of few rows need none. */
 enum { FM_TOKEN_LOGPROBS_MAX_TOP = 32 };
 FM_API size_t fm_token_logprobs_workspace_size(int64_t rows, int64_t V, int32_t dtype, int64_t top_k);
 FM_API fm_status fm_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, const int64_t* tokens,

@@ -62,6 +62,8 @@ CASES = [
     (700, 5001, 5001, torch.bfloat16, 7, 0.8),
     (1, 1500001, 1500001, torch.bfloat16, 32, 1.0),
     (2, 700001, 700001, torch.float32, 3, 1.0),
+    (300, 9001, 9001, torch.bfloat16, 4, 1.0),
+    (597, 140001, 140001, torch.float32, 3, 1.0),
 ]
 
 
@@ -139,6 +141,27 @@ def test_nan_and_infinity():
     want = torch.where(torch.isnan(x[0]), -math.inf, x[0]).topk(3).indices
     assert torch.equal(got.top_ids[0].cpu(), want) and int(got.top_ids[1, 0]) == 4999
     assert got.top_ids[2].tolist() == [0, 1, 2]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_masks_over_most_of_a_long_row(dtype):
+    """Rows long enough to be several blocks' work, of which some see -inf, the lowest value, or NaN alone."""
+    V, low = 400003, torch.finfo(dtype).min
+    x = 2.0 * torch.randn(6, V, generator=torch.Generator().manual_seed(46))
+    x[0, :V // 2 + 7] = -math.inf
+    x[1, 9:] = -math.inf
+    x[2, 100:] = low
+    x[3] = -math.inf
+    x[4] = low
+    x[5, V - 1] = math.nan
+    x = x.to(dtype).to(DEV)
+    tokens = torch.tensor([V - 1, 3, 50, 5, V // 2, 1], device=DEV)
+    for k in (0, 32):
+        got = call(x, tokens, top_k=k)
+        check(type(got)(*[t[:5] for t in got]), x[:5], tokens[:5], k, 1.0)
+        assert torch.isnan(got.logprobs[5]) and torch.isnan(got.entropy[5]) and torch.isnan(got.top_logprobs[5]).all()
+    assert torch.equal(got.top_ids[5], torch.where(torch.isnan(x[5]), -math.inf, x[5]).float().sort(stable=True, descending=True).indices[:32])
+    assert error_word() == 0
 
 
 def test_ids_outside_the_vocabulary():

@@ -88,12 +88,13 @@ def test_logprobs_refusals():
                      (dict(V=2), SHAPE), (dict(k=-1), SHAPE), (dict(V=1 << 31), SHAPE), (dict(T=0.0), INVALID),
                      (dict(T=math.nan), INVALID), (dict(T=math.inf), INVALID), (dict(logits=None), INVALID),
                      (dict(tokens=None), INVALID), (dict(ids=None), INVALID), (dict(logits=(1 << 20) + 1), ALIGN),
-                     (dict(V=151936, rows=1, ws=None), WORKSPACE), (dict(V=151936, rows=1, size=8), WORKSPACE),
-                     (dict(V=151936, rows=1, ws=(1 << 23) + 8), ALIGN)):
+                     (dict(V=151936, rows=1000, ws=None), WORKSPACE), (dict(V=151936, rows=1000, size=8), WORKSPACE),
+                     (dict(V=151936, rows=1000, ws=(1 << 23) + 8), ALIGN)):
         assert status(**kw) == want, kw
     assert status(rows=0) == 0
     assert lib.fm_token_logprobs_workspace_size(0, 100, 0, 0) == 0
-    assert lib.fm_token_logprobs_workspace_size(1, 151936, 0, 5) > 0
+    assert lib.fm_token_logprobs_workspace_size(1000, 151936, 0, 5) > 0
+    assert lib.fm_token_logprobs_workspace_size(1, 151936, 0, 5) == 0 == lib.fm_token_logprobs_workspace_size(1000, 151936, 0, 0)
 
 
 def test_four_bit_rows():
