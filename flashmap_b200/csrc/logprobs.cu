@@ -611,6 +611,8 @@ extern "C" fm_status fm_token_logprobs(const void* logits, int32_t dtype, int64_
   if (!logprob_sizes(rows, V, dtype, top_k)) return set_error(FM_ERR_SHAPE, "token_logprobs: bad shape");
   if (!(temperature > 0.0f && temperature < INFINITY))
     return set_error(FM_ERR_INVALID, "token_logprobs: the temperature must be positive");
+  if (!(LP_LOG2E / temperature < INFINITY))
+    return set_error(FM_ERR_INVALID, "token_logprobs: the temperature's reciprocal is past fp32's range");
   if (rows == 0) return FM_OK;
   if (!logits || !tokens || !logprobs || !entropy || (top_k && (!top_ids || !top_logprobs)))
     return set_error(FM_ERR_INVALID, "token_logprobs: null pointer");

@@ -86,7 +86,7 @@ def test_logprobs_refusals():
 
     for kw, want in ((dict(dtype=_lib.FM_DT_E4M3), SHAPE), (dict(rows=-1), SHAPE), (dict(V=0), SHAPE), (dict(k=33, V=100), SHAPE),
                      (dict(V=2), SHAPE), (dict(k=-1), SHAPE), (dict(V=1 << 31), SHAPE), (dict(T=0.0), INVALID),
-                     (dict(T=math.nan), INVALID), (dict(T=math.inf), INVALID), (dict(logits=None), INVALID),
+                     (dict(T=4e-39), INVALID), (dict(T=math.nan), INVALID), (dict(T=math.inf), INVALID), (dict(logits=None), INVALID),
                      (dict(tokens=None), INVALID), (dict(ids=None), INVALID), (dict(logits=(1 << 20) + 1), ALIGN),
                      (dict(V=151936, rows=1000, ws=None), WORKSPACE), (dict(V=151936, rows=1000, size=8), WORKSPACE),
                      (dict(V=151936, rows=1000, ws=(1 << 23) + 8), ALIGN)):
