@@ -31,13 +31,7 @@ constexpr int D4_TILE = 32;  // keys of a warp's tile
 // request is cut into as many chunks as CTAs are resident (100003 positions,
 // 8 kv heads: 34 us, and 40 us in three times as many), and a batch into chunks
 // of 2048 keys (128 requests of 1024 .. 8192: 163 us; of 1024 keys 173 us, of 4096 170 us).
-#ifndef RL
-#define RL 1536
-#endif
-#ifndef RM
-#define RM 2048
-#endif
-constexpr DecodeRule D4_RULE{148 * 4, 128, RL, RM, 148 * 32};
+constexpr DecodeRule D4_RULE{148 * 4, 128, 1536, 2048, 148 * 32};
 
 // P goes to f16 times 2^11, and the subtracted maximum may lag behind the true
 // one by a factor 2^4: numerators stay below 2^15, and only those under 2^-25 of
@@ -126,7 +120,6 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
     return;
   }
   const int begin = chunk * size, end = min(sp.n, begin + size);
-
 
   const uint32_t wbase = smem_u32(d4_smem_buf) + warp * Lay::WARP;
   uint32_t* wok = reinterpret_cast<uint32_t*>(d4_smem_buf + d4_smem<HD, NG, STAGES>() - 4 * STAGES * 4) + warp * STAGES;
