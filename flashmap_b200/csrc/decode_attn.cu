@@ -17,7 +17,7 @@
 // into weights, since only then are a row's maximum and sum known.
 //
 // Measured, 32 heads on 8 of 128: 1 request of 49157, 44 us (4.6 TB/s, of which
-// 6 us are the join); 64 requests of 1024 .. 8192 with sums, 225 us (5.5 TB/s,
+// 5 us are the join); 64 requests of 1024 .. 8192 with sums, 225 us (5.5 TB/s,
 // the scores and the join included); 40 heads on 8, e4m3, 192 requests of
 // 512 .. 4096, 192 us (4.7 TB/s: no unit is full, each warp waits on its own chain);
 // 64 heads on 8 of 64, a window of 2048, 92 us (5.6 TB/s).

@@ -15,7 +15,7 @@
 // are paired for V^T by exchanging half bytes before the conversion.
 //
 // Measured, 32 heads on 8 of 128: 128 requests of 1024 .. 8192, 165 us (4.1 TB/s);
-// 1 request of 100003, 34 us (3.4 TB/s, of which 7 us are the join); 201
+// 1 request of 100003, 32 us (3.6 TB/s, of which 5 us are the join); 201
 // positions, 4.8 us.  No unit is full: the arithmetic pipe that converts is at 53
 // percent and issue slots at 59, with four warps to a scheduler (registers);
 // five, and a third stage of copies, measured the same, six spill.
@@ -29,7 +29,7 @@ namespace {
 constexpr int D4_TILE = 32;  // keys of a warp's tile
 // A CTA's first copies and its merge weigh more against 4-bit keys: one long
 // request is cut into as many chunks as CTAs are resident (100003 positions,
-// 8 kv heads: 34 us, and 40 us in three times as many), and a batch into chunks
+// 8 kv heads: 34 us, and 40 us in three times as many, both with a join slower by 2 us), and a batch into chunks
 // of 2048 keys (128 requests of 1024 .. 8192: 163 us; of 1024 keys 173 us, of 4096 170 us).
 constexpr DecodeRule D4_RULE{148 * 4, 128, 1536, 2048, 148 * 32};
 
