@@ -602,7 +602,7 @@ def append_paged_context(key: torch.Tensor, value: torch.Tensor, k_cache: torch.
     and ``query (tokens, heads, head_dim)`` bf16 on the way: the pairs (i, i + rotary_dim / 2) of the first
     ``rotary_dim`` values (a multiple of 16), or (2 i, 2 i + 1) when ``interleaved``.  A token stands at
     ``positions (tokens,)`` int32 or int64, or where those are not given at its place in the cache (a context that was
-    cut holds fewer positions than its text).  Returns the rotated queries ``(tokens, heads, head_dim)``, or None.
+    cut holds fewer positions than its text); rows that are not rotated stand nowhere else than in the cache.  Returns the rotated queries ``(tokens, heads, head_dim)``, or None.
 
     A bf16 cache takes the rotated values rounded; an e4m3 cache rounded and cut to +-448; a 4-bit cache (uint8, with
     ``k_scales`` and ``v_scales``) as e2m1 codes with one e4m3 factor for 16 values, their largest magnitude / 6.  The
@@ -652,7 +652,6 @@ def append_paged_context(key: torch.Tensor, value: torch.Tensor, k_cache: torch.
             angles = rope.data_ptr()
     at, at_dtype = 0, _lib.FM_DT_I32
     if positions is not None:
-        _need(rope is not None, "positions go with a rope table")
         _on(positions, "positions", dev)
         _need(positions.dtype in (torch.int32, torch.int64) and positions.shape == (tokens,)
               and positions.is_contiguous(), "positions must be contiguous int32 or int64 (tokens,)")

@@ -624,7 +624,7 @@ typedef struct fm_append {
   int64_t out_token_stride, out_head_stride;
   int64_t tokens;
   const int32_t* cu_seqlens_q; /* or NULL */
-  const void* positions;       /* or NULL */
+  const void* positions;       /* or NULL; read where there is a rope */
   int32_t positions_dtype;     /* FM_DT_I32 or FM_DT_I64 */
   const float* rope;           /* or NULL */
   int64_t rope_rows, rotary_dim;

@@ -165,6 +165,20 @@ def test_append(case):
     assert error_word() == 0
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3", "fp4"])
+def test_positions_of_rows_that_are_not_rotated(kind):
+    """Layers without a rotation take the positions of those that have one; values outside any table mean nothing."""
+    g = torch.Generator().manual_seed(38)
+    cache = Cache(g, [40, 17], 2, 64, 16, kind, "joint")
+    k, v = ((3.0 * torch.randn(8, 2, 64, generator=g)).to(torch.bfloat16) for _ in range(2))
+    expect(cache, k, v, [5, 3], None, False, None, None, None)
+    (kc, vc, L, table), kw = cache.args()
+    at = torch.tensor([0, 1, 900, -1, 7, 1 << 40, 2, 3], device=DEV)
+    assert ops().append_paged_context(k.to(DEV), v.to(DEV), kc, vc, L, table, positions=at,
+                                      cu_seqlens_q=torch.tensor([0, 5, 8], dtype=torch.int32, device=DEV), **kw) is None
+    assert cache.same() and error_word() == 0
+
+
 def test_formula_in_64_bits():
     g = torch.Generator().manual_seed(32)
     D, KH, L = 128, 2, 200
@@ -365,7 +379,7 @@ def test_refusals():
     refused(rows, rows, kc, vc, L, table, rope=rope[:, :4], **kw)
     refused(rows, rows, kc, vc, L, table, rope=rope.double(), **kw)
     refused(rows, rows, kc, vc, L, table, rope=table_of(32, 128).to(DEV), **kw)
-    refused(rows, rows, kc, vc, L, table, positions=L, **kw)
+    refused(rows, rows, kc, vc, L, table, positions=L.float(), **kw)
     refused(rows, rows, kc, vc, L, table, rope=rope, positions=L[:1], **kw)
     refused(rows, rows, kc, vc, L.long(), table, **kw)
     refused(rows, rows, kc, vc, L, table, cu_seqlens_q=L, **kw)
