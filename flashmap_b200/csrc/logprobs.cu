@@ -9,8 +9,8 @@
 //   d' = d + a, a = c (m - m'):  S' = 2^a S,  U' = 2^a (U + a S).
 // d is formed as c x - round(c m), one multiplication and addition, and c (m - m')
 // as the difference of the same rounded products, so that their rounding
-// cancels; only where c m is no ordinary number (rows of a type's lowest value,
-// tiny T) as c (x - m).
+// cancels; only where |c m| is 2^24 or more (rows of a mask's value, tiny T) as
+// c (x - m), since a rounding of 2^7 and more would be past the exponentials' range.
 //
 // Alternatives.  The pass also leaves the maximum of every group of one or more
 // warp loads (512 bytes each).  The k largest values, equal ones by the lowest id, lie in the
@@ -140,10 +140,17 @@ __device__ __forceinline__ float2 lp_range(const uint4& u) {
 struct LpSum {
   float m, s, u;
 };
-// c (x - m); `fast` where c m is an ordinary number
-__device__ __forceinline__ bool lp_fast(float m, float c) { return fabsf(m * c) < 1e30f; }
+// A running m stands for the power c m: as the rounded product where that is
+// within a half (|c m| < 2^24: what it is off by goes into every term and out with
+// log2 S), else as c m itself, whose differences are formed as c (x - m).
+__device__ __forceinline__ bool lp_fast(float m, float c) { return fabsf(m * c) < 16777216.0f; }
+// the power of x less that of m
 __device__ __forceinline__ float lp_diff(float x, float m, float c) {
-  return lp_fast(m, c) && lp_fast(x, c) ? __fsub_rn(__fmul_rn(x, c), __fmul_rn(m, c)) : (x - m) * c;
+  const bool fx = lp_fast(x, c), fm = lp_fast(m, c);
+  return fx && fm ? __fsub_rn(__fmul_rn(x, c), __fmul_rn(m, c))
+         : fm     ? fmaf(x, c, -__fmul_rn(m, c))
+         : fx     ? -fmaf(m, c, -__fmul_rn(x, c))
+                  : (x - m) * c;
 }
 // to the same place in the first CTA of the cluster
 __device__ __forceinline__ void lp_store_first(const float* at, float v) {
@@ -390,9 +397,9 @@ __global__ void __launch_bounds__(LP_T, 4) logprob_scan_kernel(LogprobArgs a) {
     }
     const float off = v.m == -INFINITY ? 0.0f : __fmul_rn(v.m, a.c);
     float2 s2 = make_float2(v.s, 0.0f), u2 = make_float2(v.u, 0.0f);
-    // 2^d d is 0 where d is -inf; where no value is so low that d could be, and c m is an ordinary number, nothing is guarded
-    if (__any_sync(0xffffffffu, !(fabsf(off) < 1e30f && low * a.c > -1e30f))) {
-      const bool fast = fabsf(off) < 1e30f;
+    // 2^d d is 0 where d is -inf; where no value is so low that d could be, and c m goes by its rounded product, nothing is guarded
+    const bool fast = fabsf(off) < 16777216.0f;
+    if (__any_sync(0xffffffffu, !(fast && low * a.c > -1e30f))) {
       const float m = v.m == -INFINITY ? 0.0f : v.m;
 #pragma unroll
       for (int q = 0; q < LP_LOADS; ++q) {

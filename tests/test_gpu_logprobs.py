@@ -220,3 +220,31 @@ def test_refusals():
                  ((x.clone().requires_grad_(), t), {}), ((x[:, :0], t), {})):
         with pytest.raises((ValueError, RuntimeError)):
             call(*a, **k)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [9, 603])  # a cluster to a row, a block to a row
+@pytest.mark.parametrize("T", [1.0, 0.7, 0.01])
+def test_large_logits(dtype, rows, T):
+    """Logits whose products with log2(e) / T are rounded by more than the exponentials' range (masks of -1e10 or -1e30 all
+    over a row, single large ones), and ones about 2^24, where the kernel changes how it forms differences."""
+    V, g = 3001, torch.Generator().manual_seed(48)
+    x = 2.0 * torch.randn(rows, V, generator=g)
+    border = round(2.0 ** 24 * T / math.log2(math.e))
+    x[0] = -1e10
+    x[1] *= 1e10
+    x[2] = -7e29
+    x[2, 50:60] = -6.9e29
+    x[3, 77] = 1e12
+    x[4] = border + torch.randint(-4, 5, (V,), generator=g)
+    x[5] = -border + torch.randint(-4, 5, (V,), generator=g)
+    x[6] = -1e9
+    x[6, 3::7] = -1e9 + 64
+    x[7] = -3.3e30
+    x[7, :1500] = -1e4
+    x = x.to(dtype).to(DEV)
+    tokens = torch.randint(0, V, (rows,), generator=g).to(DEV)
+    for k in (0, 5):
+        got = call(x, tokens, top_k=k, temperature=T)
+        check(type(got)(*[t[:9] for t in got]), x[:9], tokens[:9], k, T)
+    assert error_word() == 0
