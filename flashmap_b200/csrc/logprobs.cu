@@ -44,7 +44,7 @@ struct LogprobArgs {
   long long ld;  // elements between rows
   int V, rows;
   const long long* tokens;
-  float c, lag;    // log2(e) / T, 8 / c
+  float t, c, lag; // T, log2(e) / T, 8 / c
   int k, gs;       // 2^gs warp loads make a group
   int groups;      // room for a row's group maxima
   int slices, per; // CTAs of a row, warp loads of each
@@ -199,7 +199,14 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float log_s = log2f(all.s);
   const bool none = all.m == -INFINITY && all.s == 0.0f;  // -inf alone
-  auto logprob = [&](float v) { return none ? -INFINITY : LP_LN2 * ((lp_fast(all.m, a.c) ? fmaf(v, a.c, -__fmul_rn(all.m, a.c)) : (v - all.m) * a.c) - log_s); };
+  auto logprob = [&](float v) {
+    if (none) return -INFINITY;
+    const float d = lp_fast(all.m, a.c) ? fmaf(v, a.c, -__fmul_rn(all.m, a.c)) : (v - all.m) * a.c;
+    // c (v - m) can be past fp32's range where (v - m) / T is not (masks of the type's lowest value); v - m can be, too,
+    // where T brings it back
+    if (d == -INFINITY && v > -INFINITY) return (a.t < 1.0f ? (v - all.m) / a.t : v / a.t - all.m / a.t) - LP_LN2 * log_s;
+    return LP_LN2 * (d - log_s);
+  };
   if (tid == 0) {
     const long long t = a.tokens[row];
     float lp = -INFINITY;
@@ -636,6 +643,7 @@ extern "C" fm_status fm_token_logprobs(const void* logits, int32_t dtype, int64_
   a.V = (int)V;
   a.rows = (int)rows;
   a.tokens = reinterpret_cast<const long long*>(tokens);
+  a.t = temperature;
   a.c = LP_LOG2E / temperature;
   a.lag = 8.0f / a.c;
   a.k = (int)top_k;

@@ -248,3 +248,25 @@ def test_large_logits(dtype, rows, T):
         got = call(x, tokens, top_k=k, temperature=T)
         check(type(got)(*[t[:9] for t in got]), x[:9], tokens[:9], k, T)
     assert error_word() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [3, 600])  # a cluster to a row, a block to a row
+@pytest.mark.parametrize("T", [1.0, 1.3, 1.5, 0.6])
+def test_tokens_of_the_lowest_value(dtype, rows, T):
+    """A mask of the type's lowest value beside ordinary and beside huge logits, as the given token and among the
+    alternatives: about -3.4e38 / T, which fp32 holds for a T of 1 and more; under 1 it is -inf."""
+    V, low, n = 3001, torch.finfo(dtype).min, 7
+    x = torch.full((rows, V), low)
+    open_ids = [3, 700, 701, 1500, 2999, 3000]
+    x[:, open_ids] = 3.0 * torch.randn(rows, 6, generator=torch.Generator().manual_seed(47))
+    x[2, open_ids] *= 1e31  # the row's largest value times log2(e) is no ordinary number
+    x = x.to(dtype)
+    tokens = torch.full((rows,), 5)
+    tokens[1] = 700
+    x, tokens = x.to(DEV), tokens.to(DEV)
+    got = call(x, tokens, top_k=n, temperature=T)
+    check(type(got)(*[t[:4] for t in got]), x[:4], tokens[:4], n, T)
+    ordinary = torch.arange(rows, device=DEV) != 2  # at T = 1 that row's masks are past fp32's range
+    assert math.isinf(float(got.logprobs[0])) == (T < 1) and (torch.isinf(got.top_logprobs[ordinary, 6]) == (T < 1)).all()
+    assert torch.isfinite(got.top_logprobs[:, :6]).all() and error_word() == 0
