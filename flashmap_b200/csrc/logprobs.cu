@@ -205,7 +205,8 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
     // c (v - m) can be past fp32's range where (v - m) / T is not (masks of the type's lowest value); v - m can be, too,
     // where T brings it back
     if (d == -INFINITY && v > -INFINITY) return (a.t < 1.0f ? (v - all.m) / a.t : v / a.t - all.m / a.t) - LP_LN2 * log_s;
-    return LP_LN2 * (d - log_s);
+    const float lp = LP_LN2 * (d - log_s);
+    return lp > 0.0f ? 0.0f : lp;  // d and log2 S of a token that is nearly certain agree but for their rounding
   };
   if (tid == 0) {
     const long long t = a.tokens[row];
@@ -215,7 +216,8 @@ __device__ void lp_finish(const LogprobArgs& a, int row, const LpSum& all, const
     else
       record_error(a.err, DEV_BAD_INDEX);
     a.logprob[row] = lp;
-    a.entropy[row] = none ? 0.0f : LP_LN2 * (log_s - all.u / all.s);
+    const float entropy = none ? 0.0f : LP_LN2 * (log_s - all.u / all.s);
+    a.entropy[row] = entropy < 0.0f ? 0.0f : entropy;
   }
   if (!TOP || a.k == 0) return;
   const int loads = (x.pieces + 31) / 32, groups = (loads + (1 << a.gs) - 1) >> a.gs;

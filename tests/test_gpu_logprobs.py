@@ -270,3 +270,21 @@ def test_tokens_of_the_lowest_value(dtype, rows, T):
     ordinary = torch.arange(rows, device=DEV) != 2  # at T = 1 that row's masks are past fp32's range
     assert math.isinf(float(got.logprobs[0])) == (T < 1) and (torch.isinf(got.top_logprobs[ordinary, 6]) == (T < 1)).all()
     assert torch.isfinite(got.top_logprobs[:, :6]).all() and error_word() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 128, 700])
+@pytest.mark.parametrize("T", [1.0, 0.7])
+def test_signs_of_certain_tokens(rows, T):
+    """One logit far above the rest, at values whose products with log2(e) / T round either way, and rows whose maximum
+    comes a little after a thread's first values: no log probability above 0, no entropy below 0."""
+    V = 5000
+    top = (1.3 + 0.37 * torch.arange(rows)) % 40
+    x = torch.full((rows, V), -80.0)
+    at = torch.arange(rows) * 7 % V
+    x[torch.arange(rows), at] = top
+    x[rows // 2:, 0] = top[rows // 2:] - 16.5  # e^-16.5 = 7e-8 of it
+    x, tokens = x.to(DEV), at.to(DEV)
+    got = call(x, tokens, top_k=3, temperature=T)
+    check(got, x, tokens, 3, T)
+    for t in (got.logprobs, got.top_logprobs, -got.entropy):
+        assert (t <= 0).all(), t.max().item()
