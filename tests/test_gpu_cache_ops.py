@@ -1007,3 +1007,36 @@ def test_head_groups_wider_than_a_row_tile(H, KH, dt):
     for r, n in enumerate(lengths):
         assert ((sums[r, :, :n].double().cpu() - w[r]).abs() <= (2.0 ** -16 + 2.0 ** -20) * w[r]).all()
     assert error_word() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 40])  # chunks of one row tile, of two
+@pytest.mark.parametrize("heavy", [0, 700])
+def test_window_many_keys_far_below_one_e4m3(rows, heavy):
+    """One key takes nearly all of the weight and has a value of 0, 1599 others 2^-22 to 2^-26 of it each: what they add
+    is the output.  As many requests (the same context) as leave the items whole.
+
+    Numerators are f16 with the row's largest at 2^11 or more: one of 2^-26 is 2^-15, whose steps are 2^-24: off by 2^-25
+    at most, 2^-36 of the largest.  n keys: n 2^-36 max |v| beside the rest."""
+    g = torch.Generator().manual_seed(71)
+    L, D, R, H = 1600, 64, 160, 4
+    pools, table, _ = make_cache(g, [L], 1, D, 16, FP8, "split")
+    j = torch.arange(L)
+    page = table[0, j // 16].long()
+    K, V = torch.zeros(L, D), torch.randn(L, D, generator=g).abs()
+    K[heavy], V[heavy] = 6.0, 0.0
+    for pool, x in zip(pools, (K, V)):
+        pool.view(torch.uint8)[page, 0, j % 16] = x.to(FP8).view(torch.uint8)
+    _, k, v = views(pools, D)
+    vmax = float(V.max())
+    lengths = torch.full((R,), L, dtype=torch.int32, device=DEV)
+    many = table.to(DEV).expand(R, -1)
+    for size in (0.3125, 0.328125, 0.375):  # e^-15, e^-15.75, e^-18
+        q = torch.full((rows, H, D), size).to(torch.bfloat16)
+        want, mag, _ = O.window_attention(q, *cpu_views(pools, D), torch.tensor([0, rows]), [L], table, D ** -0.5)
+        cu = rows * torch.arange(R + 1, dtype=torch.int32, device=DEV)
+        got = ops().paged_window_attention(q.to(DEV).repeat(R, 1, 1), k, v, cu, lengths, many, rows, L, D ** -0.5)
+        for r in (0, 77, 159):
+            err = (got[r * rows: (r + 1) * rows].double().cpu() - want).abs()
+            tol = (2.0 ** -11 + 2.0 ** -14) * mag + (2.0 ** -8 + 2.0 ** -14) * want.abs() + L * 2.0 ** -36 * vmax
+            assert (err <= tol).all(), (size, (err / tol).max().item())
+    assert error_word() == 0

@@ -373,3 +373,41 @@ def test_refusals():
     odd = torch.zeros(kc.numel() + 8, dtype=torch.uint8, device=DEV)[8:].view(kc.shape)
     with pytest.raises(_lib.FlashMapError):
         f(q, odd, vc, kf, vf, L, table, 5, 0.1)
+
+
+@pytest.mark.parametrize("rows", [1, 40])  # one row tile with both softmax warpgroups, two row tiles
+@pytest.mark.parametrize("heavy", [0, 700, 1599])
+def test_many_keys_far_below_one(rows, heavy):
+    """One key takes nearly all of the weight and has a value of 0, 1599 others 2^-22 to 2^-26 of it each: what they add
+    is the output.  As many requests (the same context) as leave the items whole.
+
+    A numerator of a row is at least 2^11 times its share of the row's largest, so one of 2^-26 is 2^-15 in f16, whose
+    steps there are 2^-24: off by 2^-25 at most, 2^-36 of the largest.  n keys: n 2^-36 max |v| beside the rest."""
+    g = torch.Generator().manual_seed(61)
+    L, D, R, H = 1600, 64, 160, 4
+    cache = Cache(g, [L], 1, D, 16, "split")
+    j = torch.arange(L)
+    page = cache.table[0, j // 16].long()
+    K, V = torch.zeros(L, D), torch.randn(L, D, generator=g).abs()
+    K[heavy], V[heavy] = 6.0, 0.0
+    for which, x in ((0, K), (1, V)):
+        codes, factors = O.quantise4(x)
+        kc, kf = cache.dev[which]
+        kc[page.to(DEV), 0, (j % 16).to(DEV)] = codes.to(DEV)
+        kf.view(torch.uint8)[page.to(DEV), 0, (j % 16).to(DEV)] = factors.view(torch.uint8).to(DEV)
+        cache.values[which][page, 0, j % 16] = O.values4(codes, factors)
+    vmax = float(cache.host()[1][page, 0, j % 16].abs().max())
+    table = cache.table.to(DEV).expand(R, -1)
+    lengths = torch.full((R,), L, dtype=torch.int32, device=DEV)
+    cu = rows * torch.arange(R + 1, dtype=torch.int32, device=DEV)
+    for size in (0.3125, 0.328125, 0.375):  # e^-15, e^-15.75, e^-18
+        q = torch.full((rows, H, D), size).to(torch.bfloat16)
+        want, mag, _ = C.window_attention(q, *cache.host(), torch.tensor([0, rows]), [L], cache.table, D ** -0.5)
+        got = ops().paged_window_attention_fp4(q.to(DEV).repeat(R, 1, 1), *cache.tensors(), cu, lengths, table, rows, L, D ** -0.5)
+        more = L * 2.0 ** -36 * vmax
+        for r in (0, 77, 159):
+            close(got[r * rows: (r + 1) * rows], want, mag, f"window, request {r}", more=more)
+        if rows == 1:
+            one = ops().paged_decode_attention_fp4(q.to(DEV).expand(R, -1, -1), *cache.tensors(), lengths, table, L, D ** -0.5)
+            close(one[159:], want, mag, "decode", more=more)
+    assert error_word() == 0
