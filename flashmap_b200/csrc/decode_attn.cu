@@ -28,6 +28,10 @@ namespace {
 
 constexpr int DA_STAGES = 2;
 constexpr int DA_TILE = 16;  // keys of a warp's tile
+// Of an e4m3 cache P goes to f16 times 2^15, the most that f16 has room for: only
+// numerators under 2^-29 of the largest meet its coarsest steps.  The lift is in
+// the subtracted maximum, so sums and gathered weights go by it, too.
+constexpr float DA_LIFT = 15.0f;
 
 template <int HD, bool KV8>
 struct DaLayout {
@@ -220,6 +224,7 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
     }
     const int key0 = begin + (t * 4 + warp) * DA_TILE;
     uint32_t pb[NG][2];
+    constexpr float LIFT = KV8 ? DA_LIFT : 0.0f;
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       float mx = -INFINITY;
@@ -240,7 +245,7 @@ __global__ void __launch_bounds__(128) decode_attn_kernel(DecodeArgs a) {
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(m[n], mx);
+      const float mn = fmaxf(m[n], mx - LIFT);
       const float u = mn == -INFINITY ? 0.0f : mn;
       if (__any_sync(0xffffffffu, mn != m[n])) {
         const float al = ex2(m[n] - u);

@@ -1040,3 +1040,30 @@ def test_window_many_keys_far_below_one_e4m3(rows, heavy):
             tol = (2.0 ** -11 + 2.0 ** -14) * mag + (2.0 ** -8 + 2.0 ** -14) * want.abs() + L * 2.0 ** -36 * vmax
             assert (err <= tol).all(), (size, (err / tol).max().item())
     assert error_word() == 0
+
+
+@pytest.mark.parametrize("heavy", [0, 700, 1599])
+@pytest.mark.parametrize("R", [1, 160])  # cut into chunks and joined, whole
+def test_decode_many_keys_far_below_one_e4m3(heavy, R):
+    """As above for one new token, with its gathered weights; numerators are f16 with a warp's largest at 2^15, so one of
+    2^-26 is 2^-11, within f16's ordinary steps."""
+    g = torch.Generator().manual_seed(72)
+    L, D, H = 1600, 64, 4
+    pools, table, _ = make_cache(g, [L], 1, D, 16, FP8, "split")
+    j = torch.arange(L)
+    page = table[0, j // 16].long()
+    K, V = torch.zeros(L, D), torch.randn(L, D, generator=g).abs()
+    K[heavy], V[heavy] = 6.0, 0.0
+    for pool, x in zip(pools, (K, V)):
+        pool.view(torch.uint8)[page, 0, j % 16] = x.to(FP8).view(torch.uint8)
+    _, k, v = views(pools, D)
+    lengths = torch.full((R,), L, dtype=torch.int32, device=DEV)
+    for size in (0.3125, 0.328125, 0.375):  # e^-15, e^-15.75, e^-18
+        q = torch.full((1, H, D), size).to(torch.bfloat16)
+        want, mag, w = O.decode_attention(q, *cpu_views(pools, D), [L], table, D ** -0.5)
+        sums = torch.zeros(R, 1, L, device=DEV)
+        args = (q.to(DEV).expand(R, -1, -1), k, v, lengths, table.to(DEV).expand(R, -1), L, D ** -0.5)
+        for kw in ({}, dict(weight_sums=sums)):
+            close(ops().paged_decode_attention(*args, **kw)[R - 1:], want, mag, "decode", True)
+        assert ((sums[R - 1].double().cpu() - w[0]).abs() <= 2.0 ** -16 * w[0] + 2.0 ** -22 * w[0]).all()
+    assert error_word() == 0
