@@ -159,6 +159,7 @@ _SIGNATURES = {
     "fm_last_error": (ctypes.c_char_p, []),
     "fm_version": (c_int, []),
     "fm_check_device": (c_int, []),
+    "fm_error_word": (c_int, [ctypes.POINTER(c_void_p)]),
     "fm_gemm_workspace_size": (c_size_t, [c_int64, c_int64, c_int64]),
     "fm_gemm_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p,
                              c_int, c_void_p, c_size_t, c_void_p, c_void_p]),

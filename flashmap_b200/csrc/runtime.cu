@@ -28,6 +28,9 @@ EncodeTiledFn encode_fn() {
   });
   return fn;
 }
+
+// The word that kernels record an index or a wait in: one to a device, zero from the library's loading on.
+__device__ __align__(256) int32_t g_error_word;
 }  // namespace
 
 fm_status set_error(fm_status code, const char* fmt, ...) {
@@ -110,5 +113,19 @@ extern "C" fm_status fm_check_device(void) {
   cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
   if (major != 10 || minor != 0)
     return fm::set_error(FM_ERR_ARCH, "device %d is sm_%d%d; this library is built for sm_100a", dev, major, minor);
+  return FM_OK;
+}
+
+extern "C" fm_status fm_error_word(int32_t** word) {
+  if (!word) return fm::set_error(FM_ERR_INVALID, "error_word: null pointer");
+  // the library may be loaded onto the device by this, which a capture in progress would refuse otherwise
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return fm::check_cuda(e, "error_word");
+  void* at = nullptr;
+  e = cudaGetSymbolAddress(&at, fm::g_error_word);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return fm::check_cuda(e, "error_word");
+  *word = static_cast<int32_t*>(at);
   return FM_OK;
 }

@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import threading
 from typing import NamedTuple
 
 import torch
@@ -29,19 +30,39 @@ def _stream():
 
 
 _ERR_WORDS: dict = {}
+_ERR_LOCK = threading.Lock()
+
+
+class _Int32:
+    """One int32 of device memory, as torch takes it over."""
+
+    def __init__(self, address: int):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False), "version": 2}
+
+
+def _new_error_word(device) -> torch.Tensor:
+    if device.type != "cuda":
+        return torch.zeros(1, dtype=torch.int32, device=device)
+    at = ctypes.c_void_p()
+    with torch.cuda.device(device):
+        _lib.call("fm_error_word", ctypes.byref(at))
+        return torch.as_tensor(_Int32(at.value))
 
 
 def error_word(device) -> torch.Tensor:
     """The device's error word (int32, zero until a kernel records an index or
-    timeout code; the first code sticks), allocated once per device so that a
-    call launches no fill kernel for it."""
+    timeout code; the first code sticks): the library's own memory, so that the
+    first call may come from any thread and while a graph is captured, and no
+    call launches a fill kernel for it."""
     key = torch.device(device)
     if key.index is None:
         key = torch.device(key.type, torch.cuda.current_device())
     w = _ERR_WORDS.get(key)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=key)
-        _ERR_WORDS[key] = w
+        with _ERR_LOCK, torch.inference_mode(False):  # the word outlives the mode that it is first asked for in
+            w = _ERR_WORDS.get(key)
+            if w is None:
+                w = _ERR_WORDS[key] = _new_error_word(key)
     return w
 
 

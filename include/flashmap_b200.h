@@ -58,6 +58,9 @@ FM_API const char* fm_last_error(void);
 FM_API int fm_version(void);
 /* 0 when the current device is an sm_100 part this library was built for. */
 FM_API fm_status fm_check_device(void);
+/* A word of the current device, zero until a kernel that it is given to as `err` records something; the library's own,
+ * the same for every caller.  May be asked for at any time, a stream capture included. */
+FM_API fm_status fm_error_word(int32_t** word);
 
 /* ------------------------------------------------------------------------
  * Primitive operators (unit-test entry points and building blocks).
