@@ -86,6 +86,14 @@ __global__ void __launch_bounds__(NT) decode_join_kernel(DecodeArgs a, int row_b
   __shared__ float2 sst[DJ_HEADS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = a.c.R * a.H;
+  // A row's length is read while the chunks are still at work: they do not write it, and since this launch's CTAs begin
+  // when all of theirs have passed their own wait, nothing before them does any more.
+  int row_n = 0;  // chunks of a block's row
+  if (!WARP_ROWS && (int)blockIdx.x < row_blocks) {
+    const Span sp = visible_span(cache_length(a.c, (int)blockIdx.x / a.H, a.err, false), a.window, a.sinks);
+    const int size = chunk_of(a, sp.n);
+    row_n = (sp.n + size - 1) / size;
+  }
   pdl_wait();
   if (WARP_ROWS && (int)blockIdx.x < row_blocks) {
     const int row = blockIdx.x * (NT / 32) + warp, r = row / a.H, h = row % a.H;
@@ -116,28 +124,28 @@ __global__ void __launch_bounds__(NT) decode_join_kernel(DecodeArgs a, int row_b
     return;
   }
   if (!WARP_ROWS && (int)blockIdx.x < row_blocks) {
+    const int n = row_n;
+    if (n <= 1) return;  // written by its only chunk
     const int row = blockIdx.x, r = row / a.H, h = row % a.H;
     const float2* stats = a.stats + (long long)row * a.chunks;
     constexpr int V = HD / 4, PER = NT / V;  // threads per chunk's row, chunks at a time
     const float4* part = reinterpret_cast<const float4*>(a.part + (long long)row * a.chunks * HD) + tid % V;
-    // The first chunks are read before it is known how many there are: what
-    // lies behind the last is not looked at (100003 positions of 4 bits in 74 chunks: 34.1 us, and 31.7 us so).
+    // The first chunks are all read at once (100003 positions of 4 bits in 74 chunks: 34.1 us, and 32.3 us so).  Reading
+    // them before the length is known gains 0.3 us more, but requests of one chunk in a call that is sized for many
+    // then read for nothing (8 of 200 positions sized for 131072, bf16: 8.6 us, and 7.9 us so).
     constexpr int F = 4, U = 4;
     float2 first[F];
     float4 x[U];
     float m[U];
 #pragma unroll
     for (int f = 0; f < F; ++f)
-      if (lane + 32 * f < a.chunks) first[f] = stats[lane + 32 * f];
+      if (lane + 32 * f < n) first[f] = stats[lane + 32 * f];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (tid / V + u * PER < a.chunks) {
+      if (tid / V + u * PER < n) {
         x[u] = part[(long long)(tid / V + u * PER) * V];
         m[u] = stats[tid / V + u * PER].x;
       }
-    const Span sp = visible_span(cache_length(a.c, r, a.err, false), a.window, a.sinks);
-    const int size = chunk_of(a, sp.n), n = (sp.n + size - 1) / size;
-    if (n <= 1) return;  // written by its only chunk
     const float2 st = row_stats(stats, n, first);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](const float4& v, float top) {

@@ -411,3 +411,18 @@ def test_many_keys_far_below_one(rows, heavy):
             one = ops().paged_decode_attention_fp4(q.to(DEV).expand(R, -1, -1), *cache.tensors(), lengths, table, L, D ** -0.5)
             close(one[159:], want, mag, "decode", more=more)
     assert error_word() == 0
+
+
+def test_short_and_long_contexts_in_a_call_sized_for_more():
+    """Requests of one chunk, of a few and of many beside one another, where rows are joined by a block each."""
+    g = torch.Generator().manual_seed(62)
+    lengths = [5, 300, 20003, 0, 200]
+    cache = Cache(g, lengths, 2, 64, 16, "joint")
+    q = torch.randn(5, 8, 64, generator=g).to(torch.bfloat16)
+    want, mag = cache.want(q)
+    L = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    table = torch.zeros(5, 8192, dtype=torch.int32)
+    table[:, : cache.table.shape[1]] = cache.table
+    got = [ops().paged_decode_attention_fp4(q.to(DEV), *cache.tensors(), L, table.to(DEV), 131072, 64 ** -0.5) for _ in range(3)]
+    close(got[0], want, mag, "decode")
+    assert all(torch.equal(got[0], x) for x in got[1:]) and error_word() == 0
