@@ -27,6 +27,7 @@ namespace fm {
 namespace {
 
 constexpr int D4_TILE = 32;  // keys of a warp's tile
+constexpr int D4_STAGES = 2;
 // A CTA's first copies and its merge weigh more against 4-bit keys: one long
 // request is cut into as many chunks as CTAs are resident (100003 positions,
 // 8 kv heads: 34 us, and 40 us in three times as many, both with a join slower by 2 us), and a batch into chunks
@@ -38,17 +39,17 @@ constexpr DecodeRule D4_RULE{148 * 4, 128, 1536, 2048, 148 * 32};
 // the largest meet f16's coarsest steps.
 constexpr float D4_LIFT = 11.0f, D4_LAG = 4.0f;
 
-template <int HD, int STAGES>
+template <int HD>
 struct D4Layout {
   static constexpr int RB = HD / 2, SB = HD / 16;  // bytes of a row's codes, of its factors
   static constexpr int V = D4_TILE * RB, KF = 2 * V, VF = KF + D4_TILE * SB;
   static constexpr int STAGE = 2 * D4_TILE * (RB + SB);
-  static constexpr int WARP = STAGES * STAGE;
+  static constexpr int WARP = D4_STAGES * STAGE;
 };
-template <int HD, int NG, int STAGES>
+template <int HD, int NG>
 constexpr int d4_smem() {
-  constexpr int merge = 4 * 8 * NG * (HD + 4) * 4 + 4 * 8 * NG * 8 + 8 * NG * 8, pipe = 4 * D4Layout<HD, STAGES>::WARP;
-  return (pipe > merge ? pipe : merge) + 4 * STAGES * 4;
+  constexpr int merge = 4 * 8 * NG * (HD + 4) * 4 + 4 * 8 * NG * 8 + 8 * NG * 8, pipe = 4 * D4Layout<HD>::WARP;
+  return (pipe > merge ? pipe : merge) + 4 * D4_STAGES * 4;
 }
 
 // Where 16-byte chunk `ch` of a tile's row lies.  A thread's rows are those of
@@ -93,9 +94,10 @@ __device__ __forceinline__ uint32_t d4_transpose(uint32_t x) {
 }
 
 // NG: groups of 8 query heads (1 or 2).  WIDE: offsets past 32 bits in NarrowRef's units.
-template <int HD, int NG, int STAGES, bool WIDE>
+template <int HD, int NG, bool WIDE>
 __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef f, NarrowRef nr) {
-  using Lay = D4Layout<HD, STAGES>;
+  using Lay = D4Layout<HD>;
+  constexpr int STAGES = D4_STAGES;
   constexpr int RB = Lay::RB, SB = Lay::SB;
   constexpr int KW = HD / 32, VW = HD / 64;  // words of a thread's piece of a key, of a value
   constexpr int KS = HD / 16;                // products along d, and rows of sixteen d of the output
@@ -122,7 +124,7 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
   const int begin = chunk * size, end = min(sp.n, begin + size);
 
   const uint32_t wbase = smem_u32(d4_smem_buf) + warp * Lay::WARP;
-  uint32_t* wok = reinterpret_cast<uint32_t*>(d4_smem_buf + d4_smem<HD, NG, STAGES>() - 4 * STAGES * 4) + warp * STAGES;
+  uint32_t* wok = reinterpret_cast<uint32_t*>(d4_smem_buf + d4_smem<HD, NG>() - 4 * STAGES * 4) + warp * STAGES;
   const int ntiles = (end - begin + 4 * D4_TILE - 1) / (4 * D4_TILE);
   const long long trow = (long long)r * a.c.tstride;
   // page and token of this lane's key of tile t, read one tile ahead of its copies
@@ -426,10 +428,10 @@ __global__ void __launch_bounds__(128) decode_fp4_kernel(DecodeArgs a, ScaleRef 
 
 template <int HD, int NG, bool WIDE>
 fm_status launch_decode_fp4(const DecodeArgs& a, const ScaleRef& f, const NarrowRef& nr, unsigned grid, cudaStream_t s) {
-  constexpr int STAGES = 2, smem = d4_smem<HD, NG, STAGES>();
-  const fm_status st = allow_smem<decode_fp4_kernel<HD, NG, STAGES, WIDE>>(smem, "paged_decode_attn_fp4");
+  constexpr int smem = d4_smem<HD, NG>();
+  const fm_status st = allow_smem<decode_fp4_kernel<HD, NG, WIDE>>(smem, "paged_decode_attn_fp4");
   if (st != FM_OK) return st;
-  return launch_kernel(decode_fp4_kernel<HD, NG, STAGES, WIDE>, dim3(grid), dim3(128), smem, s, true, a, f, nr);
+  return launch_kernel(decode_fp4_kernel<HD, NG, WIDE>, dim3(grid), dim3(128), smem, s, true, a, f, nr);
 }
 template <int HD, bool WIDE>
 fm_status launch_decode_fp4(const DecodeArgs& a, const ScaleRef& f, const NarrowRef& nr, int ng, unsigned grid, cudaStream_t s) {

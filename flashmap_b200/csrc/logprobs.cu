@@ -12,7 +12,7 @@
 // cancels; only where |c m| is 2^24 or more (rows of a mask's value, tiny T) as
 // c (x - m), since a rounding of 2^7 and more would be past the exponentials' range.
 //
-// Alternatives.  The pass also leaves the maximum of every group of one or more
+// Alternatives.  The pass also leaves the maximum of every group of two or more
 // warp loads (512 bytes each).  The k largest values, equal ones by the lowest id, lie in the
 // k groups that come first by (maximum, lowest group): an element of another
 // group is preceded by the k maxima of those.  Those groups are read once more
@@ -439,21 +439,17 @@ __global__ void __launch_bounds__(LP_T, 4) logprob_scan_kernel(LogprobArgs a) {
     v.s = s2.x + s2.y;
     v.u = u2.x + u2.y;
     if constexpr (TOP) {
-      if constexpr (!LONG) {  // groups of one, two or four loads
+      if constexpr (!LONG) {  // groups of two or four loads
         if (a.gs == 1) {
           mx[0] = fmaxf(mx[0], mx[1]);
           mx[1] = fmaxf(mx[2], mx[3]);
-        } else if (a.gs == 2) {
+        } else {
           mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         }
         float mine = lp_warp_max(mx[0]);
-        if (a.gs < 2) {
+        if (a.gs == 1) {
           const float g = lp_warp_max(mx[1]);
           mine = lane == 1 ? g : mine;
-        }
-        if (a.gs < 1) {
-          const float g = lp_warp_max(mx[2]), h = lp_warp_max(mx[3]);
-          mine = lane == 2 ? g : lane == 3 ? h : mine;
         }
         const int g0 = (l1 >> a.gs) + lane;
         if (lane < LP_LOADS >> a.gs && g0 << a.gs < loads) gmax[g0] = mine;
