@@ -31,7 +31,8 @@ writes it, and f16 holds its values exactly.
 
 Query head h reads kv head ``h // (heads / kv_heads)``.  Scores, softmax sums
 and outputs are held in fp32; the softmax numerators are rounded to bf16 (to
-f16 for an e4m3 or 4-bit cache) for the product with the values, and the output to bf16.
+f16 for an e4m3 or 4-bit cache, 2^11 or more of a row's largest) for the product with
+the values, and the output to bf16.
 A row that sees no position is zero.  A position that no row of a request may
 see is never read.  Each call checks its arguments (``OpArgumentError``; the
 alignment of addresses and strides and the limits of sizes are the library's to
@@ -39,8 +40,8 @@ check, ``FlashMapError``), records lengths, bounds and page ids out of range
 for ``check_device_errors``, runs on the current stream without a host
 synchronisation, and can be captured in a CUDA graph.  The two attentions are
 registered operators (``flashmap_b200::paged_decode_attention[_fp4]``,
-``::paged_window_attention[_fp4]``) to ``torch.compile``; they have no gradient, and
-asking for one raises.  There is no fallback.
+``::paged_window_attention[_fp4]``) to ``torch.compile``, which breaks a graph at the
+other calls; they have no gradient, and asking for one raises.  There is no fallback.
 """
 
 from __future__ import annotations

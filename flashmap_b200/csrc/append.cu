@@ -8,10 +8,11 @@
 // e2m1 codes of x / f, both to nearest even.
 //
 // Every value is read and written once, so its bytes bound a prompt: 16504 tokens
-// of 32 query heads on 8 of 128 into 4 bits, 72 us (5.1 TB/s), where a row to a
+// of 32 query heads on 8 of 128 into 4 bits, 72 to 75 us (4.9 to 5.1 TB/s), where a row to a
 // thread, each looking its request up, took 150 us, and 113 us with three rows to
 // a thread.  What is left is a warp's wait for its next four slots and the
-// roundings' instructions (issue slots 59 percent).  A few tokens cost the chain
+// roundings' instructions (issue slots 59 percent; 64 registers to a thread, of
+// which rotated rows into narrow caches spill 4 to 24 bytes).  A few tokens cost the chain
 // of row bounds, position and cosines: 2.5 us on the GPU, less than the call's
 // host time.
 #include <algorithm>

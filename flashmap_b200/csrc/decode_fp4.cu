@@ -14,11 +14,13 @@
 // bytes of a key, and 8 of a value, as they lie.  Values of two keys
 // are paired for V^T by exchanging half bytes before the conversion.
 //
-// Measured, 32 heads on 8 of 128: 128 requests of 1024 .. 8192, 165 us (4.1 TB/s);
+// Measured, 32 heads on 8 of 128: 128 requests of 1024 .. 8192, 165 to 174 us (3.9 to 4.1 TB/s);
 // 1 request of 100003, 32 us (3.6 TB/s, of which 5 us are the join); 201
 // positions, 4.8 us.  No unit is full: the arithmetic pipe that converts is at 53
 // percent and issue slots at 59, with four warps to a scheduler (registers);
-// five, and a third stage of copies, measured the same, six spill.
+// five, and a third stage of copies, measured the same, six spill.  More than 8
+// heads to a group take 230 to 240 registers, two CTAs to an SM: 64 heads on 4 read
+// the same bytes in 280 us, 2.5 TB/s.  At head_dim 64 and 32 heads on 8: 108 us, 3.2 TB/s.
 #include <type_traits>
 
 #include "decode_parts.cuh"
@@ -29,9 +31,10 @@ namespace {
 constexpr int D4_TILE = 32;  // keys of a warp's tile
 constexpr int D4_STAGES = 2;
 // A CTA's first copies and its merge weigh more against 4-bit keys: one long
-// request is cut into as many chunks as CTAs are resident (100003 positions,
-// 8 kv heads: 34 us, and 40 us in three times as many, both with a join slower by 2 us), and a batch into chunks
-// of 2048 keys (128 requests of 1024 .. 8192: 163 us; of 1024 keys 173 us, of 4096 170 us).
+// request is cut into 148 * 4 chunks, the CTAs that are resident at head_dim 128 and up to
+// 8 heads to a group (100003 positions, 8 kv heads: 34 us, and 40 us in three times as many, both with a join slower by 2 us), and a batch into chunks
+// of 2048 keys (128 requests of 1024 .. 8192, on one GPU: 163 us; of 1024 keys 173 us, of 4096 170 us).  Wider
+// groups, of which two CTAs are resident, and head_dim 64 go by the same numbers; others were not tried there.
 constexpr DecodeRule D4_RULE{148 * 4, 128, 1536, 2048, 148 * 32};
 
 // P goes to f16 times 2^11, and the subtracted maximum may lag behind the true

@@ -18,11 +18,13 @@
 // bound by the cache's bytes and the latency of a CTA's first tiles (24 x 17 rows
 // on 512 .. 4096 positions: 64 us, 3.65 TB/s).
 //
-// A cache of 4 bits halves or quarters the bytes and adds their widening: 24 x 17
-// rows take 68 us, of which 27 are a CTA's first and last tiles and 1.9 us each
-// key tile, the chain of a loading warp over its 32 rows; 2 x 2048 rows on 4100
-// .. 6200 positions 278 us (996 TFLOP/s of the visible pairs; 251 us without the
-// loading warps' work).
+// A cache of 4 bits halves or quarters the bytes and adds their widening, so it
+// is no faster than one of bf16: 24 x 17 rows take 68 us, of which 27 are a CTA's
+// first and last tiles and 1.9 us each key tile, the chain of a loading warp over
+// its 32 rows; 2 x 2048 rows on 4100 .. 6200 positions 280 to 299 us (925 to 990
+// TFLOP/s of the visible pairs; a tenth less without the loading warps' work).
+// The kernels of narrow caches spill 44 to 68 bytes of a thread's registers; those
+// of bf16 none.
 #include "paged_cache.cuh"
 
 namespace fm {

@@ -253,8 +253,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, t
     A row's values are contiguous, rows may lie further apart (a vocabulary padded in memory); more than one leading
     dimension is flattened, with a copy where its strides do not allow a view.  An id outside the vocabulary has
     log probability -inf and is recorded for ``cache_ops.check_device_errors``.  A row of -inf alone has -inf and entropy 0,
-    one with a NaN or +inf NaN throughout.  Runs on the current stream without a host synchronisation and can be
-    captured in a CUDA graph; there is no gradient."""
+    one with a NaN or +inf NaN throughout; a finite logit's is finite where fp32 holds it (a mask of the type's lowest value:
+    about -3.4e38 / temperature).  None is above 0, and no entropy below.  Runs on the current stream without a host
+    synchronisation and can be captured in a CUDA graph; it is no registered operator, so ``torch.compile`` breaks a graph
+    here, and there is no gradient."""
     if not logits.is_cuda or logits.dtype not in (torch.bfloat16, torch.float32) or logits.dim() < 1:
         raise ValueError(f"logits must be a CUDA bf16 or fp32 tensor, got {logits.dtype} on {logits.device}")
     dev, shape = logits.device, logits.shape[:-1]
